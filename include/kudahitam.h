@@ -58,7 +58,8 @@ int kh_version(void);
  * gave up set a bit).  Synchronous: reads device memory.  0 = no error.
  * Bit 0: an mbarrier wait of a compressor gave up; bit 1: a tile index fell
  * outside every segment; bit 2: kh_decode_combine_from_peers stopped waiting
- * for a peer's flag. */
+ * for a peer's flag; bit 3: a slot, position, length or page index of a paged
+ * call was out of range. */
 int kh_device_error(uint32_t* out_flags);
 int kh_clear_device_error(void);
 
@@ -397,6 +398,79 @@ int kh_decode_attn_static(const float* q, int64_t n_groups, int head_dim,
                           const float* d_v_host, const float* centroids_host,
                           int n_centroids, float sm_scale, int n_splits,
                           float* out, void* stream);
+
+/*
+ * Paged packed cache (no counterpart in the reference, which keeps one
+ * contiguous tensor per layer).  A pool of n_pages pages holds page_size rows
+ * of every KV head; row (page, head, offset) is row
+ * (page * n_kv_heads + head) * page_size + offset of the planes, which have
+ * the packed layout above (2-level codebook, residual plane).  page_size is
+ * any number >= 1.  All pointers are device pointers, planes 16-byte aligned.
+ */
+typedef struct kh_paged_cache {
+  uint32_t *k_code, *k_res;
+  float *k_norms, *k_rnorms;
+  uint32_t *v_code, *v_res;
+  float *v_norms, *v_rnorms;
+  int64_t n_pages;
+  int page_size, n_kv_heads, head_dim;
+} kh_paged_cache;
+
+/*
+ * kh_paged_append -- rotate, compress and store the keys and values of
+ * n_tokens tokens in one launch.
+ *   k, v       device, element e of head h of token t at
+ *              t * token_stride + h * head_stride + e (strides in elements)
+ *   slots      device int64 [n_tokens]: page * page_size + offset of each
+ *              token's row; -1 stores nothing (padding).  Slots of one call
+ *              must differ: two tokens of one slot leave a mixture.
+ *   positions  device int64 [n_tokens], or NULL: keys are stored unrotated.
+ *   cos, sin   device float [n_positions][rot_dim / 2]; the first rot_dim
+ *              elements of a key turn in pairs (i, i + rot_dim / 2), or
+ *              (2 i, 2 i + 1) with `interleaved`.
+ * Bits are those of the 64-bit computation (see the kernel); norms are
+ * float.  A slot outside the pool (other than -1) or a position outside the
+ * tables stores nothing and sets bit 3 of kh_device_error().
+ */
+int kh_paged_append(const kh_paged_cache* cache, const void* k, const void* v, int dtype,
+                    int64_t n_tokens, int64_t k_token_stride, int64_t k_head_stride,
+                    int64_t v_token_stride, int64_t v_head_stride, const int64_t* slots,
+                    const int64_t* positions, const float* cos, const float* sin,
+                    int64_t n_positions, int rot_dim, int interleaved, const float* d_k_host,
+                    const float* d_v_host, const float* centroids_host, int n_centroids,
+                    void* stream);
+
+/*
+ * kh_paged_attn -- decode attention of one query token per sequence over its
+ * pages: t_j = cap tanh(s_j sm_scale / cap) - slope (len - 1 - j) over rows
+ * j in [max(start, len - window), len), softmax, sum of V_hat (definitions at
+ * kh_decode_partial).  A sequence with no such row gets zeros (lse -inf).
+ *   q           device [n_seqs][n_kv_heads * n_q][head_dim] of `dtype`; query
+ *               head hq reads KV head hq / n_q.  out has q's shape and type.
+ *   table       device int32, page of block i of sequence b at
+ *               b * table_stride + i, for i < ceil(max_len / page_size)
+ *   lengths     device int32 [n_seqs], each at most max_len
+ *   starts      device int32 [n_seqs] first attended row, or NULL (0)
+ *   prefix_len  the first prefix_len rows are the same cached rows for every
+ *               sequence: they are read through sequence 0's table row, once
+ *               for all sequences.  0: nothing shared.
+ *   window      0, or how many of the last rows are attended
+ *   softcap     0, or the cap; slopes: device float [n_kv_heads * n_q] or NULL
+ *   workspace   kh_paged_workspace_bytes() bytes of device memory for the
+ *               same sizes on the current device (none read before written)
+ *   lse         device float [n_seqs][n_kv_heads * n_q] or NULL: natural log
+ *               of sum exp t_j
+ * A length outside [0, max_len] is clamped, a row whose page is outside the
+ * pool is not attended; both set bit 3 of kh_device_error().
+ */
+int64_t kh_paged_workspace_bytes(int64_t n_seqs, int n_q, int n_kv_heads, int head_dim,
+                                 int64_t max_len, int64_t prefix_len, int64_t window);
+int kh_paged_attn(const kh_paged_cache* cache, const void* q, int dtype, int64_t n_seqs, int n_q,
+                  const int32_t* table, int64_t table_stride, const int32_t* lengths,
+                  const int32_t* starts, int64_t max_len, int64_t prefix_len, int64_t window,
+                  float softcap, const float* slopes, float sm_scale, const float* d_k_host,
+                  const float* d_v_host, const float* centroids_host, int n_centroids,
+                  void* workspace, int64_t workspace_bytes, void* out, float* lse, void* stream);
 
 #ifdef __cplusplus
 }

@@ -14,6 +14,7 @@
 
 #include "kh_common.cuh"
 #include "kh_internal.h"
+#include "kh_paged.h"
 
 namespace kh {
 
@@ -627,6 +628,148 @@ int kh_decode_attn(const float* q, int64_t n_groups, int head_dim,
   if (st != KH_OK) return st;
   return kh_decode_combine(static_cast<const float*>(workspace), n_groups,
                            n_splits, head_dim, d_v_host, out, stream);
+}
+
+// The checks that both paged calls share; fills the pools.
+static int check_paged(const kh_paged_cache* c, int dtype, const float* dk, const float* dv,
+                       const float* cent, int n_c, Codebook* cb, PagedPool* kp, PagedPool* vp) {
+  if (!c) return KH_EINVAL;
+  if (dtype != KH_F32 && dtype != KH_F16 && dtype != KH_BF16) return KH_EINVAL;
+  if (!valid_head_dim(c->head_dim) || c->page_size < 1 || c->n_kv_heads < 1 || c->n_pages < 0)
+    return KH_EINVAL;
+  if (c->n_kv_heads > 65535 || c->n_pages > (int64_t(1) << 31) - 1 ||
+      c->n_pages * c->n_kv_heads > (int64_t(1) << 40) / c->page_size)
+    return KH_EINVAL;
+  if (!make_codebook(cent, n_c, cb)) return KH_EINVAL;
+  if (cb->n_c != 2) return KH_ENOTSUP;  // 2-level caches only
+  if (!check_d(dk, c->head_dim) || !check_d(dv, c->head_dim)) return KH_EINVAL;
+  *kp = PagedPool{c->k_code, c->k_res, c->k_norms, c->k_rnorms};
+  *vp = PagedPool{c->v_code, c->v_res, c->v_norms, c->v_rnorms};
+  for (const PagedPool* p : {kp, vp}) {
+    if (c->n_pages > 0 && (!p->code || !p->res || !p->norms || !p->rnorms)) return KH_EINVAL;
+    if (!aligned16(p->code) || !aligned16(p->res) || !aligned16(p->norms) || !aligned16(p->rnorms))
+      return KH_EALIGN;
+  }
+  return KH_OK;
+}
+
+static void sign_bits(const float* d, int D, uint32_t (&neg)[8]) {
+  for (int i = 0; i < D; ++i)
+    if (d[i] < 0.f) neg[i >> 5] |= 1u << (i & 31);
+}
+
+int kh_paged_append(const kh_paged_cache* cache, const void* k, const void* v, int dtype,
+                    int64_t n_tokens, int64_t k_token_stride, int64_t k_head_stride,
+                    int64_t v_token_stride, int64_t v_head_stride, const int64_t* slots,
+                    const int64_t* positions, const float* cos, const float* sin,
+                    int64_t n_positions, int rot_dim, int interleaved, const float* d_k_host,
+                    const float* d_v_host, const float* centroids_host, int n_centroids,
+                    void* stream) {
+  PagedAppendRequest r;
+  memset(&r, 0, sizeof(r));
+  Codebook cb;
+  const int st = check_paged(cache, dtype, d_k_host, d_v_host, centroids_host, n_centroids, &cb,
+                             &r.kp, &r.vp);
+  if (st != KH_OK) return st;
+  if (n_tokens < 0 || n_tokens > (int64_t(1) << 31) - 1) return KH_EINVAL;
+  if (interleaved != 0 && interleaved != 1) return KH_EINVAL;
+  if (positions) {
+    if (!cos || !sin || n_positions < 1) return KH_EINVAL;
+    if (rot_dim < 2 || rot_dim > cache->head_dim || (rot_dim & 1)) return KH_EINVAL;
+    if ((reinterpret_cast<uintptr_t>(positions) & 7) || !aligned4(cos) || !aligned4(sin))
+      return KH_EALIGN;
+  }
+  if (n_tokens == 0) return KH_OK;
+  if (!k || !v || !slots) return KH_EINVAL;
+  const uintptr_t em = dtype_size(dtype) - 1;
+  if ((reinterpret_cast<uintptr_t>(k) & em) || (reinterpret_cast<uintptr_t>(v) & em) ||
+      (reinterpret_cast<uintptr_t>(slots) & 7))
+    return KH_EALIGN;
+  r.k = k; r.v = v;
+  r.dtype = dtype;
+  r.n_tokens = n_tokens;
+  r.n_kv_heads = cache->n_kv_heads;
+  r.D = cache->head_dim;
+  r.k_stride_t = k_token_stride; r.k_stride_h = k_head_stride;
+  r.v_stride_t = v_token_stride; r.v_stride_h = v_head_stride;
+  r.slots = slots;
+  r.positions = positions;
+  r.cos = cos; r.sin = sin;
+  r.n_positions = n_positions;
+  r.rot_dim = positions ? rot_dim : 0;
+  r.interleaved = interleaved;
+  sign_bits(d_k_host, r.D, r.dk_neg);
+  sign_bits(d_v_host, r.D, r.dv_neg);
+  r.c0 = cb.c[0];
+  r.c1 = cb.c[1];
+  r.n_pages = cache->n_pages;
+  r.page_size = cache->page_size;
+  return launch_paged_append(r, static_cast<cudaStream_t>(stream));
+}
+
+int64_t kh_paged_workspace_bytes(int64_t n_seqs, int n_q, int n_kv_heads, int head_dim,
+                                 int64_t max_len, int64_t prefix_len, int64_t window) {
+  if (n_seqs < 0 || n_q < 1 || n_kv_heads < 1 || !valid_head_dim(head_dim) || max_len < 0 ||
+      max_len > (int64_t(1) << 31) - 1 || prefix_len < 0 || prefix_len > max_len || window < 0 ||
+      n_seqs * n_q > (int64_t(1) << 31) / n_kv_heads)
+    return -1;
+  const PagedPlan p = paged_plan(n_seqs, n_q, n_kv_heads, head_dim, max_len, prefix_len, window,
+                                 sm_count());
+  return n_seqs * n_q * n_kv_heads * p.parts() * (int64_t)(head_dim + 2) * 4;
+}
+
+int kh_paged_attn(const kh_paged_cache* cache, const void* q, int dtype, int64_t n_seqs, int n_q,
+                  const int32_t* table, int64_t table_stride, const int32_t* lengths,
+                  const int32_t* starts, int64_t max_len, int64_t prefix_len, int64_t window,
+                  float softcap, const float* slopes, float sm_scale, const float* d_k_host,
+                  const float* d_v_host, const float* centroids_host, int n_centroids,
+                  void* workspace, int64_t workspace_bytes, void* out, float* lse, void* stream) {
+  PagedAttnRequest r;
+  memset(&r, 0, sizeof(r));
+  Codebook cb;
+  const int st = check_paged(cache, dtype, d_k_host, d_v_host, centroids_host, n_centroids, &cb,
+                             &r.kp, &r.vp);
+  if (st != KH_OK) return st;
+  const int64_t need = kh_paged_workspace_bytes(n_seqs, n_q, cache->n_kv_heads, cache->head_dim,
+                                                max_len, prefix_len, window);
+  if (need < 0) return KH_EINVAL;
+  if (!std::isfinite(sm_scale) || !std::isfinite(softcap) || softcap < 0.f) return KH_EINVAL;
+  const int64_t blocks = (max_len + cache->page_size - 1) / cache->page_size;
+  if (table_stride < 0 || (n_seqs > 1 && table_stride < blocks)) return KH_EINVAL;
+  if (n_seqs == 0) return KH_OK;
+  if (!q || !lengths || !out || (blocks > 0 && !table)) return KH_EINVAL;
+  if (need > 0 && (!workspace || workspace_bytes < need)) return KH_EINVAL;
+  const uintptr_t em = dtype_size(dtype) - 1;
+  if ((reinterpret_cast<uintptr_t>(q) & em) || (reinterpret_cast<uintptr_t>(out) & em) ||
+      !aligned4(table) || !aligned4(lengths) || !aligned4(starts) || !aligned4(slopes) ||
+      !aligned16(workspace) || !aligned4(lse))
+    return KH_EALIGN;
+  r.q = q;
+  r.dtype = dtype;
+  r.n_seqs = n_seqs;
+  r.n_q = n_q;
+  r.n_kv_heads = cache->n_kv_heads;
+  r.D = cache->head_dim;
+  r.n_pages = cache->n_pages;
+  r.page_size = cache->page_size;
+  r.table = table;
+  r.table_stride = table_stride;
+  r.lengths = lengths;
+  r.starts = starts;
+  r.max_len = max_len;
+  r.prefix_len = prefix_len;
+  r.window = window;
+  r.softcap = softcap;
+  r.slopes = slopes;
+  r.sm_scale = sm_scale;
+  sign_bits(d_k_host, r.D, r.dk_neg);
+  sign_bits(d_v_host, r.D, r.dv_neg);
+  r.c0 = cb.c[0];
+  r.c1 = cb.c[1];
+  r.workspace = static_cast<float*>(workspace);
+  r.out = out;
+  r.lse = lse;
+  return launch_paged_attn(r, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

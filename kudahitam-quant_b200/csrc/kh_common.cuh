@@ -21,6 +21,7 @@ enum : uint32_t {
   kErrWaitTimeout = 1u << 0,   // an mbarrier wait gave up
   kErrBadSegment = 1u << 1,    // tile index fell outside every segment
   kErrPeerTimeout = 1u << 2,   // a peer's record flag did not arrive in time
+  kErrBadIndex = 1u << 3,      // a slot, position, length or page index out of range
 };
 
 // The error word lives in kh_api.cu; kernels receive its address.

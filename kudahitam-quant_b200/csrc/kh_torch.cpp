@@ -569,6 +569,141 @@ Tensor hbba_calibrate_cuda(const Tensor& sample, const Tensor& n_map, int64_t la
   return out;
 }
 
+// ------------------------------------------------------------ paged cache
+
+// The pools of a paged cache: planes of n_pages * heads * page_size rows.
+kh_paged_cache paged_of(const Tensor& kc, const Tensor& kr, const Tensor& kn, const Tensor& krn,
+                        const Tensor& vc, const Tensor& vr, const Tensor& vn, const Tensor& vrn,
+                        int64_t pages, int64_t heads, int64_t page_size, int64_t D,
+                        const c10::Device& dev) {
+  TORCH_CHECK(D == 128 || D == 256, "head_dim must be 128 or 256, got ", D);
+  TORCH_CHECK(pages >= 0 && heads >= 1 && heads <= 65535 && page_size >= 1 &&
+                  page_size <= 0x7fffffff,
+              "a paged cache is [pages, kv_heads >= 1, page_size >= 1, head_dim]");
+  const int64_t rows = pages * heads * page_size;
+  for (const Tensor* t : {&kc, &kr, &vc, &vr}) {
+    check_buf(*t, dev, "cache");
+    TORCH_CHECK(t->scalar_type() == at::kInt && t->numel() == rows * (D / 32),
+                "the planes of a paged cache hold ", rows, " rows of 1-bit codes (int32 words)");
+  }
+  for (const Tensor* t : {&kn, &krn, &vn, &vrn}) {
+    check_buf(*t, dev, "cache");
+    TORCH_CHECK(t->scalar_type() == at::kFloat && t->numel() == rows,
+                "the norms of a paged cache hold ", rows, " float32 values");
+  }
+  kh_paged_cache c;
+  c.k_code = u32(kc); c.k_res = u32(kr);
+  c.k_norms = kn.data_ptr<float>(); c.k_rnorms = krn.data_ptr<float>();
+  c.v_code = u32(vc); c.v_res = u32(vr);
+  c.v_norms = vn.data_ptr<float>(); c.v_rnorms = vrn.data_ptr<float>();
+  c.n_pages = pages;
+  c.page_size = (int)page_size;
+  c.n_kv_heads = (int)heads;
+  c.head_dim = (int)D;
+  return c;
+}
+
+// Index arrays of the paged calls: contiguous, of one type, on the device.
+const void* index_of(const Tensor& t, at::ScalarType s, int64_t n, const c10::Device& dev,
+                     const char* what) {
+  TORCH_CHECK(t.device() == dev && t.scalar_type() == s && t.is_contiguous() && t.numel() == n,
+              what, " must be a contiguous ", s, " tensor of ", n, " values on ", dev);
+  return t.data_ptr();
+}
+
+void paged_append(const Tensor& k, const Tensor& v, const Tensor& kc, const Tensor& kr,
+                  const Tensor& kn, const Tensor& krn, const Tensor& vc, const Tensor& vr,
+                  const Tensor& vn, const Tensor& vrn, int64_t pages, int64_t page_size,
+                  const Tensor& slots, const Tensor& dk, const Tensor& dv, const Tensor& c,
+                  const c10::optional<Tensor>& positions, const c10::optional<Tensor>& cos,
+                  const c10::optional<Tensor>& sin, bool interleaved) {
+  require_cuda(k, "k");
+  TORCH_CHECK(k.dim() == 3 && v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() &&
+                  v.device() == k.device(),
+              "k and v must be [tokens, kv_heads, head_dim] of one shape, dtype and device");
+  const int64_t T = k.size(0), H = k.size(1), D = k.size(2);
+  const auto dev = k.device();
+  const int dt = dtype_code(k.scalar_type());
+  const kh_paged_cache cache = paged_of(kc, kr, kn, krn, vc, vr, vn, vrn, pages, H, page_size, D,
+                                        dev);
+  const void* sl = index_of(slots, at::kLong, T, dev, "slots");
+  const void* ps = nullptr;
+  const float *cp = nullptr, *sp = nullptr;
+  int64_t n_pos = 0, rot = 0;
+  const bool rotate = positions && positions->defined();
+  TORCH_CHECK(rotate == (cos && cos->defined()) && rotate == (sin && sin->defined()),
+              "positions, cos and sin come together");
+  if (rotate) {
+    ps = index_of(*positions, at::kLong, T, dev, "positions");
+    TORCH_CHECK(cos->dim() == 2 && cos->sizes() == sin->sizes(), "cos and sin must be [n, rot / 2]");
+    n_pos = cos->size(0);
+    rot = 2 * cos->size(1);
+    TORCH_CHECK(n_pos >= 1 && rot >= 2 && rot <= D, "cos and sin must be [n >= 1, 1 .. head_dim / 2]");
+    for (const Tensor* t : {&*cos, &*sin})
+      TORCH_CHECK(t->device() == dev && t->scalar_type() == at::kFloat && t->is_contiguous(),
+                  "cos and sin must be contiguous float32 tensors on ", dev);
+    cp = cos->data_ptr<float>();
+    sp = sin->data_ptr<float>();
+  }
+  const Tensor kk = k.stride(2) == 1 ? k : k.contiguous();
+  const Tensor vv = v.stride(2) == 1 ? v : v.contiguous();
+  const float* ch = host_c(c);
+  const float *dkh = host_f32(dk, D, "dk"), *dvh = host_f32(dv, D, "dv");
+  c10::cuda::CUDAGuard guard(dev);
+  check(kh_paged_append(&cache, kk.data_ptr(), vv.data_ptr(), dt, T, kk.stride(0), kk.stride(1),
+                        vv.stride(0), vv.stride(1), static_cast<const int64_t*>(sl),
+                        static_cast<const int64_t*>(ps), cp, sp, n_pos, (int)rot,
+                        interleaved ? 1 : 0, dkh, dvh, ch, (int)c.numel(), stream_of(k)),
+        "kh_paged_append");
+}
+
+std::tuple<Tensor, Tensor> paged_attention(
+    const Tensor& q, const Tensor& kc, const Tensor& kr, const Tensor& kn, const Tensor& krn,
+    const Tensor& vc, const Tensor& vr, const Tensor& vn, const Tensor& vrn, int64_t pages,
+    int64_t heads, int64_t page_size, const Tensor& table, const Tensor& lengths, const Tensor& dk,
+    const Tensor& dv, const Tensor& c, double sm_scale, int64_t max_len, int64_t prefix_len,
+    const c10::optional<Tensor>& starts, int64_t window, double softcap,
+    const c10::optional<Tensor>& slopes, bool want_lse) {
+  require_cuda(q, "q");
+  TORCH_CHECK(q.dim() == 3, "q must be [sequences, query_heads, head_dim]");
+  const int64_t B = q.size(0), Hq = q.size(1), D = q.size(2);
+  const auto dev = q.device();
+  const int dt = dtype_code(q.scalar_type());
+  const kh_paged_cache cache = paged_of(kc, kr, kn, krn, vc, vr, vn, vrn, pages, heads, page_size,
+                                        D, dev);
+  TORCH_CHECK(Hq >= 1 && Hq % heads == 0, Hq, " query heads do not map onto ", heads, " KV heads");
+  TORCH_CHECK(max_len >= 0 && prefix_len >= 0 && prefix_len <= max_len && window >= 0,
+              "0 <= prefix_len <= max_len and window >= 0 expected");
+  TORCH_CHECK(table.dim() == 2 && table.size(0) == B && table.device() == dev &&
+                  table.scalar_type() == at::kInt && (table.size(1) <= 1 || table.stride(1) == 1),
+              "the block table must be int32 [sequences, blocks] on ", dev);
+  TORCH_CHECK(max_len <= table.size(1) * page_size, "max_len ", max_len, " needs more than the ",
+              table.size(1), " blocks of the table");
+  const void* ln = index_of(lengths, at::kInt, B, dev, "lengths");
+  const void* st = starts && starts->defined() ? index_of(*starts, at::kInt, B, dev, "starts") : nullptr;
+  const void* sp = slopes && slopes->defined() ? index_of(*slopes, at::kFloat, Hq, dev, "slopes") : nullptr;
+  const Tensor qq = q.contiguous();
+  const int n_q = (int)(Hq / heads);
+  const float* ch = host_c(c);
+  const float *dkh = host_f32(dk, D, "dk"), *dvh = host_f32(dv, D, "dv");
+  c10::cuda::CUDAGuard guard(dev);
+  const int64_t need = kh_paged_workspace_bytes(B, n_q, (int)heads, (int)D, max_len, prefix_len,
+                                                window);
+  TORCH_CHECK(need >= 0, "unsupported paged attention sizes");
+  Tensor ws = at::empty({std::max<int64_t>(need / 4, 4)}, q.options().dtype(at::kFloat));
+  Tensor out = at::empty({B, Hq, D}, q.options());
+  Tensor lse = at::empty({want_lse ? B : 0, Hq}, q.options().dtype(at::kFloat));
+  // rows of the table may lie apart (a slice of a wider one)
+  check(kh_paged_attn(&cache, qq.data_ptr(), dt, B, n_q, table.data_ptr<int>(),
+                      B > 1 ? table.stride(0) : table.size(1), static_cast<const int32_t*>(ln),
+                      static_cast<const int32_t*>(st), max_len, prefix_len, window, (float)softcap,
+                      static_cast<const float*>(sp), (float)sm_scale, dkh, dvh, ch, (int)c.numel(),
+                      ws.data_ptr(), need, out.data_ptr(),
+                      want_lse ? lse.data_ptr<float>() : nullptr, stream_of(q)),
+        "kh_paged_attn");
+  return {out, lse};
+}
+
 // ------------------------------------------------- reference-layout compat
 
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> ultra_fused_full_fusion(const Tensor& x,
@@ -660,6 +795,17 @@ TORCH_LIBRARY(kudahitam, m) {
   m.def("fused_asymmetric_attention(Tensor q, Tensor k_packed, Tensor signs, Tensor d_vec, "
         "Tensor k_norms, Tensor r_norms, Tensor centroids, int layer_id, int active_mask, "
         "float scale) -> Tensor");
+  m.def("paged_append(Tensor k, Tensor v, Tensor(a!) k_code, Tensor(b!) k_res, Tensor(c!) k_norms, "
+        "Tensor(d!) k_rnorms, Tensor(e!) v_code, Tensor(f!) v_res, Tensor(g!) v_norms, "
+        "Tensor(h!) v_rnorms, int pages, int page_size, Tensor slots, Tensor dk, Tensor dv, "
+        "Tensor centroids, Tensor? positions=None, Tensor? cos=None, Tensor? sin=None, "
+        "bool interleaved=False) -> ()");
+  m.def("paged_attention(Tensor q, Tensor k_code, Tensor k_res, Tensor k_norms, Tensor k_rnorms, "
+        "Tensor v_code, Tensor v_res, Tensor v_norms, Tensor v_rnorms, int pages, int kv_heads, "
+        "int page_size, Tensor block_table, Tensor lengths, Tensor dk, Tensor dv, "
+        "Tensor centroids, float sm_scale, int max_len, int prefix_len=0, Tensor? starts=None, "
+        "int window=0, float softcap=0.0, Tensor? slopes=None, bool lse=False) "
+        "-> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(kudahitam, CUDA, m) {
@@ -681,4 +827,6 @@ TORCH_LIBRARY_IMPL(kudahitam, CUDA, m) {
   m.impl("hbba_calibrate_cuda", &hbba_calibrate_cuda);
   m.impl("ultra_fused_full_fusion", &ultra_fused_full_fusion);
   m.impl("fused_asymmetric_attention", &fused_asymmetric_attention);
+  m.impl("paged_append", &paged_append);
+  m.impl("paged_attention", &paged_attention);
 }

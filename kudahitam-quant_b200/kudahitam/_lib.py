@@ -68,7 +68,20 @@ SIGNATURES = {
     "kh_decode_attn_static": (_c_i, [_vp, _c_i64, _c_i, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                      _vp, _c_i64, _vp, _vp, _vp, _c_i, _c_f, _c_i, _vp,
                                      _vp]),
+    "kh_paged_append": (_c_i, [_vp, _vp, _vp, _c_i, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _vp,
+                               _vp, _vp, _vp, _c_i64, _c_i, _c_i, _vp, _vp, _vp, _c_i, _vp]),
+    "kh_paged_workspace_bytes": (_c_i64, [_c_i64, _c_i, _c_i, _c_i, _c_i64, _c_i64, _c_i64]),
+    "kh_paged_attn": (_c_i, [_vp, _vp, _c_i, _c_i64, _c_i, _vp, _c_i64, _vp, _vp, _c_i64, _c_i64,
+                             _c_i64, _c_f, _vp, _c_f, _vp, _vp, _vp, _c_i, _vp, _c_i64, _vp, _vp,
+                             _vp]),
 }
+
+
+class PagedCache(ctypes.Structure):
+    """``kh_paged_cache``: the pools of a paged packed cache."""
+    _fields_ = [(n, _vp) for n in ("k_code", "k_res", "k_norms", "k_rnorms", "v_code", "v_res",
+                                   "v_norms", "v_rnorms")] + \
+        [("n_pages", _c_i64), ("page_size", _c_i), ("n_kv_heads", _c_i), ("head_dim", _c_i)]
 
 # Size of the library's fixed scratch array used by kh_decode_attn_static.
 DECODE_STATIC_SCRATCH_BYTES = 4 * 1024 * 1024

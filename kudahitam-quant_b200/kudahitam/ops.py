@@ -572,3 +572,110 @@ def fused_asymmetric_attention(q: torch.Tensor, k_packed: torch.Tensor, signs: t
                                             centroids, int(layer_id), int(active_mask),
                                             float(scale))
 
+
+
+# ------------------------------------------------------------- paged caches
+
+def empty_paged(pages: int, kv_heads: int, page_size: int, head_dim: int, device) -> PackedKV:
+    """Pool of one tensor (K or V) of a paged cache: a ``PackedKV`` of shape
+    (pages, kv_heads, page_size, head_dim), zero-filled."""
+    p = empty_packed((pages, kv_heads, page_size, head_dim), 1, True, device)
+    for t in (p.code, p.res, p.norms, p.rnorms):
+        t.zero_()
+    return p
+
+
+def _paged_pools(kc: PackedKV, vc: PackedKV) -> tuple:
+    if len(kc.shape) != 4 or tuple(kc.shape) != tuple(vc.shape):
+        raise ValueError("a paged cache is two PackedKVs of one shape "
+                         f"(pages, kv_heads, page_size, head_dim), got {kc.shape} and {vc.shape}")
+    if kc.bits != 1 or vc.bits != 1 or not (kc.residual and vc.residual):
+        raise ValueError("paged caches hold 1-bit codes with the residual plane (bits=1)")
+    return (kc.code, kc.res, kc.norms, kc.rnorms, vc.code, vc.res, vc.norms, vc.rnorms)
+
+
+def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: PackedKV, v_cache: PackedKV,
+                 slots: torch.Tensor, dk, dv, centroids,
+                 positions: Optional[torch.Tensor] = None, cos: Optional[torch.Tensor] = None,
+                 sin: Optional[torch.Tensor] = None, interleaved: bool = False) -> None:
+    """Compress the keys and values of new tokens into a paged cache, the keys
+    rotated to their positions on the way (one launch).
+
+    k, v [T, kv_heads, D] (fp32 / fp16 / bf16, any strides); slots int64 [T],
+    page * page_size + offset of each token's rows, -1 to store nothing;
+    slots of one call must differ.  positions int64 [T] with cos, sin float32
+    [n_positions, rot / 2]: the first rot elements of a key turn in pairs
+    (i, i + rot/2), or (2i, 2i+1) with ``interleaved``; all three or none.
+    The rotated key is compressed from 32 bits, it is not rounded to k's type.
+    A slot or position out of range stores nothing and sets bit 3 of
+    ``_lib.device_error()``."""
+    dev = _require_cuda(k, v, k_cache.norms, v_cache.norms, slots, positions, cos, sin)
+    if k.dtype not in _DTYPE_CODE:
+        raise TypeError(f"unsupported dtype {k.dtype}")
+    planes = _paged_pools(k_cache, v_cache)
+    P, H, page, D = k_cache.shape
+    if k.dim() != 3 or tuple(k.shape[1:]) != (H, D) or v.shape != k.shape or v.dtype != k.dtype:
+        raise ValueError(f"k and v must be [T, {H}, {D}] of one dtype, got {tuple(k.shape)} "
+                         f"{k.dtype} and {tuple(v.shape)} {v.dtype}")
+    if not (positions is None) == (cos is None) == (sin is None):
+        raise ValueError("positions, cos and sin come together")
+    ext().paged_append(k, v, *planes, P, page, slots, _host_f32(dk), _host_f32(dv),
+                       _host_f32(centroids), positions, cos, sin, interleaved)
+
+
+def _paged_attention(q, k_cache, v_cache, block_table, lengths, prefix_len, dk, dv, centroids,
+                     sm_scale, max_len, starts, window, softcap, slopes, return_lse):
+    dev = _require_cuda(q, k_cache.norms, v_cache.norms, block_table, lengths, starts, slopes)
+    if q.dtype not in _DTYPE_CODE:
+        raise TypeError(f"unsupported dtype {q.dtype}")
+    planes = _paged_pools(k_cache, v_cache)
+    P, H, page, D = k_cache.shape
+    if q.dim() != 3 or q.shape[-1] != D or q.shape[1] % H:
+        raise ValueError(f"q must be [sequences, multiple of {H} heads, {D}], got {tuple(q.shape)}")
+    if max_len is None:
+        max_len = block_table.shape[-1] * page
+    if softcap < 0 or window < 0:
+        raise ValueError("softcap and window must not be negative (0: none)")
+    if not 0 <= prefix_len <= max_len:
+        raise ValueError(f"prefix_len must be within [0, max_len = {max_len}]")
+    out, lse = ext().paged_attention(
+        q, *planes, P, H, page, block_table, lengths, _host_f32(dk), _host_f32(dv),
+        _host_f32(centroids), 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale),
+        int(max_len), int(prefix_len), starts, int(window), float(softcap), slopes, return_lse)
+    return (out, lse) if return_lse else out
+
+
+def paged_decode_attention(q: torch.Tensor, k_cache: PackedKV, v_cache: PackedKV,
+                           block_table: torch.Tensor, lengths: torch.Tensor, dk, dv, centroids,
+                           sm_scale: Optional[float] = None, max_len: Optional[int] = None,
+                           starts: Optional[torch.Tensor] = None, window: int = 0,
+                           softcap: float = 0.0, slopes: Optional[torch.Tensor] = None,
+                           return_lse: bool = False):
+    """Decode attention of one token per sequence over its pages:
+    softmax of cap * tanh(score * sm_scale / cap) - slope * (length - 1 - j)
+    over rows j in [max(start, length - window), length), times V_hat.
+
+    q [B, H_q, D] (fp32 / fp16 / bf16; the result has its type), query head h
+    reads KV head h // (H_q / kv_heads); block_table int32 [B, blocks];
+    lengths int32 [B], at most ``max_len`` (default: all the table holds; a
+    tighter bound makes fewer work items); starts int32 [B]; slopes float32
+    [H_q].  window, softcap 0: none.  A sequence with nothing to attend gets
+    zeros.  With ``return_lse`` also the natural logarithm of the sum of
+    exponentials, float32 [B, H_q] (-inf where nothing was attended)."""
+    return _paged_attention(q, k_cache, v_cache, block_table, lengths, 0, dk, dv, centroids,
+                            sm_scale, max_len, starts, window, softcap, slopes, return_lse)
+
+
+def paged_prefix_attention(q: torch.Tensor, k_cache: PackedKV, v_cache: PackedKV,
+                           block_table: torch.Tensor, lengths: torch.Tensor, prefix_len: int,
+                           dk, dv, centroids, sm_scale: Optional[float] = None,
+                           max_len: Optional[int] = None, starts: Optional[torch.Tensor] = None,
+                           window: int = 0, softcap: float = 0.0,
+                           slopes: Optional[torch.Tensor] = None, return_lse: bool = False):
+    """``paged_decode_attention`` for a batch whose sequences begin with the
+    same ``prefix_len`` cached rows: those are read once for all sequences,
+    through sequence 0's row of the block table; rows from prefix_len on are
+    each sequence's own.  ``lengths`` count the prefix."""
+    return _paged_attention(q, k_cache, v_cache, block_table, lengths, int(prefix_len), dk, dv,
+                            centroids, sm_scale, max_len, starts, window, softcap, slopes,
+                            return_lse)
