@@ -59,6 +59,10 @@ def _check_rows(pool, slots, want):
     (128, BF, 2500, 8, 64, 128, False),
     (128, HF, 2501, 7, 64, 96, True),
     (256, BF, 1203, 8, 64, 128, False),
+    (128, FL, 1501, 3, 64, 128, False),
+    (256, FL, 1100, 4, 64, 64, True),
+    (256, HF, 1302, 4, 48, 256, False),
+    (128, BF, 4100, 1, 64, 34, False),
 ])
 def test_append_is_the_64_bit_encoding(D, dtype, T, H, page, rot, inter):
     g = torch.Generator().manual_seed(T + D)
@@ -132,6 +136,26 @@ def test_append_extreme_values_and_ties():
     wk, wv = _want_append(k, k, dk, dv, c)
     _check_rows(kc, slots, wk)
     _check_rows(vc, slots, wv)
+
+
+@pytest.mark.parametrize("T", [20, 2100])
+def test_append_with_uneven_levels(T):
+    """Two levels that are not -c, c, and tokens without a slot among many."""
+    D, H = 128, 2
+    dk, dv = rademacher(D, 5), rademacher(D, 6)
+    c = torch.tensor([-0.05, 0.09])
+    g = torch.Generator().manual_seed(T)
+    k = torch.randn(T, H, D, generator=g).to(BF)
+    kc, vc = (ops.empty_paged(T // 16 + 1, H, 16, D, "cuda") for _ in range(2))
+    slots = torch.arange(T)
+    slots[3::5] = -1
+    for cb in (c, lloyd_max(1, D)):
+        ops.paged_append(k.cuda(), k.cuda(), kc, vc, slots.cuda(), dk, dv, cb)
+        on = slots >= 0
+        wk, wv = _want_append(k[on], k[on], dk, dv, cb)
+        _check_rows(kc, slots[on], wk)
+        _check_rows(vc, slots[on], wv)
+        assert int((kc.norms > 0).sum()) == int(on.sum()) * H
 
 
 def test_append_matches_compress_away_from_borders():
