@@ -140,15 +140,14 @@ struct Place {
   int64_t row;
   const float *cs, *sn;
 };
-__device__ __forceinline__ Place place_of(const AppendParams& P, int64_t t, int h, bool is_v,
-                                          bool report) {
+__device__ __forceinline__ Place place_of(const AppendParams& P, int64_t t, int h, bool report) {
   const PagedAppendRequest& r = P.r;
   Place p{-1, nullptr, nullptr};
   const int64_t slot = r.slots[t];
   if (slot == -1) return p;  // a padding token
-  const int64_t pos = !is_v && r.positions ? r.positions[t] : 0;
+  const int64_t pos = r.positions ? r.positions[t] : 0;
   if (slot < 0 || slot >= r.n_pages * r.page_size ||
-      (!is_v && r.positions && (pos < 0 || pos >= r.n_positions))) {
+      (r.positions && (pos < 0 || pos >= r.n_positions))) {
     if (report) flag_error(P.err, kErrBadIndex);
     return p;
   }
@@ -174,7 +173,7 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const __grid_constant
   const int hv = (int)(item - t * 2 * r.n_kv_heads);
   const bool is_v = hv >= r.n_kv_heads;
   const int h = is_v ? hv - r.n_kv_heads : hv;
-  const Place at = place_of(P, t, h, is_v, lane == 0);
+  const Place at = place_of(P, t, h, lane == 0);
   if (at.row < 0) return;
   const T* src = is_v ? static_cast<const T*>(r.v) + t * r.v_stride_t + h * r.v_stride_h
                       : static_cast<const T*>(r.k) + t * r.k_stride_t + h * r.k_stride_h;
@@ -225,30 +224,52 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const __grid_constant
 
 // ------------------------------------------------------------------ tiles
 //
-// Many rows: a lane owns a row (D = 128) or half of one (D = 256, the first
-// butterfly stage done while loading), so the transform stays in registers
-// on packed adds and no value is exchanged.  A warp's tile is 4096 elements:
-// 32 or 16 rows in (token, head) order, so that a token's angles serve its
-// heads from L1.  Rows come by cp.async, 16 bytes a lane, into a private
-// double buffer whose rows are 16 bytes longer than they need to be: the
-// lanes' 16-byte reads, one row each, then hit different banks.
-// 16-bit rows of D = 128 cost about 50 instructions a row against 296 bytes:
-// bound by issue, not by HBM.
+// Many rows: a lane owns 64 elements of a row, so that six stages of the
+// transform stay in registers on packed adds and only the last one (two at
+// D = 256) crosses lanes, while 16 warps fit an SM (20, with 96 registers, spilled and measured 82 us where 16 measure 74).  A warp's tile is 2048
+// elements, 32 "slots" of 64: 16 or 8 rows in (token, head) order, so that a
+// token's angles serve its heads from L1.  Slots come by cp.async, 16 bytes
+// a lane, into a private double buffer; each is 16 bytes longer than it
+// needs to be, so that the lanes' 16-byte reads hit different banks.
 constexpr int kTileWarps = 4;
+constexpr int kTileCtas = 4;
 constexpr int64_t kTileRows = 8192;
 
-template <typename T, int D>
+template <typename T>
 struct TileCfg {
-  static constexpr int kRows = 4096 / D;                // rows of a tile
-  static constexpr int kBytes = D * (int)sizeof(T);     // of a row
-  static constexpr int kPitch = kBytes + 16;
-  static constexpr int kStage = kRows * kPitch;
-  static constexpr int kSmem = kTileWarps * 2 * kStage;
+  static constexpr int N = 16 / (int)sizeof(T);           // elements of a 16-byte piece
+  static constexpr int kPieces = 64 / N;                  // of a slot
+  static constexpr int kSlot = 64 * (int)sizeof(T) + 16;  // bytes, with the pad
+  static constexpr int kStage = 32 * kSlot;
+  static constexpr int kFlips = 3 * 4 * kSlot;            // sign bits: see the kernel
+  static constexpr int kSmem = kFlips + kTileWarps * 2 * kStage;
+};
+
+// j / n for j < 2^31 by a multiplication: mul = ceil(2^shift / n) with
+// shift = 31 + ceil(log2 n), so that the error j (mul n - 2^shift) / (n 2^shift)
+// stays under 1 / n.
+struct FastDiv {
+  uint64_t mul;
+  int shift;
+  __device__ __forceinline__ uint32_t operator()(uint32_t j) const {
+    return (uint32_t)((j * mul) >> shift);
+  }
+};
+FastDiv fast_div(uint32_t n) {
+  int bits = 0;
+  while ((uint64_t(1) << bits) < n) ++bits;
+  return FastDiv{((uint64_t(1) << (31 + bits)) + n - 1) / n, 31 + bits};
+}
+
+struct TileParams {
+  AppendParams a;
+  FastDiv by_heads, by_page;
+  int contiguous;  // k's and v's rows follow one another
 };
 
 template <typename T>
-__device__ __forceinline__ void widen(const uint4& v, float (&f)[16 / sizeof(T)]) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+__device__ __forceinline__ void widen(const uint4& v, const uint4& flip, float (&f)[16 / sizeof(T)]) {
+  const uint32_t w[4] = {v.x ^ flip.x, v.y ^ flip.y, v.z ^ flip.z, v.w ^ flip.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if constexpr (std::is_same<T, float>::value) {
@@ -266,162 +287,191 @@ __device__ __forceinline__ void widen(const uint4& v, float (&f)[16 / sizeof(T)]
   }
 }
 
-// 16-byte piece c of a staged row, rotated: ROT 0 not at all, 1 in pairs
-// (i, i + rot / 2) (rot / 2 a multiple of a piece), 2 in pairs (2 i, 2 i + 1).
-template <typename T, int ROT>
-__device__ __forceinline__ void piece(const uint8_t* row, int c, int rot, const float* cs,
-                                      const float* sn, float (&f)[16 / sizeof(T)]) {
-  constexpr int N = 16 / sizeof(T);
-  widen<T>(*reinterpret_cast<const uint4*>(row + 16 * c), f);
-  if constexpr (ROT == 1) {
-    if (c * N < rot) {
-      const int half = rot / (2 * N);  // pieces
-      const bool second = c >= half;
-      const int i = (second ? c - half : c) * N;
-      float z[N];
-      widen<T>(*reinterpret_cast<const uint4*>(row + 16 * (second ? c - half : c + half)), z);
+// How the keys of a launch turn.
+enum Turn { kNone, kWhole, kPairs, kPart };  // kWhole: (i, i + D / 2); kPart: rot < D
+
+// x = slot p of the row whose slots begin at `row`, d applied, rotated.
+template <typename T, int D, int TURN>
+__device__ __forceinline__ void load_slot(const uint8_t* row, const uint8_t* flips, int p, int rot,
+                                          bool pairs, const float* cs, const float* sn,
+                                          float (&x)[64]) {
+  using C = TileCfg<T>;
+  constexpr int N = C::N, S = D / 64;
 #pragma unroll
-      for (int k = 0; k < N; k += 4) {
-        const float4 co = __ldg(reinterpret_cast<const float4*>(cs + i + k));
-        const float4 si = __ldg(reinterpret_cast<const float4*>(sn + i + k));
-        const float cc[4] = {co.x, co.y, co.z, co.w}, ss[4] = {si.x, si.y, si.z, si.w};
+  for (int c = 0; c < C::kPieces; ++c) {
+    const uint4 fl = *reinterpret_cast<const uint4*>(flips + p * C::kSlot + 16 * c);
+    const uint4 raw = *reinterpret_cast<const uint4*>(row + p * C::kSlot + 16 * c);
+    float f[N];
+    widen<T>(raw, fl, f);
+    const int e = 64 * p + N * c;
+    if (TURN == kPairs || (TURN == kPart && pairs)) {
+      if (TURN == kPairs || e < rot) {
+        // the pair's elements have signs of their own: turn them bare
+        float z[N];
+        widen<T>(raw, make_uint4(0, 0, 0, 0), z);
+        constexpr uint32_t kBit = sizeof(T) == 4 ? 0x80000000u : 0x8000u;
+        const uint32_t fw[4] = {fl.x, fl.y, fl.z, fl.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float p = z[k + e] * ss[e];
-          f[k + e] = fmaf(f[k + e], cc[e], second ? p : -p);
+        for (int k = 0; k < N; k += 2) {
+          const float co = __ldg(cs + (e + k) / 2), si = __ldg(sn + (e + k) / 2);
+          const float a = fmaf(z[k], co, -(z[k + 1] * si)), b = fmaf(z[k + 1], co, z[k] * si);
+          const bool na = sizeof(T) == 4 ? fw[k & 3] & kBit : fw[k / 2] & kBit;
+          const bool nb = sizeof(T) == 4 ? fw[(k + 1) & 3] & kBit : fw[k / 2] & (kBit << 16);
+          f[k] = na ? -a : a;
+          f[k + 1] = nb ? -b : b;
+        }
+      }
+    } else if (TURN == kWhole || TURN == kPart) {
+      if (TURN == kWhole || e < rot) {
+        const int half = TURN == kWhole ? D / 2 : rot >> 1;
+        const bool second = TURN == kWhole ? p >= S / 2 : e >= half;
+        const int o = second ? e - half : e + half, i = second ? o : e;
+        float z[N];
+        widen<T>(*reinterpret_cast<const uint4*>(row + (o >> 6) * C::kSlot +
+                                                 (o & 63) * (int)sizeof(T)),
+                 *reinterpret_cast<const uint4*>(flips + (8 + p) * C::kSlot + 16 * c), z);
+#pragma unroll
+        for (int k = 0; k < N; k += 4) {
+          const float4 co = __ldg(reinterpret_cast<const float4*>(cs + i + k));
+          const float4 si = __ldg(reinterpret_cast<const float4*>(sn + i + k));
+          const float cc[4] = {co.x, co.y, co.z, co.w}, ss[4] = {si.x, si.y, si.z, si.w};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) f[k + q] = fmaf(f[k + q], cc[q], z[k + q] * ss[q]);
         }
       }
     }
-  } else if constexpr (ROT == 2) {
-    if (c * N < rot) {
 #pragma unroll
-      for (int k = 0; k < N; k += 2) {
-        const float co = __ldg(cs + (c * N + k) / 2), si = __ldg(sn + (c * N + k) / 2);
-        const float a = f[k], b = f[k + 1];
-        f[k] = fmaf(a, co, -(b * si));
-        f[k + 1] = fmaf(b, co, a * si);
-      }
-    }
+    for (int k = 0; k < N; ++k) x[c * N + k] = f[k];
   }
 }
 
-// x[e] = this lane's 128 values of d . row: all of it at D = 128; at D = 256
-// lo + hi (lanes 0 .. 15) or lo - hi, the first stage of the transform.
-template <typename T, int D, int ROT>
-__device__ __forceinline__ void load_row(const uint8_t* row, int rot, const float* cs,
-                                         const float* sn, const uint32_t* flip, float sign,
-                                         float (&x)[128]) {
-  constexpr int N = 16 / sizeof(T);
-#pragma unroll
-  for (int c = 0; c < 128 / N; ++c) {
-    float f[N];
-    piece<T, ROT>(row, c, rot, cs, sn, f);
-    if constexpr (D == 128) {
-#pragma unroll
-      for (int k = 0; k < N; ++k)
-        x[c * N + k] = __uint_as_float(__float_as_uint(f[k]) ^ flip[c * N + k]);
-    } else {
-      float z[N];
-      piece<T, ROT>(row, c + 128 / N, rot, cs, sn, z);
-#pragma unroll
-      for (int k = 0; k < N; ++k) {
-        const float a = __uint_as_float(__float_as_uint(f[k]) ^ flip[c * N + k]);
-        const float b = __uint_as_float(__float_as_uint(z[k]) ^ flip[128 + c * N + k]);
-        x[c * N + k] = fmaf(b, sign, a);
-      }
-    }
-  }
-}
-
-struct TileParams {
-  AppendParams a;
-  uint32_t dk_flip[256], dv_flip[256];  // sign bit where d is -1
-};
-
-template <typename T, int D>
-__global__ void __launch_bounds__(32 * kTileWarps, 3)
+template <typename T, int D, int TURN>
+__global__ void __launch_bounds__(32 * kTileWarps, kTileCtas)
     paged_append_tiles_kernel(const __grid_constant__ TileParams P) {
-  using C = TileCfg<T, D>;
+  using C = TileCfg<T>;
   constexpr int J = D / 32;
+  constexpr int S = D / 64;        // slots of a row
+  constexpr int kRows = 32 / S;    // rows of a tile
   const PagedAppendRequest& r = P.a.r;
   extern __shared__ __align__(16) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint8_t* buf = smem + warp * 2 * C::kStage;
-  const int64_t rows = r.n_tokens * r.n_kv_heads;
-  const int64_t tiles = (rows + C::kRows - 1) / C::kRows * 2;  // keys and values in turn
-  const int64_t step = (int64_t)gridDim.x * kTileWarps;
+  uint8_t* buf = smem + C::kFlips + warp * 2 * C::kStage;
+  // sign bits in the slots' layout: d of keys, d of values, and d of keys
+  // times the sign of the pair's other element in the rotation
+  for (int k = threadIdx.x; k < 3 * D; k += 32 * kTileWarps) {
+    const int e = k % D, which = k / D;
+    const uint32_t* neg = which == 1 ? r.dv_neg : r.dk_neg;
+    const uint32_t bit = ((neg[e >> 5] >> (e & 31)) & 1) ^ (which == 2 && e < (r.rot_dim >> 1));
+    uint8_t* at = smem + (which * 4 + e / 64) * C::kSlot + (e & 63) * sizeof(T);
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<uint32_t*>(at) = bit << 31;
+    else *reinterpret_cast<uint16_t*>(at) = (uint16_t)(bit << 15);
+  }
+  __syncthreads();
+  const uint32_t rows = (uint32_t)(r.n_tokens * r.n_kv_heads);
+  const uint32_t tiles = (rows + kRows - 1) / kRows;
+  const uint32_t step = gridDim.x * kTileWarps;
   grid_dependency_wait();
-  // row i of the call as the source of its first element
-  auto source = [&](int64_t i, bool is_v) {
-    const int64_t t = i / r.n_kv_heads;
-    const int h = (int)(i - t * r.n_kv_heads);
+  // first element of row i
+  auto source = [&](uint32_t i, bool is_v) {
+    const uint32_t t = P.by_heads(i), h = i - t * r.n_kv_heads;
     return is_v ? static_cast<const T*>(r.v) + t * r.v_stride_t + h * r.v_stride_h
                 : static_cast<const T*>(r.k) + t * r.k_stride_t + h * r.k_stride_h;
   };
-  auto issue = [&](int64_t tile, int stage) {
+  auto issue = [&](uint32_t tile, int is_v) {
+    const int stage = is_v;
     if (tile < tiles) {
-      constexpr int kPieces = C::kBytes / 16;  // of a row: a power of two
-      const int64_t r0 = (tile >> 1) * C::kRows;
-      uint8_t* st = buf + stage * C::kStage;
-#pragma unroll 4
-      for (int k = lane; k < C::kRows * kPieces; k += 32) {
-        const int64_t i = r0 + k / kPieces;
-        if (i < rows) {
-          const uint8_t* src = reinterpret_cast<const uint8_t*>(source(i, tile & 1));
+      const uint32_t r0 = tile * kRows;
+      const uint32_t left = rows - r0;  // rows of the tile, or more
+      const uint32_t dst = smem_u32(buf + stage * C::kStage) + (lane / C::kPieces) * C::kSlot +
+                           (lane % C::kPieces) * 16;
+      const T* base = static_cast<const T*>(is_v ? r.v : r.k) + (int64_t)r0 * D + lane * C::N;
+#pragma unroll
+      for (int m = 0; m < C::kPieces; ++m) {
+        const uint32_t k = lane + 32 * m, slot = k / C::kPieces;
+        if (slot / S < left) {
+          const T* src = P.contiguous ? base + 32 * m * C::N
+                                      : source(r0 + slot / S, is_v) + (slot % S) * 64 +
+                                            (k % C::kPieces) * C::N;
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                           smem_u32(st + (k / kPieces) * C::kPitch + (k % kPieces) * 16)),
-                       "l"(src + (k % kPieces) * 16)
+                           dst + m * (32 / C::kPieces) * C::kSlot),
+                       "l"(src)
                        : "memory");
         }
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  const int64_t first = (int64_t)blockIdx.x * kTileWarps + warp;
+  const uint32_t first = blockIdx.x * kTileWarps + warp;
+  const int p = lane % S, rl = lane / S;
   issue(first, 0);
-  int stage = 0;
+  issue(first, 1);
+  // a tile's keys, then its values: both go to the same slots, and no warp is
+  // left with keys alone, which cost more
+  int64_t row = -1, angle = 0;
 #pragma unroll 1
-  for (int64_t tile = first; tile < tiles; tile += step, stage ^= 1) {
-    issue(tile + step, stage ^ 1);
-    const bool is_v = tile & 1;
-    const int rl = D == 128 ? lane : lane & 15;
-    const int64_t i = (tile >> 1) * C::kRows + rl;
-    Place at{-1, nullptr, nullptr};
-    if (i < rows) {
-      const int64_t t = i / r.n_kv_heads;
-      at = place_of(P.a, t, (int)(i - t * r.n_kv_heads), is_v, true);
+  for (uint32_t tile = first, is_v = 0; tile < tiles; tile += is_v ? step : 0, is_v ^= 1) {
+    const uint32_t i = tile * kRows + rl;
+    if (!is_v) {
+      // a lane without a row goes along on stale values
+      row = -1;
+      angle = 0;
+      if (i < rows) {
+        const uint32_t t = P.by_heads(i), h = i - t * r.n_kv_heads;
+        const int64_t slot = r.slots[t];
+        bool ok = slot >= 0 && slot < r.n_pages * r.page_size;
+        bool bad = !ok && slot != -1;
+        if (TURN != kNone && slot != -1) {
+          const int64_t pos = r.positions[t];
+          const bool in = pos >= 0 && pos < r.n_positions;
+          bad |= !in;
+          ok = ok && in;
+          angle = in ? pos * (r.rot_dim >> 1) : 0;
+        }
+        if (bad) flag_error(P.a.err, kErrBadIndex);
+        if (ok) {
+          const uint32_t page = P.by_page((uint32_t)slot);
+          row = ((int64_t)page * r.n_kv_heads + h) * r.page_size +
+                ((uint32_t)slot - page * r.page_size);
+        }
+      }
     }
-    const bool on = at.row >= 0;
     asm volatile("cp.async.wait_group 1;" ::: "memory");
     __syncwarp();
-    const uint8_t* row = buf + stage * C::kStage + (on ? rl : 0) * C::kPitch;
-    const float sign = lane < 16 ? 1.f : -1.f;
-    float x[128];
-    // a lane without a row goes along on another's (or on stale) values
-    const int rot = is_v || !on ? 0 : r.rot_dim;
-    if (is_v || !r.rot_dim) load_row<T, D, 0>(row, 0, nullptr, nullptr, is_v ? P.dv_flip : P.dk_flip, sign, x);
-    else if (r.interleaved) load_row<T, D, 2>(row, rot, at.cs, at.sn, P.dk_flip, sign, x);
-    else load_row<T, D, 1>(row, rot, at.cs, at.sn, P.dk_flip, sign, x);
+    const uint8_t* src = buf + is_v * C::kStage + rl * S * C::kSlot;
+    float x[64];
+    if (TURN == kNone || is_v)
+      load_slot<T, D, kNone>(src, smem + (is_v ? 4 * C::kSlot : 0), p, 0, false, nullptr, nullptr, x);
+    else
+      load_slot<T, D, TURN>(src, smem, p, r.rot_dim, r.interleaved, r.cos + angle, r.sin + angle, x);
+    __syncwarp();
+    issue(tile + step, is_v);  // the slots are in registers: the buffer takes the next tile's
     float2 s2 = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int e = 0; e < 128; e += 2) {
-      const float2 p = make_float2(x[e], x[e + 1]);
-      s2 = __ffma2_rn(p, p, s2);
+    for (int e = 0; e < 64; e += 2) {
+      const float2 v = make_float2(x[e], x[e + 1]);
+      s2 = __ffma2_rn(v, v, s2);
     }
     float ss = s2.x + s2.y;
-    if (D == 256) ss = 0.5f * (ss + __shfl_xor_sync(0xffffffffu, ss, 16));
+#pragma unroll
+    for (int o = 1; o < S; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     const float norm = sqrtf(ss);
     const float inv = 1.f / norm;
-    fwht_regs<128>(x);
+    fwht_regs<64>(x);
+#pragma unroll
+    for (int o = 1; o < S; o <<= 1) {
+      const float sg = p & o ? -1.f : 1.f;
+#pragma unroll
+      for (int e = 0; e < 64; ++e) x[e] = fmaf(x[e], sg, __shfl_xor_sync(0xffffffffu, x[e], o));
+    }
     // code bit = [u > 0] (an exact 0 lies inside the band); residual bit =
     // code bit xor [|y| < c1]
-    uint32_t cw[4] = {0, 0, 0, 0}, tw[4] = {0, 0, 0, 0};
+    uint32_t cw[2] = {0, 0}, tw[2] = {0, 0};
     float mu = INFINITY, mt = INFINITY;
     float2 v2 = make_float2(0.f, 0.f);
 #pragma unroll
     for (int k = 30; k >= 0; k -= 2)
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
+      for (int w = 0; w < 2; ++w) {
         const float u0 = x[32 * w + k], u1 = x[32 * w + k + 1];
         const float t0 = fmaf(fabsf(u0), inv, -P.a.c1), t1 = fmaf(fabsf(u1), inv, -P.a.c1);
         cw[w] = push_sign(push_sign(cw[w], u1), u0);
@@ -432,39 +482,36 @@ __global__ void __launch_bounds__(32 * kTileWarps, 3)
         v2 = __ffma2_rn(tt, tt, v2);
       }
     float vv = v2.x + v2.y;
+#pragma unroll
+    for (int o = 1; o < S; o <<= 1) vv += __shfl_xor_sync(0xffffffffu, vv, o);
     bool near = !(ss > kMinSquares && ss < kMaxSquares) || mu * inv < P.a.band || mt < P.a.band;
-    if (D == 256) {
-      vv += __shfl_xor_sync(0xffffffffu, vv, 16);
-      near |= __shfl_xor_sync(0xffffffffu, (int)near, 16) != 0;
+    near = near && row >= 0;
+    uint32_t todo = __ballot_sync(0xffffffffu, near);
+    // a row is near a border when one of its lanes is
+#pragma unroll
+    for (int o = 1; o < S; o <<= 1) {
+      constexpr uint32_t kLow[3] = {0, 0x55555555u, 0x33333333u};
+      todo |= ((todo & kLow[o]) << o) | ((todo >> o) & kLow[o]);
     }
-    near = near && on;
     const PagedPool& pool = is_v ? r.vp : r.kp;
-    if (on && !near) {
-      const int64_t o = D == 128 ? at.row * 4 : at.row * 8 + (lane >> 4) * 4;
-      const uint4 c = make_uint4(~cw[0], ~cw[1], ~cw[2], ~cw[3]);
-      *reinterpret_cast<uint4*>(pool.code + o) = c;
-      *reinterpret_cast<uint4*>(pool.res + o) =
-          make_uint4(c.x ^ tw[0], c.y ^ tw[1], c.z ^ tw[2], c.w ^ tw[3]);
-      if (D == 128 || lane < 16) {
+    if (row >= 0 && !(todo >> lane & 1)) {
+      const uint2 c = make_uint2(~cw[0], ~cw[1]);
+      *reinterpret_cast<uint2*>(pool.code + row * J + 2 * p) = c;
+      *reinterpret_cast<uint2*>(pool.res + row * J + 2 * p) = make_uint2(c.x ^ tw[0], c.y ^ tw[1]);
+      if (p == 0) {
         const float rn = norm * sqrtf(vv * (1.f / D));
-        pool.norms[at.row] = norm;
-        pool.rnorms[at.row] = rn == 0.f ? 1e-8f : rn;
+        pool.norms[row] = norm;
+        pool.rnorms[row] = rn == 0.f ? 1e-8f : rn;
       }
     }
-    uint32_t todo = __ballot_sync(0xffffffffu, near);
-    if (D == 256) todo &= 0xffffu;
 #pragma unroll 1
     while (todo) {
       const int l = __ffs(todo) - 1;
-      todo &= todo - 1;
-      const int64_t ti = (tile >> 1) * C::kRows + l;
-      const int64_t ro = __shfl_sync(0xffffffffu, at.row, l);
-      const float* cs = reinterpret_cast<const float*>(
-          __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(at.cs), l));
-      const float* sn = reinterpret_cast<const float*>(
-          __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(at.sn), l));
-      const Coded o = encode_row_64<T, J>(P.a, source(ti, is_v), is_v, is_v ? 0 : r.rot_dim, cs,
-                                          sn, lane);
+      todo &= ~(((1u << S) - 1) << l);
+      const int64_t ro = __shfl_sync(0xffffffffu, row, l);
+      const int64_t an = __shfl_sync(0xffffffffu, angle, l);
+      const Coded o = encode_row_64<T, J>(P.a, source(tile * kRows + l / S, is_v), is_v,
+                                          is_v ? 0 : r.rot_dim, r.cos + an, r.sin + an, lane);
       if (lane < J) {
         pool.code[ro * J + lane] = o.code;
         pool.res[ro * J + lane] = o.res;
@@ -474,7 +521,6 @@ __global__ void __launch_bounds__(32 * kTileWarps, 3)
         pool.rnorms[ro] = o.rnorm == 0.f ? 1e-8f : o.rnorm;
       }
     }
-    __syncwarp();
   }
   grid_dependents_launch();
 }
@@ -490,24 +536,27 @@ kh_status launch_rows(const AppendParams& P, cudaStream_t stream) {
   return cudaGetLastError() == cudaSuccess ? KH_OK : KH_ELAUNCH;
 }
 
-template <typename T, int D>
+template <typename T, int D, int TURN>
 kh_status launch_tiles(const AppendParams& A, cudaStream_t stream) {
-  using C = TileCfg<T, D>;
-  auto kern = paged_append_tiles_kernel<T, D>;
+  using C = TileCfg<T>;
+  auto kern = paged_append_tiles_kernel<T, D, TURN>;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return KH_ECUDA;
   static std::once_flag once[64];
   std::call_once(once[dev & 63], [&] {
     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   });
+  const PagedAppendRequest& r = A.r;
   TileParams P;
   P.a = A;
-  for (int e = 0; e < 256; ++e) {
-    P.dk_flip[e] = (A.r.dk_neg[e >> 5] >> (e & 31) & 1) << 31;
-    P.dv_flip[e] = (A.r.dv_neg[e >> 5] >> (e & 31) & 1) << 31;
-  }
-  const int64_t tiles = (A.r.n_tokens * A.r.n_kv_heads + C::kRows - 1) / C::kRows * 2;
-  const int64_t blocks = std::min<int64_t>((tiles + kTileWarps - 1) / kTileWarps, 3 * sm_count());
+  P.by_heads = fast_div(r.n_kv_heads);
+  P.by_page = fast_div(r.page_size);
+  P.contiguous = r.k_stride_h == D && r.v_stride_h == D && r.k_stride_t == D * (int64_t)r.n_kv_heads &&
+                 r.v_stride_t == r.k_stride_t;
+  const int64_t rows = 32 * 64 / D;
+  const int64_t tiles = (r.n_tokens * r.n_kv_heads + rows - 1) / rows;
+  const int64_t blocks = std::min<int64_t>((tiles + kTileWarps - 1) / kTileWarps,
+                                           (sizeof(T) == 4 ? 3 : kTileCtas) * sm_count());
   if (launch_programmatic(kern, dim3((unsigned)blocks), dim3(32 * kTileWarps), C::kSmem, stream,
                           P) != cudaSuccess)
     return KH_ELAUNCH;
@@ -515,23 +564,30 @@ kh_status launch_tiles(const AppendParams& A, cudaStream_t stream) {
 }
 
 // The tiled kernel needs 16-byte pieces of rows and angles, rotation pairs
-// that fall on whole pieces, and levels -c, c.
+// that fall on whole pieces, levels -c, c, and 31-bit row and slot numbers.
 template <typename T, int D>
 bool tiles_fit(const PagedAppendRequest& r) {
   const auto on16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
   const int64_t n = 16 / sizeof(T);
   if (r.c0 != -r.c1 || !on16(r.k) || !on16(r.v)) return false;
   if (r.k_stride_t % n || r.k_stride_h % n || r.v_stride_t % n || r.v_stride_h % n) return false;
+  if (r.n_tokens * r.n_kv_heads >= (int64_t(1) << 30) ||
+      r.n_pages * r.page_size >= (int64_t(1) << 31))
+    return false;
   if (r.rot_dim && !r.interleaved)
     return r.rot_dim % (2 * n) == 0 && r.rot_dim % 8 == 0 && on16(r.cos) && on16(r.sin);
-  return r.rot_dim == 0 || r.rot_dim % n == 0;
+  return r.rot_dim % n == 0;
 }
 
 template <typename T, int D>
 kh_status launch_typed(const AppendParams& P, cudaStream_t stream) {
-  const int64_t rows = P.r.n_tokens * P.r.n_kv_heads * 2;
-  return rows >= kTileRows && tiles_fit<T, D>(P.r) ? launch_tiles<T, D>(P, stream)
-                                                   : launch_rows<T, D>(P, stream);
+  const PagedAppendRequest& r = P.r;
+  if (r.n_tokens * r.n_kv_heads * 2 < kTileRows || !tiles_fit<T, D>(r))
+    return launch_rows<T, D>(P, stream);
+  if (!r.rot_dim) return launch_tiles<T, D, kNone>(P, stream);
+  if (r.rot_dim < D) return launch_tiles<T, D, kPart>(P, stream);
+  return r.interleaved ? launch_tiles<T, D, kPairs>(P, stream)
+                       : launch_tiles<T, D, kWhole>(P, stream);
 }
 
 template <typename T>
