@@ -19,96 +19,10 @@
 #include <mutex>
 
 #include "kh_common.cuh"
-#include "kh_paged.h"
+#include "kh_paged_attn.cuh"
 
 namespace kh {
 namespace {
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
-
-struct AttnParams {
-  PagedAttnRequest r;
-  PagedPlan plan;
-  float log_scale, inv_sd;  // sm_scale log2(e) / sqrt(D); 1 / sqrt(D)
-  // j / page_size for j < 2^31: (j * mul) >> shift, mul = ceil(2^shift / page_size),
-  // shift = 31 + ceil(log2 page_size) (the error j (mul page_size - 2^shift) / 2^shift stays under 1)
-  uint64_t div_mul;
-  int div_shift;
-  uint32_t* err;
-
-  __device__ __forceinline__ uint32_t page_div(uint32_t j) const {
-    return (uint32_t)((j * div_mul) >> div_shift);
-  }
-};
-
-__device__ __forceinline__ float ld_any(const void* p, int dtype, int64_t i) {
-  if (dtype == KH_F32) return static_cast<const float*>(p)[i];
-  if (dtype == KH_F16) return __half2float(static_cast<const __half*>(p)[i]);
-  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-}
-__device__ __forceinline__ void st_any(void* p, int dtype, int64_t i, float v) {
-  if (dtype == KH_F32) static_cast<float*>(p)[i] = v;
-  else if (dtype == KH_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
-  else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
-}
-
-// Length of sequence b, within what the table and max_len hold.
-__device__ __forceinline__ int64_t length_of(const AttnParams& P, int64_t b) {
-  int64_t n = P.r.lengths[b];
-  if (n < 0 || n > P.r.max_len) {
-    flag_error(P.err, kErrBadIndex);
-    n = n < 0 ? 0 : P.r.max_len;
-  }
-  return n;
-}
-// First attended row of sequence b.
-__device__ __forceinline__ int64_t first_of(const AttnParams& P, int64_t b, int64_t len) {
-  int64_t lo = P.r.starts ? max((int64_t)P.r.starts[b], (int64_t)0) : 0;
-  if (P.r.window > 0) lo = max(lo, len - P.r.window);
-  return lo;
-}
-// Where a sequence's own rows begin.
-__device__ __forceinline__ int64_t own_first(const AttnParams& P, int64_t b, int64_t len) {
-  return max(first_of(P, b, len), P.r.prefix_len);
-}
-// cap tanh(t / cap): 1 - 2 / (e^2x + 1) loses what is left of small x, so
-// below 0.3 the odd series (its next term is under 2^-33 of x there).
-__device__ __forceinline__ float soft_cap(float t, float cap, float inv_cap) {
-  const float x = t * inv_cap, a = fabsf(x);
-  const float big = copysignf(1.f - 2.f / (__expf(2.f * fminf(a, 20.f)) + 1.f), x);
-  const float z = x * x;
-  float s = fmaf(z, 0.0035921280f, -0.0088632355f);
-  s = fmaf(z, s, 0.021869488f);
-  s = fmaf(z, s, -0.053968254f);
-  s = fmaf(z, s, 0.13333333f);
-  s = fmaf(z, s, -0.33333333f);
-  const float small = fmaf(x * z, s, x);
-  return cap * (a < 0.3f ? small : big);
-}
-
-// Walsh-Hadamard sums of a warp's row: element 32 j + lane in x[j].
-template <int J>
-__device__ __forceinline__ void fwht_lanes(float (&x)[J], int lane) {
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const bool up = lane & o;
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const float y = __shfl_xor_sync(0xffffffffu, x[j], o);
-      x[j] = up ? y - x[j] : x[j] + y;
-    }
-  }
-#pragma unroll
-  for (int h = 1; h < J; h <<= 1)
-#pragma unroll
-    for (int j = 0; j < J; ++j)
-      if (!(j & h)) {
-        const float a = x[j], b = x[j + h];
-        x[j] = a + b;
-        x[j + h] = a - b;
-      }
-}
 
 // ------------------------------------------------------------------ rows
 //
@@ -166,22 +80,6 @@ template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float lg2(float x) {
-  float y;
-  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ float round_h(float x) { return __half2float(__float2half_rn(x)); }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -196,8 +94,6 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
 }
 
 constexpr float kPart = 2048.f;      // second fp16 parts are stored times 2^11
-constexpr float kNoRef = -1e30f;     // reference exponent before the first row
-constexpr float kMaxWeight = 4096.f;
 
 template <int D, bool HILO, bool EXACT, int NB>
 __global__ void __launch_bounds__(32 * kWarps, D == 128 ? (NB == 1 ? 4 : 3) : 3)
@@ -222,8 +118,9 @@ __global__ void __launch_bounds__(32 * kWarps, D == 128 ? (NB == 1 ? 4 : 3) : 3)
   // ---- the work item
   const int h = blockIdx.y % r.n_kv_heads;
   const int64_t item = blockIdx.y / r.n_kv_heads;  // 0: the prefix when there is one
-  const bool pre = P.plan.pre_chunks > 0 && item == 0;
-  const int64_t b = pre ? 0 : item - (P.plan.pre_chunks > 0 ? 1 : 0);
+  const bool has_pre = P.plan.pre_chunks > 0 && !P.pre_tensor;
+  const bool pre = has_pre && item == 0;
+  const int64_t b = pre ? 0 : item - has_pre;
   const int chunk = blockIdx.x;
   if (chunk >= (pre ? P.plan.pre_chunks : P.plan.own_chunks)) return;
   const int64_t n_rows = pre ? r.n_seqs * r.n_q : r.n_q;
@@ -712,12 +609,13 @@ kh_status launch_rows(const AttnParams& P, cudaStream_t stream) {
   std::call_once(once[dev & 63], [&] {
     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kRing);
   });
-  const int64_t gy = (r.n_seqs + (P.plan.pre_chunks > 0 ? 1 : 0)) * r.n_kv_heads;
-  const int64_t nq = P.plan.pre_chunks > 0 ? r.n_seqs * r.n_q : r.n_q;
+  const bool pre = P.plan.pre_chunks > 0 && !P.pre_tensor;
+  const int64_t gy = (r.n_seqs + pre) * r.n_kv_heads;
+  const int64_t nq = pre ? r.n_seqs * r.n_q : r.n_q;
   const int64_t gz = (nq + NQ - 1) / NQ;
   if (gy > 65535 || gz > 65535) return KH_EINVAL;
-  const dim3 grid((unsigned)std::max(P.plan.pre_chunks, P.plan.own_chunks), (unsigned)gy,
-                  (unsigned)gz);
+  const dim3 grid((unsigned)std::max(pre ? P.plan.pre_chunks : 0, P.plan.own_chunks),
+                  (unsigned)gy, (unsigned)gz);
   return launch_programmatic(kern, grid, dim3(32 * kWarps), C::kRing, stream, P) == cudaSuccess
              ? KH_OK
              : KH_ELAUNCH;
@@ -727,8 +625,12 @@ template <int D>
 kh_status launch_dim(const AttnParams& P, cudaStream_t stream) {
   const PagedAttnRequest& r = P.r;
   const int64_t rows = r.n_seqs * r.n_kv_heads * r.n_q;
-  if (P.plan.parts() > 0) {
-    const int64_t nq = P.plan.pre_chunks > 0 ? r.n_seqs * r.n_q : r.n_q;
+  if (P.plan.pre_chunks > 0 && P.pre_tensor) {
+    const kh_status st = launch_paged_prefix(P, stream);
+    if (st != KH_OK) return st;
+  }
+  if (P.plan.own_chunks > 0 || (P.plan.pre_chunks > 0 && !P.pre_tensor)) {
+    const int64_t nq = P.plan.pre_chunks > 0 && !P.pre_tensor ? r.n_seqs * r.n_q : r.n_q;
     kh_status st;
     if (r.dtype == KH_F32)
       st = nq > 4 && D == 128 ? launch_rows<D, true, true, D == 128 ? 2 : 1>(P, stream)
@@ -749,6 +651,9 @@ kh_status launch_dim(const AttnParams& P, cudaStream_t stream) {
 
 }  // namespace
 
+// From how many query rows a KV head's prefix is worth 128-row products.
+constexpr int64_t kPrefixTensorRows = 33;
+
 PagedPlan paged_plan(int64_t n_seqs, int n_q, int n_kv_heads, int D, int64_t max_len,
                      int64_t prefix_len, int64_t window, int n_sms) {
   PagedPlan p;
@@ -759,12 +664,19 @@ PagedPlan paged_plan(int64_t n_seqs, int n_q, int n_kv_heads, int D, int64_t max
     const int64_t even = (rows / (8 * (int64_t)n_sms) + 127) / 128 * 128;
     return std::max<int64_t>(128, std::min<int64_t>(2048, even));
   };
-  (void)D;
   const int64_t pre = std::min(prefix_len, max_len);
   int64_t own = max_len - pre;
   if (window > 0) own = std::min(own, window);
   if (pre > 0) {
-    p.pre_rows = chunk_of(pre * n_kv_heads * ((n_seqs * n_q + 7) / 8));
+    const int64_t nq = n_seqs * n_q;
+    if (nq >= kPrefixTensorRows) {
+      // one round of CTAs, one an SM, in whole tiles
+      const int64_t per = D == 128 ? 256 : 128, tile = D == 128 ? 128 : 64;
+      const int64_t ctas = std::max<int64_t>(1, n_sms / (n_kv_heads * ((nq + per - 1) / per)));
+      p.pre_rows = ((pre + ctas - 1) / ctas + tile - 1) / tile * tile;
+    } else {
+      p.pre_rows = chunk_of(pre * n_kv_heads * ((nq + 7) / 8));
+    }
     p.pre_chunks = (int)((pre + p.pre_rows - 1) / p.pre_rows);
   }
   if (own > 0) {
@@ -784,6 +696,7 @@ kh_status launch_paged_attn(const PagedAttnRequest& r, cudaStream_t stream) {
   P.inv_sd = (float)(1.0 / sd);
   int bits = 0;
   while ((int64_t(1) << bits) < r.page_size) ++bits;
+  P.pre_tensor = r.dtype == KH_BF16 && r.c0 == -r.c1 && r.n_seqs * r.n_q >= kPrefixTensorRows;
   P.div_shift = 31 + bits;
   P.div_mul = ((uint64_t(1) << P.div_shift) + r.page_size - 1) / r.page_size;
   P.err = device_error_ptr();
