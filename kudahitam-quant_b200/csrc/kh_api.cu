@@ -715,7 +715,7 @@ int64_t kh_paged_workspace_bytes(int64_t n_seqs, int n_q, int n_kv_heads, int he
     return -1;
   const PagedPlan p = paged_plan(n_seqs, n_q, n_kv_heads, head_dim, max_len, prefix_len, window,
                                  sm_count());
-  return n_seqs * n_q * n_kv_heads * p.parts() * (int64_t)(head_dim + 2) * 4;
+  return paged_workspace_bytes(p, n_seqs, n_q, n_kv_heads, head_dim);
 }
 
 int kh_paged_attn(const kh_paged_cache* cache, const void* q, int dtype, int64_t n_seqs, int n_q,

@@ -68,6 +68,7 @@ struct PagedPlan {
 };
 PagedPlan paged_plan(int64_t n_seqs, int n_q, int n_kv_heads, int D, int64_t max_len,
                      int64_t prefix_len, int64_t window, int n_sms);
+int64_t paged_workspace_bytes(const PagedPlan& p, int64_t n_seqs, int n_q, int n_kv_heads, int D);
 kh_status launch_paged_attn(const PagedAttnRequest& r, cudaStream_t stream);
 
 }  // namespace kh

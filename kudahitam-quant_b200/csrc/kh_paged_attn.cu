@@ -127,7 +127,11 @@ __global__ void __launch_bounds__(32 * kWarps, D == 128 ? (NB == 1 ? 4 : 3) : 3)
   const int64_t y0 = (int64_t)blockIdx.z * NQ;
   if (y0 >= n_rows) return;
   const int nq = (int)min((int64_t)NQ, n_rows - y0);
-  grid_dependency_wait();
+  // After a prefix launch this grid may run beside it: that one signals its
+  // dependents once all earlier work is done, and nothing here reads its
+  // records.  The wait then comes at the end, so that this grid's completion
+  // implies the prefix's.
+  if (!P.pre_tensor) grid_dependency_wait();
   int lo, hi;
   if (pre) {
     lo = (int)(chunk * P.plan.pre_rows);
@@ -135,7 +139,10 @@ __global__ void __launch_bounds__(32 * kWarps, D == 128 ? (NB == 1 ? 4 : 3) : 3)
   } else {
     const int64_t len = length_of(P, b);
     const int64_t first = own_first(P, b, len) + chunk * P.plan.own_rows;
-    if (first >= len) return;
+    if (first >= len) {
+      if (P.pre_tensor) grid_dependency_wait();
+      return;
+    }
     lo = (int)first;
     hi = (int)min(first + P.plan.own_rows, len);
   }
@@ -487,7 +494,7 @@ __global__ void __launch_bounds__(32 * kWarps, D == 128 ? (NB == 1 ? 4 : 3) : 3)
     issue(tile + (kStages - 1) * kWarps, (n + kStages - 1) % kStages, next_page);
     next_page = page_of(tile + kStages * kWarps);
   }
-  grid_dependents_launch();
+  if (!P.pre_tensor) grid_dependents_launch();
   cp_wait<0>();
   __syncthreads();
 
@@ -548,6 +555,7 @@ __global__ void __launch_bounds__(32 * kWarps, D == 128 ? (NB == 1 ? 4 : 3) : 3)
       rec[2 + 32 * j + lane] = v;
     }
   }
+  if (P.pre_tensor) grid_dependency_wait();
 }
 
 // One warp per query row: its records merged, element 32 j + lane in a[j].
@@ -569,22 +577,41 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constan
                         : 0;
   const int n = P.plan.pre_chunks + n_own;
   const float* rec = r.workspace + row * P.plan.parts() * (int64_t)(D + 2);
-  float mx = -INFINITY;
-  for (int p = lane; p < n; p += 32)
-    if (rec[p * (D + 2) + 1] != 0.f) mx = fmaxf(mx, rec[p * (D + 2)]);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  float l = 0.f, a[J];
+  // 32 records at a time: a lane each for the scales, then all lanes an
+  // element each, the loads of several records in flight
+  float mx = -INFINITY, l = 0.f, a[J];
 #pragma unroll
   for (int j = 0; j < J; ++j) a[j] = 0.f;
-  for (int p = 0; p < n; ++p) {
-    const float* q = rec + p * (D + 2);
-    const float lp = q[1];
-    if (lp == 0.f) continue;  // nothing attended there
-    const float f = exp2f(q[0] - mx);
-    l = fmaf(lp, f, l);
+  for (int p0 = 0; p0 < n; p0 += 32) {
+    const bool in = p0 + lane < n;
+    const float mp = in ? rec[(p0 + lane) * (D + 2)] : -INFINITY;
+    const float lp = in ? rec[(p0 + lane) * (D + 2) + 1] : 0.f;
+    const bool some = lp != 0.f;  // else nothing was attended there
+    float top = some ? mp : -INFINITY;
 #pragma unroll
-    for (int j = 0; j < J; ++j) a[j] = fmaf(q[2 + 32 * j + lane], f, a[j]);
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const uint32_t live = __ballot_sync(0xffffffffu, some);
+    if (!live) continue;
+    top = fmaxf(top, mx);
+    const float old = mx == -INFINITY ? 0.f : ex2(mx - top);
+    const float f = some ? ex2(mp - top) : 0.f;
+    mx = top;
+    float sum = some ? lp * f : 0.f;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    l = fmaf(l, old, sum);
+#pragma unroll
+    for (int j = 0; j < J; ++j) a[j] *= old;
+    const int m = min(32, n - p0);
+#pragma unroll 4
+    for (int p = 0; p < m; ++p) {
+      const float fp = __shfl_sync(0xffffffffu, f, p);
+      if (live >> p & 1) {
+        const float* q = rec + (p0 + p) * (D + 2) + 2;
+#pragma unroll
+        for (int j = 0; j < J; ++j) a[j] = fmaf(q[32 * j + lane], fp, a[j]);
+      }
+    }
   }
   fwht_lanes<J>(a, lane);
   const float inv = 1.f / l;
@@ -654,6 +681,18 @@ kh_status launch_dim(const AttnParams& P, cudaStream_t stream) {
 // From how many query rows a KV head's prefix is worth 128-row products.
 constexpr int64_t kPrefixTensorRows = 33;
 
+// The workspace: the records, then (16-byte aligned) the transformed queries
+// of a tensor-core prefix.
+int64_t paged_records_bytes(const PagedPlan& p, int64_t rows, int D) {
+  return (rows * p.parts() * (int64_t)(D + 2) * 4 + 15) / 16 * 16;
+}
+int64_t paged_workspace_bytes(const PagedPlan& p, int64_t n_seqs, int n_q, int n_kv_heads, int D) {
+  const int64_t nq = n_seqs * n_q;
+  int64_t n = paged_records_bytes(p, nq * n_kv_heads, D);
+  if (p.pre_chunks > 0 && nq >= kPrefixTensorRows) n += paged_queries_bytes(nq, n_kv_heads, D);
+  return n;
+}
+
 PagedPlan paged_plan(int64_t n_seqs, int n_q, int n_kv_heads, int D, int64_t max_len,
                      int64_t prefix_len, int64_t window, int n_sms) {
   PagedPlan p;
@@ -696,7 +735,10 @@ kh_status launch_paged_attn(const PagedAttnRequest& r, cudaStream_t stream) {
   P.inv_sd = (float)(1.0 / sd);
   int bits = 0;
   while ((int64_t(1) << bits) < r.page_size) ++bits;
-  P.pre_tensor = r.dtype == KH_BF16 && r.c0 == -r.c1 && r.n_seqs * r.n_q >= kPrefixTensorRows;
+  P.pre_tensor = P.plan.pre_chunks > 0 && r.dtype == KH_BF16 && r.c0 == -r.c1 &&
+                 r.n_seqs * r.n_q >= kPrefixTensorRows;
+  P.queries = reinterpret_cast<uint16_t*>(reinterpret_cast<uint8_t*>(r.workspace) +
+                                          paged_records_bytes(P.plan, r.n_seqs * r.n_q * r.n_kv_heads, r.D));
   P.div_shift = 31 + bits;
   P.div_mul = ((uint64_t(1) << P.div_shift) + r.page_size - 1) / r.page_size;
   P.err = device_error_ptr();

@@ -18,7 +18,8 @@ struct AttnParams {
   // shift = 31 + ceil(log2 page_size) (the error j (mul page_size - 2^shift) / 2^shift stays under 1)
   uint64_t div_mul;
   int div_shift;
-  int pre_tensor;  // the prefix has its own launch (launch_paged_prefix)
+  int pre_tensor;  // the prefix has its own launches (launch_paged_prefix)
+  uint16_t* queries;  // workspace of those: q~ in fp16, tile by tile
   uint32_t* err;
 
   __device__ __forceinline__ uint32_t page_div(uint32_t j) const {
@@ -40,6 +41,7 @@ __device__ __forceinline__ void st_any(void* p, int dtype, int64_t i, float v) {
 // Attention of every sequence's queries over the shared prefix, a record per
 // query row and chunk (kh_paged_prefix.cu).
 kh_status launch_paged_prefix(const AttnParams& P, cudaStream_t stream);
+int64_t paged_queries_bytes(int64_t nq, int n_kv_heads, int D);
 
 // Length of sequence b, within what the table and max_len hold.
 __device__ __forceinline__ int64_t length_of(const AttnParams& P, int64_t b) {

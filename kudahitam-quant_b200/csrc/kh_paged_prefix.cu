@@ -43,6 +43,7 @@ struct PreCfg {
   static constexpr int kQTile = kBoxes * 128 * 128;    // bytes
   static constexpr int kKvBox = ROWS * 128;
   static constexpr int kKvTile = kBoxes * kKvBox;
+  static constexpr int kGroup = MT * kQTile + 16;      // a CTA's queries in the workspace
   static constexpr int kOffK = MT * kQTile;
   static constexpr int kOffV = kOffK + 2 * kKvTile;
   static constexpr int kOffScale = kOffV + 2 * kKvTile;  // [2][kappa ROWS, r ROWS] floats
@@ -68,6 +69,64 @@ __device__ __forceinline__ float query_scale(float bound) {
   return ldexpf(1.f, max(-120, min(120, 14 - e)));
 }
 
+// Q~ of 128 MT query rows of one KV head, as the products' operand: tiles of
+// 128 rows, element e at position 2 (e & 15) + (e >> 4 & 1) of its block of
+// 32, 128-byte blocks swizzled; times log_scale and the power of two that the
+// last 4 bytes of the group hold.  Once per call, not per chunk: a warp's
+// transforms cost 4 us for 256 rows, as much as a chunk's products.
+template <int D>
+__global__ void __launch_bounds__(1024) paged_queries_kernel(const __grid_constant__ AttnParams P) {
+  using C = PreCfg<D>;
+  constexpr int W = D / 32, PER = C::MT * 4;  // query rows a warp
+  const PagedAttnRequest& r = P.r;
+  __shared__ uint32_t bound;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int h = blockIdx.y;
+  const int n_rows = (int)(r.n_seqs * r.n_q);
+  const int y0 = blockIdx.x * (C::MT * 128);
+  const uint16_t* q16 = static_cast<const uint16_t*>(r.q);
+  if (threadIdx.x == 0) bound = 0u;
+  __syncthreads();
+  grid_dependency_wait();
+  grid_dependents_launch();
+  float x[PER][W], mx = 0.f;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int i = y0 + warp * PER + k;
+    const int b = i / r.n_q;
+    const int64_t row = (int64_t)b * r.n_kv_heads * r.n_q + h * r.n_q + (i - b * r.n_q);
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      x[k][j] = i < n_rows ? __uint_as_float((uint32_t)q16[row * D + 32 * j + lane] << 16) : 0.f;
+      mx = fmaxf(mx, fabsf(x[k][j]));
+    }
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  if (lane == 0) atomicMax(&bound, __float_as_uint(mx));
+  __syncthreads();
+  const float up = query_scale(__uint_as_float(bound) * (float)D * fabsf(P.log_scale));
+  uint8_t* group = reinterpret_cast<uint8_t*>(P.queries) +
+                   (int64_t)(h * gridDim.x + blockIdx.x) * C::kGroup;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int y = warp * PER + k, row = y & 127;
+#pragma unroll
+    for (int j = 0; j < W; ++j)
+      if ((r.dk_neg[j] >> lane) & 1) x[k][j] = -x[k][j];
+    fwht_lanes<W>(x[k], lane);
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      const int pos = 32 * j + 2 * (lane & 15) + (lane >> 4);
+      const int c = (pos & 63) >> 3;
+      *reinterpret_cast<__half*>(group + (y >> 7) * C::kQTile + (pos >> 6) * (128 * 128) +
+                                 row * 128 + ((c ^ (row & 7)) << 4) + (pos & 7) * 2) =
+          __float2half_rn(x[k][j] * (P.log_scale * up));
+    }
+  }
+  if (threadIdx.x == 0) *reinterpret_cast<float*>(group + C::MT * C::kQTile) = up;
+}
+
 template <int D, bool EXTRA>
 __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
     paged_prefix_kernel(const __grid_constant__ AttnParams P) {
@@ -82,9 +141,10 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
   uint8_t* sm = smem_raw + (base - raw);
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + C::kOffBar);
   uint64_t *kfull = bars, *kempty = bars + 2, *vfull = bars + 4, *vempty = bars + 6,
-           *sfull = bars + 8, *pfull = bars + 10, *odone = bars + 12;
+           *sfull = bars + 8, *pfull = bars + 10, *odone = bars + 12, *qfull = bars + 14;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::kOffMisc);
-  uint32_t* q_bound = tmem_slot + 1;
+  const uint8_t* group = reinterpret_cast<const uint8_t*>(P.queries) +
+                         (int64_t)(blockIdx.y * gridDim.z + blockIdx.z) * C::kGroup;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   const int h = blockIdx.y;
@@ -106,8 +166,8 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
       mbar_init(&pfull[i], 4);
       mbar_init(&odone[i], 1);
     }
+    mbar_init(qfull, 32 * C::kSoftWarps);
     fence_mbar_init();
-    *q_bound = 0u;
   }
   if (warp == C::kSoftWarps + 4) {
     tmem_alloc(tmem_slot, C::kTmemCols);
@@ -117,50 +177,11 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  grid_dependency_wait();
-  grid_dependents_launch();
-
-  // ---- Q~: element e of query y at position 2 (e & 15) + (e >> 4 & 1) of its
-  // block of 32, times log_scale and a power of two
-  const uint16_t* q16 = static_cast<const uint16_t*>(r.q);
   auto query_row = [&](int y) {
     const int64_t i = y0 + y;
     const int64_t b = i / r.n_q;
     return b * hq_all + h * r.n_q + (int)(i - b * r.n_q);
   };
-  {
-    float mx = 0.f;
-    for (int y = warp; y < nq; y += C::kThreads / 32)
-#pragma unroll
-      for (int j = 0; j < W; ++j)
-        mx = fmaxf(mx, fabsf(__uint_as_float((uint32_t)q16[query_row(y) * D + 32 * j + lane] << 16)));
-#pragma unroll
-    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    if (lane == 0) atomicMax(q_bound, __float_as_uint(mx));
-  }
-  __syncthreads();
-  const float up = query_scale(__uint_as_float(*q_bound) * (float)D * fabsf(P.log_scale));
-  for (int y = warp; y < MT * 128; y += C::kThreads / 32) {
-    float x[W];
-#pragma unroll
-    for (int j = 0; j < W; ++j) {
-      float v = 0.f;
-      if (y < nq) v = __uint_as_float((uint32_t)q16[query_row(y) * D + 32 * j + lane] << 16);
-      x[j] = (r.dk_neg[j] >> lane) & 1 ? -v : v;
-    }
-    fwht_lanes<W>(x, lane);
-    const int row = y & 127;
-    uint8_t* tile = sm + (y >> 7) * C::kQTile + row * 128;
-#pragma unroll
-    for (int j = 0; j < W; ++j) {
-      const int pos = 32 * j + 2 * (lane & 15) + (lane >> 4);
-      const int c = (pos & 63) >> 3;
-      *reinterpret_cast<__half*>(tile + (pos >> 6) * (128 * 128) + ((c ^ (row & 7)) << 4) +
-                                 (pos & 7) * 2) = __float2half_rn(x[j] * (P.log_scale * up));
-    }
-  }
-  fence_proxy_async_smem();
-  __syncthreads();
 
   if (warp >= C::kSoftWarps && warp < C::kSoftWarps + 4) {
     // ------------------------------------------------------------ decoding
@@ -244,6 +265,7 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
       return m;
     };
     const float inv_sd = P.inv_sd;
+    float down = 1.f;
     int page = page_of(0);
     Row x = fetch(0, page);
     page = page_of(1);
@@ -258,11 +280,17 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&kfull[s]);
+      if (t == 0) {
+        // everything before the queries' launch was done when this grid could
+        // start, so only their scale has to be waited for
+        grid_dependency_wait();
+        down = 1.f / *reinterpret_cast<const float*>(group + MT * C::kQTile);
+      }
       if (!__all_sync(0xffffffffu, mbar_wait(&vempty[s], ph ^ 1u, P.err))) break;
       write(sm + C::kOffV + s * C::kKvTile, x.vc, x.vr, va, vb);
       if (part == 0) {
         float* sc = reinterpret_cast<float*>(sm + C::kOffScale) + s * 2 * ROWS;
-        sc[row] = kappa / up;
+        sc[row] = kappa * down;
         sc[ROWS + row] = rv;
         const uint32_t mask = __ballot_sync(0xffffffffu, x.on);
         if (lane == 0)
@@ -276,6 +304,8 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
     }
   } else if (warp == C::kSoftWarps + 4) {
     // ------------------------------------------------------------ products
+    grid_dependency_wait();
+    grid_dependents_launch();
     if (lane == 0) {
       auto scores = [&](int m, int s, int buf) {
         const uint32_t d = tmem + buf * C::kColS;
@@ -295,7 +325,7 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
           umma_f16_ta(d, pa + 8 * k, sw128_desc_mn(va + k * 2048, C::kKvBox), kIdescO,
                       more || k != 0);
       };
-      bool ok = mbar_wait(&kfull[0], 0, P.err);
+      bool ok = mbar_wait(qfull, 0, P.err) && mbar_wait(&kfull[0], 0, P.err);
       if (ok) {
         tc_fence_after();
         for (int m = 0; m < MT; ++m) {
@@ -340,6 +370,15 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
     const int m = warp >> 2, quarter = warp & 3;
     const int y = m * 128 + quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
+    // the queries, transformed by the launch before this one
+    grid_dependency_wait();
+    for (int k = threadIdx.x; k < MT * C::kQTile / 16; k += 32 * C::kSoftWarps)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(base + 16 * k),
+                   "l"(group + 16 * k)
+                   : "memory");
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    fence_proxy_async_smem();
+    mbar_arrive(qfull);
     int q_lo = 0, q_hi = 0;
     float slope = 0.f;
     if (y < nq) {
@@ -520,6 +559,12 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
   }
 }
 
+template <int D>
+int64_t queries_bytes(int64_t nq, int n_kv_heads) {
+  using C = PreCfg<D>;
+  return (nq + 128 * C::MT - 1) / (128 * C::MT) * n_kv_heads * C::kGroup;
+}
+
 template <int D, bool EXTRA>
 kh_status launch_typed(const AttnParams& P, cudaStream_t stream) {
   using C = PreCfg<D>;
@@ -534,12 +579,19 @@ kh_status launch_typed(const AttnParams& P, cudaStream_t stream) {
   const dim3 grid((unsigned)P.plan.pre_chunks, (unsigned)P.r.n_kv_heads,
                   (unsigned)((nq + per - 1) / per));
   if (grid.y > 65535 || (nq + per - 1) / per > 65535) return KH_EINVAL;
+  if (launch_programmatic(paged_queries_kernel<D>, dim3(grid.z, grid.y), dim3(1024), 0, stream,
+                          P) != cudaSuccess)
+    return KH_ELAUNCH;
   return launch_programmatic(kern, grid, dim3(C::kThreads), C::kSmem, stream, P) == cudaSuccess
              ? KH_OK
              : KH_ELAUNCH;
 }
 
 }  // namespace
+
+int64_t paged_queries_bytes(int64_t nq, int n_kv_heads, int D) {
+  return D == 128 ? queries_bytes<128>(nq, n_kv_heads) : queries_bytes<256>(nq, n_kv_heads);
+}
 
 kh_status launch_paged_prefix(const AttnParams& P, cudaStream_t stream) {
   const bool extra = P.r.softcap > 0.f || P.r.slopes;

@@ -309,6 +309,46 @@ def test_prefix_with_caps_biases_windows_and_short_sequences(dtype, D, nq):
     _attend(lengths, 2, nq, D, dtype, 64, prefix=prefix, seed=2)
 
 
+@pytest.mark.parametrize("D,B,nq", [(128, 12, 4), (128, 70, 4), (256, 9, 6)])
+@pytest.mark.parametrize("extra", [False, True])
+def test_prefix_of_many_queries_with_masks(D, B, nq, extra):
+    """Enough queries for the tensor-core prefix, each with limits of its own."""
+    prefix = 777
+    lengths = [prefix + (37 * b) % 90 for b in range(B)]
+    lengths[3:6] = [500, 0, 777]
+    starts = [(53 * b) % 1000 for b in range(B)]
+    kw = dict(softcap=12.0, slopes=2.0 ** -torch.arange(1, 2 * nq + 1, dtype=FL)) if extra else {}
+    _attend(lengths, 2, nq, D, BF, 48, prefix=prefix, seed=B, starts=starts, window=400, **kw)
+    _attend(lengths, 2, nq, D, BF, 64, prefix=prefix, seed=B + 1, **kw)
+
+
+def test_prefix_of_many_queries_with_large_and_bad_values():
+    """Norms over twelve orders in the prefix; then a NaN in one attended row,
+    which must reach every query that attends it and no other."""
+    prefix, page, H, D, B, nq = 512, 64, 1, 128, 10, 4
+    lengths = [prefix + 5] * B
+    lengths[2] = 100
+    kc, vc, dk, dv, c = R.pools(prefix // page + B, H, page, D, 12)
+    g = torch.Generator().manual_seed(12)
+    f = 10.0 ** (torch.rand(vc.norms.numel(), generator=g) * 12 - 6)
+    vc.norms *= f
+    vc.rnorms *= f
+    table = R.tables(lengths, page, prefix // page + B, 12, prefix)
+    q = (torch.randn(B, nq, D, generator=g) * 8).to(BF)
+    run = lambda: ops.paged_prefix_attention(  # noqa: E731
+        q.cuda(), R.cuda(kc), R.cuda(vc), table.cuda(),
+        torch.tensor(lengths, dtype=torch.int32).cuda(), prefix, dk, dv, c, return_lse=True)
+    R.check(*run(), R.attention(q, kc, vc, table, lengths, dk, dv, c), BF)
+    for pool in (kc, vc):
+        row = int(table[0, 300 // page]) * page + 300 % page
+        old = pool.norms[row].clone()
+        pool.norms[row] = float("nan")
+        out = run()[0].cpu().float()
+        assert torch.isfinite(out[2]).all()
+        assert torch.isnan(out[[b for b in range(B) if b != 2]]).all()
+        pool.norms[row] = old
+
+
 def test_prefix_equals_decode():
     """The shared read is the same attention as each sequence's own."""
     lengths, prefix, page = [1100, 1030, 1024], 1024, 64
