@@ -558,69 +558,87 @@ __global__ void __launch_bounds__(32 * kWarps, D == 128 ? (NB == 1 ? 4 : 3) : 3)
   if (P.pre_tensor) grid_dependency_wait();
 }
 
-// One warp per query row: its records merged, element 32 j + lane in a[j].
+// A block per query row: its records merged, back from the transformed
+// domain, divided by l, in the query's type.  What it takes is the time of a
+// few dependent loads, so each warp takes every fourth record and loads eight
+// of them at once.
 template <int D>
 __global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constant__ AttnParams P) {
-  constexpr int J = D / 32;
+  constexpr int J = D / 32, U = 8;
   const PagedAttnRequest& r = P.r;
-  const int lane = threadIdx.x & 31;
+  __shared__ float sums[4][D], tops[4], ls[4];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int hq_all = r.n_kv_heads * r.n_q;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const uint32_t row = blockIdx.x;
+  const uint32_t b = row / hq_all;
+  const float* rec = r.workspace + (int64_t)row * P.plan.parts() * (D + 2);
   grid_dependency_wait();
-  if (row >= r.n_seqs * hq_all) return;
-  const int64_t b = row / hq_all;
   const int64_t len = length_of(P, b);
   const int64_t own = max((int64_t)0, len - own_first(P, b, len));
-  const int n_own = P.plan.own_rows
-                        ? (int)min((own + P.plan.own_rows - 1) / P.plan.own_rows,
-                                   (int64_t)P.plan.own_chunks)
-                        : 0;
-  const int n = P.plan.pre_chunks + n_own;
-  const float* rec = r.workspace + row * P.plan.parts() * (int64_t)(D + 2);
-  // 32 records at a time: a lane each for the scales, then all lanes an
-  // element each, the loads of several records in flight
+  const int n = P.plan.pre_chunks +
+                (P.plan.own_rows ? (int)min((own + P.plan.own_rows - 1) / P.plan.own_rows,
+                                            (int64_t)P.plan.own_chunks)
+                                 : 0);
   float mx = -INFINITY, l = 0.f, a[J];
 #pragma unroll
   for (int j = 0; j < J; ++j) a[j] = 0.f;
-  for (int p0 = 0; p0 < n; p0 += 32) {
-    const bool in = p0 + lane < n;
-    const float mp = in ? rec[(p0 + lane) * (D + 2)] : -INFINITY;
-    const float lp = in ? rec[(p0 + lane) * (D + 2) + 1] : 0.f;
-    const bool some = lp != 0.f;  // else nothing was attended there
-    float top = some ? mp : -INFINITY;
+  for (int p0 = warp; p0 < n; p0 += 4 * U) {
+    float mp[U], lp[U], v[U][J], top = mx;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const uint32_t live = __ballot_sync(0xffffffffu, some);
-    if (!live) continue;
-    top = fmaxf(top, mx);
-    const float old = mx == -INFINITY ? 0.f : ex2(mx - top);
-    const float f = some ? ex2(mp - top) : 0.f;
-    mx = top;
-    float sum = some ? lp * f : 0.f;
+    for (int u = 0; u < U; ++u) {
+      const int p = min(p0 + 4 * u, n - 1);
+      const float* q = rec + (int64_t)p * (D + 2);
+      mp[u] = q[0];
+      lp[u] = p0 + 4 * u < n ? q[1] : 0.f;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    l = fmaf(l, old, sum);
+      for (int j = 0; j < J; ++j) v[u][j] = q[2 + 32 * j + lane];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (lp[u] != 0.f) top = fmaxf(top, mp[u]);  // else nothing was attended there
+    if (top == -INFINITY) continue;
+    const float old = ex2(mx - top);
+    l *= old;
 #pragma unroll
     for (int j = 0; j < J; ++j) a[j] *= old;
-    const int m = min(32, n - p0);
-#pragma unroll 4
-    for (int p = 0; p < m; ++p) {
-      const float fp = __shfl_sync(0xffffffffu, f, p);
-      if (live >> p & 1) {
-        const float* q = rec + (p0 + p) * (D + 2) + 2;
 #pragma unroll
-        for (int j = 0; j < J; ++j) a[j] = fmaf(q[32 * j + lane], fp, a[j]);
+    for (int u = 0; u < U; ++u)
+      if (lp[u] != 0.f) {
+        const float f = ex2(mp[u] - top);
+        l = fmaf(lp[u], f, l);
+#pragma unroll
+        for (int j = 0; j < J; ++j) a[j] = fmaf(v[u][j], f, a[j]);
       }
-    }
+    mx = top;
+  }
+#pragma unroll
+  for (int j = 0; j < J; ++j) sums[warp][32 * j + lane] = a[j];
+  if (lane == 0) {
+    tops[warp] = mx;
+    ls[warp] = l;
+  }
+  __syncthreads();
+  if (warp) return;
+  const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  l = 0.f;
+#pragma unroll
+  for (int j = 0; j < J; ++j) a[j] = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (tops[w] == -INFINITY) continue;
+    const float f = ex2(tops[w] - top);
+    l = fmaf(ls[w], f, l);
+#pragma unroll
+    for (int j = 0; j < J; ++j) a[j] = fmaf(sums[w][32 * j + lane], f, a[j]);
   }
   fwht_lanes<J>(a, lane);
   const float inv = 1.f / l;
 #pragma unroll
   for (int j = 0; j < J; ++j) {
     const float v = l == 0.f ? 0.f : a[j] * inv;
-    st_any(r.out, r.dtype, row * D + 32 * j + lane, (r.dv_neg[j] >> lane) & 1 ? -v : v);
+    st_any(r.out, r.dtype, (int64_t)row * D + 32 * j + lane, (r.dv_neg[j] >> lane) & 1 ? -v : v);
   }
-  if (r.lse && lane == 0) r.lse[row] = l == 0.f ? -INFINITY : (mx + log2f(l)) * kLn2;
+  if (r.lse && lane == 0) r.lse[row] = l == 0.f ? -INFINITY : (top + log2f(l)) * kLn2;
 }
 
 template <int D, bool HILO, bool EXACT, int NB>
@@ -670,7 +688,7 @@ kh_status launch_dim(const AttnParams& P, cudaStream_t stream) {
                               : launch_rows<D, false, false, 1>(P, stream);
     if (st != KH_OK) return st;
   }
-  if (launch_programmatic(paged_combine_kernel<D>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0,
+  if (launch_programmatic(paged_combine_kernel<D>, dim3((unsigned)rows), dim3(128), 0,
                           stream, P) != cudaSuccess)
     return KH_ELAUNCH;
   return cudaGetLastError() == cudaSuccess ? KH_OK : KH_ELAUNCH;

@@ -8,19 +8,20 @@
 //   S = Q~ K^      (queries x rows, accumulator in tensor memory)
 //   O += W V^      (W = weights, fp16, back in S's columns as the operand)
 // Row scales stay out of the tiles: K^ and V^ rows are divided by their
-// largest possible element (so any norm fits fp16), the scale multiplies the
-// column of S, or the weight, in 32 bits.  Each element is the sum of two
-// signed constants: a shift, a logic operation per plane and one packed add
-// for two elements, since elements 32 w + e and 32 w + e + 16 are neighbours
-// in the tile (the order of elements is free as long as Q~ and the output
-// follow it) and so move to the sign positions of one register together.
+// largest constant or, where a tile's rows are alike, all by one power of two
+// (so any norm fits fp16); the scale multiplies the score, or the weight, in
+// 32 bits.  Elements 32 w + e and 32 w + e + 16 are neighbours in the tile (the
+// order of elements is free as long as Q~ and the output follow it), so that
+// one mask serves both.
 //
 // Roles: 4 warps a query tile for the softmax, a thread per query row; 4 warps
-// that decode, a thread per cached row; 1 warp whose first lane issues the
-// products.  At D = 128 two query tiles alternate, so that one's exponentials
-// run beside the other's products; at D = 256 one tile alternates between two
-// score buffers.  The reference exponent of a row moves only when a weight
-// would pass 2^12: then the tile's weights are taken again and O rescaled.
+// that decode; 1 thread that issues the products.  At D = 128 two query tiles
+// alternate, so that one's exponentials run beside the other's products (two
+// buffers of 64 rows each instead of one of 128 measured slower: a product
+// 64 wide takes as long as one of 128, both read 4 KB of Q~ a step); at
+// D = 256 one tile alternates between two score buffers.  The reference exponent of
+// a row moves only when a weight would leave fp16: then the chunk's weights
+// are taken again, O and the weights before it rescaled.
 //
 // Rounding to 16 bits: q~, K^, the weights and V^ to fp16 (half a step 2^-12
 // each); sums, exponents and l in 32 bits.  That is under a result of
@@ -35,31 +36,65 @@
 namespace kh {
 namespace {
 
+// D = 128: the block launches with 4 x 128 registers a lane = 2 x 176 + 112 + 48.
+constexpr int kRegsSoft = 176, kRegsDecode = 112, kRegsIssue = 48;
+
 template <int D>
 struct PreCfg {
   static constexpr int MT = D == 128 ? 2 : 1;          // query tiles
   static constexpr int ROWS = D == 128 ? 128 : 64;     // cached rows a tile
+  static constexpr int SB = D == 128 ? 1 : 2;          // score buffers of a query tile
   static constexpr int kBoxes = D / 64;                // 64-element blocks of a row
   static constexpr int kQTile = kBoxes * 128 * 128;    // bytes
   static constexpr int kKvBox = ROWS * 128;
   static constexpr int kKvTile = kBoxes * kKvBox;
+  static constexpr int kStages = 2;                    // of K^ and of V^
   static constexpr int kGroup = MT * kQTile + 16;      // a CTA's queries in the workspace
   static constexpr int kOffK = MT * kQTile;
-  static constexpr int kOffV = kOffK + 2 * kKvTile;
-  static constexpr int kOffScale = kOffV + 2 * kKvTile;  // [2][kappa ROWS, r ROWS] floats
-  static constexpr int kOffValid = kOffScale + 2 * 2 * ROWS * 4;  // [2][4] masks
-  static constexpr int kOffBar = kOffValid + 32;
-  static constexpr int kOffMisc = kOffBar + 16 * 8;
+  static constexpr int kOffV = kOffK + kStages * kKvTile;
+  static constexpr int kOffScale = kOffV + kStages * kKvTile;  // {kappa, r} of ROWS columns
+  static constexpr int kOffValid = kOffScale + kStages * 2 * ROWS * 4;  // masks of 32 rows
+  static constexpr int kOffEven = kOffValid + kStages * 16;  // {kappa, 1 / r, log2 r, even}
+  static constexpr int kOffRange = kOffEven + kStages * 16;  // 4 warps' extremes
+  static constexpr int kOffBar = kOffRange + kStages * 64;
+  static constexpr int kBars = 4 * kStages + 4 + 4 + 2 + 1;
+  static constexpr int kOffMisc = kOffBar + kBars * 8;
   static constexpr int kSmem = 1024 + kOffMisc + 16;
   static constexpr int kSoftWarps = 4 * MT;
-  static constexpr int kThreads = 32 * (kSoftWarps + 4 + 1);
+  // whole warpgroups, so that the softmax can take registers from the others
+  static constexpr int kThreads = 32 * (kSoftWarps + 4 + 4);
   static constexpr uint32_t kTmemCols = 512;
-  static constexpr uint32_t kColO = D == 128 ? 256 : 128;  // O's first column
-  static constexpr uint32_t kColS = D == 128 ? 128 : 64;   // S buffers apart
+  // tensor memory: the score buffers of ROWS columns, then the sums
+  static constexpr uint32_t kColO = SB * MT * ROWS;
+  static_assert(kColO + MT * D <= kTmemCols, "tensor memory");
   static_assert(kSmem <= 232448, "exceeds the shared memory of a CTA");
-  // the sums of 128 queries leave through the tiles' place
-  static_assert(MT * 128 * (D + 1) * 4 <= kOffScale, "staging of the sums");
+  static_assert(MT * 128 * (D + 1) * 4 <= kOffScale, "the sums leave through the tiles' place");
 };
+
+// 2^y for two y: y = n + f with n whole (the sum with 1.5 2^23 rounds to it),
+// 2^f on [-1/2, 1/2] by the cubic of least relative error (2^-13.7, found by
+// exchange), n added to the exponent.  A quarter of the exponentials go this way: the
+// special-function pipe takes 8 cycles for a warp's 32, and two warps' 32
+// columns measured 531 cycles with none, 446 with a quarter, 489 with half.
+constexpr float kE0 = 0.999928074f, kE1 = 0.693260985f, kE2 = 0.242611122f, kE3 = 0.0551716691f;
+__device__ __forceinline__ float2 ex2_poly(float2 y) {
+  y = make_float2(fminf(fmaxf(y.x, -126.f), 127.f), fminf(fmaxf(y.y, -126.f), 127.f));
+  const float2 big = make_float2(12582912.f, 12582912.f);
+  const float2 n = __fadd2_rn(y, big);
+  const float2 f = __fadd2_rn(y, __ffma2_rn(n, make_float2(-1.f, -1.f), big));
+  float2 p = __ffma2_rn(f, make_float2(kE3, kE3), make_float2(kE2, kE2));
+  p = __ffma2_rn(p, f, make_float2(kE1, kE1));
+  p = __ffma2_rn(p, f, make_float2(kE0, kE0));
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(n.x) << 23)),
+                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(n.y) << 23)));
+}
+
+// Rows are decoded so that their largest constant becomes this or less: then
+// 2^25 times it is in fp16's range.
+constexpr float kTileScale = 0x1p-11f;
+
+// fp16 ends at 65504; 32 weights with this sum are all below it.
+constexpr float kMostSum = 32768.f;
 
 // Queries are stored times a power of two that keeps the largest |q~| of the
 // CTA under 2^14: fp16 holds elements 2^28 below that with full steps.
@@ -69,48 +104,73 @@ __device__ __forceinline__ float query_scale(float bound) {
   return ldexpf(1.f, max(-120, min(120, 14 - e)));
 }
 
-// Q~ of 128 MT query rows of one KV head, as the products' operand: tiles of
-// 128 rows, element e at position 2 (e & 15) + (e >> 4 & 1) of its block of
-// 32, 128-byte blocks swizzled; times log_scale and the power of two that the
-// last 4 bytes of the group hold.  Once per call, not per chunk: a warp's
-// transforms cost 4 us for 256 rows, as much as a chunk's products.
+// Q~ of a KV head's query rows, as the products' operand: groups of 128 MT
+// rows in tiles of 128, element e at position 2 (e & 15) + (e >> 4 & 1) of its
+// block of 32, 128-byte blocks swizzled; times log_scale and a power of two,
+// which the 4 bytes behind the group hold.  Once per call, not per chunk: the
+// transforms of 256 rows cost one CTA 4 us, as much as a chunk's products.
+// A block transforms 32 rows, and reads its whole group for the power of two
+// rather than wait for other blocks.
 template <int D>
-__global__ void __launch_bounds__(1024) paged_queries_kernel(const __grid_constant__ AttnParams P) {
+__global__ void __launch_bounds__(256) paged_queries_kernel(const __grid_constant__ AttnParams P) {
   using C = PreCfg<D>;
-  constexpr int W = D / 32, PER = C::MT * 4;  // query rows a warp
+  constexpr int W = D / 32, GROUP = C::MT * 128;
   const PagedAttnRequest& r = P.r;
-  __shared__ uint32_t bound;
+  __shared__ float most[8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int h = blockIdx.y;
   const int n_rows = (int)(r.n_seqs * r.n_q);
-  const int y0 = blockIdx.x * (C::MT * 128);
+  const int y0 = blockIdx.x / (GROUP / 32) * GROUP;
+  const int first = blockIdx.x % (GROUP / 32) * 32 + warp * 4;  // of the group
   const uint16_t* q16 = static_cast<const uint16_t*>(r.q);
-  if (threadIdx.x == 0) bound = 0u;
-  __syncthreads();
   grid_dependency_wait();
   grid_dependents_launch();
-  float x[PER][W], mx = 0.f;
+  auto row_of = [&](int y) {
+    const int i = y0 + y, b = i / r.n_q;
+    return q16 + ((int64_t)b * r.n_kv_heads * r.n_q + h * r.n_q + (i - b * r.n_q)) * D;
+  };
+  float x[4][W], mx = 0.f;
 #pragma unroll
-  for (int k = 0; k < PER; ++k) {
-    const int i = y0 + warp * PER + k;
-    const int b = i / r.n_q;
-    const int64_t row = (int64_t)b * r.n_kv_heads * r.n_q + h * r.n_q + (i - b * r.n_q);
+  for (int k = 0; k < 4; ++k)
 #pragma unroll
-    for (int j = 0; j < W; ++j) {
-      x[k][j] = i < n_rows ? __uint_as_float((uint32_t)q16[row * D + 32 * j + lane] << 16) : 0.f;
-      mx = fmaxf(mx, fabsf(x[k][j]));
+    for (int j = 0; j < W; ++j)
+      x[k][j] = y0 + first + k < n_rows
+                    ? __uint_as_float((uint32_t)row_of(first + k)[32 * j + lane] << 16)
+                    : 0.f;
+  // lanes 8 to a row; 16 bytes a lane where q's alignment allows
+  const int in_group = min(GROUP, n_rows - y0);
+  if ((reinterpret_cast<uintptr_t>(q16) & 15) == 0) {
+#pragma unroll 4
+    for (int y = warp * 4 + (lane >> 3); y < in_group; y += 32) {
+      const uint4* src = reinterpret_cast<const uint4*>(row_of(y));
+#pragma unroll
+      for (int k = 0; k < D / 64; ++k) {
+        const uint4 v = __ldg(src + 8 * k + (lane & 7));
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          mx = fmaxf(fmaxf(mx, fabsf(__uint_as_float(w[i] << 16))),
+                     fabsf(__uint_as_float(w[i] & 0xffff0000u)));
+      }
     }
+  } else {
+    for (int y = warp; y < in_group; y += 8)
+#pragma unroll
+      for (int j = 0; j < W; ++j)
+        mx = fmaxf(mx, fabsf(__uint_as_float((uint32_t)row_of(y)[32 * j + lane] << 16)));
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  if (lane == 0) atomicMax(&bound, __float_as_uint(mx));
+  if (lane == 0) most[warp] = mx;
   __syncthreads();
-  const float up = query_scale(__uint_as_float(bound) * (float)D * fabsf(P.log_scale));
-  uint8_t* group = reinterpret_cast<uint8_t*>(P.queries) +
-                   (int64_t)(h * gridDim.x + blockIdx.x) * C::kGroup;
 #pragma unroll
-  for (int k = 0; k < PER; ++k) {
-    const int y = warp * PER + k, row = y & 127;
+  for (int w = 0; w < 8; ++w) mx = fmaxf(mx, most[w]);
+  const float up = query_scale(mx * (float)D * fabsf(P.log_scale));
+  uint8_t* group = reinterpret_cast<uint8_t*>(P.queries) +
+                   (int64_t)(h * (gridDim.x / (GROUP / 32)) + blockIdx.x / (GROUP / 32)) * C::kGroup;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int y = first + k, row = y & 127;
 #pragma unroll
     for (int j = 0; j < W; ++j)
       if ((r.dk_neg[j] >> lane) & 1) x[k][j] = -x[k][j];
@@ -124,7 +184,17 @@ __global__ void __launch_bounds__(1024) paged_queries_kernel(const __grid_consta
           __float2half_rn(x[k][j] * (P.log_scale * up));
     }
   }
-  if (threadIdx.x == 0) *reinterpret_cast<float*>(group + C::MT * C::kQTile) = up;
+  if (blockIdx.x % (GROUP / 32) == 0 && threadIdx.x == 0)
+    *reinterpret_cast<float*>(group + C::MT * C::kQTile) = up;
+}
+
+template <int N>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 template <int D, bool EXTRA>
@@ -140,8 +210,10 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* sm = smem_raw + (base - raw);
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + C::kOffBar);
-  uint64_t *kfull = bars, *kempty = bars + 2, *vfull = bars + 4, *vempty = bars + 6,
-           *sfull = bars + 8, *pfull = bars + 10, *odone = bars + 12, *qfull = bars + 14;
+  constexpr int NS = C::kStages;
+  // sfull and pfull by score buffer: SB m + t % SB
+  uint64_t *kfull = bars, *kempty = kfull + NS, *vfull = kempty + NS, *vempty = vfull + NS,
+           *sfull = vempty + NS, *pfull = sfull + 4, *odone = pfull + 4, *qfull = odone + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::kOffMisc);
   const uint8_t* group = reinterpret_cast<const uint8_t*>(P.queries) +
                          (int64_t)(blockIdx.y * gridDim.z + blockIdx.z) * C::kGroup;
@@ -157,15 +229,17 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
   const int hq_all = r.n_kv_heads * r.n_q;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < NS; ++i) {
       mbar_init(&kfull[i], 4);
       mbar_init(&kempty[i], 1);
       mbar_init(&vfull[i], 4);
       mbar_init(&vempty[i], 1);
+    }
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&sfull[i], 1);
       mbar_init(&pfull[i], 4);
-      mbar_init(&odone[i], 1);
     }
+    for (int i = 0; i < 2; ++i) mbar_init(&odone[i], 1);
     mbar_init(qfull, 32 * C::kSoftWarps);
     fence_mbar_init();
   }
@@ -185,6 +259,7 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
 
   if (warp >= C::kSoftWarps && warp < C::kSoftWarps + 4) {
     // ------------------------------------------------------------ decoding
+    if constexpr (D == 128) fewer_registers<kRegsDecode>();
     const int i = threadIdx.x - 32 * C::kSoftWarps;  // row of the tile
     // at D = 256 a row is two threads', half its words each
     constexpr int kSplit = 128 / ROWS;
@@ -212,10 +287,14 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
         const uint32_t off = j - P.page_div(j) * r.page_size;
         const int64_t at = ((int64_t)page * r.n_kv_heads + h) * r.page_size + off;
         auto take = [&](const uint32_t* plane, uint32_t(&to)[WT]) {
-          const uint4 v = __ldg(reinterpret_cast<const uint4*>(plane + at * W) + part);
-          to[0] = v.x; to[1] = v.y; to[2] = v.z; to[3] = v.w;
+          if constexpr (WT == 4) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(plane + at * W) + part);
+            to[0] = v.x; to[1] = v.y; to[2] = v.z; to[3] = v.w;
+          } else {
+            const uint2 v = __ldg(reinterpret_cast<const uint2*>(plane + at * W) + part);
+            to[0] = v.x; to[1] = v.y;
+          }
         };
-        static_assert(WT == 4, "a thread decodes 128 elements");
         take(r.kp.code, x.kc);
         take(r.kp.res, x.kr);
         take(r.vp.code, x.vc);
@@ -227,54 +306,117 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
       }
       return x;
     };
-    // +-a +-b for 128 elements, divided by what the row's scale takes out
+    // +-a +-b for the thread's words: the bits masked to b = 0 .. 7 are fp16
+    // numbers 2^(b - 24), exact factors of 2 a 2^(24 - b); -a - b is added.
+    // A logic operation and a multiply-add for two elements of a plane, where
+    // moving bits to the sign took a shift and a logic operation, both on the
+    // pipe that the softmax's conversions need.
     auto write = [&](uint8_t* tile, const uint32_t(&code)[WT], const uint32_t(&res)[WT], float a,
                      float b) {
-      constexpr uint32_t M = 0x80008000u;
-      const uint32_t pa = pack_h2(a, a) ^ M, pb = pack_h2(b, b) ^ M;
+      uint32_t fa[8], fb[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float up = (float)(1 << (25 - k));
+        fa[k] = pack_h2(a * up, a * up);
+        fb[k] = pack_h2(b * up, b * up);
+      }
+      const uint32_t low = pack_h2(-a - b, -a - b);
 #pragma unroll
       for (int w = 0; w < WT; ++w) {
         const int word = part * WT + w;
-        uint32_t v[16];
+        uint32_t v[16], c = code[w], s = res[w];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const uint32_t t0 = ((code[w] << (15 - e)) & M) ^ pa;
-          const uint32_t t1 = ((res[w] << (15 - e)) & M) ^ pb;
-          asm("add.rn.f16x2 %0, %1, %2;" : "=r"(v[e]) : "r"(t0), "r"(t1));
+          if (e == 8) {
+            c >>= 8;
+            s >>= 8;
+          }
+          const uint32_t m = 0x00010001u << (e & 7);
+          asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(v[e]) : "r"(c & m), "r"(fa[e & 7]), "r"(low));
+          asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(v[e]) : "r"(s & m), "r"(fb[e & 7]));
         }
         uint8_t* at = tile + (word >> 1) * C::kKvBox + row * 128;
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-          *reinterpret_cast<uint4*>(at + ((((word & 1) * 4 + c) ^ (row & 7)) << 4)) =
-              make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+        for (int k = 0; k < 4; ++k)
+          *reinterpret_cast<uint4*>(at + ((((word & 1) * 4 + k) ^ (row & 7)) << 4)) =
+              make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
       }
     };
-    // A row's two constants divided by the larger, which is returned: any two
-    // norms fit fp16.  Norms that are not finite give a row of zeros and
-    // leave through the scale, which masked places do not take.
-    auto scaled = [&](float& a, float& b) {
+    // A row's larger constant: what it is divided by, so that any two norms fit
+    // fp16.  Norms that are not finite give a row of zeros and leave through
+    // the scale, which masked places do not take.
+    auto largest = [&](float& a, float& b) {
       const float m = fmaxf(fabsf(a), fabsf(b));
-      if (!(m > 1e-35f && m < INFINITY) || a != a || b != b) {
+      if (!(m > 1e-35f && m < 1e35f) || a != a || b != b) {
         const bool none = fabsf(a) <= 1e-35f && fabsf(b) <= 1e-35f;
         a = b = 0.f;
         return none ? 0.f : NAN;
       }
-      const float inv = 1.f / m;
-      a *= inv;
-      b *= inv;
       return m;
     };
     const float inv_sd = P.inv_sd;
     float down = 1.f;
-    int page = page_of(0);
-    Row x = fetch(0, page);
-    page = page_of(1);
+    // two tiles' rows on their way while one is decoded, their pages one ahead
+    Row ahead[2];
+    ahead[0] = fetch(0, page_of(0));
+    ahead[1] = fetch(1, page_of(1));
+    int page = page_of(2);
+#pragma unroll 2
     for (int t = 0; t < n_tiles; ++t) {
-      const int s = t & 1;
-      const uint32_t ph = (uint32_t)((t >> 1) & 1);
+      const int s = t % NS;
+      const uint32_t ph = (uint32_t)((t / NS) & 1);
+      const Row x = ahead[t & 1];
+      ahead[t & 1] = fetch(t + 2, page);
+      page = page_of(t + 3);
       float ka = x.kn * r.c1, kb = x.krn * inv_sd;
       float va = x.vn * r.c1 * inv_sd, vb = x.vrn * (0.7978845608028654f * inv_sd * inv_sd);
-      const float kappa = scaled(ka, kb), rv = scaled(va, vb);
+      float kappa = largest(ka, kb), rv = largest(va, vb);
+      // Where the tile's rows are all there and their scales lie within 2^10 of
+      // one another, one power of two serves them all: fp16 still gives every
+      // row its full steps, and the softmax needs no scale per column.
+      float* range = reinterpret_cast<float*>(sm + C::kOffRange) + s * 16;
+      {
+        const float k0 = x.on ? kappa : NAN, v0 = x.on ? rv : NAN;
+        float most[2] = {k0, v0}, least[2] = {k0, v0};
+        const bool odd = __any_sync(0xffffffffu, !(k0 > 0.f) || !(v0 > 0.f));
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int o = 16; o; o >>= 1) {
+            most[i] = fmaxf(most[i], __shfl_xor_sync(0xffffffffu, most[i], o));
+            least[i] = fminf(least[i], __shfl_xor_sync(0xffffffffu, least[i], o));
+          }
+        if (lane == 0)
+          *reinterpret_cast<float4*>(range + 4 * (warp - C::kSoftWarps)) =
+              make_float4(odd ? INFINITY : most[0], least[0], most[1], least[1]);
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      float4 all = *reinterpret_cast<const float4*>(range);
+#pragma unroll
+      for (int w = 1; w < 4; ++w) {
+        const float4 q = *reinterpret_cast<const float4*>(range + 4 * w);
+        all = make_float4(fmaxf(all.x, q.x), fminf(all.y, q.y), fmaxf(all.z, q.z), fminf(all.w, q.w));
+      }
+      const bool even = all.x <= 1024.f * all.y && all.z <= 1024.f * all.w;
+      int ve = 0;
+      float ki, vi;
+      if (even) {
+        // the power of two above the largest, its inverse and its exponent
+        const uint32_t kx = (__float_as_uint(all.x) & 0x7f800000u) + 0x00800000u;
+        const uint32_t vx = (__float_as_uint(all.z) & 0x7f800000u) + 0x00800000u;
+        kappa = __uint_as_float(kx);
+        rv = __uint_as_float(vx);
+        ki = __uint_as_float(0x7f000000u - kx);
+        vi = __uint_as_float(0x7f000000u - vx);
+        ve = (int)(vx >> 23) - 127;
+      } else {
+        ki = kappa > 0.f ? 1.f / kappa : 0.f;
+        vi = rv > 0.f ? 1.f / rv : 0.f;
+      }
+      ka *= ki * kTileScale;
+      kb *= ki * kTileScale;
+      va *= vi * kTileScale;
+      vb *= vi * kTileScale;
       if (!__all_sync(0xffffffffu, mbar_wait(&kempty[s], ph ^ 1u, P.err))) break;
       write(sm + C::kOffK + s * C::kKvTile, x.kc, x.kr, ka, kb);
       fence_proxy_async_smem();
@@ -290,83 +432,76 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
       write(sm + C::kOffV + s * C::kKvTile, x.vc, x.vr, va, vb);
       if (part == 0) {
         float* sc = reinterpret_cast<float*>(sm + C::kOffScale) + s * 2 * ROWS;
-        sc[row] = kappa * down;
+        sc[row] = kappa * (down / kTileScale);
         sc[ROWS + row] = rv;
         const uint32_t mask = __ballot_sync(0xffffffffu, x.on);
         if (lane == 0)
           reinterpret_cast<uint32_t*>(sm + C::kOffValid)[s * 4 + (row >> 5)] = mask;
+        if (i == 0)
+          *reinterpret_cast<float4*>(sm + C::kOffEven + 16 * s) =
+              make_float4(kappa * (down / kTileScale), vi, (float)ve, even ? 1.f : 0.f);
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&vfull[s]);
-      x = fetch(t + 1, page);
-      page = page_of(t + 2);
     }
-  } else if (warp == C::kSoftWarps + 4) {
+  } else if (warp >= C::kSoftWarps + 4) {
     // ------------------------------------------------------------ products
+    if constexpr (D == 128) fewer_registers<kRegsIssue>();
     grid_dependency_wait();
     grid_dependents_launch();
-    if (lane == 0) {
-      auto scores = [&](int m, int s, int buf) {
-        const uint32_t d = tmem + buf * C::kColS;
-        const uint32_t qa = base + m * C::kQTile, ka = base + C::kOffK + s * C::kKvTile;
+    if (warp == C::kSoftWarps + 4 && lane == 0) {
+      auto scores = [&](int m, int t) {  // of tile t and query tile m
+        const uint32_t ka = base + C::kOffK + (t % NS) * C::kKvTile;
+        const int i = C::SB * m + t % C::SB;
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint64_t ad = sw128_desc(qa + (k >> 2) * (128 * 128)) + 2 * (k & 3);
-          const uint64_t bd = sw128_desc(ka + (k >> 2) * C::kKvBox) + 2 * (k & 3);
-          umma_f16(d, ad, bd, kIdescS, k != 0);
-        }
+        for (int k = 0; k < D / 16; ++k)
+          umma_f16(tmem + i * ROWS, sw128_desc(base + m * C::kQTile + (k >> 2) * (128 * 128)) + 2 * (k & 3),
+                   sw128_desc(ka + (k >> 2) * C::kKvBox) + 2 * (k & 3), kIdescS, k != 0);
+        umma_commit(&sfull[i]);
+        if (m == MT - 1) umma_commit(&kempty[t % NS]);
       };
-      auto values = [&](int m, int s, int buf, bool more) {
-        const uint32_t d = tmem + C::kColO + m * 128;
-        const uint32_t pa = tmem + buf * C::kColS, va = base + C::kOffV + s * C::kKvTile;
-#pragma unroll
-        for (int k = 0; k < ROWS / 16; ++k)
-          umma_f16_ta(d, pa + 8 * k, sw128_desc_mn(va + k * 2048, C::kKvBox), kIdescO,
-                      more || k != 0);
-      };
-      bool ok = mbar_wait(qfull, 0, P.err) && mbar_wait(&kfull[0], 0, P.err);
-      if (ok) {
+      auto keys = [&](int t) {
+        const bool in = mbar_wait(&kfull[t % NS], (uint32_t)((t / NS) & 1), P.err);
         tc_fence_after();
-        for (int m = 0; m < MT; ++m) {
-          scores(m, 0, m);
-          umma_commit(&sfull[m]);
-        }
-        umma_commit(&kempty[0]);
-      }
+        return in;
+      };
+      bool ok = mbar_wait(qfull, 0, P.err) && keys(0);
+      for (int m = 0; ok && m < MT; ++m) scores(m, 0);
+#pragma unroll 1
       for (int t = 0; ok && t < n_tiles; ++t) {
-        const int s = t & 1, s1 = s ^ 1;
-        const uint32_t ph = (uint32_t)((t >> 1) & 1), ph1 = (uint32_t)(((t + 1) >> 1) & 1);
-        const bool next = t + 1 < n_tiles;
-        if (MT == 1 && next) {  // the other buffer's scores run beside this tile's softmax
-          if (!(ok = mbar_wait(&kfull[s1], ph1, P.err))) break;
-          tc_fence_after();
-          scores(0, s1, s1);
-          umma_commit(&sfull[s1]);
-          umma_commit(&kempty[s1]);
+        // The next tile's scores: beside this tile's softmax into the other
+        // buffer, or else right after its weights have been used.  Either way
+        // they take columns that held weights; the products run in the order
+        // of issue, so those have been read.
+        const bool more = t + 1 < n_tiles;
+        if (C::SB == 2 && more) {
+          if (!(ok = keys(t + 1))) break;
+          scores(0, t + 1);
         }
-        if (!(ok = mbar_wait(&vfull[s], ph, P.err))) break;
+        if (!(ok = mbar_wait(&vfull[t % NS], (uint32_t)((t / NS) & 1), P.err))) break;
+        const uint32_t va = base + C::kOffV + (t % NS) * C::kKvTile;
+#pragma unroll 1
         for (int m = 0; m < MT; ++m) {
-          const int buf = MT == 2 ? m : s;
-          if (!(ok = mbar_wait(&pfull[MT == 2 ? m : 0], (uint32_t)(t & 1), P.err))) break;
+          const int i = C::SB * m + t % C::SB;
+          if (!(ok = mbar_wait(&pfull[i], (uint32_t)((t / C::SB) & 1), P.err))) break;
           tc_fence_after();
-          values(m, s, buf, t != 0);
+#pragma unroll
+          for (int k = 0; k < ROWS / 16; ++k)
+            umma_f16_ta(tmem + C::kColO + m * D, tmem + i * ROWS + 8 * k,
+                        sw128_desc_mn(va + k * 2048, C::kKvBox), kIdescO, t != 0 || k != 0);
           umma_commit(&odone[m]);
-          if (m == MT - 1) umma_commit(&vempty[s]);
-          if (MT == 2 && next) {
-            // the products run in order: the weights have been read when the
-            // scores that take their columns are written
-            if (m == 0 && !(ok = mbar_wait(&kfull[s1], ph1, P.err))) break;
-            tc_fence_after();
-            scores(m, s1, m);
-            umma_commit(&sfull[m]);
-            if (m == 1) umma_commit(&kempty[s1]);
+          if (m == MT - 1) umma_commit(&vempty[t % NS]);
+          if (C::SB == 1 && more) {
+            if (m == 0 && !(ok = keys(t + 1))) break;
+            scores(m, t + 1);
           }
         }
       }
     }
   } else {
     // ------------------------------------------------------------ softmax
+    if constexpr (D == 128) more_registers<kRegsSoft>();
     const int m = warp >> 2, quarter = warp & 3;
     const int y = m * 128 + quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
@@ -392,19 +527,19 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
     float ref = kNoRef, l = 0.f;
     bool ok = true;
     for (int t = 0; ok && t < n_tiles; ++t) {
-      const int s = t & 1, buf = MT == 2 ? m : s;
+      const int s = t % NS, i = C::SB * m + t % C::SB;
       const int j0 = lo + t * ROWS;
-      ok = mbar_wait(&vfull[s], (uint32_t)((t >> 1) & 1), P.err);
-      ok = ok && mbar_wait(&sfull[buf], (uint32_t)(MT == 2 ? t & 1 : (t >> 1) & 1), P.err);
+      const uint32_t scores = tmem + lanes + i * ROWS;  // and the weights
+      ok = mbar_wait(&vfull[s], (uint32_t)((t / NS) & 1), P.err);
+      ok = ok && mbar_wait(&sfull[i], (uint32_t)((t / C::SB) & 1), P.err);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
       const float* kap = reinterpret_cast<const float*>(sm + C::kOffScale) + s * 2 * ROWS;
       const float* rv = kap + ROWS;
       const uint32_t* valid = reinterpret_cast<const uint32_t*>(sm + C::kOffValid) + s * 4;
-      bool whole = j0 >= q_lo && j0 + ROWS <= q_hi;
-#pragma unroll
-      for (int c = 0; c < ROWS / 32; ++c) whole = whole && valid[c] == 0xffffffffu;
+      const float4 tile = *reinterpret_cast<const float4*>(sm + C::kOffEven + 16 * s);
+      const bool whole = j0 >= q_lo && j0 + ROWS <= q_hi && tile.w != 0.f;
       // places of chunk c that this query attends
       auto places = [&](int c) {
         const int a = max(q_lo - (j0 + 32 * c), 0), z = min(q_hi - (j0 + 32 * c), 32);
@@ -412,112 +547,125 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
         const uint32_t below = z == 32 ? 0xffffffffu : (1u << z) - 1u;
         return valid[c] & below & (0xffffffffu << a);
       };
-      // exponents of chunk c, without the reference
-      auto exponents = [&](int c, float (&v)[32]) {
-        tmem_ld32(tmem + lanes + buf * C::kColS + 32 * c, v);
-        tmem_wait_ld();
-        if constexpr (EXTRA) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            float x = v[i] * kap[32 * c + i];
-            if (r.softcap > 0.f) x = soft_cap(x, cap, inv_cap);
-            if (r.slopes) x = fmaf(slope, (float)(j0 + 32 * c + i + 1 - q_hi), x);
-            v[i] = x;
-          }
-        }
+      // 32 columns at a time; their weights take the columns of scores already
+      // read (half as many), so a chunk's own scores stay until it is settled
+      auto load = [&](int c, float (&x)[32]) { tmem_ld32(scores + 32 * c, x); };
+      // a score as an exponent of two, without the reference
+      auto exponent = [&](int j, float x, float k) {
+        x *= k;
+        if (EXTRA && r.softcap > 0.f) x = soft_cap(x, cap, inv_cap);
+        if (EXTRA && r.slopes) x = fmaf(slope, (float)(j0 + j + 1 - q_hi), x);
+        return x;
       };
-      uint32_t p[ROWS / 32][16];
+      uint32_t p[16];
       float lt;
-      const bool all_whole = __all_sync(0xffffffffu, whole);
-      auto pass = [&](auto masked) {
+      // Weights of chunk c into p, their sum (without the rows' scale) into lt;
+      // false when one may pass fp16: none does while 32 sum to less.
+      // A whole, even tile: w = 2^(x kappa - ref + log2 r).
+      auto weigh_even = [&](int c, const float (&x)[32]) {
         float2 sum = make_float2(0.f, 0.f);
-        float top = 0.f;
-        const float2 nref = make_float2(-ref, -ref);
+        const float shift = tile.z - ref;
+        const float2 kk = make_float2(tile.x, tile.x), sh = make_float2(shift, shift);
 #pragma unroll
-        for (int c = 0; c < ROWS / 32; ++c) {
-          float v[32];
-          exponents(c, v);
-          const uint32_t on = decltype(masked)::value ? places(c) : 0u;
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const float4 k4 = EXTRA ? make_float4(1.f, 1.f, 1.f, 1.f)
-                                    : *reinterpret_cast<const float4*>(kap + 32 * c + i);
-            const float4 r4 = *reinterpret_cast<const float4*>(rv + 32 * c + i);
-#pragma unroll
-            for (int o = 0; o < 4; o += 2) {
-              const float2 kk = o ? make_float2(k4.z, k4.w) : make_float2(k4.x, k4.y);
-              const float2 rr = o ? make_float2(r4.z, r4.w) : make_float2(r4.x, r4.y);
-              float2 x = __ffma2_rn(make_float2(v[i + o], v[i + o + 1]), kk, nref);
-              if constexpr (decltype(masked)::value) {
-                if (!(on >> (i + o) & 1)) x.x = -INFINITY;
-                if (!(on >> (i + o + 1) & 1)) x.y = -INFINITY;
-              }
-              const float2 e = make_float2(ex2(x.x), ex2(x.y));
-              sum = __fadd2_rn(sum, e);
-              float2 w = __fmul2_rn(e, rr);
-              if constexpr (decltype(masked)::value) {
-                if (!(on >> (i + o) & 1)) w.x = 0.f;  // whatever the row's norms hold
-                if (!(on >> (i + o + 1) & 1)) w.y = 0.f;
-              }
-              top = fmaxf(fmaxf(top, w.x), w.y);
-              p[c][(i + o) >> 1] = pack_h2(w.x, w.y);
-            }
-          }
+        for (int i = 0; i < 32; i += 2) {
+          float2 y;
+          if constexpr (EXTRA)
+            y = __fadd2_rn(make_float2(exponent(32 * c + i, x[i], tile.x),
+                                       exponent(32 * c + i + 1, x[i + 1], tile.x)), sh);
+          else
+            y = __ffma2_rn(make_float2(x[i], x[i + 1]), kk, sh);
+          const float2 w = (i & 6) == 2 ? ex2_poly(y) : make_float2(ex2(y.x), ex2(y.y));
+          sum = __fadd2_rn(sum, w);
+          p[i >> 1] = pack_h2(w.x, w.y);
         }
-        lt = sum.x + sum.y;
-        return !(top <= kMaxWeight && lt < 0x1p60f);
+        const float s0 = sum.x + sum.y;
+        lt = s0 * tile.y;
+        return s0 <= kMostSum && lt < 0x1p60f;
       };
-      auto weigh = [&] {
-        return all_whole ? pass(std::false_type{}) : pass(std::true_type{});
+      // Any tile: scales and places by column.
+      auto weigh_any = [&](int c, const float (&x)[32], uint32_t on) {
+        float sum = 0.f, total = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          float w[2];
+#pragma unroll
+          for (int o = 0; o < 2; ++o) {
+            const int j = 32 * c + i + o;
+            const float e = on >> (i + o) & 1 ? ex2(exponent(j, x[i + o], kap[j]) - ref) : 0.f;
+            w[o] = on >> (i + o) & 1 ? e * rv[j] : 0.f;  // whatever the row's norms hold
+            sum += e;
+            total += w[o];
+          }
+          p[i >> 1] = pack_h2(w[0], w[1]);
+        }
+        lt = sum;
+        return total <= kMostSum && sum < 0x1p60f;
       };
-      bool over = weigh();
-      if (__any_sync(0xffffffffu, over)) {
-        float top = kNoRef;
+      const bool all_whole = __all_sync(0xffffffffu, whole);
+      float v[2][32];
+      if (!EXTRA) load(0, v[0]);  // the next chunk loads while one is weighed
+      auto chunk = [&](int c, float (&x)[32], float (&next)[32]) {
+        if (EXTRA) load(c, x);  // no registers left for two
+        tmem_wait_ld();
+        tmem_pin(x);
+        if (!EXTRA && c + 1 < ROWS / 32) load(c + 1, next);
+        const uint32_t on = all_whole ? 0xffffffffu : places(c);
 #pragma unroll 1
-        for (int c = 0; c < ROWS / 32; ++c) {
-          float v[32];
-          exponents(c, v);
-          const uint32_t on = places(c);
+        for (bool again = false;; again = true) {
+          const bool fits = all_whole ? weigh_even(c, x) : weigh_any(c, x, on);
+          if (again || __all_sync(0xffffffffu, fits)) break;
+          // a weight would leave fp16: the reference moves up to this chunk's
+          // largest, what has been summed and stored so far follows
+          float top = kNoRef;
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
-            const float x = EXTRA ? v[i] : v[i] * kap[32 * c + i];
-            if (on >> i & 1) top = fmaxf(top, x + lg2(fmaxf(rv[32 * c + i], 0x1p-40f)));
+            const int j = 32 * c + i;
+            const float y = exponent(j, x[i], kap[j]) + lg2(fmaxf(rv[j], 0x1p-40f));
+            if (on >> i & 1) top = fmaxf(top, y);
           }
-        }
-        const float to = fmaxf(ref, top), f = ex2(ref - to);
-        ref = to;
-        l *= f;
-        if (t > 0) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&odone[m], (uint32_t)((t - 1) & 1), P.err));
-          if (!ok) break;
-          tc_fence_after();
+          const float to = fmaxf(ref, top), f = ex2(ref - to);
+          ref = to;
+          l *= f;
+          const uint32_t f2 = pack_h2(f, f);
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            const uint32_t at = tmem + lanes + C::kColO + m * 128 + 32 * c;
-            float v[32];
-            uint32_t u[32];
-            tmem_ld32(at, v);
+          for (int k = 0; k < c; ++k) {
+            const uint32_t at = scores + 16 * k;
+            tmem_ld16(at, p);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(v[i] * f);
-            tmem_st32(at, u);
+            for (int i = 0; i < 16; ++i)
+              asm volatile("mul.rn.f16x2 %0, %0, %1;" : "+r"(p[i]) : "r"(f2));
+            tmem_st16(at, p);
+          }
+          if (t > 0) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&odone[m], (uint32_t)((t - 1) & 1), P.err)) && ok;
+            tc_fence_after();
+#pragma unroll 1
+            for (int k = 0; k < D / 16; ++k) {
+              const uint32_t at = tmem + lanes + C::kColO + m * D + 16 * k;
+              tmem_ld16(at, p);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                asm volatile("mul.rn.f32 %0, %0, %1;" : "+r"(p[i]) : "r"(__float_as_uint(f)));
+              tmem_st16(at, p);
+            }
           }
           tmem_wait_st();
         }
-        weigh();
+        l += lt;
+        tmem_st16(scores + 16 * c, p);
+      };
+#pragma unroll 1
+      for (int c = 0; c < ROWS / 32; c += 2) {
+        chunk(c, v[0], v[1]);
+        chunk(c + 1, v[1], v[0]);
       }
-      l += lt;
-#pragma unroll
-      for (int c = 0; c < ROWS / 64; ++c) {
-        uint32_t u[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) u[i] = p[2 * c + (i >> 4)][i & 15];
-        tmem_st32(tmem + lanes + buf * C::kColS + 32 * c, u);
-      }
+      if (!ok) break;
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&pfull[m]);
+      if (lane == 0) mbar_arrive(&pfull[i]);
     }
     // ---- the sums leave through the tiles' shared memory
     if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&odone[m], (uint32_t)((n_tiles - 1) & 1), P.err));
@@ -531,24 +679,26 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         float v[32];
-        tmem_ld32(tmem + lanes + C::kColO + m * 128 + 32 * c, v);
+        tmem_ld32(tmem + lanes + C::kColO + m * D + 32 * c, v);
         tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) out[lane * (D + 1) + 32 * c + (i >> 1) + 16 * (i & 1)] = v[i];
+        for (int i = 0; i < 32; ++i) 
+          out[lane * (D + 1) + 32 * c + (i >> 1) + 16 * (i & 1)] = v[i] * (1.f / kTileScale);
       }
     }
     __syncwarp();
+    const int64_t mine = y < nq ? (query_row(y) * P.plan.parts() + blockIdx.x) * (int64_t)(D + 2) : -1;
+    if (!ok) l = 0.f;
+#pragma unroll 4
     for (int k = 0; k < 32; ++k) {
-      const int yk = m * 128 + quarter * 32 + k;
-      if (yk >= nq) break;
-      float* rec = r.workspace + (query_row(yk) * P.plan.parts() + blockIdx.x) * (int64_t)(D + 2);
+      const int64_t at = __shfl_sync(0xffffffffu, mine, k);
       const float mk = __shfl_sync(0xffffffffu, ref, k), lk = __shfl_sync(0xffffffffu, l, k);
-      if (lane == 0) {
-        rec[0] = mk;
-        rec[1] = ok ? lk : 0.f;
-      }
+      if (at < 0) break;
+      float* rec = r.workspace + at;
+      if (lane < 2) rec[lane] = lane ? lk : mk;
 #pragma unroll
-      for (int j = 0; j < W; ++j) rec[2 + 32 * j + lane] = out[k * (D + 1) + 32 * j + lane];
+      for (int j = 0; j < W; ++j)
+        rec[2 + 32 * j + lane] = ok ? out[k * (D + 1) + 32 * j + lane] : 0.f;
     }
   }
   tc_fence_before();
@@ -579,7 +729,7 @@ kh_status launch_typed(const AttnParams& P, cudaStream_t stream) {
   const dim3 grid((unsigned)P.plan.pre_chunks, (unsigned)P.r.n_kv_heads,
                   (unsigned)((nq + per - 1) / per));
   if (grid.y > 65535 || (nq + per - 1) / per > 65535) return KH_EINVAL;
-  if (launch_programmatic(paged_queries_kernel<D>, dim3(grid.z, grid.y), dim3(1024), 0, stream,
+  if (launch_programmatic(paged_queries_kernel<D>, dim3(grid.z * C::MT * 4, grid.y), dim3(256), 0, stream,
                           P) != cudaSuccess)
     return KH_ELAUNCH;
   return launch_programmatic(kern, grid, dim3(C::kThreads), C::kSmem, stream, P) == cudaSuccess
