@@ -463,7 +463,7 @@ int kh_paged_append(const kh_paged_cache* cache, const void* k, const void* v, i
  * A length outside [0, max_len] is clamped, a row whose page is outside the
  * pool is not attended; both set bit 3 of kh_device_error().
  */
-int64_t kh_paged_workspace_bytes(int64_t n_seqs, int n_q, int n_kv_heads, int head_dim,
+int64_t kh_paged_workspace_bytes(int64_t n_seqs, int n_q, int n_kv_heads, int head_dim, int dtype,
                                  int64_t max_len, int64_t prefix_len, int64_t window);
 int kh_paged_attn(const kh_paged_cache* cache, const void* q, int dtype, int64_t n_seqs, int n_q,
                   const int32_t* table, int64_t table_stride, const int32_t* lengths,

@@ -707,14 +707,15 @@ int kh_paged_append(const kh_paged_cache* cache, const void* k, const void* v, i
   return launch_paged_append(r, static_cast<cudaStream_t>(stream));
 }
 
-int64_t kh_paged_workspace_bytes(int64_t n_seqs, int n_q, int n_kv_heads, int head_dim,
+int64_t kh_paged_workspace_bytes(int64_t n_seqs, int n_q, int n_kv_heads, int head_dim, int dtype,
                                  int64_t max_len, int64_t prefix_len, int64_t window) {
+  if (dtype != KH_F32 && dtype != KH_F16 && dtype != KH_BF16) return -1;
   if (n_seqs < 0 || n_q < 1 || n_kv_heads < 1 || !valid_head_dim(head_dim) || max_len < 0 ||
       max_len > (int64_t(1) << 31) - 1 || prefix_len < 0 || prefix_len > max_len || window < 0 ||
       n_seqs * n_q > (int64_t(1) << 31) / n_kv_heads)
     return -1;
   const PagedPlan p = paged_plan(n_seqs, n_q, n_kv_heads, head_dim, max_len, prefix_len, window,
-                                 sm_count());
+                                 dtype, sm_count());
   return paged_workspace_bytes(p, n_seqs, n_q, n_kv_heads, head_dim);
 }
 
@@ -731,7 +732,7 @@ int kh_paged_attn(const kh_paged_cache* cache, const void* q, int dtype, int64_t
                              &r.kp, &r.vp);
   if (st != KH_OK) return st;
   const int64_t need = kh_paged_workspace_bytes(n_seqs, n_q, cache->n_kv_heads, cache->head_dim,
-                                                max_len, prefix_len, window);
+                                                dtype, max_len, prefix_len, window);
   if (need < 0) return KH_EINVAL;
   if (!std::isfinite(sm_scale) || !std::isfinite(softcap) || softcap < 0.f) return KH_EINVAL;
   const int64_t blocks = (max_len + cache->page_size - 1) / cache->page_size;

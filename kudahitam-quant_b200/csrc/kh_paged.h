@@ -59,15 +59,19 @@ struct PagedAttnRequest {
   float* lse;  // may be null
 };
 
-// How a call's rows are cut into work items.  Every query row has
-// `parts()` record slots: the shared prefix's chunks, then its own chunks.
+// How a call's rows are cut.  Every query row has parts() record slots: those
+// of the shared prefix, then those of its own rows.
 struct PagedPlan {
-  int pre_chunks = 0, own_chunks = 0;
-  int64_t pre_rows = 0, own_rows = 0;  // rows per chunk
-  __host__ __device__ int parts() const { return pre_chunks + own_chunks; }
+  int pre_parts = 0, own_parts = 0;  // slots
+  int64_t own_rows = 0;              // most own rows of a sequence
+  int64_t unit = 64;                 // pairs of a row and a group that a warp claims
+  // the prefix on the tensor cores: chunks of pre_rows rows, a slot each
+  int pre_chunks = 0;
+  int64_t pre_rows = 0;
+  __host__ __device__ int parts() const { return pre_parts + own_parts; }
 };
 PagedPlan paged_plan(int64_t n_seqs, int n_q, int n_kv_heads, int D, int64_t max_len,
-                     int64_t prefix_len, int64_t window, int n_sms);
+                     int64_t prefix_len, int64_t window, int dtype, int n_sms);
 int64_t paged_workspace_bytes(const PagedPlan& p, int64_t n_seqs, int n_q, int n_kv_heads, int D);
 kh_status launch_paged_attn(const PagedAttnRequest& r, cudaStream_t stream);
 

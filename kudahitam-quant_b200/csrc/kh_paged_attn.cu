@@ -17,6 +17,7 @@
 #include <cfloat>
 #include <cmath>
 #include <mutex>
+#include <type_traits>
 
 #include "kh_common.cuh"
 #include "kh_paged_attn.cuh"
@@ -26,34 +27,35 @@ namespace {
 
 // ------------------------------------------------------------------ rows
 //
-// paged_rows_kernel: the two products of a chunk on mma.sync, fed from
-// registers.  A row's bits need no shared-memory expansion: a 16-bit lane of
-// a packed word, masked to bit b, IS the fp16 number 2^(b - 24) (a
-// subnormal) or zero, exactly, so one LOP3 makes two matrix elements and
-// the factor goes into the other operand (q~ 2^(24 - b)) or into the
-// accumulator's scale.  What bit belongs to what index of the product is
-// free, as long as both operands agree:
-//   scores  A = 16 rows x 16 elements: lane (g, t) holds word t of rows
-//           pi(g) and pi(g) + 8; step i takes its bits 2 i and 2 i + 1 in
-//           both halves.  B = q~ of 8 columns.
-//   values  A = 16 elements x 16 rows: lane (g, t) holds halfword g (word g
-//           at D = 256) of rows t, t + 4, t + 8, t + 12.  B = the weights
-//           p norm' and p rnorm', which movmatrix turns from the scores'
-//           accumulator layout into the operand's.
-// With bits as 0 / 1, sum w sign = 2 sum w bit - sum w.  That difference
-// costs the values a few bits of 24, nothing next to a 16-bit result's
-// rounding; for fp32 results (EXACT) the bits are moved to the sign
-// of +-1 instead, one more shift each.
-//
-// Columns: HILO splits a query (and its weights) into two fp16 parts, the
-// second times 2^11: 22 bits from 4 queries a block of 8 columns.  Without,
-// 8 queries of 11 bits: for bf16 results of groups over 4.
+// paged_rows_kernel: both products on mma.sync, fed from registers, so that a
+// row's bits are never written out as elements.  A packed word masked to one
+// bit a byte (or halfword) IS a register of matrix elements, each 2^b or zero
+// (8-bit integers), or 2^(b - 24) or zero (fp16, subnormal): one logic
+// operation makes four elements, or two.  The factor 2^b goes into the other
+// operand or into the accumulator's scale.  What bit belongs to what index of
+// the product is free, as long as both operands agree:
+//   scores  A = 16 rows: lane (g, t) holds word t of rows pi(g) and pi(g) + 8
+//           (words 2 t, 2 t + 1 at D = 256).  B = q~, a query in two columns.
+//   values  A = 16 elements of lane g's halfword (word at D = 256), of rows
+//           t, t + 4, t + 8, t + 12 (and 16 more).  B = the weights p norm' and
+//           p rnorm', which movmatrix turns from the scores' accumulator
+//           layout into the operand's.
+// A query's (and a weight's) two columns are its high and low part:
+//   I8    (16-bit queries) 16-bit fixed point in two bytes, sums exact in 32-bit
+//         integers.  q~ keeps 2^-13 of its largest element (2^-16 for three
+//         bits of four), a weight 2^-16 of the largest of its unit, whose
+//         rounding errors average out; together under a tenth of a bf16 step.
+//         Bits count as 0 / 1: sum w sign = 2 sum w bit - sum w, exactly.
+//   else  (32-bit queries) two fp16 parts of 11 bits, the second times 2^11.
+//         There the difference would cost bits, so values move their bits
+//         to the sign of +-1, one more shift each.
+// Measured on the ragged batch (32 sequences up to 8192, 8 x 4 heads): fp16
+// parts for bf16 queries 25 instructions a row, 63 us.
 //
 // A warp runs on its own: 32-row tiles in a ring of cp.async stages, one lane
-// fetching one row (so pages may end anywhere), no block barrier until the
-// warps' sums are joined.  The reference exponent of a column moves only when
-// a weight would leave fp16's upper range (2^12), so most tiles rescale
-// nothing.
+// fetching one row (so pages may end anywhere).  The reference exponent of a
+// column moves only when a weight would leave its type's range, so most tiles
+// rescale nothing.
 constexpr int kWarps = 4;
 
 template <int D>
@@ -61,7 +63,7 @@ struct RowsCfg {
   static constexpr int W = D / 32;
   static constexpr int kStages = D == 128 ? 4 : 3;
   static constexpr int kPlane = 32 * W * 4;             // one plane of a tile
-  static constexpr int kStage = 4 * kPlane + 4 * 128 + 16;  // + norms + valid mask
+  static constexpr int kStage = 4 * kPlane + 512 + 16;  // + norms by row + valid mask
   static constexpr int kRing = kWarps * kStages * kStage;
 };
 
@@ -93,65 +95,267 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// ---- how a call's rows are split
+//
+// All (group, row) pairs of the call lie one after another: first the prefix's
+// groups (KV head, block of NQ of every sequence's query rows), then for each
+// sequence its groups (KV head, block of NQ of its own).  They are cut into
+// units of equal length, which the warps claim one by one: lengths live on the
+// device, and neither CTAs with a chunk of a fixed length nor equal ranges per
+// CTA kept the GPU busy to the end (an SM's CTAs progress unevenly, and one
+// left alone runs at a third of the SM's rate).  A unit may hold pieces of
+// several groups; a group has a record slot for every unit it touches.
+//
+// What the claims need is prepared by a launch before: where each sequence's
+// pairs start, its first row, the claim counter, and each group's queries as
+// operand fragments.
+template <int D, bool I8, int NB>
+struct Frags {  // of a group
+  static constexpr int kSteps = D / (I8 ? 32 : 16);
+  uint2 q[NB * kSteps][32];
+  float sum[NB * 4], scale[NB * 4];  // per query: sum of q~ and the exponent's scale
+};
+
+// Groups: [0, n_pre) the prefix's, then those of each sequence.
+struct Group {
+  bool pre;
+  int h, z;
+  int64_t b;  // sequence whose table is read
+};
+__device__ __forceinline__ Group group_of(const AttnParams& P, int64_t i) {
+  Group g;
+  const int64_t n_pre = (int64_t)P.r.n_kv_heads * P.pre_blocks;
+  g.pre = i < n_pre;
+  const int blocks = g.pre ? P.pre_blocks : P.own_blocks;
+  const int64_t per = (int64_t)P.r.n_kv_heads * blocks, x = g.pre ? i : i - n_pre;
+  g.b = g.pre ? 0 : x / per;
+  const int hz = (int)(x - g.b * per);
+  g.h = hz / blocks;
+  g.z = hz - g.h * blocks;
+  return g;
+}
+
+__device__ __forceinline__ void mma16832(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {  // u8 x s8
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16832u(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                          uint32_t a3, uint32_t b0, uint32_t b1) {  // u8 x u8
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+constexpr int64_t kFragBytes = 4352;  // of a group's Frags, at most
+
 constexpr float kPart = 2048.f;      // second fp16 parts are stored times 2^11
 
-template <int D, bool HILO, bool EXACT, int NB>
-__global__ void __launch_bounds__(32 * kWarps, D == 128 ? (NB == 1 ? 4 : 3) : 3)
+// Block 0: starts, first rows, the counter.  The others: a group each.
+template <int D, bool I8, int NB>
+__global__ void __launch_bounds__(128) paged_prepare_kernel(const __grid_constant__ AttnParams P) {
+  using F = Frags<D, I8, NB>;
+  constexpr int W = D / 32, KS = F::kSteps, NQ = NB * 4;
+  const PagedAttnRequest& r = P.r;
+  __shared__ float qs[NQ][D];
+  __shared__ int64_t part[4];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  grid_dependency_wait();
+  grid_dependents_launch();
+  if (blockIdx.x == 0) {
+    if (threadIdx.x == 0) *P.next_unit = 0u;
+    int64_t base = 0;
+    for (int64_t b0 = 0; b0 < r.n_seqs; b0 += 128) {
+      const int64_t b = b0 + threadIdx.x;
+      int64_t n = 0;
+      if (b < r.n_seqs) {
+        const int64_t len = length_of(P, b), first = own_first(P, b, len);
+        n = max((int64_t)0, len - first);
+        P.first_row[b] = (int32_t)min(first, (int64_t)0x7fffffff);
+      }
+      int64_t upto = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += x;
+      }
+      __syncthreads();
+      if (lane == 31) part[warp] = upto;
+      __syncthreads();
+      int64_t before = base;
+      for (int w = 0; w < 4; ++w) {
+        if (w < warp) before += part[w];
+        base += part[w];
+      }
+      if (b < r.n_seqs) P.starts[b] = before + upto - n;
+    }
+    if (threadIdx.x == 0) P.starts[r.n_seqs] = base;
+    return;
+  }
+  const int64_t gi = blockIdx.x - 1;
+  const Group grp = group_of(P, gi);
+  const int64_t y0 = (int64_t)grp.z * NQ;
+  const int nq = (int)min((int64_t)NQ, (grp.pre ? r.n_seqs * r.n_q : (int64_t)r.n_q) - y0);
+  F* out = reinterpret_cast<F*>(P.frags) + gi;
+  for (int y = warp; y < NQ; y += 4) {
+    float x[W], mx = 0.f, sum = 0.f;
+    const int64_t i = y0 + y, b = grp.pre ? i / r.n_q : grp.b;
+    const int64_t row = (b * r.n_kv_heads + grp.h) * r.n_q + (grp.pre ? i - b * r.n_q : i);
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      const float v = y < nq ? ld_any(r.q, r.dtype, row * D + 32 * j + lane) : 0.f;
+      x[j] = (r.dk_neg[j] >> lane) & 1 ? -v : v;
+    }
+    fwht_lanes<W>(x, lane);
+#pragma unroll
+    for (int j = 0; j < W; ++j) mx = fmaxf(mx, fabsf(x[j]));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    float up;
+    if constexpr (I8) {
+      // whole numbers up to 32639 = 127 x 256 + 127 where a bit counts once
+      up = mx > 0.f && mx < INFINITY ? 32639.f / mx : 1.f;
+    } else {
+      // the largest element into [2^-10, 2^-9): q~ 2^(24 - b) stays inside fp16
+      int e = 0;
+      if (mx > 0.f && mx < INFINITY) frexpf(mx, &e);
+      up = ldexpf(1.f, max(-120, min(-9 - e, 120)));
+    }
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      float v = x[j] * up;
+      if constexpr (I8) {  // element 32 j + lane counts 2^(bit & 3) times
+        const float times = (float)(1 << (lane & 3));
+        v = rintf(v / times) * times;
+      }
+      sum += v;
+      qs[y][32 * j + lane] = v;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) {
+      out->sum[y] = sum;
+      out->scale[y] = P.log_scale / up;  // sm_scale log2(e) / sqrt(D) and the scale above
+    }
+  }
+  __syncthreads();
+  // column g: query g / 2, its high part (even) or low part
+  const int g = lane >> 2, t = lane & 3;
+  for (int k = warp; k < NB * KS; k += 4) {
+    const int i = k % KS, y = k / KS * 4 + (g >> 1);
+    if constexpr (I8) {
+      // k = 4 t + j is bit 2 i of byte j of the lane's word, k = 4 t + 16 + j bit 2 i + 1
+      const int word = D == 128 ? t : 2 * t + (i >> 2);
+      uint32_t f[2] = {0, 0};
+#pragma unroll
+      for (int o = 0; o < 2; ++o)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int bit = 2 * (i & 3) + o;
+          const int v = (int)qs[y][32 * word + 8 * j + bit] >> (bit & 3);
+          const int low = ((v + 128) & 255) - 128;
+          f[o] |= (uint32_t)((g & 1 ? low : (v - low) >> 8) & 255) << (8 * j);
+        }
+      out->q[k][lane] = make_uint2(f[0], f[1]);
+    } else {
+      // k = 2 t, 2 t + 1 are bit 2 i of the two halves of the lane's word,
+      // k = 2 t + 8, 2 t + 9 bit 2 i + 1
+      auto value = [&](int e, int bit) {
+        const float v = qs[y][e] * (float)(1 << (24 - (bit & 7)));
+        const float hi_part = round_h(v);
+        return g & 1 ? (v - hi_part) * kPart : hi_part;
+      };
+      const int e = (D == 128 ? 32 * t : 64 * t + 32 * (i >> 3)), bit = 2 * (i & 7);
+      out->q[k][lane] =
+          make_uint2(pack_h2(value(e + bit, bit), value(e + 16 + bit, bit)),
+                     pack_h2(value(e + bit + 1, bit + 1), value(e + 17 + bit, bit + 1)));
+    }
+  }
+}
+
+// Sequence b with starts[b] * per <= x < starts[b + 1] * per: a warp looks at
+// 32 places at once.
+__device__ __forceinline__ int64_t find_sequence(const AttnParams& P, int64_t x, int64_t per,
+                                                 int lane) {
+  int64_t lo = 0, n = P.r.n_seqs;  // it is among [lo, lo + n)
+  while (n > 1) {
+    const int64_t step = (n + 31) / 32, i = min(lo + (lane + 1) * step, lo + n);
+    const int below = __popc(__ballot_sync(0xffffffffu, i < lo + n && P.starts[i] * per <= x));
+    lo += below * step;
+    n = min(step, n - below * step);
+  }
+  return lo;
+}
+
+// CTAs an SM that the registers are bounded for.
+template <int D, bool I8, int NB>
+constexpr int rows_ctas() {
+  return D == 256 || NB == 2 ? 3 : I8 ? 5 : 4;
+}
+
+template <int D, bool I8, bool EXTRA, int NB>
+__global__ void __launch_bounds__(32 * kWarps, rows_ctas<D, I8, NB>())
     paged_rows_kernel(const __grid_constant__ AttnParams P) {
   using C = RowsCfg<D>;
+  using F = Frags<D, I8, NB>;
+  using Acc = std::conditional_t<I8, int, float>;
   constexpr int W = C::W;
   constexpr int kStages = C::kStages;
-  constexpr int KS = D / 16;            // steps of the score product
+  constexpr int KS = F::kSteps;         // steps of the score product
   constexpr int MT = D / 16;            // element tiles of the value product
-  constexpr int QB = HILO ? 4 : 8;      // queries a column block
-  constexpr int QT = HILO ? 1 : 2;      // of them this thread's
-  constexpr int NQ = NB * QB;
+  constexpr int NQ = NB * 4;
+  constexpr bool kRegs = NB * KS <= 8;  // query fragments in registers
   const PagedAttnRequest& r = P.r;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float qs[NQ][D];
-  __shared__ float q_sum[NQ], q_scale[NQ];
-  __shared__ float rec_m[kWarps][NQ], rec_l[kWarps][NQ];
-  __shared__ uint2 q_frag[(D == 128 && NB == 1) ? 1 : NB * KS][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
-
-  // ---- the work item
-  const int h = blockIdx.y % r.n_kv_heads;
-  const int64_t item = blockIdx.y / r.n_kv_heads;  // 0: the prefix when there is one
-  const bool has_pre = P.plan.pre_chunks > 0 && !P.pre_tensor;
-  const bool pre = has_pre && item == 0;
-  const int64_t b = pre ? 0 : item - has_pre;
-  const int chunk = blockIdx.x;
-  if (chunk >= (pre ? P.plan.pre_chunks : P.plan.own_chunks)) return;
-  const int64_t n_rows = pre ? r.n_seqs * r.n_q : r.n_q;
-  const int64_t y0 = (int64_t)blockIdx.z * NQ;
-  if (y0 >= n_rows) return;
-  const int nq = (int)min((int64_t)NQ, n_rows - y0);
+  const int hq_all = r.n_kv_heads * r.n_q;
+  uint8_t* ring = smem + warp * kStages * C::kStage;
+  uint2(*q_frag)[32] = reinterpret_cast<uint2(*)[32]>(smem + C::kRing + warp * NB * KS * 256);
   // After a prefix launch this grid may run beside it: that one signals its
   // dependents once all earlier work is done, and nothing here reads its
   // records.  The wait then comes at the end, so that this grid's completion
   // implies the prefix's.
   if (!P.pre_tensor) grid_dependency_wait();
-  int lo, hi;
-  if (pre) {
-    lo = (int)(chunk * P.plan.pre_rows);
-    hi = (int)min(lo + P.plan.pre_rows, r.prefix_len);
-  } else {
-    const int64_t len = length_of(P, b);
-    const int64_t first = own_first(P, b, len) + chunk * P.plan.own_rows;
-    if (first >= len) {
-      if (P.pre_tensor) grid_dependency_wait();
-      return;
-    }
-    lo = (int)first;
-    hi = (int)min(first + P.plan.own_rows, len);
-  }
-  const int hq_all = r.n_kv_heads * r.n_q;
+  const int64_t n_pre = (int64_t)r.n_kv_heads * P.pre_blocks * r.prefix_len;
+  const int64_t per = (int64_t)r.n_kv_heads * P.own_blocks;
+  const int64_t total = n_pre + P.starts[r.n_seqs] * per;
+
+#pragma unroll 1
+  for (;;) {
+  uint32_t unit = 0;
+  if (lane == 0) unit = atomicAdd(P.next_unit, 1u);
+  unit = __shfl_sync(0xffffffffu, unit, 0);
+  int64_t at = (int64_t)unit * P.unit;
+  if (at >= total) break;
+  const int64_t end = min(at + P.unit, total);
+#pragma unroll 1
+  while (at < end) {
+  // ---- the piece: rows [lo, hi) of a sequence (or of the prefix, for every
+  // sequence's queries) for query rows y0 .. y0 + nq of KV head h
+  const bool pre = at < n_pre;
+  const int64_t b = pre ? 0 : find_sequence(P, at - n_pre, per, lane);
+  const int64_t start = pre ? 0 : n_pre + P.starts[b] * per;
+  const int64_t rows = pre ? r.prefix_len : P.starts[b + 1] - P.starts[b];
+  const int hz = (int)((at - start) / rows);
+  const int64_t begin = start + hz * rows;
+  const int lo = (pre ? 0 : P.first_row[b]) + (int)(at - begin);
+  const int hi = lo + (int)min(rows - (at - begin), end - at);
+  at += hi - lo;
+  const int blocks = pre ? P.pre_blocks : P.own_blocks;
+  const int h = hz / blocks;
+  const int64_t y0 = (int64_t)(hz - h * blocks) * NQ;
+  const int nq = (int)min((int64_t)NQ, (pre ? r.n_seqs * r.n_q : (int64_t)r.n_q) - y0);
+  const int part = (int)(unit - begin / P.unit) + (pre ? 0 : P.plan.pre_parts);
+  const F* frags = reinterpret_cast<const F*>(P.frags) +
+                              (pre ? hz : r.n_kv_heads * P.pre_blocks + b * per + hz);
   auto seq_of = [&](int y) { return pre ? (y0 + y) / r.n_q : b; };
   auto head_of = [&](int y) { return h * r.n_q + (int)(pre ? (y0 + y) % r.n_q : y0 + y); };
 
-  // ---- tiles: lane = row
-  uint8_t* ring = smem + warp * kStages * C::kStage;
+  // ---- tiles of 32 rows: lane = row
   const int n_tiles = (hi - lo + 31) >> 5;
   const int32_t* tab = r.table + b * r.table_stride;
   auto page_of = [&](int tile) {
@@ -176,139 +380,93 @@ __global__ void __launch_bounds__(32 * kWarps, D == 128 ? (NB == 1 ? 4 : 3) : 3)
         cp_async16(d + 2 * C::kPlane, r.vp.code + row * W + 4 * v, on);
         cp_async16(d + 3 * C::kPlane, r.vp.res + row * W + 4 * v, on);
       }
-      const uint32_t n = s + 4 * C::kPlane + lane * 4;
+      const uint32_t n = s + 4 * C::kPlane + lane * 16;
       cp_async4(n, r.kp.norms + row, on);
-      cp_async4(n + 128, r.kp.rnorms + row, on);
-      cp_async4(n + 256, r.vp.norms + row, on);
-      cp_async4(n + 384, r.vp.rnorms + row, on);
+      cp_async4(n + 4, r.kp.rnorms + row, on);
+      cp_async4(n + 8, r.vp.norms + row, on);
+      cp_async4(n + 12, r.vp.rnorms + row, on);
       const uint32_t mask = __ballot_sync(0xffffffffu, on);
       if (lane == 0) *reinterpret_cast<uint32_t*>(st + 4 * C::kPlane + 512) = mask;
     }
     cp_commit();
   };
 #pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) issue(warp + s * kWarps, s, page_of(warp + s * kWarps));
-  int next_page = page_of(warp + (kStages - 1) * kWarps);
+  for (int s = 0; s < kStages - 1; ++s) issue(s, s, page_of(s));
+  int next_page = page_of(kStages - 1);
 
-  // ---- queries: q~ times a power of two that brings its largest element to
-  // [2^-10, 2^-9), so that q~ 2^(24 - b) stays inside fp16 for b = 0 .. 7
-  for (int y = warp; y < NQ; y += kWarps) {
-    float x[W], mx = 0.f, sum = 0.f;
+  uint2 qf[kRegs ? NB * KS : 1];
 #pragma unroll
-    for (int j = 0; j < W; ++j) {
-      float v = 0.f;
-      if (y < nq) v = ld_any(r.q, r.dtype, (seq_of(y) * hq_all + head_of(y)) * D + 32 * j + lane);
-      x[j] = (r.dk_neg[j] >> lane) & 1 ? -v : v;
-    }
-    fwht_lanes<W>(x, lane);
-#pragma unroll
-    for (int j = 0; j < W; ++j) mx = fmaxf(mx, fabsf(x[j]));
-#pragma unroll
-    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    int e = 0;
-    if (mx > 0.f && mx < INFINITY) frexpf(mx, &e);
-    const float up = ldexpf(1.f, min(-9 - e, 120));
-#pragma unroll
-    for (int j = 0; j < W; ++j) {
-      float v = x[j] * up;
-      if (!HILO) v = round_h(v * 16777216.f) * (1.f / 16777216.f);
-      sum += v;
-      qs[y][32 * j + lane] = v;
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) {
-      q_sum[y] = sum;
-      q_scale[y] = P.log_scale / up;  // sm_scale log2(e) / sqrt(D) and the power of two
-    }
+  for (int i = 0; i < NB * KS; ++i) {
+    const uint2 f = frags->q[i][lane];
+    if constexpr (kRegs) qf[i] = f;
+    else q_frag[i][lane] = f;
   }
-  __syncthreads();
-  // B fragments: column g; k = 2 t, 2 t + 1 are bit 2 i of the two halves of
-  // the lane's word, k = 2 t + 8, 2 t + 9 bit 2 i + 1
-  uint2 qf[(D == 128 && NB == 1) ? KS : 1];
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    const int y = nb * QB + (HILO ? g >> 1 : g);
-    auto part = [&](int e, int bit) {
-      const float v = qs[y][e] * (float)(1 << (24 - (bit & 7)));
-      const float hi_part = round_h(v);
-      return HILO && (g & 1) ? (v - hi_part) * kPart : hi_part;
-    };
-#pragma unroll
-    for (int i = 0; i < KS; ++i) {
-      const int e = (D == 128 ? 32 * t : 64 * t + 32 * (i >> 3)), bit = 2 * (i & 7);
-      if ((D != 128 || NB != 1) && (i & 3) != warp) continue;
-      const uint2 f = make_uint2(pack_h2(part(e + bit, bit), part(e + 16 + bit, bit)),
-                                 pack_h2(part(e + bit + 1, bit + 1), part(e + 17 + bit, bit + 1)));
-      if constexpr (D == 128 && NB == 1) qf[i] = f;
-      else q_frag[nb * KS + i][lane] = f;
-    }
-  }
-  if (D != 128 || NB != 1) __syncthreads();
 
-  // ---- per-thread constants of its queries
+  // ---- constants of this thread's query of each block
   //   t2 = norm (a1 M1 + b1) + rnorm (a2 M2 + b2), M the masked sums
   const float ch = 0.5f * (r.c1 - r.c0), cm = 0.5f * (r.c1 + r.c0);
   const float inv_sd = P.inv_sd;
-  float a1[NB][QT], b1[NB][QT], a2[NB][QT], b2[NB][QT], slope[NB][QT];
-  int q_lo[NB][QT], q_hi[NB][QT];
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-    for (int qq = 0; qq < QT; ++qq) {
-      const int y = nb * QB + (HILO ? t : 2 * t + qq);
-      const float k = q_scale[y], sum = q_sum[y] * k;
-      a1[nb][qq] = 2.f * ch * k;
-      b1[nb][qq] = (cm - ch) * sum;
-      a2[nb][qq] = 2.f * inv_sd * k;
-      b2[nb][qq] = -inv_sd * sum;
-      slope[nb][qq] = 0.f;
-      q_lo[nb][qq] = 0;
-      q_hi[nb][qq] = 0x7fffffff;
-      if (y < nq) {
-        if (pre || r.slopes) {
-          const int64_t len = length_of(P, seq_of(y));
-          q_hi[nb][qq] = (int)len;
-          if (pre) q_lo[nb][qq] = (int)min(first_of(P, seq_of(y), len), (int64_t)0x7fffffff);
-        }
-        if (r.slopes) slope[nb][qq] = r.slopes[head_of(y)] * kLog2e;
-      }
-    }
-  const float va = ch * inv_sd, vb = 0.7978845608028654f * inv_sd * inv_sd;
-  const float cap = r.softcap * kLog2e, inv_cap = r.softcap > 0.f ? 1.f / cap : 0.f;
-
-  float ref[NB][QT], l[NB][QT], w1s[NB][QT], w2s[NB][QT], acc[NB][MT][4];
+  float a1[NB], b1[NB], a2[NB], b2[NB], slope[NB];
+  int q_lo[NB], q_hi[NB];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-    for (int qq = 0; qq < QT; ++qq) {
-      ref[nb][qq] = kNoRef;
-      l[nb][qq] = w1s[nb][qq] = w2s[nb][qq] = 0.f;
+    const int y = nb * 4 + t;
+    const float k = frags->scale[y], sum = frags->sum[y] * k;
+    a1[nb] = 2.f * ch * k;
+    b1[nb] = (cm - ch) * sum;
+    a2[nb] = 2.f * inv_sd * k;
+    b2[nb] = -inv_sd * sum;
+    slope[nb] = 0.f;
+    q_lo[nb] = 0;
+    q_hi[nb] = 0x7fffffff;
+    if (y < nq) {
+      if (pre || (EXTRA && r.slopes)) {
+        const int64_t len = length_of(P, seq_of(y));
+        q_hi[nb] = (int)len;
+        if (pre) q_lo[nb] = (int)min(first_of(P, seq_of(y), len), (int64_t)0x7fffffff);
+      }
+      if (EXTRA && r.slopes) slope[nb] = r.slopes[head_of(y)] * kLog2e;
     }
+  }
+  constexpr float kUnitWeight = I8 ? 32768.f : 1.f;  // how weight 1 is stored
+  constexpr float kMost = I8 ? 65535.f : kMaxWeight;
+  const float va = ch * inv_sd * kUnitWeight;
+  const float vb = 0.7978845608028654f * inv_sd * inv_sd * kUnitWeight;
+  const float cap = r.softcap * kLog2e, inv_cap = r.softcap > 0.f ? 1.f / cap : 0.f;
+
+  // w1s, w2s: sums of weights; in i1, i2 those since the reference last moved
+  float ref[NB], l[NB], w1s[NB], w2s[NB];
+  uint32_t i1[NB], i2[NB];
+  Acc acc[NB][MT][4];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    ref[nb] = kNoRef;
+    l[nb] = w1s[nb] = w2s[nb] = 0.f;
+    i1[nb] = i2[nb] = 0u;
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) acc[nb][i][k] = 0.f;
+      for (int k = 0; k < 4; ++k) acc[nb][i][k] = 0;
   }
   const int pg = (g >> 1) + 4 * (g & 1);  // pi(g)
 
 #pragma unroll 1
-  for (int n = 0, tile = warp; tile < n_tiles; ++n, tile += kWarps) {
+  for (int tile = 0; tile < n_tiles; ++tile) {
     cp_wait<kStages - 2>();
     __syncwarp();
-    const uint8_t* st = ring + (n % kStages) * C::kStage;
-    const float* nrm = reinterpret_cast<const float*>(st + 4 * C::kPlane);
+    const uint8_t* st = ring + (tile % kStages) * C::kStage;
+    const float4* nrm = reinterpret_cast<const float4*>(st + 4 * C::kPlane);
     const uint32_t valid = *reinterpret_cast<const uint32_t*>(st + 4 * C::kPlane + 512);
     const int j0 = lo + tile * 32;
 
-    // scores of the tile's two 16-row halves
-    float s1[2][NB][4], s2[2][NB][4];
+    // scores of the tile's two 16-row halves, both planes
+    Acc s1[2][NB][4], s2[2][NB][4];
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) s1[hf][nb][k] = s2[hf][nb][k] = 0.f;
+        for (int k = 0; k < 4; ++k) s1[hf][nb][k] = s2[hf][nb][k] = 0;
 #pragma unroll
     for (int v = 0; v < W / 4; ++v) {
       uint32_t w[2][2][2];  // half, plane, row
@@ -320,251 +478,293 @@ __global__ void __launch_bounds__(32 * kWarps, D == 128 ? (NB == 1 ? 4 : 3) : 3)
           for (int rr = 0; rr < 2; ++rr)
             w[hf][p][rr] = reinterpret_cast<const uint32_t*>(
                 st + p * C::kPlane)[(16 * hf + pg + 8 * rr) * W + (D == 128 ? t : 2 * t + v)];
+      constexpr int kPer = KS / (W / 4);  // steps of a word
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (i == 4)
+      for (int i = 0; i < kPer; ++i) {
+        if (i == kPer / 2)
 #pragma unroll
-          for (int k = 0; k < 8; ++k) w[k >> 2][(k >> 1) & 1][k & 1] >>= 8;
-        const uint32_t m0 = 0x00010001u << ((2 * i) & 7), m1 = m0 << 1;
+          for (int k = 0; k < 8; ++k) w[k >> 2][(k >> 1) & 1][k & 1] >>= kPer;
+        const uint32_t m0 = (I8 ? 0x01010101u : 0x00010001u) << ((2 * i) % kPer), m1 = m0 << 1;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
           uint2 f;
-          if constexpr (D == 128 && NB == 1) f = qf[i];
-          else f = q_frag[nb * KS + v * 8 + i][lane];
+          if constexpr (kRegs) f = qf[nb * KS + v * kPer + i];
+          else f = q_frag[nb * KS + v * kPer + i][lane];
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            mma16816(s1[hf][nb], w[hf][0][0] & m0, w[hf][0][1] & m0, w[hf][0][0] & m1,
-                     w[hf][0][1] & m1, f.x, f.y);
-            mma16816(s2[hf][nb], w[hf][1][0] & m0, w[hf][1][1] & m0, w[hf][1][0] & m1,
-                     w[hf][1][1] & m1, f.x, f.y);
-          }
+          for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+              auto& c = p == 0 ? s1[hf][nb] : s2[hf][nb];
+              const uint32_t x0 = w[hf][p][0], x1 = w[hf][p][1];
+              if constexpr (I8) mma16832(c, x0 & m0, x1 & m0, x0 & m1, x1 & m1, f.x, f.y);
+              else mma16816(c, x0 & m0, x1 & m0, x0 & m1, x1 & m1, f.x, f.y);
+            }
         }
       }
     }
 
-    // exponents and weights
+    // exponents
     bool full = valid == 0xffffffffu;
     if (pre) {
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int qq = 0; qq < QT; ++qq)
-          full = full && j0 >= q_lo[nb][qq] && j0 + 32 <= q_hi[nb][qq];
+      for (int nb = 0; nb < NB; ++nb) full = full && j0 >= q_lo[nb] && j0 + 32 <= q_hi[nb];
       full = __all_sync(0xffffffffu, full);
     }
-    float tt[2][2][NB][QT], ra[2][2], rb[2][2];
-    float w1[2][2][NB][QT], w2[2][2][NB][QT];
-    bool over = false;
+    float tt[2][2][NB], ra[2][2], rb[2][2];
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
       for (int rr = 0; rr < 2; ++rr) {
         const int row = 16 * hf + pg + 8 * rr;
-        const float kn = nrm[row], krn = nrm[32 + row];
-        ra[hf][rr] = nrm[64 + row] * va;
-        rb[hf][rr] = nrm[96 + row] * vb;
+        const float4 n = nrm[row];
+        ra[hf][rr] = n.z * va;
+        rb[hf][rr] = n.w * vb;
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-          for (int qq = 0; qq < QT; ++qq) {
-            const float m1 = HILO ? fmaf(s1[hf][nb][2 * rr + 1], 1.f / kPart, s1[hf][nb][2 * rr])
-                                  : s1[hf][nb][2 * rr + qq];
-            const float m2 = HILO ? fmaf(s2[hf][nb][2 * rr + 1], 1.f / kPart, s2[hf][nb][2 * rr])
-                                  : s2[hf][nb][2 * rr + qq];
-            float x = kn * fmaf(a1[nb][qq], m1, b1[nb][qq]);
-            x = fmaf(krn, fmaf(a2[nb][qq], m2, b2[nb][qq]), x);
-            if (r.softcap > 0.f) x = soft_cap(x, cap, inv_cap);
-            if (r.slopes) x = fmaf(slope[nb][qq], (float)(j0 + row + 1 - q_hi[nb][qq]), x);
-            if (!full) {
-              const int j = j0 + row;
-              const bool on = ((valid >> row) & 1) && j >= q_lo[nb][qq] && j < q_hi[nb][qq];
-              x = on ? x : -INFINITY;
-            }
-            tt[hf][rr][nb][qq] = x;
-            const float e = ex2(x - ref[nb][qq]);
-            w1[hf][rr][nb][qq] = e * ra[hf][rr];
-            w2[hf][rr][nb][qq] = e * rb[hf][rr];
-            // not <=: a NaN of 0 * infinity has to go the long way too
-            over |= !(fmaxf(fmaxf(w1[hf][rr][nb][qq], w2[hf][rr][nb][qq]), e * 0x1p-40f) <=
-                      kMaxWeight);
+        for (int nb = 0; nb < NB; ++nb) {
+          float m1, m2;
+          if constexpr (I8) {
+            m1 = (float)(s1[hf][nb][2 * rr] * 256 + s1[hf][nb][2 * rr + 1]);
+            m2 = (float)(s2[hf][nb][2 * rr] * 256 + s2[hf][nb][2 * rr + 1]);
+          } else {
+            m1 = fmaf(s1[hf][nb][2 * rr + 1], 1.f / kPart, s1[hf][nb][2 * rr]);
+            m2 = fmaf(s2[hf][nb][2 * rr + 1], 1.f / kPart, s2[hf][nb][2 * rr]);
           }
+          float x = n.x * fmaf(a1[nb], m1, b1[nb]);
+          x = fmaf(n.y, fmaf(a2[nb], m2, b2[nb]), x);
+          if (EXTRA && r.softcap > 0.f) x = soft_cap(x, cap, inv_cap);
+          if (EXTRA && r.slopes) x = fmaf(slope[nb], (float)(j0 + row + 1 - q_hi[nb]), x);
+          tt[hf][rr][nb] = x;
+        }
       }
-    if (__any_sync(0xffffffffu, over)) {
+    if (!full) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          const int row = 16 * (k >> 1) + pg + 8 * (k & 1), j = j0 + row;
+          const bool on = ((valid >> row) & 1) && j >= q_lo[nb] && j < q_hi[nb];
+          if (!on) tt[k >> 1][k & 1][nb] = -INFINITY;
+        }
+    }
+    // weights: e = 2^(t2 - ref); a row's larger weight decides whether they fit
+    float ee[2][2][NB];
+#pragma unroll 1
+    for (bool again = false;; again = true) {
+      float top = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          const float e = ex2(tt[k >> 1][k & 1][nb] - ref[nb]);
+          ee[k >> 1][k & 1][nb] = e;
+          const float most =
+              fmaxf(fmaxf(ra[k >> 1][k & 1], rb[k >> 1][k & 1]), kUnitWeight * 0x1p-40f);
+          // nothing attended: 0 times whatever the row's norms hold
+          top = fmaxf(top, e == 0.f ? 0.f : e * most);
+        }
+      if (again || !__any_sync(0xffffffffu, !(top <= kMost))) break;
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
-        float f[QT];
+        float mx = kNoRef;
 #pragma unroll
-        for (int qq = 0; qq < QT; ++qq) {
-          float mx = kNoRef;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float x = tt[k >> 1][k & 1][nb][qq];
-            const float a = lg2(fmaxf(fmaxf(ra[k >> 1][k & 1], rb[k >> 1][k & 1]), 0x1p-40f));
-            if (x > -INFINITY) mx = fmaxf(mx, x + a);
-          }
-#pragma unroll
-          for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-          const float to = fmaxf(ref[nb][qq], mx);
-          f[qq] = ex2(ref[nb][qq] - to);
-          ref[nb][qq] = to;
-          l[nb][qq] *= f[qq];
-          w1s[nb][qq] *= f[qq];
-          w2s[nb][qq] *= f[qq];
+        for (int k = 0; k < 4; ++k) {
+          const float most =
+              fmaxf(fmaxf(ra[k >> 1][k & 1], rb[k >> 1][k & 1]), kUnitWeight * 0x1p-40f);
+          const float x = tt[k >> 1][k & 1][nb];
+          if (x > -INFINITY) mx = fmaxf(mx, x + lg2(most * (1.f / kUnitWeight)));
         }
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        if (mx == INFINITY) l[nb] = NAN;  // an infinite norm has no average
+        // whole exponents: integer sums move by shifts
+        const float to = fmaxf(ref[nb], I8 ? ceilf(mx) : mx), f = ex2(ref[nb] - to);
+        const int shift = (int)fminf(to - ref[nb], 31.f);
+        if constexpr (I8) {
+          w1s[nb] += (float)i1[nb];
+          w2s[nb] += (float)i2[nb];
+          i1[nb] = i2[nb] = 0u;
+        }
+        ref[nb] = to;
+        l[nb] *= f;
+        w1s[nb] *= f;
+        w2s[nb] *= f;
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) acc[nb][i][k] *= f[HILO ? 0 : k & 1];
+          for (int k = 0; k < 4; ++k) {
+            if constexpr (I8) acc[nb][i][k] = (acc[nb][i][k] + (int)((1u << shift) >> 1)) >> shift;
+            else acc[nb][i][k] *= f;
+          }
       }
     }
     uint32_t p1[2][NB][2], p2[2][NB][2];
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
-      for (int rr = 0; rr < 2; ++rr)
+      for (int nb = 0; nb < NB; ++nb) {
+        uint32_t u1[2], u2[2];
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          float u1[2], u2[2];
-#pragma unroll
-          for (int qq = 0; qq < QT; ++qq) {
-            const float x = tt[hf][rr][nb][qq];
-            const float e = ex2(x - ref[nb][qq]);
-            l[nb][qq] += e;
-            float v1 = e * ra[hf][rr], v2 = e * rb[hf][rr];
-            if (!full && x == -INFINITY) v1 = v2 = 0.f;  // whatever the row's norms hold
-            if constexpr (HILO) {
-              w1s[nb][0] += v1;
-              w2s[nb][0] += v2;
-              u1[0] = v1;
-              u2[0] = v2;
-              u1[1] = (v1 - round_h(v1)) * kPart;
-              u2[1] = (v2 - round_h(v2)) * kPart;
-            } else {
-              u1[qq] = round_h(v1);
-              u2[qq] = round_h(v2);
-              w1s[nb][qq] += u1[qq];
-              w2s[nb][qq] += u2[qq];
-            }
+        for (int rr = 0; rr < 2; ++rr) {
+          const float e = ee[hf][rr][nb];
+          l[nb] += e;
+          float x1, x2;
+          if constexpr (I8) {
+            // 2^23 + w: the low bits are w as a whole number
+            x1 = fmaf(e, ra[hf][rr], 8388608.f);
+            x2 = fmaf(e, rb[hf][rr], 8388608.f);
+          } else {
+            x1 = e * ra[hf][rr];
+            x2 = e * rb[hf][rr];
           }
-          p1[hf][nb][rr] = transpose8(pack_h2(u1[0], u1[1]));
-          p2[hf][nb][rr] = transpose8(pack_h2(u2[0], u2[1]));
+          if (!full && tt[hf][rr][nb] == -INFINITY) x1 = x2 = I8 ? 8388608.f : 0.f;
+          if constexpr (I8) {
+            u1[rr] = __float_as_uint(x1);
+            u2[rr] = __float_as_uint(x2);
+          } else {
+            w1s[nb] += x1;
+            w2s[nb] += x2;
+            p1[hf][nb][rr] = transpose8(pack_h2(x1, (x1 - round_h(x1)) * kPart));
+            p2[hf][nb][rr] = transpose8(pack_h2(x2, (x2 - round_h(x2)) * kPart));
+          }
         }
+        if constexpr (I8) {
+          i1[nb] += u1[0] + u1[1];
+          i2[nb] += u2[0] + u2[1];
+          // columns 2 t, 2 t + 1: high and low bytes, of both rows
+          p1[hf][nb][0] = transpose8(__byte_perm(u1[0], u1[1], 0x4051));
+          p2[hf][nb][0] = transpose8(__byte_perm(u2[0], u2[1], 0x4051));
+        }
+      }
 
     // values
+    if constexpr (I8) {
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf)
+      for (int nb = 0; nb < NB; ++nb) {  // without the four exponent fields of 2^23
+        i1[nb] -= 4u * 0x4B000000u;
+        i2[nb] -= 4u * 0x4B000000u;
+      }
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
-        const uint32_t* pl = reinterpret_cast<const uint32_t*>(st + (2 + p) * C::kPlane) +
-                             (16 * hf + t) * W + (D == 128 ? g >> 1 : g);
-        const uint32_t r0 = pl[0], r1 = pl[4 * W], r2 = pl[8 * W], r3 = pl[12 * W];
+        uint32_t x[2][W / 4], y[2][W / 4];  // even and odd bytes of four rows, by half
 #pragma unroll
-        for (int v = 0; v < W / 4; ++v) {
-          const uint32_t sel = (D == 128 ? (g & 1) : v) ? 0x7632u : 0x5410u;
-          uint32_t x0 = __byte_perm(r0, r1, sel), x1 = __byte_perm(r2, r3, sel);
+        for (int hf = 0; hf < 2; ++hf) {
+          const uint32_t* pl = reinterpret_cast<const uint32_t*>(st + (2 + p) * C::kPlane) +
+                               (16 * hf + t) * W + (D == 128 ? g >> 1 : g);
+          const uint32_t r0 = pl[0], r1 = pl[8 * W], r2 = pl[4 * W], r3 = pl[12 * W];
+#pragma unroll
+          for (int v = 0; v < W / 4; ++v) {
+            const uint32_t sel = (D == 128 ? (g & 1) : v) ? 0x7362u : 0x5140u;
+            const uint32_t a = __byte_perm(r0, r1, sel), b = __byte_perm(r2, r3, sel);
+            x[hf][v] = __byte_perm(a, b, 0x5410);
+            y[hf][v] = __byte_perm(a, b, 0x7632);
+          }
+        }
+#pragma unroll
+        for (int v = 0; v < W / 4; ++v)
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            uint32_t a[4];
-            if constexpr (EXACT) {
-              const int s0 = 15 - 2 * i, s1x = 14 - 2 * i;
-              a[0] = ((x0 << s0) & 0x80008000u) ^ 0xBC00BC00u;
-              a[1] = ((x0 << s1x) & 0x80008000u) ^ 0xBC00BC00u;
-              a[2] = ((x1 << s0) & 0x80008000u) ^ 0xBC00BC00u;
-              a[3] = ((x1 << s1x) & 0x80008000u) ^ 0xBC00BC00u;
-            } else {
-              if (i == 4) {
-                x0 >>= 8;
-                x1 >>= 8;
-              }
-              const uint32_t m0 = 0x00010001u << ((2 * i) & 7), m1 = m0 << 1;
-              a[0] = x0 & m0;
-              a[1] = x0 & m1;
-              a[2] = x1 & m0;
-              a[3] = x1 & m1;
-            }
+            const uint32_t m = 0x01010101u << i;
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-              const uint32_t(&f)[2] = p == 0 ? p1[hf][nb] : p2[hf][nb];
-              mma16816(acc[nb][8 * v + i], a[0], a[1], a[2], a[3], f[0], f[1]);
+              const auto& f = p == 0 ? p1 : p2;
+              mma16832u(acc[nb][8 * v + i], x[0][v] & m, y[0][v] & m, x[1][v] & m, y[1][v] & m,
+                        f[0][nb][0], f[1][nb][0]);
+            }
+          }
+      }
+    } else {
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const uint32_t* pl = reinterpret_cast<const uint32_t*>(st + (2 + p) * C::kPlane) +
+                               (16 * hf + t) * W + (D == 128 ? g >> 1 : g);
+          const uint32_t r0 = pl[0], r1 = pl[4 * W], r2 = pl[8 * W], r3 = pl[12 * W];
+#pragma unroll
+          for (int v = 0; v < W / 4; ++v) {
+            const uint32_t sel = (D == 128 ? (g & 1) : v) ? 0x7632u : 0x5410u;
+            const uint32_t x0 = __byte_perm(r0, r1, sel), x1 = __byte_perm(r2, r3, sel);
+            auto sign = [](uint32_t x, int bit) {
+              return ((x << (15 - bit)) & 0x80008000u) ^ 0xBC00BC00u;
+            };
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const uint32_t a0 = sign(x0, 2 * i), b0 = sign(x0, 2 * i + 1);
+              const uint32_t a1 = sign(x1, 2 * i), b1 = sign(x1, 2 * i + 1);
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb) {
+                const uint32_t(&f)[2] = p == 0 ? p1[hf][nb] : p2[hf][nb];
+                mma16816(acc[nb][8 * v + i], a0, b0, a1, b1, f[0], f[1]);
+              }
             }
           }
         }
-      }
+    }
     __syncwarp();
-    issue(tile + (kStages - 1) * kWarps, (n + kStages - 1) % kStages, next_page);
-    next_page = page_of(tile + kStages * kWarps);
+    issue(tile + kStages - 1, (tile + kStages - 1) % kStages, next_page);
+    next_page = page_of(tile + kStages);
   }
-  if (!P.pre_tensor) grid_dependents_launch();
   cp_wait<0>();
-  __syncthreads();
+  __syncwarp();
 
-  // ---- the warps' sums: element e of query y of warp w in out[w][y][e]
-  float* out = reinterpret_cast<float*>(smem);
+  // ---- the record: 16 consecutive elements a lane (32 at D = 256)
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
+    if constexpr (I8) {
+      w1s[nb] += (float)i1[nb];
+      w2s[nb] += (float)i2[nb];
+    }
 #pragma unroll
-    for (int qq = 0; qq < QT; ++qq) {
-#pragma unroll
-      for (int o = 4; o < 32; o <<= 1) {
-        l[nb][qq] += __shfl_xor_sync(0xffffffffu, l[nb][qq], o);
-        w1s[nb][qq] += __shfl_xor_sync(0xffffffffu, w1s[nb][qq], o);
-        w2s[nb][qq] += __shfl_xor_sync(0xffffffffu, w2s[nb][qq], o);
-      }
-      const int y = nb * QB + (HILO ? t : 2 * t + qq);
-      if (g == 0) {
-        rec_m[warp][y] = ref[nb][qq];
-        rec_l[warp][y] = l[nb][qq];
-      }
-      const float base = (EXACT ? 0.f : -w1s[nb][qq] - w2s[nb][qq]) + (cm / ch) * w1s[nb][qq];
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int bit = 2 * (i & 7) + k;
-          const int e = (D == 128 ? 16 * g : 32 * g + 16 * (i >> 3)) + bit;
-          float v = HILO ? fmaf(acc[nb][i][2 * k + 1], 1.f / kPart, acc[nb][i][2 * k])
-                         : acc[nb][i][2 * k + qq];
-          if (!EXACT) v *= (float)(1 << (25 - (bit & 7)));  // 2 sum w bit
-          out[(warp * NQ + y) * D + e] = v + base;
+    for (int o = 4; o < 32; o <<= 1) {
+      l[nb] += __shfl_xor_sync(0xffffffffu, l[nb], o);
+      w1s[nb] += __shfl_xor_sync(0xffffffffu, w1s[nb], o);
+      w2s[nb] += __shfl_xor_sync(0xffffffffu, w2s[nb], o);
+    }
+    const int y = nb * 4 + t;
+    if (y < nq) {
+      float* rec = r.workspace +
+                   ((seq_of(y) * hq_all + head_of(y)) * P.plan.parts() + part) * (int64_t)(D + 2);
+      if (g == 0) *reinterpret_cast<float2*>(rec) = make_float2(ref[nb], l[nb]);
+      const float base = (I8 ? -w1s[nb] - w2s[nb] : 0.f) + (cm / ch) * w1s[nb];
+      // element i of part k of the lane's 16 (or 32)
+      auto element = [&](int i, int k) {
+        if constexpr (I8) {  // 2 sum w bit, bit i counting 2^(i & 7) times
+          const float x = fmaf((float)acc[nb][i][2 * k], 256.f, (float)acc[nb][i][2 * k + 1]);
+          return (fmaf(x, 2.f / (float)(1 << (i & 7)), base)) * (1.f / kUnitWeight);
+        } else {
+          return fmaf(acc[nb][i][2 * k + 1], 1.f / kPart, acc[nb][i][2 * k]) + base;
         }
+      };
+      const int e0 = 2 + (D == 128 ? 16 : 32) * g;
+#pragma unroll
+      for (int i = 0; i < MT; i += 2) {
+        if constexpr (I8) {  // tile i: elements i and 8 + i of each 16
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            *reinterpret_cast<float2*>(rec + e0 + 16 * (i >> 3) + 8 * k + (i & 7)) =
+                make_float2(element(i, k), element(i + 1, k));
+        } else {  // tile i: elements 2 i and 2 i + 1
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            *reinterpret_cast<float2*>(rec + e0 + 2 * (i + k)) =
+                make_float2(element(i + k, 0), element(i + k, 1));
+        }
+      }
     }
   }
-  __syncthreads();
-  const int part = pre ? chunk : P.plan.pre_chunks + chunk;
-  for (int y = warp; y < nq; y += kWarps) {
-    float mx = rec_m[0][y];
-#pragma unroll
-    for (int w = 1; w < kWarps; ++w) mx = fmaxf(mx, rec_m[w][y]);
-    float f[kWarps], sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      f[w] = ex2(rec_m[w][y] - mx);
-      sum = fmaf(rec_l[w][y], f[w], sum);
-    }
-    float* rec = r.workspace +
-                 ((seq_of(y) * hq_all + head_of(y)) * P.plan.parts() + part) * (int64_t)(D + 2);
-    if (lane == 0) {
-      rec[0] = mx;
-      rec[1] = sum;
-    }
-#pragma unroll
-    for (int j = 0; j < W; ++j) {
-      float v = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) v = fmaf(out[(w * NQ + y) * D + 32 * j + lane], f[w], v);
-      rec[2 + 32 * j + lane] = v;
-    }
+  }
   }
   if (P.pre_tensor) grid_dependency_wait();
+  else grid_dependents_launch();
 }
 
 // A block per query row: its records merged, back from the transformed
 // domain, divided by l, in the query's type.  What it takes is the time of a
-// few dependent loads, so each warp takes every fourth record and loads eight
+// few dependent loads, so each warp takes every fourth record and loads four
 // of them at once.
 template <int D>
 __global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constant__ AttnParams P) {
-  constexpr int J = D / 32, U = 8;
+  constexpr int J = D / 32, U = 4;
   const PagedAttnRequest& r = P.r;
   __shared__ float sums[4][D], tops[4], ls[4];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -573,43 +773,72 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constan
   const uint32_t b = row / hq_all;
   const float* rec = r.workspace + (int64_t)row * P.plan.parts() * (D + 2);
   grid_dependency_wait();
-  const int64_t len = length_of(P, b);
-  const int64_t own = max((int64_t)0, len - own_first(P, b, len));
-  const int n = P.plan.pre_chunks +
-                (P.plan.own_rows ? (int)min((own + P.plan.own_rows - 1) / P.plan.own_rows,
-                                            (int64_t)P.plan.own_chunks)
-                                 : 0);
+  // slots of the units that the row's groups touch
+  const int hq = (int)(row - b * hq_all), h = hq / r.n_q, y = hq - h * r.n_q;
+  auto slots = [&](int64_t begin, int64_t rows) {
+    return rows > 0 ? (int)((begin + rows - 1) / P.unit - begin / P.unit) + 1 : 0;
+  };
+  const int n_pre = P.pre_tensor ? P.plan.pre_chunks
+                    : P.pre_blocks
+                        ? slots((int64_t)(h * P.pre_blocks + (b * r.n_q + y) / P.block) * r.prefix_len,
+                                r.prefix_len)
+                        : 0;
+  int n = n_pre;
+  if (P.plan.own_parts) {
+    const int64_t first = P.starts[b], rows = P.starts[b + 1] - first;
+    n += slots(((int64_t)P.pre_blocks * r.prefix_len + first * P.own_blocks) * r.n_kv_heads +
+                   (int64_t)(h * P.own_blocks + y / P.block) * rows,
+               rows);
+  }
   float mx = -INFINITY, l = 0.f, a[J];
 #pragma unroll
   for (int j = 0; j < J; ++j) a[j] = 0.f;
-  for (int p0 = warp; p0 < n; p0 += 4 * U) {
-    float mp[U], lp[U], v[U][J], top = mx;
+  // 32 slots at a time: a lane each for m and l (0 where nothing was attended)
+  for (int p0 = 0; p0 < n; p0 += 32) {
+    const int i = p0 + lane, slot = i < n_pre ? i : i - n_pre + P.plan.pre_parts;
+    const float* mine = rec + (int64_t)(i < n ? slot : 0) * (D + 2);
+    const float mp = mine[0], lp = i < n ? mine[1] : 0.f;
+    uint32_t live = __ballot_sync(0xffffffffu, lp != 0.f);
+    if (!live) continue;
+    float top = lp != 0.f ? mp : -INFINITY;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int p = min(p0 + 4 * u, n - 1);
-      const float* q = rec + (int64_t)p * (D + 2);
-      mp[u] = q[0];
-      lp[u] = p0 + 4 * u < n ? q[1] : 0.f;
-#pragma unroll
-      for (int j = 0; j < J; ++j) v[u][j] = q[2 + 32 * j + lane];
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (lp[u] != 0.f) top = fmaxf(top, mp[u]);  // else nothing was attended there
-    if (top == -INFINITY) continue;
-    const float old = ex2(mx - top);
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    top = fmaxf(top, mx);
+    const float old = mx == -INFINITY ? 0.f : ex2(mx - top), f = lp != 0.f ? ex2(mp - top) : 0.f;
+    mx = top;
     l *= old;
 #pragma unroll
     for (int j = 0; j < J; ++j) a[j] *= old;
+    // this warp's share of them: every fourth
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (lp[u] != 0.f) {
-        const float f = ex2(mp[u] - top);
-        l = fmaf(lp[u], f, l);
+    for (int k = 0; k < 4; ++k)
+      if (k < warp) live &= live - 1;
+    while (live) {
+      int q[U];
+      float v[U][J];
 #pragma unroll
-        for (int j = 0; j < J; ++j) a[j] = fmaf(v[u][j], f, a[j]);
+      for (int u = 0; u < U; ++u) {
+        q[u] = live ? __ffs(live) - 1 : -1;
+        live &= live - 1;
+        live &= live - 1;
+        live &= live - 1;
+        live &= live - 1;
+        const int at = __shfl_sync(0xffffffffu, slot, max(q[u], 0));
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+          v[u][j] = q[u] >= 0 ? rec[(int64_t)at * (D + 2) + 2 + 32 * j + lane] : 0.f;
       }
-    mx = top;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float fu = __shfl_sync(0xffffffffu, f, max(q[u], 0));
+        const float lu = __shfl_sync(0xffffffffu, lp, max(q[u], 0));
+        if (q[u] >= 0) {
+          l = fmaf(lu, fu, l);
+#pragma unroll
+          for (int j = 0; j < J; ++j) a[j] = fmaf(v[u][j], fu, a[j]);
+        }
+      }
+    }
   }
 #pragma unroll
   for (int j = 0; j < J; ++j) sums[warp][32 * j + lane] = a[j];
@@ -641,27 +870,52 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constan
   if (r.lse && lane == 0) r.lse[row] = l == 0.f ? -INFINITY : (top + log2f(l)) * kLn2;
 }
 
-template <int D, bool HILO, bool EXACT, int NB>
-kh_status launch_rows(const AttnParams& P, cudaStream_t stream) {
+template <int D, bool I8, bool EXTRA, int NB>
+kh_status launch_rows(AttnParams P, cudaStream_t stream) {
   const PagedAttnRequest& r = P.r;
-  constexpr int NQ = NB * (HILO ? 4 : 8);
+  constexpr int NQ = NB * 4, KS = Frags<D, I8, NB>::kSteps;
   using C = RowsCfg<D>;
-  auto kern = paged_rows_kernel<D, HILO, EXACT, NB>;
-  static_assert(kWarps * NQ * D * 4 <= C::kRing, "the warps' sums take the ring's place");
+  auto kern = paged_rows_kernel<D, I8, EXTRA, NB>;
+  constexpr int kSmem = C::kRing + (NB * KS <= 8 ? 0 : kWarps * NB * KS * 256);
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return KH_ECUDA;
   static std::once_flag once[64];
+  static int ctas[64];  // that fit an SM
   std::call_once(once[dev & 63], [&] {
-    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kRing);
+    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas[dev & 63], kern, 32 * kWarps, kSmem) !=
+        cudaSuccess)
+      ctas[dev & 63] = 0;
   });
-  const bool pre = P.plan.pre_chunks > 0 && !P.pre_tensor;
-  const int64_t gy = (r.n_seqs + pre) * r.n_kv_heads;
-  const int64_t nq = pre ? r.n_seqs * r.n_q : r.n_q;
-  const int64_t gz = (nq + NQ - 1) / NQ;
-  if (gy > 65535 || gz > 65535) return KH_EINVAL;
-  const dim3 grid((unsigned)std::max(pre ? P.plan.pre_chunks : 0, P.plan.own_chunks),
-                  (unsigned)gy, (unsigned)gz);
-  return launch_programmatic(kern, grid, dim3(32 * kWarps), C::kRing, stream, P) == cudaSuccess
+  P.block = NQ;
+  P.own_blocks = P.plan.own_parts > 0 ? (r.n_q + NQ - 1) / NQ : 0;
+  P.pre_blocks =
+      P.plan.pre_parts > 0 && !P.pre_tensor ? (int)((r.n_seqs * r.n_q + NQ - 1) / NQ) : 0;
+  const int64_t groups = (int64_t)r.n_kv_heads * (P.pre_blocks + r.n_seqs * P.own_blocks);
+  const int64_t pairs = (int64_t)r.n_kv_heads * (P.pre_blocks * r.prefix_len +
+                                                 r.n_seqs * P.own_blocks * P.plan.own_rows);
+  if (groups > 0x7ffffff0ll || pairs / P.unit > 0x7ffffff0ll) return KH_EINVAL;
+  static_assert(sizeof(Frags<D, I8, NB>) <= kFragBytes, "workspace of the fragments");
+  if (P.plan.parts() > 0 &&
+      launch_programmatic(paged_prepare_kernel<D, I8, NB>, dim3((unsigned)(groups + 1)),
+                          dim3(128), 0, stream, P) != cudaSuccess)
+    return KH_ELAUNCH;
+  if (P.pre_tensor) {
+    const kh_status st = launch_paged_prefix(P, stream);
+    if (st != KH_OK) return st;
+  }
+  if (pairs > 0) {
+    const int64_t units = (pairs + P.unit - 1) / P.unit;
+    const int64_t grid = std::min<int64_t>((int64_t)std::max(1, ctas[dev & 63]) * sm_count(),
+                                           (units + kWarps - 1) / kWarps);
+    if (launch_programmatic(kern, dim3((unsigned)grid), dim3(32 * kWarps), kSmem, stream, P) !=
+        cudaSuccess)
+      return KH_ELAUNCH;
+  }
+  const int64_t rows = r.n_seqs * r.n_kv_heads * r.n_q;
+  if (rows > 0x7fffffffll) return KH_EINVAL;
+  return launch_programmatic(paged_combine_kernel<D>, dim3((unsigned)rows), dim3(128), 0, stream,
+                             P) == cudaSuccess
              ? KH_OK
              : KH_ELAUNCH;
 }
@@ -669,28 +923,21 @@ kh_status launch_rows(const AttnParams& P, cudaStream_t stream) {
 template <int D>
 kh_status launch_dim(const AttnParams& P, cudaStream_t stream) {
   const PagedAttnRequest& r = P.r;
-  const int64_t rows = r.n_seqs * r.n_kv_heads * r.n_q;
-  if (P.plan.pre_chunks > 0 && P.pre_tensor) {
-    const kh_status st = launch_paged_prefix(P, stream);
-    if (st != KH_OK) return st;
-  }
-  if (P.plan.own_chunks > 0 || (P.plan.pre_chunks > 0 && !P.pre_tensor)) {
-    const int64_t nq = P.plan.pre_chunks > 0 && !P.pre_tensor ? r.n_seqs * r.n_q : r.n_q;
-    kh_status st;
-    if (r.dtype == KH_F32)
-      st = nq > 4 && D == 128 ? launch_rows<D, true, true, D == 128 ? 2 : 1>(P, stream)
-                              : launch_rows<D, true, true, 1>(P, stream);
-    else if (nq <= 4 || r.dtype == KH_F16)
-      st = nq > 4 && D == 128 ? launch_rows<D, true, false, D == 128 ? 2 : 1>(P, stream)
-                              : launch_rows<D, true, false, 1>(P, stream);
-    else
-      st = nq > 8 && D == 128 ? launch_rows<D, false, false, D == 128 ? 2 : 1>(P, stream)
-                              : launch_rows<D, false, false, 1>(P, stream);
-    if (st != KH_OK) return st;
-  }
-  if (launch_programmatic(paged_combine_kernel<D>, dim3((unsigned)rows), dim3(128), 0,
-                          stream, P) != cudaSuccess)
-    return KH_ELAUNCH;
+  const int64_t nq = P.plan.pre_parts > 0 && !P.pre_tensor ? r.n_seqs * r.n_q : r.n_q;
+  constexpr int kTwo = D == 128 ? 2 : 1;  // column blocks a pass, where there are queries for two
+  // 32-bit queries need more than 16-bit parts, and so do units so long that
+  // a 32-bit integer could not hold a column's sum (255 x 128 a row)
+  const bool i8 = r.dtype != KH_F32 && P.unit <= 32768;
+  const bool extra = r.softcap > 0.f || r.slopes;
+  auto go = [&](auto i8c, auto extrac) {
+    return nq > 4 ? launch_rows<D, decltype(i8c)::value, decltype(extrac)::value, kTwo>(P, stream)
+                  : launch_rows<D, decltype(i8c)::value, decltype(extrac)::value, 1>(P, stream);
+  };
+  const kh_status st = i8 ? (extra ? go(std::true_type{}, std::true_type{})
+                                   : go(std::true_type{}, std::false_type{}))
+                          : (extra ? go(std::false_type{}, std::true_type{})
+                                   : go(std::false_type{}, std::false_type{}));
+  if (st != KH_OK) return st;
   return cudaGetLastError() == cudaSuccess ? KH_OK : KH_ELAUNCH;
 }
 
@@ -699,66 +946,86 @@ kh_status launch_dim(const AttnParams& P, cudaStream_t stream) {
 // From how many query rows a KV head's prefix is worth 128-row products.
 constexpr int64_t kPrefixTensorRows = 33;
 
-// The workspace: the records, then (16-byte aligned) the transformed queries
-// of a tensor-core prefix.
-int64_t paged_records_bytes(const PagedPlan& p, int64_t rows, int D) {
-  return (rows * p.parts() * (int64_t)(D + 2) * 4 + 15) / 16 * 16;
+// The workspace: the records; then, each 16-byte aligned, the sequences'
+// starts and first rows, the claim counter, the queries' fragments (blocks of
+// 4 queries at least, so n_q / 4 of them at most) and, of a tensor-core
+// prefix, its transformed queries.
+struct Layout {
+  int64_t starts, first, next, frags, queries, bytes;
+};
+Layout layout_of(const PagedPlan& p, int64_t n_seqs, int n_q, int n_kv_heads, int D) {
+  auto up = [](int64_t x) { return (x + 15) / 16 * 16; };
+  const int64_t nq = n_seqs * n_q, blocks = (n_q + 3) / 4;
+  Layout l;
+  l.starts = up(nq * n_kv_heads * p.parts() * (int64_t)(D + 2) * 4);
+  l.first = l.starts + up((n_seqs + 1) * 8);
+  l.next = l.first + up(n_seqs * 4);
+  l.frags = l.next + 16;
+  int64_t groups = p.own_parts > 0 ? n_seqs * blocks : 0;
+  if (p.pre_parts > 0) groups += (nq + 3) / 4;
+  l.queries = l.frags + groups * n_kv_heads * kFragBytes;
+  l.bytes = l.queries;
+  if (p.pre_chunks > 0) l.bytes += paged_queries_bytes(nq, n_kv_heads, D);
+  return l;
 }
 int64_t paged_workspace_bytes(const PagedPlan& p, int64_t n_seqs, int n_q, int n_kv_heads, int D) {
-  const int64_t nq = n_seqs * n_q;
-  int64_t n = paged_records_bytes(p, nq * n_kv_heads, D);
-  if (p.pre_chunks > 0 && nq >= kPrefixTensorRows) n += paged_queries_bytes(nq, n_kv_heads, D);
-  return n;
+  return p.parts() > 0 ? layout_of(p, n_seqs, n_q, n_kv_heads, D).bytes : 0;
 }
 
 PagedPlan paged_plan(int64_t n_seqs, int n_q, int n_kv_heads, int D, int64_t max_len,
-                     int64_t prefix_len, int64_t window, int n_sms) {
+                     int64_t prefix_len, int64_t window, int dtype, int n_sms) {
   PagedPlan p;
-  // Two rounds of the CTAs that fit (4 an SM), so that uneven sequences even
-  // out, but at least a tile for each warp of a CTA and at most 16.
-  const int64_t qb = (n_q + 3) / 4;
-  auto chunk_of = [&](int64_t rows) {
-    const int64_t even = (rows / (8 * (int64_t)n_sms) + 127) / 128 * 128;
-    return std::max<int64_t>(128, std::min<int64_t>(2048, even));
-  };
-  const int64_t pre = std::min(prefix_len, max_len);
+  const int64_t rows = n_seqs * n_q * n_kv_heads, record = (D + 2) * 4;
+  const int64_t pre = std::min(prefix_len, max_len), nq = n_seqs * n_q;
   int64_t own = max_len - pre;
   if (window > 0) own = std::min(own, window);
-  if (pre > 0) {
-    const int64_t nq = n_seqs * n_q;
-    if (nq >= kPrefixTensorRows) {
-      // one round of CTAs, one an SM, in whole tiles
-      const int64_t per = D == 128 ? 256 : 128, tile = D == 128 ? 128 : 64;
-      const int64_t ctas = std::max<int64_t>(1, n_sms / (n_kv_heads * ((nq + per - 1) / per)));
-      p.pre_rows = ((pre + ctas - 1) / ctas + tile - 1) / tile * tile;
-    } else {
-      p.pre_rows = chunk_of(pre * n_kv_heads * ((nq + 7) / 8));
-    }
+  // the prefix's chunks on the tensor cores: one round of CTAs, one an SM, in
+  // whole tiles
+  if (pre > 0 && nq >= kPrefixTensorRows && dtype == KH_BF16) {
+    const int64_t each = D == 128 ? 256 : 128, tile = D == 128 ? 128 : 64;
+    const int64_t ctas = std::max<int64_t>(1, n_sms / (n_kv_heads * ((nq + each - 1) / each)));
+    p.pre_rows = ((pre + ctas - 1) / ctas + tile - 1) / tile * tile;
     p.pre_chunks = (int)((pre + p.pre_rows - 1) / p.pre_rows);
   }
-  if (own > 0) {
-    p.own_rows = chunk_of(n_seqs * n_kv_heads * qb * own);
-    p.own_chunks = (int)((own + p.own_rows - 1) / p.own_rows);
-  }
+  // Units: six for each of the 16 warps of an SM where the longest sequences
+  // give that many, so that the last ones end together; not under two tiles
+  // (a unit's fixed cost is about one tile's) nor over 64, and not so short
+  // that the records take over 64 MB (at least 6 slots a row).
+  const int64_t blocks = (n_q + 3) / 4;
+  const int64_t pairs = n_kv_heads * (n_seqs * blocks * own + (p.pre_chunks ? 0 : (nq + 3) / 4 * pre));
+  const int64_t room =
+      rows > 0 ? std::max<int64_t>(6, (int64_t(64) << 20) / (rows * record)) - 4 : 2;
+  int64_t unit = std::max<int64_t>(64, std::min<int64_t>(2048, pairs / (96 * (int64_t)n_sms)));
+  unit = std::max(unit, (own + (p.pre_chunks ? 0 : pre) + room - 1) / room);
+  p.unit = (unit + 31) / 32 * 32;
+  // a group touches at most this many units
+  if (pre > 0) p.pre_parts = p.pre_chunks ? p.pre_chunks : (int)(pre / p.unit + 2);
+  if (own > 0) p.own_parts = (int)(own / p.unit + 2);
+  p.own_rows = own;
   return p;
 }
 
 kh_status launch_paged_attn(const PagedAttnRequest& r, cudaStream_t stream) {
-  AttnParams P;
+  AttnParams P{};
   P.r = r;
   P.plan = paged_plan(r.n_seqs, r.n_q, r.n_kv_heads, r.D, r.max_len, r.prefix_len, r.window,
-                      sm_count());
+                      r.dtype, sm_count());
   const double sd = std::sqrt((double)r.D);
   P.log_scale = (float)(r.sm_scale * 1.4426950408889634 / sd);
   P.inv_sd = (float)(1.0 / sd);
   int bits = 0;
   while ((int64_t(1) << bits) < r.page_size) ++bits;
-  P.pre_tensor = P.plan.pre_chunks > 0 && r.dtype == KH_BF16 && r.c0 == -r.c1 &&
-                 r.n_seqs * r.n_q >= kPrefixTensorRows;
-  P.queries = reinterpret_cast<uint16_t*>(reinterpret_cast<uint8_t*>(r.workspace) +
-                                          paged_records_bytes(P.plan, r.n_seqs * r.n_q * r.n_kv_heads, r.D));
   P.div_shift = 31 + bits;
   P.div_mul = ((uint64_t(1) << P.div_shift) + r.page_size - 1) / r.page_size;
+  P.pre_tensor = P.plan.pre_chunks > 0;
+  P.unit = P.plan.unit;
+  const Layout l = layout_of(P.plan, r.n_seqs, r.n_q, r.n_kv_heads, r.D);
+  uint8_t* ws = reinterpret_cast<uint8_t*>(r.workspace);
+  P.starts = reinterpret_cast<int64_t*>(ws + l.starts);
+  P.first_row = reinterpret_cast<int32_t*>(ws + l.first);
+  P.next_unit = reinterpret_cast<uint32_t*>(ws + l.next);
+  P.frags = ws + l.frags;
+  P.queries = reinterpret_cast<uint16_t*>(ws + l.queries);
   P.err = device_error_ptr();
   return r.D == 128 ? launch_dim<128>(P, stream) : launch_dim<256>(P, stream);
 }

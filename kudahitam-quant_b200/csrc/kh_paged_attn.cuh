@@ -18,6 +18,13 @@ struct AttnParams {
   // shift = 31 + ceil(log2 page_size) (the error j (mul page_size - 2^shift) / 2^shift stays under 1)
   uint64_t div_mul;
   int div_shift;
+  // units and groups of the rows kernel (kh_paged_attn.cu)
+  int64_t unit;
+  int block, own_blocks, pre_blocks;  // queries of a block; blocks of a KV head
+  int64_t* starts;
+  int32_t* first_row;
+  uint32_t* next_unit;
+  void* frags;
   int pre_tensor;  // the prefix has its own launches (launch_paged_prefix)
   uint16_t* queries;  // workspace of those: q~ in fp16, tile by tile
   uint32_t* err;

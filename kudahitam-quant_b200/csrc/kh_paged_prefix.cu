@@ -306,13 +306,14 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
       }
       return x;
     };
-    // +-a +-b for the thread's words: the bits masked to b = 0 .. 7 are fp16
-    // numbers 2^(b - 24), exact factors of 2 a 2^(24 - b); -a - b is added.
+    // The thread's words decoded: the bits masked to b = 0 .. 7 are fp16
+    // numbers 2^(b - 24), exact factors of 2 a 2^(24 - b); what both planes'
+    // zeros stand for is added.
     // A logic operation and a multiply-add for two elements of a plane, where
     // moving bits to the sign took a shift and a logic operation, both on the
     // pipe that the softmax's conversions need.
     auto write = [&](uint8_t* tile, const uint32_t(&code)[WT], const uint32_t(&res)[WT], float a,
-                     float b) {
+                     float b, float least) {
       uint32_t fa[8], fb[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
@@ -320,7 +321,7 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
         fa[k] = pack_h2(a * up, a * up);
         fb[k] = pack_h2(b * up, b * up);
       }
-      const uint32_t low = pack_h2(-a - b, -a - b);
+      const uint32_t low = pack_h2(least, least);
 #pragma unroll
       for (int w = 0; w < WT; ++w) {
         const int word = part * WT + w;
@@ -342,13 +343,15 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
               make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
       }
     };
-    // A row's larger constant: what it is divided by, so that any two norms fit
+    // The larger of a row's two constants, a times a level and b: what it is
+    // divided by, so that any two norms fit
     // fp16.  Norms that are not finite give a row of zeros and leave through
     // the scale, which masked places do not take.
+    const float c_most = fmaxf(fabsf(r.c0), fabsf(r.c1)), c_half = 0.5f * (r.c1 - r.c0);
     auto largest = [&](float& a, float& b) {
-      const float m = fmaxf(fabsf(a), fabsf(b));
+      const float m = fmaxf(fabsf(a) * c_most, fabsf(b));
       if (!(m > 1e-35f && m < 1e35f) || a != a || b != b) {
-        const bool none = fabsf(a) <= 1e-35f && fabsf(b) <= 1e-35f;
+        const bool none = m <= 1e-35f && a == a && b == b;
         a = b = 0.f;
         return none ? 0.f : NAN;
       }
@@ -368,8 +371,8 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
       const Row x = ahead[t & 1];
       ahead[t & 1] = fetch(t + 2, page);
       page = page_of(t + 3);
-      float ka = x.kn * r.c1, kb = x.krn * inv_sd;
-      float va = x.vn * r.c1 * inv_sd, vb = x.vrn * (0.7978845608028654f * inv_sd * inv_sd);
+      float ka = x.kn, kb = x.krn * inv_sd;
+      float va = x.vn * inv_sd, vb = x.vrn * (0.7978845608028654f * inv_sd * inv_sd);
       float kappa = largest(ka, kb), rv = largest(va, vb);
       // Where the tile's rows are all there and their scales lie within 2^10 of
       // one another, one power of two serves them all: fp16 still gives every
@@ -418,7 +421,7 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
       va *= vi * kTileScale;
       vb *= vi * kTileScale;
       if (!__all_sync(0xffffffffu, mbar_wait(&kempty[s], ph ^ 1u, P.err))) break;
-      write(sm + C::kOffK + s * C::kKvTile, x.kc, x.kr, ka, kb);
+      write(sm + C::kOffK + s * C::kKvTile, x.kc, x.kr, ka * c_half, kb, ka * r.c0 - kb);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&kfull[s]);
@@ -429,7 +432,7 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
         down = 1.f / *reinterpret_cast<const float*>(group + MT * C::kQTile);
       }
       if (!__all_sync(0xffffffffu, mbar_wait(&vempty[s], ph ^ 1u, P.err))) break;
-      write(sm + C::kOffV + s * C::kKvTile, x.vc, x.vr, va, vb);
+      write(sm + C::kOffV + s * C::kKvTile, x.vc, x.vr, va * c_half, vb, va * r.c0 - vb);
       if (part == 0) {
         float* sc = reinterpret_cast<float*>(sm + C::kOffScale) + s * 2 * ROWS;
         sc[row] = kappa * (down / kTileScale);

@@ -687,8 +687,8 @@ std::tuple<Tensor, Tensor> paged_attention(
   const float* ch = host_c(c);
   const float *dkh = host_f32(dk, D, "dk"), *dvh = host_f32(dv, D, "dv");
   c10::cuda::CUDAGuard guard(dev);
-  const int64_t need = kh_paged_workspace_bytes(B, n_q, (int)heads, (int)D, max_len, prefix_len,
-                                                window);
+  const int64_t need = kh_paged_workspace_bytes(B, n_q, (int)heads, (int)D, dt, max_len,
+                                                prefix_len, window);
   TORCH_CHECK(need >= 0, "unsupported paged attention sizes");
   Tensor ws = at::empty({std::max<int64_t>(need / 4, 4)}, q.options().dtype(at::kFloat));
   Tensor out = at::empty({B, Hq, D}, q.options());

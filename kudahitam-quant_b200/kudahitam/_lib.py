@@ -70,7 +70,7 @@ SIGNATURES = {
                                      _vp]),
     "kh_paged_append": (_c_i, [_vp, _vp, _vp, _c_i, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _vp,
                                _vp, _vp, _vp, _c_i64, _c_i, _c_i, _vp, _vp, _vp, _c_i, _vp]),
-    "kh_paged_workspace_bytes": (_c_i64, [_c_i64, _c_i, _c_i, _c_i, _c_i64, _c_i64, _c_i64]),
+    "kh_paged_workspace_bytes": (_c_i64, [_c_i64, _c_i, _c_i, _c_i, _c_i, _c_i64, _c_i64, _c_i64]),
     "kh_paged_attn": (_c_i, [_vp, _vp, _c_i, _c_i64, _c_i, _vp, _c_i64, _vp, _vp, _c_i64, _c_i64,
                              _c_i64, _c_f, _vp, _c_f, _vp, _vp, _vp, _c_i, _vp, _c_i64, _vp, _vp,
                              _vp]),

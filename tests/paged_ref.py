@@ -56,8 +56,10 @@ def rows(p: ops.PackedKV, c, key: bool) -> torch.Tensor:
 
 def attention(q, kc, vc, table, lengths, dk, dv, c, sm_scale=None, starts=None, window=0,
               softcap=0.0, slopes=None):
-    """(out, lse, spread, reach): 64-bit attention of every query row; spread
-    is sum p |V_hat|, reach the largest |q| |K| sm_scale among its rows."""
+    """(out, lse, spread, reach, peak, largest): 64-bit attention of every query
+    row; spread is sum p |V_hat|, reach the largest |q| |K| sm_scale among its
+    rows, peak the same with sqrt(D) max |q~| for |q|, largest the rows' largest
+    p |V_hat| times the square root of their number."""
     B, Hq, D = q.shape
     P, H, page, _ = kc.shape
     nq = Hq // H
@@ -66,7 +68,7 @@ def attention(q, kc, vc, table, lengths, dk, dv, c, sm_scale=None, starts=None, 
     qt = (q.cpu().double() * dk.double()) @ hadamard(D) / math.sqrt(D)
     out = torch.zeros(B, Hq, D, dtype=torch.float64)
     lse = torch.full((B, Hq), -math.inf, dtype=torch.float64)
-    spread, reach = torch.zeros(B, Hq, dtype=torch.float64), torch.zeros(B, Hq, dtype=torch.float64)
+    spread, reach, peak, largest = (torch.zeros(B, Hq, dtype=torch.float64) for _ in range(4))
     table = table.cpu().long()
     for b in range(B):
         n = int(lengths[b])
@@ -88,26 +90,40 @@ def attention(q, kc, vc, table, lengths, dk, dv, c, sm_scale=None, starts=None, 
             out[b, hq] = p @ v
             spread[b, hq] = p @ v.norm(dim=-1) * math.sqrt(D)
             reach[b, hq] = k.norm(dim=-1).max() * qt[b, hq].norm() * abs(scale)
-    return (out @ hadamard(D)) * dv.double(), lse, spread, reach
+            peak[b, hq] = k.norm(dim=-1).max() * qt[b, hq].abs().max() * math.sqrt(D) * abs(scale)
+            largest[b, hq] = (p * v.norm(dim=-1)).max() * math.sqrt(D * len(p))
+    return (out @ hadamard(D)) * dv.double(), lse, spread, reach, peak, largest
 
 
 def check(got, lse, want, dtype):
     """Holds an output (and lse, or None) to the accuracy that the operators document.
 
-    With u = 2^-20 for fp32 and fp16 queries (values split into two fp16
-    parts) and 2^-11 for bf16 ones (two operands rounded to fp16, 2^-12 each):
-    a score is off by at most u |q| |K| sm_scale (the cap and the bias do not
-    enlarge that); p by twice that, relatively, as numerator and denominator
-    move apart; the weighted sum by another u.  In the 2-norm of a row:
-    (2 u reach + u) sum p |V_hat|, and half a step of the output's type."""
-    out, ref_lse, spread, reach = want
-    u = 2.0 ** -11 if dtype == torch.bfloat16 else 2.0 ** -20
+    A score is off by at most `ds` (the cap and the bias do not enlarge that):
+      fp32 queries: 2^-20 |q| |K| sm_scale (two fp16 parts, sums in 32 bits);
+      16-bit ones: q~ in fixed point, off by 2^-13 of its largest element for a
+      quarter of the elements, half of that for the next and so on, in the
+      2-norm sqrt(D / 4 (1 + 1/4 + 1/16 + 1/64)) 2^-13 max |q~|, which is under
+      2^-13.7 sqrt(D) max |q~|;  bf16 may take the tensor-core prefix instead:
+      two operands rounded to fp16, 2^-11 |q| |K| sm_scale.
+    p is off by twice that, relatively, as numerator and denominator move
+    apart.  The weighted sum adds `dw` sum p |V_hat| (2^-20; 2^-11 for bf16, two
+    fp16 operands) and, for 16-bit queries, roundings to 2^-14 (half of that
+    at most) of the largest weight of a unit: independent, so the root of their
+    number counts, 1 / sqrt(12) of a step each; a whole 2^-14 is 7 deviations.
+    The output's own rounding is half a step."""
+    out, ref_lse, spread, reach, peak, largest = want
+    ds, dw = 2.0 ** -20 * reach, 2.0 ** -20
+    if dtype != torch.float32:
+        ds = ds + 2.0 ** -13.7 * peak
+    if dtype == torch.bfloat16:
+        ds, dw = torch.maximum(ds, 2.0 ** -11 * reach), 2.0 ** -11
+    extra = 2.0 ** -14 * largest if dtype != torch.float32 else 0
     got = got.detach().cpu().double()
     # a value past the type's largest rounds to an infinity of its sign
     over = torch.isinf(got) & (out.abs() >= torch.finfo(dtype).max) & (got.sign() == out.sign())
     got = torch.where(over, out, got)
     off = (got - out).norm(dim=-1)
-    most = (2 * u * reach + u) * spread + torch.finfo(dtype).eps / 2 * out.norm(dim=-1)
+    most = (2 * ds + dw) * spread + extra + torch.finfo(dtype).eps / 2 * out.norm(dim=-1)
     bad = off > most
     assert torch.isfinite(got).all()
     assert not bad.any(), (off[bad].max(), most[bad].min(), bad.nonzero()[:4].tolist())
@@ -117,7 +133,7 @@ def check(got, lse, want, dtype):
         assert torch.equal(torch.isinf(lse), none) and (lse[none] < 0).all()
         # the logarithm and its parts are 32-bit: 2^-22 of its size
         dl = (lse - ref_lse).abs()[~none]
-        ml = (u * reach + 2.0 ** -20 + 2.0 ** -22 * ref_lse.abs())[~none]
+        ml = (ds + 2.0 ** -20 + 2.0 ** -22 * ref_lse.abs())[~none]
         assert (dl <= ml).all(), (dl.max(), ml.min())
 
 

@@ -94,14 +94,18 @@ def test_attention_refuses_bad_arguments(kw, status):
 
 
 def test_workspace_sizes():
-    f = _lib.lib().kh_paged_workspace_bytes
-    assert f(0, 1, 1, 128, 10, 0, 0) == 0 and f(3, 1, 1, 128, 0, 0, 0) == 0
-    a = f(2, 4, 8, 128, 100, 0, 0)
-    assert a > 0 and a % (2 * 4 * 8 * 130 * 4) == 0
-    assert f(2, 4, 8, 96, 100, 0, 0) == -1 and f(2, 4, 8, 128, 100, 101, 0) == -1
-    assert f(2, 0, 8, 128, 100, 0, 0) == -1 and f(-1, 1, 1, 128, 1, 0, 0) == -1
-    # a window bounds what a sequence needs
-    assert f(64, 1, 8, 128, 100000, 0, 64) <= f(64, 1, 8, 128, 100000, 0, 0)
+    def f(n_seqs, n_q, heads, D, max_len, prefix=0, window=0, dtype=_lib.KH_BF16):
+        return _lib.lib().kh_paged_workspace_bytes(n_seqs, n_q, heads, D, dtype, max_len, prefix,
+                                                   window)
+    assert f(3, 1, 1, 128, 0) == 0  # nothing can be attended
+    assert f(2, 4, 8, 128, 100) >= 2 * 4 * 8 * 130 * 4
+    assert f(2, 4, 8, 96, 100) == -1 and f(2, 4, 8, 128, 100, 101) == -1
+    assert f(2, 0, 8, 128, 100) == -1 and f(-1, 1, 1, 128, 1) == -1
+    assert f(2, 4, 8, 128, 100, dtype=7) == -1
+    # a window bounds what a sequence needs; records do not grow without bound
+    assert f(64, 1, 8, 128, 100000, 0, 64) < f(64, 1, 8, 128, 100000)
+    assert f(64, 4, 8, 128, 10 ** 9) < 1 << 28
+    assert f(64, 4, 8, 128, 10 ** 9, 10 ** 8, dtype=_lib.KH_F32) < 1 << 28
 
 
 def _pool(bits=1, residual=True, shape=(2, 2, 16, 128)):
