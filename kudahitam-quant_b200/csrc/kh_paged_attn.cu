@@ -142,6 +142,13 @@ __device__ __forceinline__ void mma16832(int (&c)[4], uint32_t a0, uint32_t a1, 
       : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma16832_0(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                           uint32_t a3, uint32_t b0, uint32_t b1) {  // from zero
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%10,%10,%10};"
+      : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
+}
 __device__ __forceinline__ void mma16832u(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                           uint32_t a3, uint32_t b0, uint32_t b1) {  // u8 x u8
   asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
@@ -461,12 +468,14 @@ __global__ void __launch_bounds__(32 * kWarps, rows_ctas<D, I8, NB>())
 
     // scores of the tile's two 16-row halves, both planes
     Acc s1[2][NB][4], s2[2][NB][4];
+    if constexpr (!I8) {
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf)
+      for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) s1[hf][nb][k] = s2[hf][nb][k] = 0;
+          for (int k = 0; k < 4; ++k) s1[hf][nb][k] = s2[hf][nb][k] = 0;
+    }
 #pragma unroll
     for (int v = 0; v < W / 4; ++v) {
       uint32_t w[2][2][2];  // half, plane, row
@@ -496,8 +505,10 @@ __global__ void __launch_bounds__(32 * kWarps, rows_ctas<D, I8, NB>())
             for (int p = 0; p < 2; ++p) {
               auto& c = p == 0 ? s1[hf][nb] : s2[hf][nb];
               const uint32_t x0 = w[hf][p][0], x1 = w[hf][p][1];
-              if constexpr (I8) mma16832(c, x0 & m0, x1 & m0, x0 & m1, x1 & m1, f.x, f.y);
-              else mma16816(c, x0 & m0, x1 & m0, x0 & m1, x1 & m1, f.x, f.y);
+              if constexpr (I8) {
+                if (v == 0 && i == 0) mma16832_0(c, x0 & m0, x1 & m0, x0 & m1, x1 & m1, f.x, f.y);
+                else mma16832(c, x0 & m0, x1 & m0, x0 & m1, x1 & m1, f.x, f.y);
+              } else mma16816(c, x0 & m0, x1 & m0, x0 & m1, x1 & m1, f.x, f.y);
             }
         }
       }
@@ -585,6 +596,7 @@ __global__ void __launch_bounds__(32 * kWarps, rows_ctas<D, I8, NB>())
           i1[nb] = i2[nb] = 0u;
         }
         ref[nb] = to;
+        if (tile == 0) continue;  // nothing summed yet
         l[nb] *= f;
         w1s[nb] *= f;
         w2s[nb] *= f;
@@ -987,7 +999,7 @@ PagedPlan paged_plan(int64_t n_seqs, int n_q, int n_kv_heads, int D, int64_t max
     p.pre_rows = ((pre + ctas - 1) / ctas + tile - 1) / tile * tile;
     p.pre_chunks = (int)((pre + p.pre_rows - 1) / p.pre_rows);
   }
-  // Units: six for each of the 16 warps of an SM where the longest sequences
+  // Units: three for every two warps (20 an SM) where the longest sequences
   // give that many, so that the last ones end together; not under two tiles
   // (a unit's fixed cost is about one tile's) nor over 64, and not so short
   // that the records take over 64 MB (at least 6 slots a row).
@@ -995,7 +1007,7 @@ PagedPlan paged_plan(int64_t n_seqs, int n_q, int n_kv_heads, int D, int64_t max
   const int64_t pairs = n_kv_heads * (n_seqs * blocks * own + (p.pre_chunks ? 0 : (nq + 3) / 4 * pre));
   const int64_t room =
       rows > 0 ? std::max<int64_t>(6, (int64_t(64) << 20) / (rows * record)) - 4 : 2;
-  int64_t unit = std::max<int64_t>(64, std::min<int64_t>(2048, pairs / (96 * (int64_t)n_sms)));
+  int64_t unit = std::max<int64_t>(64, std::min<int64_t>(2048, pairs / (32 * (int64_t)n_sms)));
   unit = std::max(unit, (own + (p.pre_chunks ? 0 : pre) + room - 1) / room);
   p.unit = (unit + 31) / 32 * 32;
   // a group touches at most this many units
