@@ -27,36 +27,41 @@ namespace {
 
 // ------------------------------------------------------------------ rows
 //
-// paged_rows_kernel: both products on mma.sync, fed from registers, so that a
-// row's bits are never written out as elements.  A packed word masked to one
-// bit a byte (or halfword) IS a register of matrix elements, each 2^b or zero
-// (8-bit integers), or 2^(b - 24) or zero (fp16, subnormal): one logic
-// operation makes four elements, or two.  The factor 2^b goes into the other
-// operand or into the accumulator's scale.  What bit belongs to what index of
-// the product is free, as long as both operands agree:
+// paged_rows_kernel: both products on mma.sync with 8-bit integers, fed from
+// registers, so that a row's bits are never written out as elements.  A packed
+// word masked to one bit a byte IS a register of four matrix elements, each 2^b
+// or zero; the factor 2^b goes into the other operand or into the
+// accumulator's scale.  What bit belongs to what index of the product is free,
+// as long as both operands agree:
 //   scores  A = 16 rows: lane (g, t) holds word t of rows pi(g) and pi(g) + 8
-//           (words 2 t, 2 t + 1 at D = 256).  B = q~, a query in two columns.
+//           (words 2 t, 2 t + 1 at D = 256).  B = q~.
 //   values  A = 16 elements of lane g's halfword (word at D = 256), of rows
-//           t, t + 4, t + 8, t + 12 (and 16 more).  B = the weights p norm' and
+//           t, t + 8, t + 4, t + 12 (and 16 more).  B = the weights p norm' and
 //           p rnorm', which movmatrix turns from the scores' accumulator
 //           layout into the operand's.
-// A query's (and a weight's) two columns are its high and low part:
-//   I8    (16-bit queries) 16-bit fixed point in two bytes, sums exact in 32-bit
-//         integers.  q~ keeps 2^-13 of its largest element (2^-16 for three
-//         bits of four), a weight 2^-16 of the largest of its unit, whose
-//         rounding errors average out; together under a tenth of a bf16 step.
-//         Bits count as 0 / 1: sum w sign = 2 sum w bit - sum w, exactly.
-//   else  (32-bit queries) two fp16 parts of 11 bits, the second times 2^11.
-//         There the difference would cost bits, so values move their bits
-//         to the sign of +-1, one more shift each.
-// Measured on the ragged batch (32 sequences up to 8192, 8 x 4 heads): fp16
-// parts for bf16 queries 25 instructions a row, 63 us.
+// Queries and weights are fixed point, PARTS bytes of them a column each, and
+// sums are exact in 32 bits.  Bits count as 0 / 1: sum w sign = 2 sum w bit -
+// sum w, exactly too.
+//   PARTS = 2 (16-bit queries, 4 a block of 8 columns): q~ to 2^-13 of its
+//     largest element (2^-16 for bits that count once), weights to 2^-16 of
+//     the largest of their unit, whose roundings average out; together under
+//     a tenth of a bf16 step.
+//   PARTS = 4 (32-bit queries, 2 a block): q~ to 2^-28, weights to 2^-22.
+// What bounds it is issue: 128 logic operations a 32-row tile at half rate,
+// and as many around them.  As fp16 products (two elements a logic operation,
+// half the rate of the products) it took 25 instructions a row and 63 us on
+// the ragged batch (32 sequences up to 8192 rows, 8 KV heads x 4), now 20 and
+// 42 us.
 //
 // A warp runs on its own: 32-row tiles in a ring of cp.async stages, one lane
 // fetching one row (so pages may end anywhere).  The reference exponent of a
-// column moves only when a weight would leave its type's range, so most tiles
-// rescale nothing.
+// column is a whole number and moves only when a weight would leave its range,
+// so that most tiles rescale nothing and sums move by shifts.
+// A piece of a unit is at most 16384 rows: 32-bit sums hold those (weights up
+// to 255 x 128 each), and what is summed as floats keeps its bits; the next
+// piece's record joins in.
 constexpr int kWarps = 4;
+constexpr int64_t kPieceRows = 16384;
 
 template <int D>
 struct RowsCfg {
@@ -82,19 +87,16 @@ template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
+  uint32_t y;
+  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(y) : "r"(a), "r"(b), "r"(sel));
+  return y;
+}
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                         uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
 // ---- how a call's rows are split
 //
 // All (group, row) pairs of the call lie one after another: first the prefix's
@@ -109,9 +111,9 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
 // What the claims need is prepared by a launch before: where each sequence's
 // pairs start, its first row, the claim counter, and each group's queries as
 // operand fragments.
-template <int D, bool I8, int NB>
+template <int D, int NB>
 struct Frags {  // of a group
-  static constexpr int kSteps = D / (I8 ? 32 : 16);
+  static constexpr int kSteps = D / 32;
   uint2 q[NB * kSteps][32];
   float sum[NB * 4], scale[NB * 4];  // per query: sum of q~ and the exponent's scale
 };
@@ -157,20 +159,21 @@ __device__ __forceinline__ void mma16832u(int (&c)[4], uint32_t a0, uint32_t a1,
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-constexpr int64_t kFragBytes = 4352;  // of a group's Frags, at most
+constexpr int64_t kFragBytes = 2176;  // of a group's Frags, at most
 
-constexpr float kPart = 2048.f;      // second fp16 parts are stored times 2^11
 
 // Block 0: starts, first rows, the counter.  The others: a group each.
-template <int D, bool I8, int NB>
+template <int D, int PARTS, int NB>
 __global__ void __launch_bounds__(128) paged_prepare_kernel(const __grid_constant__ AttnParams P) {
-  using F = Frags<D, I8, NB>;
-  constexpr int W = D / 32, KS = F::kSteps, NQ = NB * 4;
+  using F = Frags<D, NB>;
+  constexpr int W = D / 32, KS = F::kSteps, QB = 8 / PARTS, NQ = NB * QB;
   const PagedAttnRequest& r = P.r;
   __shared__ float qs[NQ][D];
   __shared__ int64_t part[4];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  grid_dependency_wait();
+  // Behind the launch that transforms a tensor-core prefix's queries, which
+  // signals once all earlier work is done, this one waits at its end only.
+  if (!P.pre_tensor) grid_dependency_wait();
   grid_dependents_launch();
   if (blockIdx.x == 0) {
     if (threadIdx.x == 0) *P.next_unit = 0u;
@@ -200,6 +203,7 @@ __global__ void __launch_bounds__(128) paged_prepare_kernel(const __grid_constan
       if (b < r.n_seqs) P.starts[b] = before + upto - n;
     }
     if (threadIdx.x == 0) P.starts[r.n_seqs] = base;
+    if (P.pre_tensor) grid_dependency_wait();
     return;
   }
   const int64_t gi = blockIdx.x - 1;
@@ -221,23 +225,14 @@ __global__ void __launch_bounds__(128) paged_prepare_kernel(const __grid_constan
     for (int j = 0; j < W; ++j) mx = fmaxf(mx, fabsf(x[j]));
 #pragma unroll
     for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    float up;
-    if constexpr (I8) {
-      // whole numbers up to 32639 = 127 x 256 + 127 where a bit counts once
-      up = mx > 0.f && mx < INFINITY ? 32639.f / mx : 1.f;
-    } else {
-      // the largest element into [2^-10, 2^-9): q~ 2^(24 - b) stays inside fp16
-      int e = 0;
-      if (mx > 0.f && mx < INFINITY) frexpf(mx, &e);
-      up = ldexpf(1.f, max(-120, min(-9 - e, 120)));
-    }
+    // whole numbers that PARTS signed bytes hold: 127 x 256 + 127, or 127 x 2^24
+    constexpr float kLargest = PARTS == 2 ? 32639.f : 2130706432.f;
+    const float up = mx > 0.f && mx < INFINITY ? kLargest / mx : 1.f;
 #pragma unroll
     for (int j = 0; j < W; ++j) {
-      float v = x[j] * up;
-      if constexpr (I8) {  // element 32 j + lane counts 2^(bit & 3) times
-        const float times = (float)(1 << (lane & 3));
-        v = rintf(v / times) * times;
-      }
+      // element 32 j + lane: its bit's place in the masked byte counts 2^(bit & 3) times
+      const float times = (float)(1 << (lane & 3));
+      const float v = rintf(x[j] * up / times) * times;
       sum += v;
       qs[y][32 * j + lane] = v;
     }
@@ -249,38 +244,25 @@ __global__ void __launch_bounds__(128) paged_prepare_kernel(const __grid_constan
     }
   }
   __syncthreads();
-  // column g: query g / 2, its high part (even) or low part
+  // column g: byte PARTS - 1 - g % PARTS of query g / PARTS; k = 4 t + j is bit
+  // 2 i of byte j of the lane's word, k = 4 t + 16 + j bit 2 i + 1
   const int g = lane >> 2, t = lane & 3;
   for (int k = warp; k < NB * KS; k += 4) {
-    const int i = k % KS, y = k / KS * 4 + (g >> 1);
-    if constexpr (I8) {
-      // k = 4 t + j is bit 2 i of byte j of the lane's word, k = 4 t + 16 + j bit 2 i + 1
-      const int word = D == 128 ? t : 2 * t + (i >> 2);
-      uint32_t f[2] = {0, 0};
+    const int i = k % KS, y = k / KS * QB + g / PARTS;
+    const int word = D == 128 ? t : 2 * t + (i >> 2);
+    uint32_t f[2] = {0, 0};
 #pragma unroll
-      for (int o = 0; o < 2; ++o)
+    for (int o = 0; o < 2; ++o)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int bit = 2 * (i & 3) + o;
-          const int v = (int)qs[y][32 * word + 8 * j + bit] >> (bit & 3);
-          const int low = ((v + 128) & 255) - 128;
-          f[o] |= (uint32_t)((g & 1 ? low : (v - low) >> 8) & 255) << (8 * j);
-        }
-      out->q[k][lane] = make_uint2(f[0], f[1]);
-    } else {
-      // k = 2 t, 2 t + 1 are bit 2 i of the two halves of the lane's word,
-      // k = 2 t + 8, 2 t + 9 bit 2 i + 1
-      auto value = [&](int e, int bit) {
-        const float v = qs[y][e] * (float)(1 << (24 - (bit & 7)));
-        const float hi_part = round_h(v);
-        return g & 1 ? (v - hi_part) * kPart : hi_part;
-      };
-      const int e = (D == 128 ? 32 * t : 64 * t + 32 * (i >> 3)), bit = 2 * (i & 7);
-      out->q[k][lane] =
-          make_uint2(pack_h2(value(e + bit, bit), value(e + 16 + bit, bit)),
-                     pack_h2(value(e + bit + 1, bit + 1), value(e + 17 + bit, bit + 1)));
-    }
+      for (int j = 0; j < 4; ++j) {
+        const int bit = 2 * (i & 3) + o;
+        int v = (int)qs[y][32 * word + 8 * j + bit] >> (bit & 3);
+        for (int d = PARTS - 1 - g % PARTS; d > 0; --d) v = (v - (((v + 128) & 255) - 128)) >> 8;
+        f[o] |= (uint32_t)(v & 255) << (8 * j);
+      }
+    out->q[k][lane] = make_uint2(f[0], f[1]);
   }
+  if (P.pre_tensor) grid_dependency_wait();
 }
 
 // Sequence b with starts[b] * per <= x < starts[b + 1] * per: a warp looks at
@@ -298,30 +280,30 @@ __device__ __forceinline__ int64_t find_sequence(const AttnParams& P, int64_t x,
 }
 
 // CTAs an SM that the registers are bounded for.
-template <int D, bool I8, int NB>
+template <int D, int NB>
 constexpr int rows_ctas() {
-  return D == 256 || NB == 2 ? 3 : I8 ? 5 : 4;
+  return D == 256 || NB == 2 ? 3 : 5;
 }
 
-template <int D, bool I8, bool EXTRA, int NB>
-__global__ void __launch_bounds__(32 * kWarps, rows_ctas<D, I8, NB>())
+template <int D, int PARTS, bool EXTRA, int NB>
+__global__ void __launch_bounds__(32 * kWarps, rows_ctas<D, NB>())
     paged_rows_kernel(const __grid_constant__ AttnParams P) {
   using C = RowsCfg<D>;
-  using F = Frags<D, I8, NB>;
-  using Acc = std::conditional_t<I8, int, float>;
+  using F = Frags<D, NB>;
   constexpr int W = C::W;
   constexpr int kStages = C::kStages;
   constexpr int KS = F::kSteps;         // steps of the score product
   constexpr int MT = D / 16;            // element tiles of the value product
-  constexpr int NQ = NB * 4;
-  constexpr bool kRegs = NB * KS <= 8;  // query fragments in registers
+  constexpr int QB = 8 / PARTS;         // queries a column block
+  constexpr int NQ = NB * QB;
   const PagedAttnRequest& r = P.r;
   extern __shared__ __align__(16) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
+  const int mine = PARTS == 2 ? t : t >> 1;   // this lane's query of a block
+  const bool low = PARTS == 4 && (t & 1);     // it holds the query's low bytes
   const int hq_all = r.n_kv_heads * r.n_q;
   uint8_t* ring = smem + warp * kStages * C::kStage;
-  uint2(*q_frag)[32] = reinterpret_cast<uint2(*)[32]>(smem + C::kRing + warp * NB * KS * 256);
   // After a prefix launch this grid may run beside it: that one signals its
   // dependents once all earlier work is done, and nothing here reads its
   // records.  The wait then comes at the end, so that this grid's completion
@@ -350,13 +332,14 @@ __global__ void __launch_bounds__(32 * kWarps, rows_ctas<D, I8, NB>())
   const int hz = (int)((at - start) / rows);
   const int64_t begin = start + hz * rows;
   const int lo = (pre ? 0 : P.first_row[b]) + (int)(at - begin);
-  const int hi = lo + (int)min(rows - (at - begin), end - at);
+  const int hi = lo + (int)min(min(rows - (at - begin), end - at), kPieceRows);
+  const bool more = at > begin && at > (int64_t)unit * P.unit;  // the slot holds rows already
   at += hi - lo;
   const int blocks = pre ? P.pre_blocks : P.own_blocks;
   const int h = hz / blocks;
   const int64_t y0 = (int64_t)(hz - h * blocks) * NQ;
   const int nq = (int)min((int64_t)NQ, (pre ? r.n_seqs * r.n_q : (int64_t)r.n_q) - y0);
-  const int part = (int)(unit - begin / P.unit) + (pre ? 0 : P.plan.pre_parts);
+  const int part = (int)(unit - P.unit_of(begin)) + (pre ? 0 : P.plan.pre_parts);
   const F* frags = reinterpret_cast<const F*>(P.frags) +
                               (pre ? hz : r.n_kv_heads * P.pre_blocks + b * per + hz);
   auto seq_of = [&](int y) { return pre ? (y0 + y) / r.n_q : b; };
@@ -401,13 +384,9 @@ __global__ void __launch_bounds__(32 * kWarps, rows_ctas<D, I8, NB>())
   for (int s = 0; s < kStages - 1; ++s) issue(s, s, page_of(s));
   int next_page = page_of(kStages - 1);
 
-  uint2 qf[kRegs ? NB * KS : 1];
+  uint2 qf[NB * KS];
 #pragma unroll
-  for (int i = 0; i < NB * KS; ++i) {
-    const uint2 f = frags->q[i][lane];
-    if constexpr (kRegs) qf[i] = f;
-    else q_frag[i][lane] = f;
-  }
+  for (int i = 0; i < NB * KS; ++i) qf[i] = frags->q[i][lane];
 
   // ---- constants of this thread's query of each block
   //   t2 = norm (a1 M1 + b1) + rnorm (a2 M2 + b2), M the masked sums
@@ -417,7 +396,7 @@ __global__ void __launch_bounds__(32 * kWarps, rows_ctas<D, I8, NB>())
   int q_lo[NB], q_hi[NB];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    const int y = nb * 4 + t;
+    const int y = nb * QB + mine;
     const float k = frags->scale[y], sum = frags->sum[y] * k;
     a1[nb] = 2.f * ch * k;
     b1[nb] = (cm - ch) * sum;
@@ -435,21 +414,19 @@ __global__ void __launch_bounds__(32 * kWarps, rows_ctas<D, I8, NB>())
       if (EXTRA && r.slopes) slope[nb] = r.slopes[head_of(y)] * kLog2e;
     }
   }
-  constexpr float kUnitWeight = I8 ? 32768.f : 1.f;  // how weight 1 is stored
-  constexpr float kMost = I8 ? 65535.f : kMaxWeight;
-  const float va = ch * inv_sd * kUnitWeight;
-  const float vb = 0.7978845608028654f * inv_sd * inv_sd * kUnitWeight;
+  // weight 1 as a whole number, and the most one may be
+  constexpr float kOne = PARTS == 2 ? 32768.f : 4194304.f;
+  constexpr float kMost = PARTS == 2 ? 65535.f : 8388607.f;
+  const float va = ch * inv_sd * kOne;
+  const float vb = 0.7978845608028654f * inv_sd * inv_sd * kOne;
   const float cap = r.softcap * kLog2e, inv_cap = r.softcap > 0.f ? 1.f / cap : 0.f;
 
-  // w1s, w2s: sums of weights; in i1, i2 those since the reference last moved
   float ref[NB], l[NB], w1s[NB], w2s[NB];
-  uint32_t i1[NB], i2[NB];
-  Acc acc[NB][MT][4];
+  int acc[NB][MT][4];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     ref[nb] = kNoRef;
     l[nb] = w1s[nb] = w2s[nb] = 0.f;
-    i1[nb] = i2[nb] = 0u;
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -467,15 +444,7 @@ __global__ void __launch_bounds__(32 * kWarps, rows_ctas<D, I8, NB>())
     const int j0 = lo + tile * 32;
 
     // scores of the tile's two 16-row halves, both planes
-    Acc s1[2][NB][4], s2[2][NB][4];
-    if constexpr (!I8) {
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) s1[hf][nb][k] = s2[hf][nb][k] = 0;
-    }
+    int s1[2][NB][4], s2[2][NB][4];
 #pragma unroll
     for (int v = 0; v < W / 4; ++v) {
       uint32_t w[2][2][2];  // half, plane, row
@@ -487,28 +456,23 @@ __global__ void __launch_bounds__(32 * kWarps, rows_ctas<D, I8, NB>())
           for (int rr = 0; rr < 2; ++rr)
             w[hf][p][rr] = reinterpret_cast<const uint32_t*>(
                 st + p * C::kPlane)[(16 * hf + pg + 8 * rr) * W + (D == 128 ? t : 2 * t + v)];
-      constexpr int kPer = KS / (W / 4);  // steps of a word
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        if (i == kPer / 2)
+      for (int i = 0; i < 4; ++i) {
+        if (i == 2)
 #pragma unroll
-          for (int k = 0; k < 8; ++k) w[k >> 2][(k >> 1) & 1][k & 1] >>= kPer;
-        const uint32_t m0 = (I8 ? 0x01010101u : 0x00010001u) << ((2 * i) % kPer), m1 = m0 << 1;
+          for (int k = 0; k < 8; ++k) w[k >> 2][(k >> 1) & 1][k & 1] >>= 4;
+        const uint32_t m0 = 0x01010101u << ((2 * i) & 3), m1 = m0 << 1;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-          uint2 f;
-          if constexpr (kRegs) f = qf[nb * KS + v * kPer + i];
-          else f = q_frag[nb * KS + v * kPer + i][lane];
+          const uint2 f = qf[nb * KS + v * 4 + i];
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
               auto& c = p == 0 ? s1[hf][nb] : s2[hf][nb];
               const uint32_t x0 = w[hf][p][0], x1 = w[hf][p][1];
-              if constexpr (I8) {
-                if (v == 0 && i == 0) mma16832_0(c, x0 & m0, x1 & m0, x0 & m1, x1 & m1, f.x, f.y);
-                else mma16832(c, x0 & m0, x1 & m0, x0 & m1, x1 & m1, f.x, f.y);
-              } else mma16816(c, x0 & m0, x1 & m0, x0 & m1, x1 & m1, f.x, f.y);
+              if (v == 0 && i == 0) mma16832_0(c, x0 & m0, x1 & m0, x0 & m1, x1 & m1, f.x, f.y);
+              else mma16832(c, x0 & m0, x1 & m0, x0 & m1, x1 & m1, f.x, f.y);
             }
         }
       }
@@ -521,6 +485,13 @@ __global__ void __launch_bounds__(32 * kWarps, rows_ctas<D, I8, NB>())
       for (int nb = 0; nb < NB; ++nb) full = full && j0 >= q_lo[nb] && j0 + 32 <= q_hi[nb];
       full = __all_sync(0xffffffffu, full);
     }
+    // a query's masked sum from its columns' (2 PARTS bytes of them)
+    auto joined = [&](const int(&s)[4], int rr) {
+      const float x = (float)(s[2 * rr] * 256 + s[2 * rr + 1]);
+      if constexpr (PARTS == 2) return x;
+      const float y = __shfl_xor_sync(0xffffffffu, x, 1);
+      return low ? fmaf(y, 65536.f, x) : fmaf(x, 65536.f, y);
+    };
     float tt[2][2][NB], ra[2][2], rb[2][2];
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf)
@@ -532,16 +503,8 @@ __global__ void __launch_bounds__(32 * kWarps, rows_ctas<D, I8, NB>())
         rb[hf][rr] = n.w * vb;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-          float m1, m2;
-          if constexpr (I8) {
-            m1 = (float)(s1[hf][nb][2 * rr] * 256 + s1[hf][nb][2 * rr + 1]);
-            m2 = (float)(s2[hf][nb][2 * rr] * 256 + s2[hf][nb][2 * rr + 1]);
-          } else {
-            m1 = fmaf(s1[hf][nb][2 * rr + 1], 1.f / kPart, s1[hf][nb][2 * rr]);
-            m2 = fmaf(s2[hf][nb][2 * rr + 1], 1.f / kPart, s2[hf][nb][2 * rr]);
-          }
-          float x = n.x * fmaf(a1[nb], m1, b1[nb]);
-          x = fmaf(n.y, fmaf(a2[nb], m2, b2[nb]), x);
+          float x = n.x * fmaf(a1[nb], joined(s1[hf][nb], rr), b1[nb]);
+          x = fmaf(n.y, fmaf(a2[nb], joined(s2[hf][nb], rr), b2[nb]), x);
           if (EXTRA && r.softcap > 0.f) x = soft_cap(x, cap, inv_cap);
           if (EXTRA && r.slopes) x = fmaf(slope[nb], (float)(j0 + row + 1 - q_hi[nb]), x);
           tt[hf][rr][nb] = x;
@@ -568,8 +531,7 @@ __global__ void __launch_bounds__(32 * kWarps, rows_ctas<D, I8, NB>())
         for (int nb = 0; nb < NB; ++nb) {
           const float e = ex2(tt[k >> 1][k & 1][nb] - ref[nb]);
           ee[k >> 1][k & 1][nb] = e;
-          const float most =
-              fmaxf(fmaxf(ra[k >> 1][k & 1], rb[k >> 1][k & 1]), kUnitWeight * 0x1p-40f);
+          const float most = fmaxf(fmaxf(ra[k >> 1][k & 1], rb[k >> 1][k & 1]), kOne * 0x1p-40f);
           // nothing attended: 0 times whatever the row's norms hold
           top = fmaxf(top, e == 0.f ? 0.f : e * most);
         }
@@ -579,136 +541,100 @@ __global__ void __launch_bounds__(32 * kWarps, rows_ctas<D, I8, NB>())
         float mx = kNoRef;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const float most =
-              fmaxf(fmaxf(ra[k >> 1][k & 1], rb[k >> 1][k & 1]), kUnitWeight * 0x1p-40f);
+          const float most = fmaxf(fmaxf(ra[k >> 1][k & 1], rb[k >> 1][k & 1]), kOne * 0x1p-40f);
           const float x = tt[k >> 1][k & 1][nb];
-          if (x > -INFINITY) mx = fmaxf(mx, x + lg2(most * (1.f / kUnitWeight)));
+          if (x > -INFINITY) mx = fmaxf(mx, x + lg2(most * (1.f / kOne)));
         }
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
         if (mx == INFINITY) l[nb] = NAN;  // an infinite norm has no average
-        // whole exponents: integer sums move by shifts
-        const float to = fmaxf(ref[nb], I8 ? ceilf(mx) : mx), f = ex2(ref[nb] - to);
-        const int shift = (int)fminf(to - ref[nb], 31.f);
-        if constexpr (I8) {
-          w1s[nb] += (float)i1[nb];
-          w2s[nb] += (float)i2[nb];
-          i1[nb] = i2[nb] = 0u;
-        }
+        const float to = fmaxf(ref[nb], ceilf(mx)), f = ex2(ref[nb] - to);
+        int left = (int)fminf(to - ref[nb], 48.f);
         ref[nb] = to;
         if (tile == 0) continue;  // nothing summed yet
         l[nb] *= f;
         w1s[nb] *= f;
         w2s[nb] *= f;
+        // sums move right; what a column loses its next lower one takes up
+#pragma unroll 1
+        while (__any_sync(0xffffffffu, left > 0)) {
+          const int sh = min(left, 16);
+          const uint32_t lost = (1u << sh) - 1u, half = (1u << sh) >> 1;
+          left -= sh;
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+          for (int i = 0; i < MT; ++i)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if constexpr (I8) acc[nb][i][k] = (acc[nb][i][k] + (int)((1u << shift) >> 1)) >> shift;
-            else acc[nb][i][k] *= f;
-          }
+            for (int k = 0; k < 4; k += 2) {
+              uint32_t h = acc[nb][i][k], o = acc[nb][i][k + 1];
+              if constexpr (PARTS == 2) {
+                o += ((h & lost) << 8) + half;
+              } else {  // the low lanes hold one column, in h
+                if (!low) o += (h & lost) << 8;
+                const uint32_t down = __shfl_xor_sync(0xffffffffu, o & lost, 1);
+                if (low) h += (down << 8) + half;
+              }
+              acc[nb][i][k] = (int)(h >> sh);
+              acc[nb][i][k + 1] = (int)(o >> sh);
+            }
+        }
       }
     }
-    uint32_t p1[2][NB][2], p2[2][NB][2];
+    uint32_t p1[2][NB], p2[2][NB];
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf)
+    for (int nb = 0; nb < NB; ++nb) {
+      uint32_t i1 = 0u, i2 = 0u;
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
+      for (int hf = 0; hf < 2; ++hf) {
         uint32_t u1[2], u2[2];
 #pragma unroll
         for (int rr = 0; rr < 2; ++rr) {
           const float e = ee[hf][rr][nb];
           l[nb] += e;
-          float x1, x2;
-          if constexpr (I8) {
-            // 2^23 + w: the low bits are w as a whole number
-            x1 = fmaf(e, ra[hf][rr], 8388608.f);
-            x2 = fmaf(e, rb[hf][rr], 8388608.f);
-          } else {
-            x1 = e * ra[hf][rr];
-            x2 = e * rb[hf][rr];
-          }
-          if (!full && tt[hf][rr][nb] == -INFINITY) x1 = x2 = I8 ? 8388608.f : 0.f;
-          if constexpr (I8) {
-            u1[rr] = __float_as_uint(x1);
-            u2[rr] = __float_as_uint(x2);
-          } else {
-            w1s[nb] += x1;
-            w2s[nb] += x2;
-            p1[hf][nb][rr] = transpose8(pack_h2(x1, (x1 - round_h(x1)) * kPart));
-            p2[hf][nb][rr] = transpose8(pack_h2(x2, (x2 - round_h(x2)) * kPart));
-          }
+          // 2^23 + w: the low bits are w as a whole number
+          float x1 = fmaf(e, ra[hf][rr], 8388608.f), x2 = fmaf(e, rb[hf][rr], 8388608.f);
+          if (!full && tt[hf][rr][nb] == -INFINITY) x1 = x2 = 8388608.f;
+          u1[rr] = __float_as_uint(x1);
+          u2[rr] = __float_as_uint(x2);
         }
-        if constexpr (I8) {
-          i1[nb] += u1[0] + u1[1];
-          i2[nb] += u2[0] + u2[1];
-          // columns 2 t, 2 t + 1: high and low bytes, of both rows
-          p1[hf][nb][0] = transpose8(__byte_perm(u1[0], u1[1], 0x4051));
-          p2[hf][nb][0] = transpose8(__byte_perm(u2[0], u2[1], 0x4051));
-        }
+        i1 += u1[0] + u1[1];
+        i2 += u2[0] + u2[1];
+        // this lane's two columns, high byte first, of both rows
+        // (the low lanes' second is zero: the sign of byte 3, repeated)
+        const uint32_t sel = PARTS == 2 ? 0x4051u : low ? 0xfb40u : 0x5162u;
+        p1[hf][nb] = transpose8(prmt(u1[0], u1[1], sel));
+        p2[hf][nb] = transpose8(prmt(u2[0], u2[1], sel));
       }
+      w1s[nb] += (float)(i1 - 4u * 0x4B000000u);  // without the exponent fields
+      w2s[nb] += (float)(i2 - 4u * 0x4B000000u);
+    }
 
     // values
-    if constexpr (I8) {
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {  // without the four exponent fields of 2^23
-        i1[nb] -= 4u * 0x4B000000u;
-        i2[nb] -= 4u * 0x4B000000u;
-      }
+    for (int p = 0; p < 2; ++p) {
+      uint32_t x[2][W / 4], y[2][W / 4];  // even and odd bytes of four rows, by half
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        uint32_t x[2][W / 4], y[2][W / 4];  // even and odd bytes of four rows, by half
+      for (int hf = 0; hf < 2; ++hf) {
+        const uint32_t* pl = reinterpret_cast<const uint32_t*>(st + (2 + p) * C::kPlane) +
+                             (16 * hf + t) * W + (D == 128 ? g >> 1 : g);
+        const uint32_t r0 = pl[0], r1 = pl[8 * W], r2 = pl[4 * W], r3 = pl[12 * W];
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          const uint32_t* pl = reinterpret_cast<const uint32_t*>(st + (2 + p) * C::kPlane) +
-                               (16 * hf + t) * W + (D == 128 ? g >> 1 : g);
-          const uint32_t r0 = pl[0], r1 = pl[8 * W], r2 = pl[4 * W], r3 = pl[12 * W];
-#pragma unroll
-          for (int v = 0; v < W / 4; ++v) {
-            const uint32_t sel = (D == 128 ? (g & 1) : v) ? 0x7362u : 0x5140u;
-            const uint32_t a = __byte_perm(r0, r1, sel), b = __byte_perm(r2, r3, sel);
-            x[hf][v] = __byte_perm(a, b, 0x5410);
-            y[hf][v] = __byte_perm(a, b, 0x7632);
-          }
+        for (int v = 0; v < W / 4; ++v) {
+          const uint32_t sel = (D == 128 ? (g & 1) : v) ? 0x7362u : 0x5140u;
+          const uint32_t a = __byte_perm(r0, r1, sel), b = __byte_perm(r2, r3, sel);
+          x[hf][v] = __byte_perm(a, b, 0x5410);
+          y[hf][v] = __byte_perm(a, b, 0x7632);
         }
-#pragma unroll
-        for (int v = 0; v < W / 4; ++v)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint32_t m = 0x01010101u << i;
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-              const auto& f = p == 0 ? p1 : p2;
-              mma16832u(acc[nb][8 * v + i], x[0][v] & m, y[0][v] & m, x[1][v] & m, y[1][v] & m,
-                        f[0][nb][0], f[1][nb][0]);
-            }
-          }
       }
-    } else {
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf)
+      for (int v = 0; v < W / 4; ++v)
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          const uint32_t* pl = reinterpret_cast<const uint32_t*>(st + (2 + p) * C::kPlane) +
-                               (16 * hf + t) * W + (D == 128 ? g >> 1 : g);
-          const uint32_t r0 = pl[0], r1 = pl[4 * W], r2 = pl[8 * W], r3 = pl[12 * W];
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t m = 0x01010101u << i;
 #pragma unroll
-          for (int v = 0; v < W / 4; ++v) {
-            const uint32_t sel = (D == 128 ? (g & 1) : v) ? 0x7632u : 0x5410u;
-            const uint32_t x0 = __byte_perm(r0, r1, sel), x1 = __byte_perm(r2, r3, sel);
-            auto sign = [](uint32_t x, int bit) {
-              return ((x << (15 - bit)) & 0x80008000u) ^ 0xBC00BC00u;
-            };
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const uint32_t a0 = sign(x0, 2 * i), b0 = sign(x0, 2 * i + 1);
-              const uint32_t a1 = sign(x1, 2 * i), b1 = sign(x1, 2 * i + 1);
-#pragma unroll
-              for (int nb = 0; nb < NB; ++nb) {
-                const uint32_t(&f)[2] = p == 0 ? p1[hf][nb] : p2[hf][nb];
-                mma16816(acc[nb][8 * v + i], a0, b0, a1, b1, f[0], f[1]);
-              }
-            }
+          for (int nb = 0; nb < NB; ++nb) {
+            const auto& f = p == 0 ? p1 : p2;
+            mma16832u(acc[nb][8 * v + i], x[0][v] & m, y[0][v] & m, x[1][v] & m, y[1][v] & m,
+                      f[0][nb], f[1][nb]);
           }
         }
     }
@@ -719,51 +645,57 @@ __global__ void __launch_bounds__(32 * kWarps, rows_ctas<D, I8, NB>())
   cp_wait<0>();
   __syncwarp();
 
-  // ---- the record: 16 consecutive elements a lane (32 at D = 256)
+  // ---- the record: 16 consecutive elements a lane (32 at D = 256), tile i's
+  // parts elements i and 8 + i of each 16
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    if constexpr (I8) {
-      w1s[nb] += (float)i1[nb];
-      w2s[nb] += (float)i2[nb];
-    }
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) {
       l[nb] += __shfl_xor_sync(0xffffffffu, l[nb], o);
       w1s[nb] += __shfl_xor_sync(0xffffffffu, w1s[nb], o);
       w2s[nb] += __shfl_xor_sync(0xffffffffu, w2s[nb], o);
     }
-    const int y = nb * 4 + t;
-    if (y < nq) {
-      float* rec = r.workspace +
-                   ((seq_of(y) * hq_all + head_of(y)) * P.plan.parts() + part) * (int64_t)(D + 2);
-      if (g == 0) *reinterpret_cast<float2*>(rec) = make_float2(ref[nb], l[nb]);
-      const float base = (I8 ? -w1s[nb] - w2s[nb] : 0.f) + (cm / ch) * w1s[nb];
-      // element i of part k of the lane's 16 (or 32)
-      auto element = [&](int i, int k) {
-        if constexpr (I8) {  // 2 sum w bit, bit i counting 2^(i & 7) times
-          const float x = fmaf((float)acc[nb][i][2 * k], 256.f, (float)acc[nb][i][2 * k + 1]);
-          return (fmaf(x, 2.f / (float)(1 << (i & 7)), base)) * (1.f / kUnitWeight);
-        } else {
-          return fmaf(acc[nb][i][2 * k + 1], 1.f / kPart, acc[nb][i][2 * k]) + base;
-        }
-      };
-      const int e0 = 2 + (D == 128 ? 16 : 32) * g;
+    const int y = nb * QB + mine;
+    float* rec = r.workspace +
+                 ((y < nq ? seq_of(y) * hq_all + head_of(y) : 0) * P.plan.parts() + part) *
+                     (int64_t)(D + 2);
+    float is = 1.f / kOne, was = 0.f;
+    if (more && y < nq) {  // joins the record
+      const float2 old = *reinterpret_cast<const float2*>(rec);
+      const float top = fmaxf(old.x, ref[nb]), f = ex2(ref[nb] - top);
+      ref[nb] = top;
+      is *= f;
+      was = ex2(old.x - top);
+      l[nb] = fmaf(l[nb], f, old.y * was);
+    }
+    __syncwarp();
+    if (y < nq && g == 0 && !low) *reinterpret_cast<float2*>(rec) = make_float2(ref[nb], l[nb]);
+    const float base = -w1s[nb] - w2s[nb] + (cm / ch) * w1s[nb];
+    auto element = [&](int i, int k) {  // 2 sum w bit, bit i counting 2^(i & 7) times
+      const float h = (float)acc[nb][i][2 * k], o = (float)acc[nb][i][2 * k + 1];
+      float x;
+      if constexpr (PARTS == 2) {
+        x = fmaf(h, 256.f, o);
+      } else {
+        x = low ? h : fmaf(h, 65536.f, o * 256.f);
+        x += __shfl_xor_sync(0xffffffffu, x, 1);
+      }
+      return fmaf(x, 2.f / (float)(1 << (i & 7)), base) * is;
+    };
+    const int e0 = 2 + (D == 128 ? 16 : 32) * g;
 #pragma unroll
-      for (int i = 0; i < MT; i += 2) {
-        if constexpr (I8) {  // tile i: elements i and 8 + i of each 16
+    for (int i = 0; i < MT; i += 2)
 #pragma unroll
-          for (int k = 0; k < 2; ++k)
-            *reinterpret_cast<float2*>(rec + e0 + 16 * (i >> 3) + 8 * k + (i & 7)) =
-                make_float2(element(i, k), element(i + 1, k));
-        } else {  // tile i: elements 2 i and 2 i + 1
-#pragma unroll
-          for (int k = 0; k < 2; ++k)
-            *reinterpret_cast<float2*>(rec + e0 + 2 * (i + k)) =
-                make_float2(element(i + k, 0), element(i + k, 1));
+      for (int k = 0; k < 2; ++k) {
+        float2 v = make_float2(element(i, k), element(i + 1, k));
+        if (y < nq && (PARTS == 2 || (t & 1) == k)) {
+          float2* at2 = reinterpret_cast<float2*>(rec + e0 + 16 * (i >> 3) + 8 * k + (i & 7));
+          if (more) v = make_float2(fmaf(at2->x, was, v.x), fmaf(at2->y, was, v.y));
+          *at2 = v;
         }
       }
-    }
   }
+  __syncwarp();
   }
   }
   if (P.pre_tensor) grid_dependency_wait();
@@ -772,8 +704,9 @@ __global__ void __launch_bounds__(32 * kWarps, rows_ctas<D, I8, NB>())
 
 // A block per query row: its records merged, back from the transformed
 // domain, divided by l, in the query's type.  What it takes is the time of a
-// few dependent loads, so each warp takes every fourth record and loads four
-// of them at once.
+// few dependent steps: which slots hold records is worked out before the wait
+// for them (the launch before can only have started when that was known), and
+// a warp takes every fourth, four at once.
 template <int D>
 __global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constant__ AttnParams P) {
   constexpr int J = D / 32, U = 4;
@@ -784,17 +717,17 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constan
   const uint32_t row = blockIdx.x;
   const uint32_t b = row / hq_all;
   const float* rec = r.workspace + (int64_t)row * P.plan.parts() * (D + 2);
-  grid_dependency_wait();
-  // slots of the units that the row's groups touch
+  if (P.plan.parts() == 0) grid_dependency_wait();
   const int hq = (int)(row - b * hq_all), h = hq / r.n_q, y = hq - h * r.n_q;
   auto slots = [&](int64_t begin, int64_t rows) {
-    return rows > 0 ? (int)((begin + rows - 1) / P.unit - begin / P.unit) + 1 : 0;
+    return rows > 0 ? (int)(P.unit_of(begin + rows - 1) - P.unit_of(begin)) + 1 : 0;
   };
-  const int n_pre = P.pre_tensor ? P.plan.pre_chunks
-                    : P.pre_blocks
-                        ? slots((int64_t)(h * P.pre_blocks + (b * r.n_q + y) / P.block) * r.prefix_len,
-                                r.prefix_len)
-                        : 0;
+  const int n_pre =
+      P.pre_tensor ? P.plan.pre_chunks
+      : P.pre_blocks
+          ? slots((int64_t)(h * P.pre_blocks + (int)((b * r.n_q + y) / P.block)) * r.prefix_len,
+                  r.prefix_len)
+          : 0;
   int n = n_pre;
   if (P.plan.own_parts) {
     const int64_t first = P.starts[b], rows = P.starts[b + 1] - first;
@@ -802,55 +735,41 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constan
                    (int64_t)(h * P.own_blocks + y / P.block) * rows,
                rows);
   }
+  grid_dependency_wait();
   float mx = -INFINITY, l = 0.f, a[J];
 #pragma unroll
   for (int j = 0; j < J; ++j) a[j] = 0.f;
-  // 32 slots at a time: a lane each for m and l (0 where nothing was attended)
-  for (int p0 = 0; p0 < n; p0 += 32) {
-    const int i = p0 + lane, slot = i < n_pre ? i : i - n_pre + P.plan.pre_parts;
-    const float* mine = rec + (int64_t)(i < n ? slot : 0) * (D + 2);
-    const float mp = mine[0], lp = i < n ? mine[1] : 0.f;
-    uint32_t live = __ballot_sync(0xffffffffu, lp != 0.f);
-    if (!live) continue;
-    float top = lp != 0.f ? mp : -INFINITY;
+  for (int p0 = warp; p0 < n; p0 += 4 * U) {
+    float2 ml[U];
+    float v[U][J];
 #pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    top = fmaxf(top, mx);
-    const float old = mx == -INFINITY ? 0.f : ex2(mx - top), f = lp != 0.f ? ex2(mp - top) : 0.f;
+    for (int u = 0; u < U; ++u) {
+      const int i = min(p0 + 4 * u, n - 1), slot = i < n_pre ? i : i - n_pre + P.plan.pre_parts;
+      const float* q = rec + (int64_t)slot * (D + 2);
+      ml[u] = *reinterpret_cast<const float2*>(q);
+#pragma unroll
+      for (int j = 0; j < J; ++j) v[u][j] = q[2 + 32 * j + lane];
+    }
+    float top = mx;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (p0 + 4 * u >= n) ml[u].y = 0.f;
+      if (ml[u].y != 0.f) top = fmaxf(top, ml[u].x);  // else nothing was attended there
+    }
+    if (top == -INFINITY) continue;
+    const float old = ex2(mx - top);
     mx = top;
     l *= old;
 #pragma unroll
     for (int j = 0; j < J; ++j) a[j] *= old;
-    // this warp's share of them: every fourth
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (k < warp) live &= live - 1;
-    while (live) {
-      int q[U];
-      float v[U][J];
+    for (int u = 0; u < U; ++u)
+      if (ml[u].y != 0.f) {
+        const float f = ex2(ml[u].x - top);
+        l = fmaf(ml[u].y, f, l);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        q[u] = live ? __ffs(live) - 1 : -1;
-        live &= live - 1;
-        live &= live - 1;
-        live &= live - 1;
-        live &= live - 1;
-        const int at = __shfl_sync(0xffffffffu, slot, max(q[u], 0));
-#pragma unroll
-        for (int j = 0; j < J; ++j)
-          v[u][j] = q[u] >= 0 ? rec[(int64_t)at * (D + 2) + 2 + 32 * j + lane] : 0.f;
+        for (int j = 0; j < J; ++j) a[j] = fmaf(v[u][j], f, a[j]);
       }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const float fu = __shfl_sync(0xffffffffu, f, max(q[u], 0));
-        const float lu = __shfl_sync(0xffffffffu, lp, max(q[u], 0));
-        if (q[u] >= 0) {
-          l = fmaf(lu, fu, l);
-#pragma unroll
-          for (int j = 0; j < J; ++j) a[j] = fmaf(v[u][j], fu, a[j]);
-        }
-      }
-    }
   }
 #pragma unroll
   for (int j = 0; j < J; ++j) sums[warp][32 * j + lane] = a[j];
@@ -882,13 +801,11 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constan
   if (r.lse && lane == 0) r.lse[row] = l == 0.f ? -INFINITY : (top + log2f(l)) * kLn2;
 }
 
-template <int D, bool I8, bool EXTRA, int NB>
+template <int D, int PARTS, bool EXTRA, int NB>
 kh_status launch_rows(AttnParams P, cudaStream_t stream) {
   const PagedAttnRequest& r = P.r;
-  constexpr int NQ = NB * 4, KS = Frags<D, I8, NB>::kSteps;
-  using C = RowsCfg<D>;
-  auto kern = paged_rows_kernel<D, I8, EXTRA, NB>;
-  constexpr int kSmem = C::kRing + (NB * KS <= 8 ? 0 : kWarps * NB * KS * 256);
+  constexpr int NQ = NB * 8 / PARTS, kSmem = RowsCfg<D>::kRing;
+  auto kern = paged_rows_kernel<D, PARTS, EXTRA, NB>;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return KH_ECUDA;
   static std::once_flag once[64];
@@ -906,10 +823,16 @@ kh_status launch_rows(AttnParams P, cudaStream_t stream) {
   const int64_t groups = (int64_t)r.n_kv_heads * (P.pre_blocks + r.n_seqs * P.own_blocks);
   const int64_t pairs = (int64_t)r.n_kv_heads * (P.pre_blocks * r.prefix_len +
                                                  r.n_seqs * P.own_blocks * P.plan.own_rows);
-  if (groups > 0x7ffffff0ll || pairs / P.unit > 0x7ffffff0ll) return KH_EINVAL;
-  static_assert(sizeof(Frags<D, I8, NB>) <= kFragBytes, "workspace of the fragments");
+  if (groups > 0x7ffffff0ll || pairs / P.unit > 0x7ffffff0ll ||
+      pairs > (int64_t(1) << 62) / P.unit)
+    return KH_EINVAL;
+  static_assert(sizeof(Frags<D, NB>) <= kFragBytes, "workspace of the fragments");
+  if (P.pre_tensor) {
+    const kh_status st = launch_paged_queries(P, stream);
+    if (st != KH_OK) return st;
+  }
   if (P.plan.parts() > 0 &&
-      launch_programmatic(paged_prepare_kernel<D, I8, NB>, dim3((unsigned)(groups + 1)),
+      launch_programmatic(paged_prepare_kernel<D, PARTS, NB>, dim3((unsigned)(groups + 1)),
                           dim3(128), 0, stream, P) != cudaSuccess)
     return KH_ELAUNCH;
   if (P.pre_tensor) {
@@ -937,18 +860,19 @@ kh_status launch_dim(const AttnParams& P, cudaStream_t stream) {
   const PagedAttnRequest& r = P.r;
   const int64_t nq = P.plan.pre_parts > 0 && !P.pre_tensor ? r.n_seqs * r.n_q : r.n_q;
   constexpr int kTwo = D == 128 ? 2 : 1;  // column blocks a pass, where there are queries for two
-  // 32-bit queries need more than 16-bit parts, and so do units so long that
-  // a 32-bit integer could not hold a column's sum (255 x 128 a row)
-  const bool i8 = r.dtype != KH_F32 && P.unit <= 32768;
   const bool extra = r.softcap > 0.f || r.slopes;
-  auto go = [&](auto i8c, auto extrac) {
-    return nq > 4 ? launch_rows<D, decltype(i8c)::value, decltype(extrac)::value, kTwo>(P, stream)
-                  : launch_rows<D, decltype(i8c)::value, decltype(extrac)::value, 1>(P, stream);
+  auto go = [&](auto parts, auto with) {
+    constexpr int kParts = decltype(parts)::value;
+    return nq > 8 / kParts ? launch_rows<D, kParts, decltype(with)::value, kTwo>(P, stream)
+                           : launch_rows<D, kParts, decltype(with)::value, 1>(P, stream);
   };
-  const kh_status st = i8 ? (extra ? go(std::true_type{}, std::true_type{})
-                                   : go(std::true_type{}, std::false_type{}))
-                          : (extra ? go(std::false_type{}, std::true_type{})
-                                   : go(std::false_type{}, std::false_type{}));
+  using std::integral_constant;
+  const kh_status st =
+      r.dtype == KH_F32
+          ? (extra ? go(integral_constant<int, 4>{}, std::true_type{})
+                   : go(integral_constant<int, 4>{}, std::false_type{}))
+          : (extra ? go(integral_constant<int, 2>{}, std::true_type{})
+                   : go(integral_constant<int, 2>{}, std::false_type{}));
   if (st != KH_OK) return st;
   return cudaGetLastError() == cudaSuccess ? KH_OK : KH_ELAUNCH;
 }
@@ -960,21 +884,21 @@ constexpr int64_t kPrefixTensorRows = 33;
 
 // The workspace: the records; then, each 16-byte aligned, the sequences'
 // starts and first rows, the claim counter, the queries' fragments (blocks of
-// 4 queries at least, so n_q / 4 of them at most) and, of a tensor-core
+// 2 queries at least, so n_q / 2 of them at most) and, of a tensor-core
 // prefix, its transformed queries.
 struct Layout {
   int64_t starts, first, next, frags, queries, bytes;
 };
 Layout layout_of(const PagedPlan& p, int64_t n_seqs, int n_q, int n_kv_heads, int D) {
   auto up = [](int64_t x) { return (x + 15) / 16 * 16; };
-  const int64_t nq = n_seqs * n_q, blocks = (n_q + 3) / 4;
+  const int64_t nq = n_seqs * n_q, blocks = (n_q + 1) / 2;
   Layout l;
   l.starts = up(nq * n_kv_heads * p.parts() * (int64_t)(D + 2) * 4);
   l.first = l.starts + up((n_seqs + 1) * 8);
   l.next = l.first + up(n_seqs * 4);
   l.frags = l.next + 16;
   int64_t groups = p.own_parts > 0 ? n_seqs * blocks : 0;
-  if (p.pre_parts > 0) groups += (nq + 3) / 4;
+  if (p.pre_parts > 0) groups += (nq + 1) / 2;
   l.queries = l.frags + groups * n_kv_heads * kFragBytes;
   l.bytes = l.queries;
   if (p.pre_chunks > 0) l.bytes += paged_queries_bytes(nq, n_kv_heads, D);
@@ -1031,6 +955,7 @@ kh_status launch_paged_attn(const PagedAttnRequest& r, cudaStream_t stream) {
   P.div_mul = ((uint64_t(1) << P.div_shift) + r.page_size - 1) / r.page_size;
   P.pre_tensor = P.plan.pre_chunks > 0;
   P.unit = P.plan.unit;
+  P.unit_mul = ~uint64_t(0) / (uint64_t)P.unit + 1;
   const Layout l = layout_of(P.plan, r.n_seqs, r.n_q, r.n_kv_heads, r.D);
   uint8_t* ws = reinterpret_cast<uint8_t*>(r.workspace);
   P.starts = reinterpret_cast<int64_t*>(ws + l.starts);

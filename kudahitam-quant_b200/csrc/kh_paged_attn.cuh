@@ -20,6 +20,7 @@ struct AttnParams {
   int div_shift;
   // units and groups of the rows kernel (kh_paged_attn.cu)
   int64_t unit;
+  uint64_t unit_mul;  // floor(2^64 / unit) + 1: x / unit for x unit < 2^64
   int block, own_blocks, pre_blocks;  // queries of a block; blocks of a KV head
   int64_t* starts;
   int32_t* first_row;
@@ -29,6 +30,9 @@ struct AttnParams {
   uint16_t* queries;  // workspace of those: q~ in fp16, tile by tile
   uint32_t* err;
 
+  __device__ __forceinline__ int64_t unit_of(int64_t x) const {
+    return (int64_t)__umul64hi((uint64_t)x, unit_mul);
+  }
   __device__ __forceinline__ uint32_t page_div(uint32_t j) const {
     return (uint32_t)((j * div_mul) >> div_shift);
   }
@@ -47,6 +51,7 @@ __device__ __forceinline__ void st_any(void* p, int dtype, int64_t i, float v) {
 
 // Attention of every sequence's queries over the shared prefix, a record per
 // query row and chunk (kh_paged_prefix.cu).
+kh_status launch_paged_queries(const AttnParams& P, cudaStream_t stream);  // before it
 kh_status launch_paged_prefix(const AttnParams& P, cudaStream_t stream);
 int64_t paged_queries_bytes(int64_t nq, int n_kv_heads, int D);
 
@@ -122,9 +127,6 @@ __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-__device__ __forceinline__ float round_h(float x) { return __half2float(__float2half_rn(x)); }
-// Records: a weight above kMaxWeight (fp16 holds 65504) moves the reference.
-constexpr float kNoRef = -1e30f;     // reference exponent before the first row
-constexpr float kMaxWeight = 4096.f;
+constexpr float kNoRef = -1e30f;  // reference exponent before the first row
 
 }  // namespace kh

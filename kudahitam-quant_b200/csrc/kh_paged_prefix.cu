@@ -732,9 +732,6 @@ kh_status launch_typed(const AttnParams& P, cudaStream_t stream) {
   const dim3 grid((unsigned)P.plan.pre_chunks, (unsigned)P.r.n_kv_heads,
                   (unsigned)((nq + per - 1) / per));
   if (grid.y > 65535 || (nq + per - 1) / per > 65535) return KH_EINVAL;
-  if (launch_programmatic(paged_queries_kernel<D>, dim3(grid.z * C::MT * 4, grid.y), dim3(256), 0, stream,
-                          P) != cudaSuccess)
-    return KH_ELAUNCH;
   return launch_programmatic(kern, grid, dim3(C::kThreads), C::kSmem, stream, P) == cudaSuccess
              ? KH_OK
              : KH_ELAUNCH;
@@ -744,6 +741,22 @@ kh_status launch_typed(const AttnParams& P, cudaStream_t stream) {
 
 int64_t paged_queries_bytes(int64_t nq, int n_kv_heads, int D) {
   return D == 128 ? queries_bytes<128>(nq, n_kv_heads) : queries_bytes<256>(nq, n_kv_heads);
+}
+
+template <int D>
+static kh_status launch_queries(const AttnParams& P, cudaStream_t stream) {
+  using C = PreCfg<D>;
+  const int64_t nq = P.r.n_seqs * P.r.n_q, per = 128 * C::MT;
+  const int64_t groups = (nq + per - 1) / per;
+  if (groups * C::MT * 4 > 0x7fffffffll) return KH_EINVAL;
+  return launch_programmatic(paged_queries_kernel<D>,
+                             dim3((unsigned)(groups * C::MT * 4), (unsigned)P.r.n_kv_heads),
+                             dim3(256), 0, stream, P) == cudaSuccess
+             ? KH_OK
+             : KH_ELAUNCH;
+}
+kh_status launch_paged_queries(const AttnParams& P, cudaStream_t stream) {
+  return P.r.D == 128 ? launch_queries<128>(P, stream) : launch_queries<256>(P, stream);
 }
 
 kh_status launch_paged_prefix(const AttnParams& P, cudaStream_t stream) {

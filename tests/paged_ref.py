@@ -99,7 +99,8 @@ def check(got, lse, want, dtype):
     """Holds an output (and lse, or None) to the accuracy that the operators document.
 
     A score is off by at most `ds` (the cap and the bias do not enlarge that):
-      fp32 queries: 2^-20 |q| |K| sm_scale (two fp16 parts, sums in 32 bits);
+      fp32 queries: 2^-20 |q| |K| sm_scale (32-bit transforms, q~ in 32-bit fixed
+      point, sums of whole numbers);
       16-bit ones: q~ in fixed point, off by 2^-13 of its largest element for a
       quarter of the elements, half of that for the next and so on, in the
       2-norm sqrt(D / 4 (1 + 1/4 + 1/16 + 1/64)) 2^-13 max |q~|, which is under
@@ -107,9 +108,9 @@ def check(got, lse, want, dtype):
       two operands rounded to fp16, 2^-11 |q| |K| sm_scale.
     p is off by twice that, relatively, as numerator and denominator move
     apart.  The weighted sum adds `dw` sum p |V_hat| (2^-20; 2^-11 for bf16, two
-    fp16 operands) and, for 16-bit queries, roundings to 2^-14 (half of that
-    at most) of the largest weight of a unit: independent, so the root of their
-    number counts, 1 / sqrt(12) of a step each; a whole 2^-14 is 7 deviations.
+    fp16 operands) and roundings of the weights to 2^-14 (2^-21 for fp32 queries)
+    of the largest weight of a unit: independent, so the root of their number
+    counts, 1 / sqrt(12) of a step each; a whole 2^-14 is over 3 deviations.
     The output's own rounding is half a step."""
     out, ref_lse, spread, reach, peak, largest = want
     ds, dw = 2.0 ** -20 * reach, 2.0 ** -20
@@ -117,7 +118,7 @@ def check(got, lse, want, dtype):
         ds = ds + 2.0 ** -13.7 * peak
     if dtype == torch.bfloat16:
         ds, dw = torch.maximum(ds, 2.0 ** -11 * reach), 2.0 ** -11
-    extra = 2.0 ** -14 * largest if dtype != torch.float32 else 0
+    extra = 2.0 ** (-21 if dtype == torch.float32 else -14) * largest
     got = got.detach().cpu().double()
     # a value past the type's largest rounds to an infinity of its sign
     over = torch.isinf(got) & (out.abs() >= torch.finfo(dtype).max) & (got.sign() == out.sign())

@@ -262,6 +262,27 @@ def test_decode_caps_biases_windows_and_starts(dtype, D, nq, kw):
     _attend(lengths, 2, nq, D, dtype, 48, seed=nq, pad=3, **kw)
 
 
+@pytest.mark.parametrize("dtype,D", [(BF, 128), (HF, 256), (FL, 128)])
+def test_decode_units_of_half_a_million_rows(dtype, D):
+    """So many query rows that each gets a few records only, and one sequence of
+    a million rows: five pages over and over, which is attention over the five
+    once."""
+    page, pages, times, B, nq = 500, 5, 420, 80, 256
+    n = page * pages
+    kc, vc, dk, dv, c = R.pools(pages, 1, page, D, 21)
+    table = torch.arange(pages, dtype=torch.int32).repeat(B, times)
+    lengths = [n * times] + [3] * (B - 1)
+    q = torch.randn(B, nq, D, generator=torch.Generator().manual_seed(21)) / 8
+    q = q.to(dtype)
+    out, lse = ops.paged_decode_attention(q.cuda(), R.cuda(kc), R.cuda(vc), table.cuda(),
+                                          torch.tensor(lengths, dtype=torch.int32).cuda(), dk, dv,
+                                          c, return_lse=True)
+    few = q[:2, :3]
+    want = list(R.attention(few, kc, vc, table[:2], [n, 3], dk, dv, c))
+    want[1][0] += math.log(times)
+    R.check(out[:2, :3], lse[:2, :3], want, dtype)
+
+
 def test_decode_negative_scale_and_large_values():
     """A negative scale, and rows whose norms span many orders."""
     _attend([400, 90], 1, 4, 128, FL, 16, seed=5, sm_scale=-0.2)
@@ -278,6 +299,25 @@ def test_decode_negative_scale_and_large_values():
                                               torch.tensor(lengths, dtype=torch.int32).cuda(), dk,
                                               dv, c, return_lse=True)
         R.check(out, lse, R.attention(q, kc, vc, table, lengths, dk, dv, c), dtype)
+
+
+@pytest.mark.parametrize("dtype,D,B,nq", [(BF, 128, 3, 4), (FL, 256, 2, 2), (BF, 128, 12, 4),
+                                          (BF, 256, 20, 2)])
+def test_attention_with_uneven_levels(dtype, D, B, nq):
+    """A caller's codebook need not be symmetric, nor around zero."""
+    prefix, page = 200, 16
+    lengths = [prefix + 30 + b for b in range(B)]
+    kc, vc, dk, dv, _ = R.pools(prefix // page + 1 + 6 * B, 1, page, D, 8)
+    c = torch.tensor([-0.3, 1.7])
+    table = R.tables(lengths, page, kc.shape[0], 8, prefix // page * page)
+    g = torch.Generator().manual_seed(8)
+    q = torch.randn(B, nq, D, generator=g).to(dtype)
+    a = (q.cuda(), R.cuda(kc), R.cuda(vc), table.cuda(),
+         torch.tensor(lengths, dtype=torch.int32).cuda())
+    want = R.attention(q, kc, vc, table, lengths, dk, dv, c)
+    R.check(*ops.paged_decode_attention(*a, dk, dv, c, return_lse=True), want, dtype)
+    R.check(*ops.paged_prefix_attention(*a, prefix // page * page, dk, dv, c, return_lse=True),
+            want, dtype)
 
 
 @pytest.mark.parametrize("dtype,D,H,nq,page,prefix,suffix", [
