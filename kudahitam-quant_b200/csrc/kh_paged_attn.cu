@@ -698,8 +698,8 @@ __global__ void __launch_bounds__(32 * kWarps, rows_ctas<D, NB>())
   __syncwarp();
   }
   }
+  grid_dependents_launch();
   if (P.pre_tensor) grid_dependency_wait();
-  else grid_dependents_launch();
 }
 
 // A block per query row: its records merged, back from the transformed

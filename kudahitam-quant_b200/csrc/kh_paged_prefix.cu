@@ -360,16 +360,15 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
     const float inv_sd = P.inv_sd;
     float down = 1.f;
     // two tiles' rows on their way while one is decoded, their pages one ahead
-    Row ahead[2];
-    ahead[0] = fetch(0, page_of(0));
-    ahead[1] = fetch(1, page_of(1));
+    Row now = fetch(0, page_of(0)), next = fetch(1, page_of(1));
     int page = page_of(2);
-#pragma unroll 2
+#pragma unroll 1
     for (int t = 0; t < n_tiles; ++t) {
       const int s = t % NS;
       const uint32_t ph = (uint32_t)((t / NS) & 1);
-      const Row x = ahead[t & 1];
-      ahead[t & 1] = fetch(t + 2, page);
+      Row x = now;
+      now = next;
+      next = fetch(t + 2, page);
       page = page_of(t + 3);
       float ka = x.kn, kb = x.krn * inv_sd;
       float va = x.vn * inv_sd, vb = x.vrn * (0.7978845608028654f * inv_sd * inv_sd);
@@ -420,33 +419,44 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
       kb *= ki * kTileScale;
       va *= vi * kTileScale;
       vb *= vi * kTileScale;
-      if (!__all_sync(0xffffffffu, mbar_wait(&kempty[s], ph ^ 1u, P.err))) break;
-      write(sm + C::kOffK + s * C::kKvTile, x.kc, x.kr, ka * c_half, kb, ka * r.c0 - kb);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&kfull[s]);
-      if (t == 0) {
-        // everything before the queries' launch was done when this grid could
-        // start, so only their scale has to be waited for
-        grid_dependency_wait();
-        down = 1.f / *reinterpret_cast<const float*>(group + MT * C::kQTile);
+      // Keys, then values, through the same code: written out twice (and for
+      // two tiles) it did not stay in the instruction cache beside the softmax.
+      bool in = true;
+#pragma unroll 1
+      for (int kv = 0; kv < 2; ++kv) {
+        in = __all_sync(0xffffffffu, mbar_wait(kv ? &vempty[s] : &kempty[s], ph ^ 1u, P.err));
+        if (!in) break;
+        write(sm + (kv ? C::kOffV : C::kOffK) + s * C::kKvTile, x.kc, x.kr, ka * c_half, kb,
+              ka * r.c0 - kb);
+        if (kv == 0 && t == 0) {
+          // everything before the queries' launch was done when this grid could
+          // start, so only their scale has to be waited for
+          grid_dependency_wait();
+          down = 1.f / *reinterpret_cast<const float*>(group + MT * C::kQTile);
+        }
+        if (kv == 1 && part == 0) {
+          float* sc = reinterpret_cast<float*>(sm + C::kOffScale) + s * 2 * ROWS;
+          sc[row] = kappa * (down / kTileScale);
+          sc[ROWS + row] = rv;
+          const uint32_t mask = __ballot_sync(0xffffffffu, x.on);
+          if (lane == 0)
+            reinterpret_cast<uint32_t*>(sm + C::kOffValid)[s * 4 + (row >> 5)] = mask;
+          if (i == 0)
+            *reinterpret_cast<float4*>(sm + C::kOffEven + 16 * s) =
+                make_float4(kappa * (down / kTileScale), vi, (float)ve, even ? 1.f : 0.f);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(kv ? &vfull[s] : &kfull[s]);
+        ka = va;
+        kb = vb;
+#pragma unroll
+        for (int w = 0; w < WT; ++w) {
+          x.kc[w] = x.vc[w];
+          x.kr[w] = x.vr[w];
+        }
       }
-      if (!__all_sync(0xffffffffu, mbar_wait(&vempty[s], ph ^ 1u, P.err))) break;
-      write(sm + C::kOffV + s * C::kKvTile, x.vc, x.vr, va * c_half, vb, va * r.c0 - vb);
-      if (part == 0) {
-        float* sc = reinterpret_cast<float*>(sm + C::kOffScale) + s * 2 * ROWS;
-        sc[row] = kappa * (down / kTileScale);
-        sc[ROWS + row] = rv;
-        const uint32_t mask = __ballot_sync(0xffffffffu, x.on);
-        if (lane == 0)
-          reinterpret_cast<uint32_t*>(sm + C::kOffValid)[s * 4 + (row >> 5)] = mask;
-        if (i == 0)
-          *reinterpret_cast<float4*>(sm + C::kOffEven + 16 * s) =
-              make_float4(kappa * (down / kTileScale), vi, (float)ve, even ? 1.f : 0.f);
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&vfull[s]);
+      if (!in) break;
     }
   } else if (warp >= C::kSoftWarps + 4) {
     // ------------------------------------------------------------ products
@@ -552,7 +562,6 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
       };
       // 32 columns at a time; their weights take the columns of scores already
       // read (half as many), so a chunk's own scores stay until it is settled
-      auto load = [&](int c, float (&x)[32]) { tmem_ld32(scores + 32 * c, x); };
       // a score as an exponent of two, without the reference
       auto exponent = [&](int j, float x, float k) {
         x *= k;
@@ -605,13 +614,12 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
         return total <= kMostSum && sum < 0x1p60f;
       };
       const bool all_whole = __all_sync(0xffffffffu, whole);
-      float v[2][32];
-      if (!EXTRA) load(0, v[0]);  // the next chunk loads while one is weighed
-      auto chunk = [&](int c, float (&x)[32], float (&next)[32]) {
-        if (EXTRA) load(c, x);  // no registers left for two
+#pragma unroll 1
+      for (int c = 0; c < ROWS / 32; ++c) {
+        float x[32];
+        tmem_ld32(scores + 32 * c, x);
         tmem_wait_ld();
         tmem_pin(x);
-        if (!EXTRA && c + 1 < ROWS / 32) load(c + 1, next);
         const uint32_t on = all_whole ? 0xffffffffu : places(c);
 #pragma unroll 1
         for (bool again = false;; again = true) {
@@ -658,11 +666,6 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
         }
         l += lt;
         tmem_st16(scores + 16 * c, p);
-      };
-#pragma unroll 1
-      for (int c = 0; c < ROWS / 32; c += 2) {
-        chunk(c, v[0], v[1]);
-        chunk(c + 1, v[1], v[0]);
       }
       if (!ok) break;
       tmem_wait_st();
