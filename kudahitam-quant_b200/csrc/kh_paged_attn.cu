@@ -162,7 +162,62 @@ __device__ __forceinline__ void mma16832u(int (&c)[4], uint32_t a0, uint32_t a1,
 constexpr int64_t kFragBytes = 2176;  // of a group's Frags, at most
 
 
-// Block 0: starts, first rows, the counter.  The others: a group each.
+// Sixteen query rows of a KV head as the tensor-core prefix's operand: element
+// e at position 2 (e & 15) + (e >> 4 & 1) of its block of 32, 128-byte blocks
+// swizzled; times log_scale and a power of two that brings the row's largest
+// under 2^14 (fp16 holds elements 2^28 below that with full steps).
+template <int D>
+__device__ __forceinline__ void write_query_tiles(const AttnParams& P, int64_t block, int lane,
+                                                  int warp) {
+  using Q = QueryTiles<D>;
+  constexpr int W = D / 32, GROUP = Q::MT * 128;
+  const PagedAttnRequest& r = P.r;
+  const int64_t n_rows = r.n_seqs * r.n_q, per = (n_rows + GROUP - 1) / GROUP * (GROUP / 16);
+  const int h = (int)(block / per);
+  const int64_t first = (block - h * per) * 16 + warp * 4;
+  uint8_t* group = reinterpret_cast<uint8_t*>(P.queries) +
+                   (h * (per / (GROUP / 16)) + first / GROUP) * (int64_t)Q::kGroup;
+  float x[4][W];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int64_t i = first + k, b = i / r.n_q;
+    const int64_t row = (b * r.n_kv_heads + h) * r.n_q + (i - b * r.n_q);
+#pragma unroll
+    for (int j = 0; j < W; ++j)
+      x[k][j] = i < n_rows ? ld_any(r.q, r.dtype, row * D + 32 * j + lane) : 0.f;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int y = (int)((first + k) % GROUP);
+    float mx = 0.f;
+#pragma unroll
+    for (int j = 0; j < W; ++j)
+      if ((r.dk_neg[j] >> lane) & 1) x[k][j] = -x[k][j];
+    fwht_lanes<W>(x[k], lane);
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      x[k][j] *= P.log_scale;
+      mx = fmaxf(mx, fabsf(x[k][j]));
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    int e = 14;
+    if (mx > 0.f && mx < INFINITY) frexpf(mx, &e);
+    const float up = ldexpf(1.f, max(-120, min(120, 14 - e)));
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      const int pos = 32 * j + 2 * (lane & 15) + (lane >> 4);
+      const int c = (pos & 63) >> 3;
+      *reinterpret_cast<__half*>(group + (y >> 7) * Q::kTile + (pos >> 6) * (128 * 128) +
+                                 (y & 127) * 128 + ((c ^ (y & 7)) << 4) + (pos & 7) * 2) =
+          __float2half_rn(x[k][j] * up);
+    }
+    if (lane == 0) reinterpret_cast<float*>(group + Q::MT * Q::kTile)[y] = up;
+  }
+}
+
+// Block 0: starts, first rows, the counter.  Then a group each; then, where the
+// prefix goes to the tensor cores, sixteen rows of its operand each.
 template <int D, int PARTS, int NB>
 __global__ void __launch_bounds__(128) paged_prepare_kernel(const __grid_constant__ AttnParams P) {
   using F = Frags<D, NB>;
@@ -171,9 +226,7 @@ __global__ void __launch_bounds__(128) paged_prepare_kernel(const __grid_constan
   __shared__ float qs[NQ][D];
   __shared__ int64_t part[4];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  // Behind the launch that transforms a tensor-core prefix's queries, which
-  // signals once all earlier work is done, this one waits at its end only.
-  if (!P.pre_tensor) grid_dependency_wait();
+  grid_dependency_wait();
   grid_dependents_launch();
   if (blockIdx.x == 0) {
     if (threadIdx.x == 0) *P.next_unit = 0u;
@@ -203,10 +256,13 @@ __global__ void __launch_bounds__(128) paged_prepare_kernel(const __grid_constan
       if (b < r.n_seqs) P.starts[b] = before + upto - n;
     }
     if (threadIdx.x == 0) P.starts[r.n_seqs] = base;
-    if (P.pre_tensor) grid_dependency_wait();
     return;
   }
   const int64_t gi = blockIdx.x - 1;
+  if (gi >= P.groups) {
+    write_query_tiles<D>(P, gi - P.groups, lane, warp);
+    return;
+  }
   const Group grp = group_of(P, gi);
   const int64_t y0 = (int64_t)grp.z * NQ;
   const int nq = (int)min((int64_t)NQ, (grp.pre ? r.n_seqs * r.n_q : (int64_t)r.n_q) - y0);
@@ -262,7 +318,6 @@ __global__ void __launch_bounds__(128) paged_prepare_kernel(const __grid_constan
       }
     out->q[k][lane] = make_uint2(f[0], f[1]);
   }
-  if (P.pre_tensor) grid_dependency_wait();
 }
 
 // Sequence b with starts[b] * per <= x < starts[b + 1] * per: a warp looks at
@@ -823,16 +878,16 @@ kh_status launch_rows(AttnParams P, cudaStream_t stream) {
   const int64_t groups = (int64_t)r.n_kv_heads * (P.pre_blocks + r.n_seqs * P.own_blocks);
   const int64_t pairs = (int64_t)r.n_kv_heads * (P.pre_blocks * r.prefix_len +
                                                  r.n_seqs * P.own_blocks * P.plan.own_rows);
-  if (groups > 0x7ffffff0ll || pairs / P.unit > 0x7ffffff0ll ||
+  constexpr int kGroup = 128 * QueryTiles<D>::MT;
+  const int64_t tiles =
+      P.pre_tensor ? r.n_kv_heads * ((r.n_seqs * r.n_q + kGroup - 1) / kGroup) * (kGroup / 16) : 0;
+  P.groups = groups;
+  if (groups + tiles > 0x7ffffff0ll || pairs / P.unit > 0x7ffffff0ll ||
       pairs > (int64_t(1) << 62) / P.unit)
     return KH_EINVAL;
   static_assert(sizeof(Frags<D, NB>) <= kFragBytes, "workspace of the fragments");
-  if (P.pre_tensor) {
-    const kh_status st = launch_paged_queries(P, stream);
-    if (st != KH_OK) return st;
-  }
   if (P.plan.parts() > 0 &&
-      launch_programmatic(paged_prepare_kernel<D, PARTS, NB>, dim3((unsigned)(groups + 1)),
+      launch_programmatic(paged_prepare_kernel<D, PARTS, NB>, dim3((unsigned)(groups + tiles + 1)),
                           dim3(128), 0, stream, P) != cudaSuccess)
     return KH_ELAUNCH;
   if (P.pre_tensor) {
@@ -901,7 +956,9 @@ Layout layout_of(const PagedPlan& p, int64_t n_seqs, int n_q, int n_kv_heads, in
   if (p.pre_parts > 0) groups += (nq + 1) / 2;
   l.queries = l.frags + groups * n_kv_heads * kFragBytes;
   l.bytes = l.queries;
-  if (p.pre_chunks > 0) l.bytes += paged_queries_bytes(nq, n_kv_heads, D);
+  if (p.pre_chunks > 0)
+    l.bytes += D == 128 ? (nq + 255) / 256 * n_kv_heads * QueryTiles<128>::kGroup
+                        : (nq + 127) / 128 * n_kv_heads * QueryTiles<256>::kGroup;
   return l;
 }
 int64_t paged_workspace_bytes(const PagedPlan& p, int64_t n_seqs, int n_q, int n_kv_heads, int D) {

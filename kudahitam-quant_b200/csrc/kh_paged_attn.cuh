@@ -22,6 +22,7 @@ struct AttnParams {
   int64_t unit;
   uint64_t unit_mul;  // floor(2^64 / unit) + 1: x / unit for x unit < 2^64
   int block, own_blocks, pre_blocks;  // queries of a block; blocks of a KV head
+  int64_t groups;
   int64_t* starts;
   int32_t* first_row;
   uint32_t* next_unit;
@@ -51,9 +52,16 @@ __device__ __forceinline__ void st_any(void* p, int dtype, int64_t i, float v) {
 
 // Attention of every sequence's queries over the shared prefix, a record per
 // query row and chunk (kh_paged_prefix.cu).
-kh_status launch_paged_queries(const AttnParams& P, cudaStream_t stream);  // before it
 kh_status launch_paged_prefix(const AttnParams& P, cudaStream_t stream);
-int64_t paged_queries_bytes(int64_t nq, int n_kv_heads, int D);
+
+// Its operand in the workspace: a KV head's query rows in groups of MT tiles of
+// 128, then the group's scales, a float a row.
+template <int D>
+struct QueryTiles {
+  static constexpr int MT = D == 128 ? 2 : 1;
+  static constexpr int kTile = 128 * D * 2;  // bytes
+  static constexpr int kGroup = MT * (kTile + 512);
+};
 
 // Length of sequence b, within what the table and max_len hold.
 __device__ __forceinline__ int64_t length_of(const AttnParams& P, int64_t b) {

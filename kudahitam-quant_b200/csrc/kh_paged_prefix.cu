@@ -41,15 +41,15 @@ constexpr int kRegsSoft = 176, kRegsDecode = 112, kRegsIssue = 48;
 
 template <int D>
 struct PreCfg {
-  static constexpr int MT = D == 128 ? 2 : 1;          // query tiles
+  static constexpr int MT = QueryTiles<D>::MT;         // query tiles
   static constexpr int ROWS = D == 128 ? 128 : 64;     // cached rows a tile
   static constexpr int SB = D == 128 ? 1 : 2;          // score buffers of a query tile
   static constexpr int kBoxes = D / 64;                // 64-element blocks of a row
-  static constexpr int kQTile = kBoxes * 128 * 128;    // bytes
+  static constexpr int kQTile = QueryTiles<D>::kTile;  // bytes
   static constexpr int kKvBox = ROWS * 128;
   static constexpr int kKvTile = kBoxes * kKvBox;
   static constexpr int kStages = 2;                    // of K^ and of V^
-  static constexpr int kGroup = MT * kQTile + 16;      // a CTA's queries in the workspace
+  static constexpr int kGroup = QueryTiles<D>::kGroup; // a CTA's queries in the workspace
   static constexpr int kOffK = MT * kQTile;
   static constexpr int kOffV = kOffK + kStages * kKvTile;
   static constexpr int kOffScale = kOffV + kStages * kKvTile;  // {kappa, r} of ROWS columns
@@ -95,98 +95,6 @@ constexpr float kTileScale = 0x1p-11f;
 
 // fp16 ends at 65504; 32 weights with this sum are all below it.
 constexpr float kMostSum = 32768.f;
-
-// Queries are stored times a power of two that keeps the largest |q~| of the
-// CTA under 2^14: fp16 holds elements 2^28 below that with full steps.
-__device__ __forceinline__ float query_scale(float bound) {
-  int e = 0;
-  if (bound > 0.f && bound < INFINITY) frexpf(bound, &e);
-  return ldexpf(1.f, max(-120, min(120, 14 - e)));
-}
-
-// Q~ of a KV head's query rows, as the products' operand: groups of 128 MT
-// rows in tiles of 128, element e at position 2 (e & 15) + (e >> 4 & 1) of its
-// block of 32, 128-byte blocks swizzled; times log_scale and a power of two,
-// which the 4 bytes behind the group hold.  Once per call, not per chunk: the
-// transforms of 256 rows cost one CTA 4 us, as much as a chunk's products.
-// A block transforms 32 rows, and reads its whole group for the power of two
-// rather than wait for other blocks.
-template <int D>
-__global__ void __launch_bounds__(256) paged_queries_kernel(const __grid_constant__ AttnParams P) {
-  using C = PreCfg<D>;
-  constexpr int W = D / 32, GROUP = C::MT * 128;
-  const PagedAttnRequest& r = P.r;
-  __shared__ float most[8];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h = blockIdx.y;
-  const int n_rows = (int)(r.n_seqs * r.n_q);
-  const int y0 = blockIdx.x / (GROUP / 32) * GROUP;
-  const int first = blockIdx.x % (GROUP / 32) * 32 + warp * 4;  // of the group
-  const uint16_t* q16 = static_cast<const uint16_t*>(r.q);
-  grid_dependency_wait();
-  grid_dependents_launch();
-  auto row_of = [&](int y) {
-    const int i = y0 + y, b = i / r.n_q;
-    return q16 + ((int64_t)b * r.n_kv_heads * r.n_q + h * r.n_q + (i - b * r.n_q)) * D;
-  };
-  float x[4][W], mx = 0.f;
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-#pragma unroll
-    for (int j = 0; j < W; ++j)
-      x[k][j] = y0 + first + k < n_rows
-                    ? __uint_as_float((uint32_t)row_of(first + k)[32 * j + lane] << 16)
-                    : 0.f;
-  // lanes 8 to a row; 16 bytes a lane where q's alignment allows
-  const int in_group = min(GROUP, n_rows - y0);
-  if ((reinterpret_cast<uintptr_t>(q16) & 15) == 0) {
-#pragma unroll 4
-    for (int y = warp * 4 + (lane >> 3); y < in_group; y += 32) {
-      const uint4* src = reinterpret_cast<const uint4*>(row_of(y));
-#pragma unroll
-      for (int k = 0; k < D / 64; ++k) {
-        const uint4 v = __ldg(src + 8 * k + (lane & 7));
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          mx = fmaxf(fmaxf(mx, fabsf(__uint_as_float(w[i] << 16))),
-                     fabsf(__uint_as_float(w[i] & 0xffff0000u)));
-      }
-    }
-  } else {
-    for (int y = warp; y < in_group; y += 8)
-#pragma unroll
-      for (int j = 0; j < W; ++j)
-        mx = fmaxf(mx, fabsf(__uint_as_float((uint32_t)row_of(y)[32 * j + lane] << 16)));
-  }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  if (lane == 0) most[warp] = mx;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < 8; ++w) mx = fmaxf(mx, most[w]);
-  const float up = query_scale(mx * (float)D * fabsf(P.log_scale));
-  uint8_t* group = reinterpret_cast<uint8_t*>(P.queries) +
-                   (int64_t)(h * (gridDim.x / (GROUP / 32)) + blockIdx.x / (GROUP / 32)) * C::kGroup;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int y = first + k, row = y & 127;
-#pragma unroll
-    for (int j = 0; j < W; ++j)
-      if ((r.dk_neg[j] >> lane) & 1) x[k][j] = -x[k][j];
-    fwht_lanes<W>(x[k], lane);
-#pragma unroll
-    for (int j = 0; j < W; ++j) {
-      const int pos = 32 * j + 2 * (lane & 15) + (lane >> 4);
-      const int c = (pos & 63) >> 3;
-      *reinterpret_cast<__half*>(group + (y >> 7) * C::kQTile + (pos >> 6) * (128 * 128) +
-                                 row * 128 + ((c ^ (row & 7)) << 4) + (pos & 7) * 2) =
-          __float2half_rn(x[k][j] * (P.log_scale * up));
-    }
-  }
-  if (blockIdx.x % (GROUP / 32) == 0 && threadIdx.x == 0)
-    *reinterpret_cast<float*>(group + C::MT * C::kQTile) = up;
-}
 
 template <int N>
 __device__ __forceinline__ void more_registers() {
@@ -259,6 +167,8 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
 
   if (warp >= C::kSoftWarps && warp < C::kSoftWarps + 4) {
     // ------------------------------------------------------------ decoding
+    // (no wait: what was before the queries' launch was done when this grid
+    // could start)
     if constexpr (D == 128) fewer_registers<kRegsDecode>();
     const int i = threadIdx.x - 32 * C::kSoftWarps;  // row of the tile
     // at D = 256 a row is two threads', half its words each
@@ -358,7 +268,6 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
       return m;
     };
     const float inv_sd = P.inv_sd;
-    float down = 1.f;
     // two tiles' rows on their way while one is decoded, their pages one ahead
     Row now = fetch(0, page_of(0)), next = fetch(1, page_of(1));
     int page = page_of(2);
@@ -428,22 +337,16 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
         if (!in) break;
         write(sm + (kv ? C::kOffV : C::kOffK) + s * C::kKvTile, x.kc, x.kr, ka * c_half, kb,
               ka * r.c0 - kb);
-        if (kv == 0 && t == 0) {
-          // everything before the queries' launch was done when this grid could
-          // start, so only their scale has to be waited for
-          grid_dependency_wait();
-          down = 1.f / *reinterpret_cast<const float*>(group + MT * C::kQTile);
-        }
         if (kv == 1 && part == 0) {
           float* sc = reinterpret_cast<float*>(sm + C::kOffScale) + s * 2 * ROWS;
-          sc[row] = kappa * (down / kTileScale);
+          sc[row] = kappa * (1.f / kTileScale);
           sc[ROWS + row] = rv;
           const uint32_t mask = __ballot_sync(0xffffffffu, x.on);
           if (lane == 0)
             reinterpret_cast<uint32_t*>(sm + C::kOffValid)[s * 4 + (row >> 5)] = mask;
           if (i == 0)
             *reinterpret_cast<float4*>(sm + C::kOffEven + 16 * s) =
-                make_float4(kappa * (down / kTileScale), vi, (float)ve, even ? 1.f : 0.f);
+                make_float4(kappa * (1.f / kTileScale), vi, (float)ve, even ? 1.f : 0.f);
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -527,6 +430,8 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
     asm volatile("cp.async.wait_all;" ::: "memory");
     fence_proxy_async_smem();
     mbar_arrive(qfull);
+    // q~ is stored times log_scale and a power of two
+    const float down = 1.f / reinterpret_cast<const float*>(group + MT * C::kQTile)[y];
     int q_lo = 0, q_hi = 0;
     float slope = 0.f;
     if (y < nq) {
@@ -577,13 +482,14 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
       auto weigh_even = [&](int c, const float (&x)[32]) {
         float2 sum = make_float2(0.f, 0.f);
         const float shift = tile.z - ref;
-        const float2 kk = make_float2(tile.x, tile.x), sh = make_float2(shift, shift);
+        const float k = tile.x * down;
+        const float2 kk = make_float2(k, k), sh = make_float2(shift, shift);
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
           float2 y;
           if constexpr (EXTRA)
-            y = __fadd2_rn(make_float2(exponent(32 * c + i, x[i], tile.x),
-                                       exponent(32 * c + i + 1, x[i + 1], tile.x)), sh);
+            y = __fadd2_rn(make_float2(exponent(32 * c + i, x[i], k),
+                                       exponent(32 * c + i + 1, x[i + 1], k)), sh);
           else
             y = __ffma2_rn(make_float2(x[i], x[i + 1]), kk, sh);
           const float2 w = (i & 6) == 2 ? ex2_poly(y) : make_float2(ex2(y.x), ex2(y.y));
@@ -603,7 +509,7 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
 #pragma unroll
           for (int o = 0; o < 2; ++o) {
             const int j = 32 * c + i + o;
-            const float e = on >> (i + o) & 1 ? ex2(exponent(j, x[i + o], kap[j]) - ref) : 0.f;
+            const float e = on >> (i + o) & 1 ? ex2(exponent(j, x[i + o], kap[j] * down) - ref) : 0.f;
             w[o] = on >> (i + o) & 1 ? e * rv[j] : 0.f;  // whatever the row's norms hold
             sum += e;
             total += w[o];
@@ -631,7 +537,7 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             const int j = 32 * c + i;
-            const float y = exponent(j, x[i], kap[j]) + lg2(fmaxf(rv[j], 0x1p-40f));
+            const float y = exponent(j, x[i], kap[j] * down) + lg2(fmaxf(rv[j], 0x1p-40f));
             if (on >> i & 1) top = fmaxf(top, y);
           }
           const float to = fmaxf(ref, top), f = ex2(ref - to);
@@ -715,12 +621,6 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
   }
 }
 
-template <int D>
-int64_t queries_bytes(int64_t nq, int n_kv_heads) {
-  using C = PreCfg<D>;
-  return (nq + 128 * C::MT - 1) / (128 * C::MT) * n_kv_heads * C::kGroup;
-}
-
 template <int D, bool EXTRA>
 kh_status launch_typed(const AttnParams& P, cudaStream_t stream) {
   using C = PreCfg<D>;
@@ -741,26 +641,6 @@ kh_status launch_typed(const AttnParams& P, cudaStream_t stream) {
 }
 
 }  // namespace
-
-int64_t paged_queries_bytes(int64_t nq, int n_kv_heads, int D) {
-  return D == 128 ? queries_bytes<128>(nq, n_kv_heads) : queries_bytes<256>(nq, n_kv_heads);
-}
-
-template <int D>
-static kh_status launch_queries(const AttnParams& P, cudaStream_t stream) {
-  using C = PreCfg<D>;
-  const int64_t nq = P.r.n_seqs * P.r.n_q, per = 128 * C::MT;
-  const int64_t groups = (nq + per - 1) / per;
-  if (groups * C::MT * 4 > 0x7fffffffll) return KH_EINVAL;
-  return launch_programmatic(paged_queries_kernel<D>,
-                             dim3((unsigned)(groups * C::MT * 4), (unsigned)P.r.n_kv_heads),
-                             dim3(256), 0, stream, P) == cudaSuccess
-             ? KH_OK
-             : KH_ELAUNCH;
-}
-kh_status launch_paged_queries(const AttnParams& P, cudaStream_t stream) {
-  return P.r.D == 128 ? launch_queries<128>(P, stream) : launch_queries<256>(P, stream);
-}
 
 kh_status launch_paged_prefix(const AttnParams& P, cudaStream_t stream) {
   const bool extra = P.r.softcap > 0.f || P.r.slopes;
