@@ -59,16 +59,15 @@ struct PagedAttnRequest {
   float* lse;  // may be null
 };
 
-// How a call's rows are cut.  Every query row has parts() record slots: those
-// of the shared prefix, then those of its own rows.
+// How a call's rows are cut, from what the host knows of it.
 struct PagedPlan {
-  int pre_parts = 0, own_parts = 0;  // slots
-  int64_t own_rows = 0;              // most own rows of a sequence
-  int64_t unit = 64;                 // pairs of a row and a group that a warp claims
-  // the prefix on the tensor cores: chunks of pre_rows rows, a slot each
+  // the rows kernel: query rows of a group, groups of a KV head (the prefix's,
+  // and a sequence's own), their rows at most, units at most
+  int block = 1, pre_blocks = 0, own_blocks = 0;
+  int64_t pre_rows = 0, own_rows = 0, groups = 0, pairs = 0, max_units = 0;
+  // the prefix on the tensor cores: chunks of chunk_rows rows
   int pre_chunks = 0;
-  int64_t pre_rows = 0;
-  __host__ __device__ int parts() const { return pre_parts + own_parts; }
+  int64_t chunk_rows = 0;
 };
 PagedPlan paged_plan(int64_t n_seqs, int n_q, int n_kv_heads, int D, int64_t max_len,
                      int64_t prefix_len, int64_t window, int dtype, int n_sms);

@@ -102,15 +102,18 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 // All (group, row) pairs of the call lie one after another: first the prefix's
 // groups (KV head, block of NQ of every sequence's query rows), then for each
 // sequence its groups (KV head, block of NQ of its own).  They are cut into
-// units of equal length, which the warps claim one by one: lengths live on the
-// device, and neither CTAs with a chunk of a fixed length nor equal ranges per
-// CTA kept the GPU busy to the end (an SM's CTAs progress unevenly, and one
-// left alone runs at a third of the SM's rate).  A unit may hold pieces of
-// several groups; a group has a record slot for every unit it touches.
+// units of equal length, which the warps claim one by one: one for every warp
+// that the GPU holds, up to kRounds where that leaves them long.  Lengths live
+// on the device, so the cut is made there: units from what max_len allows left
+// a quarter of the SM time idle on the ragged batch, CTAs with a chunk of a
+// fixed length more.  A unit may hold pieces of several groups; piece (unit u,
+// group G) has record u + G, as a unit's or a group's begin starts a new piece.
 //
 // What the claims need is prepared by a launch before: where each sequence's
-// pairs start, its first row, the claim counter, and each group's queries as
-// operand fragments.
+// pairs start, its first row, the units, and each group's queries as operand
+// fragments.
+constexpr int kRounds = 4;
+
 template <int D, int NB>
 struct Frags {  // of a group
   static constexpr int kSteps = D / 32;
@@ -126,9 +129,9 @@ struct Group {
 };
 __device__ __forceinline__ Group group_of(const AttnParams& P, int64_t i) {
   Group g;
-  const int64_t n_pre = (int64_t)P.r.n_kv_heads * P.pre_blocks;
+  const int64_t n_pre = (int64_t)P.r.n_kv_heads * P.plan.pre_blocks;
   g.pre = i < n_pre;
-  const int blocks = g.pre ? P.pre_blocks : P.own_blocks;
+  const int blocks = g.pre ? P.plan.pre_blocks : P.plan.own_blocks;
   const int64_t per = (int64_t)P.r.n_kv_heads * blocks, x = g.pre ? i : i - n_pre;
   g.b = g.pre ? 0 : x / per;
   const int hz = (int)(x - g.b * per);
@@ -229,7 +232,6 @@ __global__ void __launch_bounds__(128) paged_prepare_kernel(const __grid_constan
   grid_dependency_wait();
   grid_dependents_launch();
   if (blockIdx.x == 0) {
-    if (threadIdx.x == 0) *P.next_unit = 0u;
     int64_t base = 0;
     for (int64_t b0 = 0; b0 < r.n_seqs; b0 += 128) {
       const int64_t b = b0 + threadIdx.x;
@@ -255,12 +257,23 @@ __global__ void __launch_bounds__(128) paged_prepare_kernel(const __grid_constan
       }
       if (b < r.n_seqs) P.starts[b] = before + upto - n;
     }
-    if (threadIdx.x == 0) P.starts[r.n_seqs] = base;
+    if (threadIdx.x == 0) {
+      P.starts[r.n_seqs] = base;
+      const int64_t total =
+          r.n_kv_heads * (P.plan.pre_blocks * P.plan.pre_rows + base * P.plan.own_blocks);
+      const int64_t each = total / (P.n_warps * 512);
+      const int64_t n = P.n_warps * max((int64_t)1, min(each, (int64_t)kRounds));
+      Units u;
+      u.size = max((int64_t)64, ((total + n - 1) / n + 31) / 32 * 32);
+      u.mul = ~uint64_t(0) / (uint64_t)u.size + 1;
+      u.next = 0;
+      *P.units = u;
+    }
     return;
   }
   const int64_t gi = blockIdx.x - 1;
-  if (gi >= P.groups) {
-    write_query_tiles<D>(P, gi - P.groups, lane, warp);
+  if (gi >= P.plan.groups) {
+    write_query_tiles<D>(P, gi - P.plan.groups, lane, warp);
     return;
   }
   const Group grp = group_of(P, gi);
@@ -357,25 +370,24 @@ __global__ void __launch_bounds__(32 * kWarps, rows_ctas<D, NB>())
   const int g = lane >> 2, t = lane & 3;
   const int mine = PARTS == 2 ? t : t >> 1;   // this lane's query of a block
   const bool low = PARTS == 4 && (t & 1);     // it holds the query's low bytes
-  const int hq_all = r.n_kv_heads * r.n_q;
   uint8_t* ring = smem + warp * kStages * C::kStage;
   // After a prefix launch this grid may run beside it: that one signals its
   // dependents once all earlier work is done, and nothing here reads its
   // records.  The wait then comes at the end, so that this grid's completion
   // implies the prefix's.
   if (!P.pre_tensor) grid_dependency_wait();
-  const int64_t n_pre = (int64_t)r.n_kv_heads * P.pre_blocks * r.prefix_len;
-  const int64_t per = (int64_t)r.n_kv_heads * P.own_blocks;
+  const int64_t n_pre = r.n_kv_heads * P.plan.pre_blocks * P.plan.pre_rows;
+  const int64_t per = (int64_t)r.n_kv_heads * P.plan.own_blocks, size = P.units->size;
   const int64_t total = n_pre + P.starts[r.n_seqs] * per;
 
 #pragma unroll 1
   for (;;) {
   uint32_t unit = 0;
-  if (lane == 0) unit = atomicAdd(P.next_unit, 1u);
+  if (lane == 0) unit = atomicAdd(&P.units->next, 1u);
   unit = __shfl_sync(0xffffffffu, unit, 0);
-  int64_t at = (int64_t)unit * P.unit;
+  int64_t at = (int64_t)unit * size;
   if (at >= total) break;
-  const int64_t end = min(at + P.unit, total);
+  const int64_t end = min(at + size, total);
 #pragma unroll 1
   while (at < end) {
   // ---- the piece: rows [lo, hi) of a sequence (or of the prefix, for every
@@ -383,20 +395,19 @@ __global__ void __launch_bounds__(32 * kWarps, rows_ctas<D, NB>())
   const bool pre = at < n_pre;
   const int64_t b = pre ? 0 : find_sequence(P, at - n_pre, per, lane);
   const int64_t start = pre ? 0 : n_pre + P.starts[b] * per;
-  const int64_t rows = pre ? r.prefix_len : P.starts[b + 1] - P.starts[b];
+  const int64_t rows = pre ? P.plan.pre_rows : P.starts[b + 1] - P.starts[b];
   const int hz = (int)((at - start) / rows);
   const int64_t begin = start + hz * rows;
   const int lo = (pre ? 0 : P.first_row[b]) + (int)(at - begin);
   const int hi = lo + (int)min(min(rows - (at - begin), end - at), kPieceRows);
-  const bool more = at > begin && at > (int64_t)unit * P.unit;  // the slot holds rows already
+  const bool more = at > begin && at > (int64_t)unit * size;  // the record holds rows already
   at += hi - lo;
-  const int blocks = pre ? P.pre_blocks : P.own_blocks;
+  const int blocks = pre ? P.plan.pre_blocks : P.plan.own_blocks;
   const int h = hz / blocks;
   const int64_t y0 = (int64_t)(hz - h * blocks) * NQ;
   const int nq = (int)min((int64_t)NQ, (pre ? r.n_seqs * r.n_q : (int64_t)r.n_q) - y0);
-  const int part = (int)(unit - P.unit_of(begin)) + (pre ? 0 : P.plan.pre_parts);
-  const F* frags = reinterpret_cast<const F*>(P.frags) +
-                              (pre ? hz : r.n_kv_heads * P.pre_blocks + b * per + hz);
+  const int64_t group = pre ? hz : r.n_kv_heads * P.plan.pre_blocks + b * per + hz;
+  const F* frags = reinterpret_cast<const F*>(P.frags) + group;
   auto seq_of = [&](int y) { return pre ? (y0 + y) / r.n_q : b; };
   auto head_of = [&](int y) { return h * r.n_q + (int)(pre ? (y0 + y) % r.n_q : y0 + y); };
 
@@ -711,9 +722,7 @@ __global__ void __launch_bounds__(32 * kWarps, rows_ctas<D, NB>())
       w2s[nb] += __shfl_xor_sync(0xffffffffu, w2s[nb], o);
     }
     const int y = nb * QB + mine;
-    float* rec = r.workspace +
-                 ((y < nq ? seq_of(y) * hq_all + head_of(y) : 0) * P.plan.parts() + part) *
-                     (int64_t)(D + 2);
+    float* rec = P.records + ((unit + group) * NQ + y) * (int64_t)(D + 2);
     float is = 1.f / kOne, was = 0.f;
     if (more && y < nq) {  // joins the record
       const float2 old = *reinterpret_cast<const float2*>(rec);
@@ -771,25 +780,39 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constan
   const int hq_all = r.n_kv_heads * r.n_q;
   const uint32_t row = blockIdx.x;
   const uint32_t b = row / hq_all;
-  const float* rec = r.workspace + (int64_t)row * P.plan.parts() * (D + 2);
-  if (P.plan.parts() == 0) grid_dependency_wait();
+  if (!P.plan.pre_chunks && P.plan.groups == 0) grid_dependency_wait();
   const int hq = (int)(row - b * hq_all), h = hq / r.n_q, y = hq - h * r.n_q;
-  auto slots = [&](int64_t begin, int64_t rows) {
-    return rows > 0 ? (int)(P.unit_of(begin + rows - 1) - P.unit_of(begin)) + 1 : 0;
+  constexpr int64_t kRec = D + 2;
+  const int64_t stride = P.plan.block * kRec;
+  // record 0 and how many there are of the prefix, and of the sequence's own rows
+  struct Run {
+    const float* at;
+    int n;
   };
-  const int n_pre =
-      P.pre_tensor ? P.plan.pre_chunks
-      : P.pre_blocks
-          ? slots((int64_t)(h * P.pre_blocks + (int)((b * r.n_q + y) / P.block)) * r.prefix_len,
-                  r.prefix_len)
-          : 0;
-  int n = n_pre;
-  if (P.plan.own_parts) {
-    const int64_t first = P.starts[b], rows = P.starts[b + 1] - first;
-    n += slots(((int64_t)P.pre_blocks * r.prefix_len + first * P.own_blocks) * r.n_kv_heads +
-                   (int64_t)(h * P.own_blocks + y / P.block) * rows,
-               rows);
+  auto run = [&](int64_t begin, int64_t rows, int64_t group, int place) {
+    if (rows <= 0) return Run{P.records, 0};
+    const int64_t u = P.units->of(begin);
+    return Run{P.records + (u + group) * stride + place * kRec,
+               (int)(P.units->of(begin + rows - 1) - u) + 1};
+  };
+  Run pre{P.records, 0}, own{P.records, 0};
+  int64_t pre_stride = stride;
+  if (P.plan.pre_chunks) {
+    pre = Run{r.workspace + (int64_t)row * P.plan.pre_chunks * kRec, P.plan.pre_chunks};
+    pre_stride = kRec;
+  } else if (P.plan.pre_blocks) {
+    const uint32_t i = b * r.n_q + y, z = i / P.plan.block;
+    const int64_t group = (int64_t)h * P.plan.pre_blocks + z;
+    pre = run(group * P.plan.pre_rows, P.plan.pre_rows, group, i - z * P.plan.block);
   }
+  if (P.plan.own_blocks) {
+    const int64_t first = P.starts[b], rows = P.starts[b + 1] - first;
+    const int z = y / P.plan.block, hz = h * P.plan.own_blocks + z;
+    const int64_t per = (int64_t)r.n_kv_heads * P.plan.own_blocks;
+    own = run(r.n_kv_heads * P.plan.pre_blocks * P.plan.pre_rows + first * per + hz * rows, rows,
+              r.n_kv_heads * P.plan.pre_blocks + b * per + hz, y - z * P.plan.block);
+  }
+  const int n = pre.n + own.n;
   grid_dependency_wait();
   float mx = -INFINITY, l = 0.f, a[J];
 #pragma unroll
@@ -799,8 +822,8 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constan
     float v[U][J];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = min(p0 + 4 * u, n - 1), slot = i < n_pre ? i : i - n_pre + P.plan.pre_parts;
-      const float* q = rec + (int64_t)slot * (D + 2);
+      const int i = min(p0 + 4 * u, n - 1);
+      const float* q = i < pre.n ? pre.at + i * pre_stride : own.at + (i - pre.n) * stride;
       ml[u] = *reinterpret_cast<const float2*>(q);
 #pragma unroll
       for (int j = 0; j < J; ++j) v[u][j] = q[2 + 32 * j + lane];
@@ -871,22 +894,19 @@ kh_status launch_rows(AttnParams P, cudaStream_t stream) {
         cudaSuccess)
       ctas[dev & 63] = 0;
   });
-  P.block = NQ;
-  P.own_blocks = P.plan.own_parts > 0 ? (r.n_q + NQ - 1) / NQ : 0;
-  P.pre_blocks =
-      P.plan.pre_parts > 0 && !P.pre_tensor ? (int)((r.n_seqs * r.n_q + NQ - 1) / NQ) : 0;
-  const int64_t groups = (int64_t)r.n_kv_heads * (P.pre_blocks + r.n_seqs * P.own_blocks);
-  const int64_t pairs = (int64_t)r.n_kv_heads * (P.pre_blocks * r.prefix_len +
-                                                 r.n_seqs * P.own_blocks * P.plan.own_rows);
   constexpr int kGroup = 128 * QueryTiles<D>::MT;
   const int64_t tiles =
       P.pre_tensor ? r.n_kv_heads * ((r.n_seqs * r.n_q + kGroup - 1) / kGroup) * (kGroup / 16) : 0;
-  P.groups = groups;
-  if (groups + tiles > 0x7ffffff0ll || pairs / P.unit > 0x7ffffff0ll ||
-      pairs > (int64_t(1) << 62) / P.unit)
+  const int64_t groups = P.plan.groups, pairs = P.plan.pairs;
+  if (P.plan.block != NQ || groups + tiles > 0x7ffffff0ll || pairs >= int64_t(1) << 36)
     return KH_EINVAL;
+  const int64_t grid =
+      std::min<int64_t>((int64_t)std::min(std::max(1, ctas[dev & 63]), rows_ctas<D, NB>()) *
+                            sm_count(),
+                        (pairs / 64 + kWarps) / kWarps);
+  P.n_warps = grid * kWarps;
   static_assert(sizeof(Frags<D, NB>) <= kFragBytes, "workspace of the fragments");
-  if (P.plan.parts() > 0 &&
+  if (groups + tiles > 0 &&
       launch_programmatic(paged_prepare_kernel<D, PARTS, NB>, dim3((unsigned)(groups + tiles + 1)),
                           dim3(128), 0, stream, P) != cudaSuccess)
     return KH_ELAUNCH;
@@ -895,9 +915,6 @@ kh_status launch_rows(AttnParams P, cudaStream_t stream) {
     if (st != KH_OK) return st;
   }
   if (pairs > 0) {
-    const int64_t units = (pairs + P.unit - 1) / P.unit;
-    const int64_t grid = std::min<int64_t>((int64_t)std::max(1, ctas[dev & 63]) * sm_count(),
-                                           (units + kWarps - 1) / kWarps);
     if (launch_programmatic(kern, dim3((unsigned)grid), dim3(32 * kWarps), kSmem, stream, P) !=
         cudaSuccess)
       return KH_ELAUNCH;
@@ -913,12 +930,11 @@ kh_status launch_rows(AttnParams P, cudaStream_t stream) {
 template <int D>
 kh_status launch_dim(const AttnParams& P, cudaStream_t stream) {
   const PagedAttnRequest& r = P.r;
-  const int64_t nq = P.plan.pre_parts > 0 && !P.pre_tensor ? r.n_seqs * r.n_q : r.n_q;
-  constexpr int kTwo = D == 128 ? 2 : 1;  // column blocks a pass, where there are queries for two
+  constexpr int kTwo = D == 128 ? 2 : 1;
   const bool extra = r.softcap > 0.f || r.slopes;
   auto go = [&](auto parts, auto with) {
     constexpr int kParts = decltype(parts)::value;
-    return nq > 8 / kParts ? launch_rows<D, kParts, decltype(with)::value, kTwo>(P, stream)
+    return P.plan.block > 8 / kParts ? launch_rows<D, kParts, decltype(with)::value, kTwo>(P, stream)
                            : launch_rows<D, kParts, decltype(with)::value, 1>(P, stream);
   };
   using std::integral_constant;
@@ -937,24 +953,22 @@ kh_status launch_dim(const AttnParams& P, cudaStream_t stream) {
 // From how many query rows a KV head's prefix is worth 128-row products.
 constexpr int64_t kPrefixTensorRows = 33;
 
-// The workspace: the records; then, each 16-byte aligned, the sequences'
-// starts and first rows, the claim counter, the queries' fragments (blocks of
-// 2 queries at least, so n_q / 2 of them at most) and, of a tensor-core
-// prefix, its transformed queries.
+// The workspace, each part 16-byte aligned: a tensor-core prefix's records, by
+// query row and chunk; the other records; the sequences' starts and first rows;
+// the units; the groups' fragments; a tensor-core prefix's queries.
 struct Layout {
-  int64_t starts, first, next, frags, queries, bytes;
+  int64_t records, starts, first, units, frags, queries, bytes;
 };
 Layout layout_of(const PagedPlan& p, int64_t n_seqs, int n_q, int n_kv_heads, int D) {
   auto up = [](int64_t x) { return (x + 15) / 16 * 16; };
-  const int64_t nq = n_seqs * n_q, blocks = (n_q + 1) / 2;
+  const int64_t nq = n_seqs * n_q, record = (D + 2) * 4;
   Layout l;
-  l.starts = up(nq * n_kv_heads * p.parts() * (int64_t)(D + 2) * 4);
+  l.records = up(nq * n_kv_heads * p.pre_chunks * record);
+  l.starts = l.records + up((p.max_units + p.groups) * p.block * record);
   l.first = l.starts + up((n_seqs + 1) * 8);
-  l.next = l.first + up(n_seqs * 4);
-  l.frags = l.next + 16;
-  int64_t groups = p.own_parts > 0 ? n_seqs * blocks : 0;
-  if (p.pre_parts > 0) groups += (nq + 1) / 2;
-  l.queries = l.frags + groups * n_kv_heads * kFragBytes;
+  l.units = l.first + up(n_seqs * 4);
+  l.frags = l.units + up(sizeof(Units));
+  l.queries = l.frags + p.groups * kFragBytes;
   l.bytes = l.queries;
   if (p.pre_chunks > 0)
     l.bytes += D == 128 ? (nq + 255) / 256 * n_kv_heads * QueryTiles<128>::kGroup
@@ -962,39 +976,33 @@ Layout layout_of(const PagedPlan& p, int64_t n_seqs, int n_q, int n_kv_heads, in
   return l;
 }
 int64_t paged_workspace_bytes(const PagedPlan& p, int64_t n_seqs, int n_q, int n_kv_heads, int D) {
-  return p.parts() > 0 ? layout_of(p, n_seqs, n_q, n_kv_heads, D).bytes : 0;
+  return p.pre_chunks || p.groups ? layout_of(p, n_seqs, n_q, n_kv_heads, D).bytes : 0;
 }
 
 PagedPlan paged_plan(int64_t n_seqs, int n_q, int n_kv_heads, int D, int64_t max_len,
                      int64_t prefix_len, int64_t window, int dtype, int n_sms) {
   PagedPlan p;
-  const int64_t rows = n_seqs * n_q * n_kv_heads, record = (D + 2) * 4;
   const int64_t pre = std::min(prefix_len, max_len), nq = n_seqs * n_q;
-  int64_t own = max_len - pre;
-  if (window > 0) own = std::min(own, window);
+  p.own_rows = max_len - pre;
+  if (window > 0) p.own_rows = std::min(p.own_rows, window);
   // the prefix's chunks on the tensor cores: one round of CTAs, one an SM, in
   // whole tiles
   if (pre > 0 && nq >= kPrefixTensorRows && dtype == KH_BF16) {
     const int64_t each = D == 128 ? 256 : 128, tile = D == 128 ? 128 : 64;
     const int64_t ctas = std::max<int64_t>(1, n_sms / (n_kv_heads * ((nq + each - 1) / each)));
-    p.pre_rows = ((pre + ctas - 1) / ctas + tile - 1) / tile * tile;
-    p.pre_chunks = (int)((pre + p.pre_rows - 1) / p.pre_rows);
+    p.chunk_rows = ((pre + ctas - 1) / ctas + tile - 1) / tile * tile;
+    p.pre_chunks = (int)((pre + p.chunk_rows - 1) / p.chunk_rows);
+  } else {
+    p.pre_rows = pre;
   }
-  // Units: three for every two warps (20 an SM) where the longest sequences
-  // give that many, so that the last ones end together; not under two tiles
-  // (a unit's fixed cost is about one tile's) nor over 64, and not so short
-  // that the records take over 64 MB (at least 6 slots a row).
-  const int64_t blocks = (n_q + 3) / 4;
-  const int64_t pairs = n_kv_heads * (n_seqs * blocks * own + (p.pre_chunks ? 0 : (nq + 3) / 4 * pre));
-  const int64_t room =
-      rows > 0 ? std::max<int64_t>(6, (int64_t(64) << 20) / (rows * record)) - 4 : 2;
-  int64_t unit = std::max<int64_t>(64, std::min<int64_t>(2048, pairs / (32 * (int64_t)n_sms)));
-  unit = std::max(unit, (own + (p.pre_chunks ? 0 : pre) + room - 1) / room);
-  p.unit = (unit + 31) / 32 * 32;
-  // a group touches at most this many units
-  if (pre > 0) p.pre_parts = p.pre_chunks ? p.pre_chunks : (int)(pre / p.unit + 2);
-  if (own > 0) p.own_parts = (int)(own / p.unit + 2);
-  p.own_rows = own;
+  // a column block's queries, or two blocks' where there are queries for them
+  const int64_t most = p.pre_rows > 0 ? nq : n_q, one = dtype == KH_F32 ? 2 : 4;
+  p.block = (int)(D == 128 && most > one ? 2 * one : one);
+  if (p.pre_rows > 0) p.pre_blocks = (int)((nq + p.block - 1) / p.block);
+  if (p.own_rows > 0) p.own_blocks = (n_q + p.block - 1) / p.block;
+  p.groups = n_kv_heads * (p.pre_blocks + n_seqs * p.own_blocks);
+  p.pairs = n_kv_heads * (p.pre_blocks * p.pre_rows + n_seqs * p.own_blocks * p.own_rows);
+  p.max_units = std::min<int64_t>((int64_t)kRounds * 5 * kWarps * n_sms, p.pairs / 64 + 1);
   return p;
 }
 
@@ -1011,13 +1019,12 @@ kh_status launch_paged_attn(const PagedAttnRequest& r, cudaStream_t stream) {
   P.div_shift = 31 + bits;
   P.div_mul = ((uint64_t(1) << P.div_shift) + r.page_size - 1) / r.page_size;
   P.pre_tensor = P.plan.pre_chunks > 0;
-  P.unit = P.plan.unit;
-  P.unit_mul = ~uint64_t(0) / (uint64_t)P.unit + 1;
   const Layout l = layout_of(P.plan, r.n_seqs, r.n_q, r.n_kv_heads, r.D);
   uint8_t* ws = reinterpret_cast<uint8_t*>(r.workspace);
   P.starts = reinterpret_cast<int64_t*>(ws + l.starts);
   P.first_row = reinterpret_cast<int32_t*>(ws + l.first);
-  P.next_unit = reinterpret_cast<uint32_t*>(ws + l.next);
+  P.units = reinterpret_cast<Units*>(ws + l.units);
+  P.records = reinterpret_cast<float*>(ws + l.records);
   P.frags = ws + l.frags;
   P.queries = reinterpret_cast<uint16_t*>(ws + l.queries);
   P.err = device_error_ptr();

@@ -10,6 +10,16 @@ namespace kh {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
+// How the rows kernel's (group, row) pairs are cut (kh_paged_attn.cu).
+struct Units {
+  int64_t size;
+  uint64_t mul;   // floor(2^64 / size) + 1: x / size while x size < 2^64
+  uint32_t next;  // unclaimed
+  __device__ __forceinline__ int64_t of(int64_t x) const {
+    return (int64_t)__umul64hi((uint64_t)x, mul);
+  }
+};
+
 struct AttnParams {
   PagedAttnRequest r;
   PagedPlan plan;
@@ -18,22 +28,17 @@ struct AttnParams {
   // shift = 31 + ceil(log2 page_size) (the error j (mul page_size - 2^shift) / 2^shift stays under 1)
   uint64_t div_mul;
   int div_shift;
-  // units and groups of the rows kernel (kh_paged_attn.cu)
-  int64_t unit;
-  uint64_t unit_mul;  // floor(2^64 / unit) + 1: x / unit for x unit < 2^64
-  int block, own_blocks, pre_blocks;  // queries of a block; blocks of a KV head
-  int64_t groups;
+  // of the rows kernel (kh_paged_attn.cu)
+  int64_t n_warps;
+  float* records;
   int64_t* starts;
   int32_t* first_row;
-  uint32_t* next_unit;
+  Units* units;
   void* frags;
   int pre_tensor;  // the prefix has its own launches (launch_paged_prefix)
   uint16_t* queries;  // workspace of those: q~ in fp16, tile by tile
   uint32_t* err;
 
-  __device__ __forceinline__ int64_t unit_of(int64_t x) const {
-    return (int64_t)__umul64hi((uint64_t)x, unit_mul);
-  }
   __device__ __forceinline__ uint32_t page_div(uint32_t j) const {
     return (uint32_t)((j * div_mul) >> div_shift);
   }

@@ -131,8 +131,8 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
   const int64_t n_rows = r.n_seqs * r.n_q;
   const int64_t y0 = (int64_t)blockIdx.z * (MT * 128);
   const int nq = (int)min((int64_t)(MT * 128), n_rows - y0);
-  const int lo = (int)(blockIdx.x * P.plan.pre_rows);
-  const int hi = (int)min(lo + P.plan.pre_rows, r.prefix_len);
+  const int lo = (int)(blockIdx.x * P.plan.chunk_rows);
+  const int hi = (int)min(lo + P.plan.chunk_rows, r.prefix_len);
   const int n_tiles = (hi - lo + ROWS - 1) / ROWS;
   const int hq_all = r.n_kv_heads * r.n_q;
 
@@ -599,7 +599,7 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
       }
     }
     __syncwarp();
-    const int64_t mine = y < nq ? (query_row(y) * P.plan.parts() + blockIdx.x) * (int64_t)(D + 2) : -1;
+    const int64_t mine = y < nq ? (query_row(y) * P.plan.pre_chunks + blockIdx.x) * (int64_t)(D + 2) : -1;
     if (!ok) l = 0.f;
 #pragma unroll 4
     for (int k = 0; k < 32; ++k) {

@@ -263,15 +263,15 @@ def test_decode_caps_biases_windows_and_starts(dtype, D, nq, kw):
 
 
 @pytest.mark.parametrize("dtype,D", [(BF, 128), (HF, 256), (FL, 128)])
-def test_decode_units_of_half_a_million_rows(dtype, D):
-    """So many query rows that each gets a few records only, and one sequence of
-    a million rows: five pages over and over, which is attention over the five
-    once."""
-    page, pages, times, B, nq = 500, 5, 420, 80, 256
+def test_decode_units_of_many_thousand_rows(dtype, D):
+    """So many rows that a unit is longer than what 32-bit sums hold: sequences
+    of a million rows, five pages over and over, which is attention over the
+    five once."""
+    page, pages, times, B, nq = 500, 5, 420, 8, 256
     n = page * pages
     kc, vc, dk, dv, c = R.pools(pages, 1, page, D, 21)
     table = torch.arange(pages, dtype=torch.int32).repeat(B, times)
-    lengths = [n * times] + [3] * (B - 1)
+    lengths = [n * times, 3] + [n * times - 1] * (B - 2)
     q = torch.randn(B, nq, D, generator=torch.Generator().manual_seed(21)) / 8
     q = q.to(dtype)
     out, lse = ops.paged_decode_attention(q.cuda(), R.cuda(kc), R.cuda(vc), table.cuda(),
