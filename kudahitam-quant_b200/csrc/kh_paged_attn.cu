@@ -350,7 +350,7 @@ __device__ __forceinline__ int64_t find_sequence(const AttnParams& P, int64_t x,
 // CTAs an SM that the registers are bounded for.
 template <int D, int NB>
 constexpr int rows_ctas() {
-  return D == 256 || NB == 2 ? 3 : 5;
+  return 3;
 }
 
 template <int D, int PARTS, bool EXTRA, int NB>
@@ -411,21 +411,27 @@ __global__ void __launch_bounds__(32 * kWarps, rows_ctas<D, NB>())
   auto seq_of = [&](int y) { return pre ? (y0 + y) / r.n_q : b; };
   auto head_of = [&](int y) { return h * r.n_q + (int)(pre ? (y0 + y) % r.n_q : y0 + y); };
 
-  // ---- tiles of 32 rows: lane = row
+  // ---- tiles of 32 rows: lane = row.  Its place in the table and in the page
+  // moves on by 32 rows a tile; pages are read a tile before they are used.
   const int n_tiles = (hi - lo + 31) >> 5;
   const int32_t* tab = r.table + b * r.table_stride;
-  auto page_of = [&](int tile) {
-    const uint32_t j = lo + tile * 32 + lane;
-    return (tile < n_tiles && (int)j < hi) ? tab[P.page_div(j)] : -1;
+  uint32_t block = P.page_div(lo + lane), off = lo + lane - block * r.page_size;
+  int left = hi - lo - lane;
+  auto take = [&](int& page, uint32_t& place) {
+    page = left > 0 ? tab[block] : -1;
+    place = off;
+    left -= 32;
+    block += P.step_blocks;
+    off += P.step_off;
+    if (off >= (uint32_t)r.page_size) {
+      off -= r.page_size;
+      ++block;
+    }
   };
-  auto issue = [&](int tile, int stage, int page) {
+  auto issue = [&](int tile, int stage, int page, uint32_t place) {
     if (tile < n_tiles) {
-      const uint32_t j = lo + tile * 32 + lane;
-      const bool in = (int)j < hi;
-      const bool on = in && (uint32_t)page < (uint32_t)r.n_pages;
-      if (in && !on) flag_error(P.err, kErrBadIndex);
-      const uint32_t off = j - P.page_div(j) * r.page_size;
-      const int64_t row = on ? ((int64_t)page * r.n_kv_heads + h) * r.page_size + off : 0;
+      const bool on = (uint32_t)page < (uint32_t)r.n_pages;
+      const int64_t row = on ? ((int64_t)page * r.n_kv_heads + h) * r.page_size + place : 0;
       uint8_t* st = ring + stage * C::kStage;
       const uint32_t s = smem_u32(st);
 #pragma unroll
@@ -443,12 +449,24 @@ __global__ void __launch_bounds__(32 * kWarps, rows_ctas<D, NB>())
       cp_async4(n + 12, r.vp.rnorms + row, on);
       const uint32_t mask = __ballot_sync(0xffffffffu, on);
       if (lane == 0) *reinterpret_cast<uint32_t*>(st + 4 * C::kPlane + 512) = mask;
+      // rows that there are, and pages that there are not
+      const int n_rows = hi - lo - 32 * tile;
+      if (mask != (n_rows >= 32 ? 0xffffffffu : (1u << n_rows) - 1u))
+        flag_error(P.err, kErrBadIndex);
     }
     cp_commit();
   };
+  int next_page;
+  uint32_t next_place;
+  {
+    int pages[kStages - 1];
+    uint32_t places[kStages - 1];
 #pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) issue(s, s, page_of(s));
-  int next_page = page_of(kStages - 1);
+    for (int s = 0; s < kStages - 1; ++s) take(pages[s], places[s]);
+    take(next_page, next_place);
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) issue(s, s, pages[s], places[s]);
+  }
 
   uint2 qf[NB * KS];
 #pragma unroll
@@ -500,17 +518,14 @@ __global__ void __launch_bounds__(32 * kWarps, rows_ctas<D, NB>())
   }
   const int pg = (g >> 1) + 4 * (g & 1);  // pi(g)
 
-#pragma unroll 1
-  for (int tile = 0; tile < n_tiles; ++tile) {
-    cp_wait<kStages - 2>();
-    __syncwarp();
-    const uint8_t* st = ring + (tile % kStages) * C::kStage;
-    const float4* nrm = reinterpret_cast<const float4*>(st + 4 * C::kPlane);
-    const uint32_t valid = *reinterpret_cast<const uint32_t*>(st + 4 * C::kPlane + 512);
-    const int j0 = lo + tile * 32;
-
-    // scores of the tile's two 16-row halves, both planes
-    int s1[2][NB][4], s2[2][NB][4];
+  // A tile's scores and a tile's values are independent: in the loop the next
+  // tile's scores and exponents run between this tile's value products.
+  int s1[2][NB][4], s2[2][NB][4];
+  float tt[2][2][NB], ra[2][2], rb[2][2], ee[2][2][NB];
+  uint32_t p1[2][NB], p2[2][NB];
+  bool full;
+  // scores of a tile's two 16-row halves, both planes
+  auto scores = [&](const uint8_t* st) {
 #pragma unroll
     for (int v = 0; v < W / 4; ++v) {
       uint32_t w[2][2][2];  // half, plane, row
@@ -544,8 +559,12 @@ __global__ void __launch_bounds__(32 * kWarps, rows_ctas<D, NB>())
       }
     }
 
-    // exponents
-    bool full = valid == 0xffffffffu;
+  };
+  // their exponents without the reference, -inf where nothing is attended
+  auto exponents = [&](const uint8_t* st, int j0) {
+    const float4* nrm = reinterpret_cast<const float4*>(st + 4 * C::kPlane);
+    const uint32_t valid = *reinterpret_cast<const uint32_t*>(st + 4 * C::kPlane + 512);
+    full = valid == 0xffffffffu;
     if (pre) {
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) full = full && j0 >= q_lo[nb] && j0 + 32 <= q_hi[nb];
@@ -558,7 +577,6 @@ __global__ void __launch_bounds__(32 * kWarps, rows_ctas<D, NB>())
       const float y = __shfl_xor_sync(0xffffffffu, x, 1);
       return low ? fmaf(y, 65536.f, x) : fmaf(x, 65536.f, y);
     };
-    float tt[2][2][NB], ra[2][2], rb[2][2];
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
@@ -586,66 +604,68 @@ __global__ void __launch_bounds__(32 * kWarps, rows_ctas<D, NB>())
           if (!on) tt[k >> 1][k & 1][nb] = -INFINITY;
         }
     }
-    // weights: e = 2^(t2 - ref); a row's larger weight decides whether they fit
-    float ee[2][2][NB];
-#pragma unroll 1
-    for (bool again = false;; again = true) {
-      float top = 0.f;
+  };
+  // weights e = 2^(t2 - ref); true where they fit: a row's larger one decides
+  auto weigh = [&] {
+    float top = 0.f;
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          const float e = ex2(tt[k >> 1][k & 1][nb] - ref[nb]);
-          ee[k >> 1][k & 1][nb] = e;
-          const float most = fmaxf(fmaxf(ra[k >> 1][k & 1], rb[k >> 1][k & 1]), kOne * 0x1p-40f);
-          // nothing attended: 0 times whatever the row's norms hold
-          top = fmaxf(top, e == 0.f ? 0.f : e * most);
-        }
-      if (again || !__any_sync(0xffffffffu, !(top <= kMost))) break;
+    for (int k = 0; k < 4; ++k)
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
-        float mx = kNoRef;
+        const float e = ex2(tt[k >> 1][k & 1][nb] - ref[nb]);
+        ee[k >> 1][k & 1][nb] = e;
+        const float most = fmaxf(fmaxf(ra[k >> 1][k & 1], rb[k >> 1][k & 1]), kOne * 0x1p-40f);
+        // nothing attended: 0 times whatever the row's norms hold
+        top = fmaxf(top, e == 0.f ? 0.f : e * most);
+      }
+    return top <= kMost;
+  };
+  // the reference moves up to the tile's largest, what has been summed follows
+  auto rescale = [&](bool first) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float most = fmaxf(fmaxf(ra[k >> 1][k & 1], rb[k >> 1][k & 1]), kOne * 0x1p-40f);
-          const float x = tt[k >> 1][k & 1][nb];
-          if (x > -INFINITY) mx = fmaxf(mx, x + lg2(most * (1.f / kOne)));
-        }
+    for (int nb = 0; nb < NB; ++nb) {
+      float mx = kNoRef;
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        if (mx == INFINITY) l[nb] = NAN;  // an infinite norm has no average
-        const float to = fmaxf(ref[nb], ceilf(mx)), f = ex2(ref[nb] - to);
-        int left = (int)fminf(to - ref[nb], 48.f);
-        ref[nb] = to;
-        if (tile == 0) continue;  // nothing summed yet
-        l[nb] *= f;
-        w1s[nb] *= f;
-        w2s[nb] *= f;
-        // sums move right; what a column loses its next lower one takes up
+      for (int k = 0; k < 4; ++k) {
+        const float most = fmaxf(fmaxf(ra[k >> 1][k & 1], rb[k >> 1][k & 1]), kOne * 0x1p-40f);
+        const float x = tt[k >> 1][k & 1][nb];
+        if (x > -INFINITY) mx = fmaxf(mx, x + lg2(most * (1.f / kOne)));
+      }
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      if (mx == INFINITY) l[nb] = NAN;  // an infinite norm has no average
+      const float to = fmaxf(ref[nb], ceilf(mx)), f = ex2(ref[nb] - to);
+      int left = (int)fminf(to - ref[nb], 48.f);
+      ref[nb] = to;
+      if (first) continue;  // nothing summed yet
+      l[nb] *= f;
+      w1s[nb] *= f;
+      w2s[nb] *= f;
+      // sums move right; what a column loses its next lower one takes up
 #pragma unroll 1
-        while (__any_sync(0xffffffffu, left > 0)) {
-          const int sh = min(left, 16);
-          const uint32_t lost = (1u << sh) - 1u, half = (1u << sh) >> 1;
-          left -= sh;
+      while (__any_sync(0xffffffffu, left > 0)) {
+        const int sh = min(left, 16);
+        const uint32_t lost = (1u << sh) - 1u, half = (1u << sh) >> 1;
+        left -= sh;
 #pragma unroll
-          for (int i = 0; i < MT; ++i)
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int k = 0; k < 4; k += 2) {
-              uint32_t h = acc[nb][i][k], o = acc[nb][i][k + 1];
-              if constexpr (PARTS == 2) {
-                o += ((h & lost) << 8) + half;
-              } else {  // the low lanes hold one column, in h
-                if (!low) o += (h & lost) << 8;
-                const uint32_t down = __shfl_xor_sync(0xffffffffu, o & lost, 1);
-                if (low) h += (down << 8) + half;
-              }
-              acc[nb][i][k] = (int)(h >> sh);
-              acc[nb][i][k + 1] = (int)(o >> sh);
+          for (int k = 0; k < 4; k += 2) {
+            uint32_t h = acc[nb][i][k], o = acc[nb][i][k + 1];
+            if constexpr (PARTS == 2) {
+              o += ((h & lost) << 8) + half;
+            } else {  // the low lanes hold one column, in h
+              if (!low) o += (h & lost) << 8;
+              const uint32_t down = __shfl_xor_sync(0xffffffffu, o & lost, 1);
+              if (low) h += (down << 8) + half;
             }
-        }
+            acc[nb][i][k] = (int)(h >> sh);
+            acc[nb][i][k + 1] = (int)(o >> sh);
+          }
       }
     }
-    uint32_t p1[2][NB], p2[2][NB];
+  };
+  auto pack = [&] {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       uint32_t i1 = 0u, i2 = 0u;
@@ -673,41 +693,67 @@ __global__ void __launch_bounds__(32 * kWarps, rows_ctas<D, NB>())
       w1s[nb] += (float)(i1 - 4u * 0x4B000000u);  // without the exponent fields
       w2s[nb] += (float)(i2 - 4u * 0x4B000000u);
     }
-
-    // values
+  };
+  auto values = [&](const uint8_t* st, int p) {
+    uint32_t x[2][W / 4], y[2][W / 4];  // even and odd bytes of four rows, by half
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      uint32_t x[2][W / 4], y[2][W / 4];  // even and odd bytes of four rows, by half
+    for (int hf = 0; hf < 2; ++hf) {
+      const uint32_t* pl = reinterpret_cast<const uint32_t*>(st + (2 + p) * C::kPlane) +
+                           (16 * hf + t) * W + (D == 128 ? g >> 1 : g);
+      const uint32_t r0 = pl[0], r1 = pl[8 * W], r2 = pl[4 * W], r3 = pl[12 * W];
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const uint32_t* pl = reinterpret_cast<const uint32_t*>(st + (2 + p) * C::kPlane) +
-                             (16 * hf + t) * W + (D == 128 ? g >> 1 : g);
-        const uint32_t r0 = pl[0], r1 = pl[8 * W], r2 = pl[4 * W], r3 = pl[12 * W];
+      for (int v = 0; v < W / 4; ++v) {
+        const uint32_t sel = (D == 128 ? (g & 1) : v) ? 0x7362u : 0x5140u;
+        const uint32_t a = __byte_perm(r0, r1, sel), b = __byte_perm(r2, r3, sel);
+        x[hf][v] = __byte_perm(a, b, 0x5410);
+        y[hf][v] = __byte_perm(a, b, 0x7632);
+      }
+    }
 #pragma unroll
-        for (int v = 0; v < W / 4; ++v) {
-          const uint32_t sel = (D == 128 ? (g & 1) : v) ? 0x7362u : 0x5140u;
-          const uint32_t a = __byte_perm(r0, r1, sel), b = __byte_perm(r2, r3, sel);
-          x[hf][v] = __byte_perm(a, b, 0x5410);
-          y[hf][v] = __byte_perm(a, b, 0x7632);
+    for (int v = 0; v < W / 4; ++v)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t m = 0x01010101u << i;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          const auto& f = p == 0 ? p1 : p2;
+          mma16832u(acc[nb][8 * v + i], x[0][v] & m, y[0][v] & m, x[1][v] & m, y[1][v] & m,
+                    f[0][nb], f[1][nb]);
         }
       }
-#pragma unroll
-      for (int v = 0; v < W / 4; ++v)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t m = 0x01010101u << i;
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            const auto& f = p == 0 ? p1 : p2;
-            mma16832u(acc[nb][8 * v + i], x[0][v] & m, y[0][v] & m, x[1][v] & m, y[1][v] & m,
-                      f[0][nb], f[1][nb]);
-          }
-        }
+  };
+  auto settle = [&](bool first) {
+    if (!__all_sync(0xffffffffu, weigh())) {
+      rescale(first);
+      weigh();
     }
+    pack();
+  };
+
+  cp_wait<kStages - 2>();
+  __syncwarp();
+  scores(ring);
+  exponents(ring, lo);
+  settle(true);
+  int stage = 0;
+#pragma unroll 1
+  for (int tile = 0; tile + 1 < n_tiles; ++tile) {
+    const uint8_t* st = ring + stage * C::kStage;
+    issue(tile + kStages - 1, stage == 0 ? kStages - 1 : stage - 1, next_page, next_place);
+    take(next_page, next_place);
+    stage = stage == kStages - 1 ? 0 : stage + 1;
+    cp_wait<kStages - 2>();
     __syncwarp();
-    issue(tile + kStages - 1, (tile + kStages - 1) % kStages, next_page);
-    next_page = page_of(tile + kStages);
+    const uint8_t* next = ring + stage * C::kStage;
+    scores(next);
+    values(st, 0);
+    exponents(next, lo + (tile + 1) * 32);
+    values(st, 1);
+    settle(false);
+    __syncwarp();
   }
+  values(ring + stage * C::kStage, 0);
+  values(ring + stage * C::kStage, 1);
   cp_wait<0>();
   __syncwarp();
 
@@ -1018,6 +1064,8 @@ kh_status launch_paged_attn(const PagedAttnRequest& r, cudaStream_t stream) {
   while ((int64_t(1) << bits) < r.page_size) ++bits;
   P.div_shift = 31 + bits;
   P.div_mul = ((uint64_t(1) << P.div_shift) + r.page_size - 1) / r.page_size;
+  P.step_blocks = 32 / r.page_size;
+  P.step_off = 32 % r.page_size;
   P.pre_tensor = P.plan.pre_chunks > 0;
   const Layout l = layout_of(P.plan, r.n_seqs, r.n_q, r.n_kv_heads, r.D);
   uint8_t* ws = reinterpret_cast<uint8_t*>(r.workspace);

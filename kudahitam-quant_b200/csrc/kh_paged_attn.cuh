@@ -28,6 +28,7 @@ struct AttnParams {
   // shift = 31 + ceil(log2 page_size) (the error j (mul page_size - 2^shift) / 2^shift stays under 1)
   uint64_t div_mul;
   int div_shift;
+  uint32_t step_blocks, step_off;  // 32 rows on: whole pages and the rest
   // of the rows kernel (kh_paged_attn.cu)
   int64_t n_warps;
   float* records;
