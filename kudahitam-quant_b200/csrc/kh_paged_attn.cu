@@ -814,15 +814,18 @@ __global__ void __launch_bounds__(32 * kWarps, rows_ctas<D, NB>())
 
 // A block per query row: its records merged, back from the transformed
 // domain, divided by l, in the query's type.  What it takes is the time of a
-// few dependent steps: which slots hold records is worked out before the wait
+// few dependent steps: which records there are is worked out before the wait
 // for them (the launch before can only have started when that was known), and
-// a warp takes every fourth, four at once.
+// a warp takes four at once.  4 warps; 8 or 16 where there are so few query
+// rows that the GPU holds them (a row of a long cache has a hundred records).
+constexpr int kMostJoin = 16;
 template <int D>
-__global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constant__ AttnParams P) {
+__global__ void __launch_bounds__(32 * kMostJoin)
+    paged_combine_kernel(const __grid_constant__ AttnParams P) {
   constexpr int J = D / 32, U = 4;
   const PagedAttnRequest& r = P.r;
-  __shared__ float sums[4][D], tops[4], ls[4];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ float sums[kMostJoin][D], tops[kMostJoin], ls[kMostJoin];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const int hq_all = r.n_kv_heads * r.n_q;
   const uint32_t row = blockIdx.x;
   const uint32_t b = row / hq_all;
@@ -863,12 +866,12 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constan
   float mx = -INFINITY, l = 0.f, a[J];
 #pragma unroll
   for (int j = 0; j < J; ++j) a[j] = 0.f;
-  for (int p0 = warp; p0 < n; p0 += 4 * U) {
+  for (int p0 = warp; p0 < n; p0 += warps * U) {
     float2 ml[U];
     float v[U][J];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = min(p0 + 4 * u, n - 1);
+      const int i = min(p0 + warps * u, n - 1);
       const float* q = i < pre.n ? pre.at + i * pre_stride : own.at + (i - pre.n) * stride;
       ml[u] = *reinterpret_cast<const float2*>(q);
 #pragma unroll
@@ -877,7 +880,7 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constan
     float top = mx;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (p0 + 4 * u >= n) ml[u].y = 0.f;
+      if (p0 + warps * u >= n) ml[u].y = 0.f;
       if (ml[u].y != 0.f) top = fmaxf(top, ml[u].x);  // else nothing was attended there
     }
     if (top == -INFINITY) continue;
@@ -903,12 +906,13 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constan
   }
   __syncthreads();
   if (warp) return;
-  const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  float top = tops[0];
+  for (int w = 1; w < warps; ++w) top = fmaxf(top, tops[w]);
   l = 0.f;
 #pragma unroll
   for (int j = 0; j < J; ++j) a[j] = 0.f;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
+#pragma unroll 4
+  for (int w = 0; w < warps; ++w) {
     if (tops[w] == -INFINITY) continue;
     const float f = ex2(tops[w] - top);
     l = fmaf(ls[w], f, l);
@@ -967,8 +971,9 @@ kh_status launch_rows(AttnParams P, cudaStream_t stream) {
   }
   const int64_t rows = r.n_seqs * r.n_kv_heads * r.n_q;
   if (rows > 0x7fffffffll) return KH_EINVAL;
-  return launch_programmatic(paged_combine_kernel<D>, dim3((unsigned)rows), dim3(128), 0, stream,
-                             P) == cudaSuccess
+  const int join = rows <= sm_count() ? kMostJoin : rows <= 4 * sm_count() ? 8 : 4;
+  return launch_programmatic(paged_combine_kernel<D>, dim3((unsigned)rows), dim3(32 * join), 0,
+                             stream, P) == cudaSuccess
              ? KH_OK
              : KH_ELAUNCH;
 }
@@ -996,8 +1001,17 @@ kh_status launch_dim(const AttnParams& P, cudaStream_t stream) {
 
 }  // namespace
 
-// From how many query rows a KV head's prefix is worth 128-row products.
-constexpr int64_t kPrefixTensorRows = 33;
+// Above how many query rows a KV head's prefix goes to the tensor cores: their
+// products have 128 query rows whatever there are, the rows kernel's time grows
+// with them.  Measured (us, rows kernel / tensor cores, 8 KV heads, bf16):
+//                 16 rows      32           48           64           128
+//   D 128, 1024   15.5 / 18.3  16.8 / 18.4  18.6 / 18.6  19.6 / 18.6  24.8 / 19.0
+//   D 128, 8192   24.3 / 30.9  33.0 / 30.2  40.7 / 31.1  51.6 / 30.7  88.0 / 31.8
+//   D 256, 1024   18.3 / 20.5  21.7 / 20.5  23.4 / 22.3  26.2 / 24.7  34.5 / 29.3
+//   D 256, 8192   33.1 / 33.9  51.0 / 32.7  66.9 / 34.8  87.6 / 34.0   132 / 35.1
+// (Of one KV head and 1024 rows the rows kernel stays ahead up to 64 query
+// rows, by 1 us at D 128 and 4 us at D 256.)
+int64_t prefix_tensor_rows(int D) { return D == 128 ? 32 : 16; }
 
 // The workspace, each part 16-byte aligned: a tensor-core prefix's records, by
 // query row and chunk; the other records; the sequences' starts and first rows;
@@ -1033,7 +1047,7 @@ PagedPlan paged_plan(int64_t n_seqs, int n_q, int n_kv_heads, int D, int64_t max
   if (window > 0) p.own_rows = std::min(p.own_rows, window);
   // the prefix's chunks on the tensor cores: one round of CTAs, one an SM, in
   // whole tiles
-  if (pre > 0 && nq >= kPrefixTensorRows && dtype == KH_BF16) {
+  if (pre > 0 && nq > prefix_tensor_rows(D) && dtype == KH_BF16) {
     const int64_t each = D == 128 ? 256 : 128, tile = D == 128 ? 128 : 64;
     const int64_t ctas = std::max<int64_t>(1, n_sms / (n_kv_heads * ((nq + each - 1) / each)));
     p.chunk_rows = ((pre + ctas - 1) / ctas + tile - 1) / tile * tile;
