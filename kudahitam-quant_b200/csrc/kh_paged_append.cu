@@ -233,11 +233,11 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const __grid_constant
 // needs to be, so that the lanes' 16-byte reads hit different banks.
 constexpr int kTileWarps = 4;
 constexpr int kTileCtas = 4;
-// From how many rows (tokens x heads) they come in tiles: fewer do not give the
+// From how many keys (tokens x heads) they come in tiles: fewer do not give the
 // 592 CTAs' warps a tile each.  Measured (us, a warp per row / tiles, bf16, whole
-// keys rotated), D 128: 4096 rows 6.9 / 10.1, 8192 11.2 / 9.4, 32768 36.1 / 14.0;
+// keys rotated), D 128: 4096 keys 6.9 / 10.1, 8192 11.2 / 9.4, 32768 36.1 / 14.0;
 // D 256: 4096 9.9 / 13.5, 8192 16.3 / 14.2, 32768 53.5 / 30.1.
-constexpr int64_t kTileRows = 8192;
+constexpr int64_t kTileRows = 6656;
 
 template <typename T>
 struct TileCfg {
@@ -586,7 +586,7 @@ bool tiles_fit(const PagedAppendRequest& r) {
 template <typename T, int D>
 kh_status launch_typed(const AppendParams& P, cudaStream_t stream) {
   const PagedAppendRequest& r = P.r;
-  if (r.n_tokens * r.n_kv_heads * 2 < kTileRows || !tiles_fit<T, D>(r))
+  if (r.n_tokens * r.n_kv_heads < kTileRows || !tiles_fit<T, D>(r))
     return launch_rows<T, D>(P, stream);
   if (!r.rot_dim) return launch_tiles<T, D, kNone>(P, stream);
   if (r.rot_dim < D) return launch_tiles<T, D, kPart>(P, stream);

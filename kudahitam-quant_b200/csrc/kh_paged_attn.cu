@@ -47,11 +47,14 @@ namespace {
 //     the largest of their unit, whose roundings average out; together under
 //     a tenth of a bf16 step.
 //   PARTS = 4 (32-bit queries, 2 a block): q~ to 2^-28, weights to 2^-22.
-// What bounds it is issue: 128 logic operations a 32-row tile at half rate,
-// and as many around them.  As fp16 products (two elements a logic operation,
-// half the rate of the products) it took 25 instructions a row and 63 us on
-// the ragged batch (32 sequences up to 8192 rows, 8 KV heads x 4), now 20 and
-// 42 us.
+// What bounds it is issue: a 32-row tile takes 128 logic operations at half
+// rate, 32 products of 7.5 cycles, and some 370 other instructions.  On a ragged
+// batch (32 sequences up to 8192 rows, 8 KV heads x 4, D 128, bf16) the kernel
+// takes 41 us (half of the cycles issue); as fp16 products, two elements a logic
+// operation, 63 us.  Two column blocks, where a KV head has queries for them,
+// take the same masked bits: 16 sequences of 4096 rows, 8 KV heads x 5 bf16
+// queries 33.9 us (one block at a time 37.6), x 16 54.9 (65.9), x 3 fp32 queries
+// 36.3 (39.8); at D 256 two blocks' sums do not fit the registers.
 //
 // A warp runs on its own: 32-row tiles in a ring of cp.async stages, one lane
 // fetching one row (so pages may end anywhere).  The reference exponent of a
@@ -102,17 +105,18 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 // All (group, row) pairs of the call lie one after another: first the prefix's
 // groups (KV head, block of NQ of every sequence's query rows), then for each
 // sequence its groups (KV head, block of NQ of its own).  They are cut into
-// units of equal length, which the warps claim one by one: one for every warp
-// that the GPU holds, up to kRounds where that leaves them long.  Lengths live
-// on the device, so the cut is made there: units from what max_len allows left
-// a quarter of the SM time idle on the ragged batch, CTAs with a chunk of a
-// fixed length more.  A unit may hold pieces of several groups; piece (unit u,
-// group G) has record u + G, as a unit's or a group's begin starts a new piece.
+// units of equal length, one for every warp that the GPU holds (two to four a
+// warp made more records and measured the same, or 119 us instead of 110 on 8
+// sequences up to 40000 rows), which the warps claim, as those beside a prefix
+// come late.  Lengths live on the device, so the cut is made there: units from
+// what max_len allows left a quarter of the SM time idle on the ragged batch,
+// CTAs with a chunk of a fixed length more.  A unit may hold pieces of several
+// groups; piece (unit u, group G) has record u + G, as a unit's or a group's
+// begin starts a new piece.
 //
 // What the claims need is prepared by a launch before: where each sequence's
 // pairs start, its first row, the units, and each group's queries as operand
 // fragments.
-constexpr int kRounds = 4;
 
 template <int D, int NB>
 struct Frags {  // of a group
@@ -261,10 +265,8 @@ __global__ void __launch_bounds__(128) paged_prepare_kernel(const __grid_constan
       P.starts[r.n_seqs] = base;
       const int64_t total =
           r.n_kv_heads * (P.plan.pre_blocks * P.plan.pre_rows + base * P.plan.own_blocks);
-      const int64_t each = total / (P.n_warps * 512);
-      const int64_t n = P.n_warps * max((int64_t)1, min(each, (int64_t)kRounds));
       Units u;
-      u.size = max((int64_t)64, ((total + n - 1) / n + 31) / 32 * 32);
+      u.size = max((int64_t)64, ((total + P.n_warps - 1) / P.n_warps + 31) / 32 * 32);
       u.mul = ~uint64_t(0) / (uint64_t)u.size + 1;
       u.next = 0;
       *P.units = u;
@@ -347,14 +349,13 @@ __device__ __forceinline__ int64_t find_sequence(const AttnParams& P, int64_t x,
   return lo;
 }
 
-// CTAs an SM that the registers are bounded for.
-template <int D, int NB>
-constexpr int rows_ctas() {
-  return 3;
-}
+// CTAs an SM that the registers are bounded for (168 of them).  Four or five at
+// D 128 measured 46 and 51 us on the ragged batch instead of 43.5, two at D 256
+// 54.6 instead of 49.2 for 13 x 28 fp16 queries over a prefix of 5001 rows.
+constexpr int kRowsCtas = 3;
 
 template <int D, int PARTS, bool EXTRA, int NB>
-__global__ void __launch_bounds__(32 * kWarps, rows_ctas<D, NB>())
+__global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
     paged_rows_kernel(const __grid_constant__ AttnParams P) {
   using C = RowsCfg<D>;
   using F = Frags<D, NB>;
@@ -951,7 +952,7 @@ kh_status launch_rows(AttnParams P, cudaStream_t stream) {
   if (P.plan.block != NQ || groups + tiles > 0x7ffffff0ll || pairs >= int64_t(1) << 36)
     return KH_EINVAL;
   const int64_t grid =
-      std::min<int64_t>((int64_t)std::min(std::max(1, ctas[dev & 63]), rows_ctas<D, NB>()) *
+      std::min<int64_t>((int64_t)std::min(std::max(1, ctas[dev & 63]), kRowsCtas) *
                             sm_count(),
                         (pairs / 64 + kWarps) / kWarps);
   P.n_warps = grid * kWarps;
@@ -1062,7 +1063,7 @@ PagedPlan paged_plan(int64_t n_seqs, int n_q, int n_kv_heads, int D, int64_t max
   if (p.own_rows > 0) p.own_blocks = (n_q + p.block - 1) / p.block;
   p.groups = n_kv_heads * (p.pre_blocks + n_seqs * p.own_blocks);
   p.pairs = n_kv_heads * (p.pre_blocks * p.pre_rows + n_seqs * p.own_blocks * p.own_rows);
-  p.max_units = std::min<int64_t>((int64_t)kRounds * 5 * kWarps * n_sms, p.pairs / 64 + 1);
+  p.max_units = std::min<int64_t>((int64_t)kRowsCtas * kWarps * n_sms, p.pairs / 64 + 1);
   return p;
 }
 

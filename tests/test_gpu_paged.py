@@ -63,6 +63,11 @@ def _check_rows(pool, slots, want):
     (256, FL, 1100, 4, 64, 64, True),
     (256, HF, 1302, 4, 48, 256, False),
     (128, BF, 4100, 1, 64, 34, False),
+    (128, FL, 2301, 3, 64, 128, False),
+    (256, FL, 1700, 4, 64, 64, True),
+    (256, HF, 1702, 4, 48, 256, False),
+    (256, BF, 3400, 2, 64, 256, True),
+    (128, BF, 6700, 1, 64, 34, False),
 ])
 def test_append_is_the_64_bit_encoding(D, dtype, T, H, page, rot, inter):
     g = torch.Generator().manual_seed(T + D)
@@ -120,7 +125,8 @@ def test_append_without_rotation_strided_inputs_and_padding():
     _check_rows(vc, slots[on], wv)
 
 
-def test_append_extreme_values_and_ties():
+@pytest.mark.parametrize("times", [1, 110])
+def test_append_extreme_values_and_ties(times):
     """Squares that leave 32 bits, and sums that are exactly zero."""
     D, H = 128, 1
     dk, dv, c = rademacher(D, 5), rademacher(D, 6), lloyd_max(1, D)
@@ -130,15 +136,16 @@ def test_append_extreme_values_and_ties():
     k[16:32] *= 1e18
     k[32:48] = torch.randint(-2, 3, (16, H, D), generator=g).float()  # many sums are zero
     k[48:] = torch.where(torch.rand(16, H, D, generator=g) < 0.5, 1.0, -1.0)
-    kc, vc = (ops.empty_paged(1, H, 64, D, "cuda") for _ in range(2))
-    slots = torch.arange(64)
+    k = k.repeat(times, 1, 1)
+    kc, vc = (ops.empty_paged(times, H, 64, D, "cuda") for _ in range(2))
+    slots = torch.arange(64 * times)
     ops.paged_append(k.cuda(), k.cuda(), kc, vc, slots.cuda(), dk, dv, c)
     wk, wv = _want_append(k, k, dk, dv, c)
     _check_rows(kc, slots, wk)
     _check_rows(vc, slots, wv)
 
 
-@pytest.mark.parametrize("T", [20, 2100])
+@pytest.mark.parametrize("T", [20, 2100, 3400])
 def test_append_with_uneven_levels(T):
     """Two levels that are not -c, c, and tokens without a slot among many."""
     D, H = 128, 2
@@ -159,14 +166,24 @@ def test_append_with_uneven_levels(T):
 
 
 def test_append_matches_compress_away_from_borders():
-    """The engine's own compressor writes the same planes (borders aside)."""
+    """The engine's own compressor writes the same planes, but for elements so
+    near a border that its 32-bit sums may fall on the other side: D additions
+    in at most 16 roundings of 2^-23 of sum |x| <= sqrt(D) norm are 2^-19 of
+    y = u / (norm sqrt(D)), the norm's own error is far below; twice that."""
     D, H, T = 128, 4, 512
     dk, dv, c = rademacher(D, 7), rademacher(D, 8), lloyd_max(1, D)
     x = torch.randn(T, H, D, device="cuda").to(BF)
     kc, vc = (ops.empty_paged(1, H, T, D, "cuda") for _ in range(2))
     ops.paged_append(x, x, kc, vc, torch.arange(T, device="cuda"), dk, dv, c)
-    p = ops.compress(x.transpose(0, 1).contiguous(), dk, c)
-    assert int((p.code != kc.code).sum()) + int((p.res != kc.res).sum()) <= 2
+    rows = x.transpose(0, 1).contiguous()
+    p = ops.compress(rows, dk, c)
+    z = rows.cpu().double().view(H * T, D)
+    y = (z * dk.double()) @ R.hadamard(D) / (z.norm(dim=-1, keepdim=True) * math.sqrt(D))
+    off = torch.stack([y.abs()] + [(y - float(b)).abs() for b in c]).amin(0)
+    for a, b in ((p.code, kc.code), (p.res, kc.res)):
+        other = R.unpack(a.cpu().view(H * T, -1)) != R.unpack(b.cpu().view(H * T, -1))
+        assert (off[other] <= 2.0 ** -18).all()
+        assert int(other.sum()) < 0.001 * other.numel()
 
 
 def test_append_flags_bad_slots_and_positions():
