@@ -107,14 +107,13 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 // sequence its groups (KV head, block of NQ of its own).  They are cut into
 // units of equal length, one for every warp that the GPU holds (two to four a
 // warp made more records and measured the same, or 119 us instead of 110 on 8
-// sequences up to 40000 rows), which the warps claim, as those beside a prefix
-// come late.  Lengths live on the device, so the cut is made there: units from
+// sequences up to 40000 rows).  Lengths live on the device, so the cut is made there: units from
 // what max_len allows left a quarter of the SM time idle on the ragged batch,
 // CTAs with a chunk of a fixed length more.  A unit may hold pieces of several
 // groups; piece (unit u, group G) has record u + G, as a unit's or a group's
 // begin starts a new piece.
 //
-// What the claims need is prepared by a launch before: where each sequence's
+// What the warps need is prepared by a launch before: where each sequence's
 // pairs start, its first row, the units, and each group's queries as operand
 // fragments.
 
@@ -268,7 +267,6 @@ __global__ void __launch_bounds__(128) paged_prepare_kernel(const __grid_constan
       Units u;
       u.size = max((int64_t)64, ((total + P.n_warps - 1) / P.n_warps + 31) / 32 * 32);
       u.mul = ~uint64_t(0) / (uint64_t)u.size + 1;
-      u.next = 0;
       *P.units = u;
     }
     return;
@@ -336,13 +334,22 @@ __global__ void __launch_bounds__(128) paged_prepare_kernel(const __grid_constan
 }
 
 // Sequence b with starts[b] * per <= x < starts[b + 1] * per: a warp looks at
-// 32 places at once.
+// 128 places at once.
 __device__ __forceinline__ int64_t find_sequence(const AttnParams& P, int64_t x, int64_t per,
                                                  int lane) {
   int64_t lo = 0, n = P.r.n_seqs;  // it is among [lo, lo + n)
   while (n > 1) {
-    const int64_t step = (n + 31) / 32, i = min(lo + (lane + 1) * step, lo + n);
-    const int below = __popc(__ballot_sync(0xffffffffu, i < lo + n && P.starts[i] * per <= x));
+    const int64_t step = (n + 127) / 128;
+    int64_t start[4];
+    int below = 0;  // of the places lo + step, lo + 2 step, ... those that are not after x
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t i = lo + (32 * k + lane + 1) * step;
+      start[k] = i < lo + n ? P.starts[i] : -1;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      below += __popc(__ballot_sync(0xffffffffu, start[k] >= 0 && start[k] * per <= x));
     lo += below * step;
     n = min(step, n - below * step);
   }
@@ -380,14 +387,8 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
   const int64_t n_pre = r.n_kv_heads * P.plan.pre_blocks * P.plan.pre_rows;
   const int64_t per = (int64_t)r.n_kv_heads * P.plan.own_blocks, size = P.units->size;
   const int64_t total = n_pre + P.starts[r.n_seqs] * per;
-
-#pragma unroll 1
-  for (;;) {
-  uint32_t unit = 0;
-  if (lane == 0) unit = atomicAdd(&P.units->next, 1u);
-  unit = __shfl_sync(0xffffffffu, unit, 0);
-  int64_t at = (int64_t)unit * size;
-  if (at >= total) break;
+  const int64_t unit = (int64_t)blockIdx.x * kWarps + warp;
+  int64_t at = unit * size;
   const int64_t end = min(at + size, total);
 #pragma unroll 1
   while (at < end) {
@@ -401,7 +402,7 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
   const int64_t begin = start + hz * rows;
   const int lo = (pre ? 0 : P.first_row[b]) + (int)(at - begin);
   const int hi = lo + (int)min(min(rows - (at - begin), end - at), kPieceRows);
-  const bool more = at > begin && at > (int64_t)unit * size;  // the record holds rows already
+  const bool more = at > begin && at > unit * size;  // the record holds rows already
   at += hi - lo;
   const int blocks = pre ? P.plan.pre_blocks : P.plan.own_blocks;
   const int h = hz / blocks;
@@ -807,7 +808,6 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
       }
   }
   __syncwarp();
-  }
   }
   grid_dependents_launch();
   if (P.pre_tensor) grid_dependency_wait();

@@ -13,8 +13,7 @@ constexpr float kLn2 = 0.6931471805599453f;
 // How the rows kernel's (group, row) pairs are cut (kh_paged_attn.cu).
 struct Units {
   int64_t size;
-  uint64_t mul;   // floor(2^64 / size) + 1: x / size while x size < 2^64
-  uint32_t next;  // unclaimed
+  uint64_t mul;  // floor(2^64 / size) + 1: x / size while x size < 2^64
   __device__ __forceinline__ int64_t of(int64_t x) const {
     return (int64_t)__umul64hi((uint64_t)x, mul);
   }
