@@ -100,6 +100,7 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
+
 // ---- how a call's rows are split
 //
 // All (group, row) pairs of the call lie one after another: first the prefix's
@@ -107,16 +108,15 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 // sequence its groups (KV head, block of NQ of its own).  They are cut into
 // units of equal length, one for every warp that the GPU holds (two to four a
 // warp made more records and measured the same, or 119 us instead of 110 on 8
-// sequences up to 40000 rows).  Lengths live on the device, so the cut is made there: units from
-// what max_len allows left a quarter of the SM time idle on the ragged batch,
-// CTAs with a chunk of a fixed length more.  A unit may hold pieces of several
-// groups; piece (unit u, group G) has record u + G, as a unit's or a group's
-// begin starts a new piece.
+// sequences up to 40000 rows).  Lengths live on the device, so the cut is made
+// there: units from what max_len allows left a quarter of the SM time idle on
+// the ragged batch, CTAs with a chunk of a fixed length more.  A unit may hold
+// pieces of several groups; piece (unit u, group G) has record u + G, as a
+// unit's or a group's begin starts a new piece.
 //
 // What the warps need is prepared by a launch before: where each sequence's
 // pairs start, its first row, the units, and each group's queries as operand
 // fragments.
-
 template <int D, int NB>
 struct Frags {  // of a group
   static constexpr int kSteps = D / 32;
@@ -222,7 +222,7 @@ __device__ __forceinline__ void write_query_tiles(const AttnParams& P, int64_t b
   }
 }
 
-// Block 0: starts, first rows, the counter.  Then a group each; then, where the
+// Block 0: starts, first rows, the units.  Then a group each; then, where the
 // prefix goes to the tensor cores, sixteen rows of its operand each.
 template <int D, int PARTS, int NB>
 __global__ void __launch_bounds__(128) paged_prepare_kernel(const __grid_constant__ AttnParams P) {
@@ -821,7 +821,7 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
 // rows that the GPU holds them (a row of a long cache has a hundred records).
 constexpr int kMostJoin = 16;
 template <int D>
-__global__ void __launch_bounds__(32 * kMostJoin)
+__global__ void __launch_bounds__(32 * kMostJoin, D == 128 ? 3 : 2)
     paged_combine_kernel(const __grid_constant__ AttnParams P) {
   constexpr int J = D / 32, U = 4;
   const PagedAttnRequest& r = P.r;
@@ -876,7 +876,11 @@ __global__ void __launch_bounds__(32 * kMostJoin)
       const float* q = i < pre.n ? pre.at + i * pre_stride : own.at + (i - pre.n) * stride;
       ml[u] = *reinterpret_cast<const float2*>(q);
 #pragma unroll
-      for (int j = 0; j < J; ++j) v[u][j] = q[2 + 32 * j + lane];
+      for (int j = 0; j < J; j += 2) {  // elements 32 j + 2 lane and the next
+        const float2 two = *reinterpret_cast<const float2*>(q + 2 + 32 * j + 2 * lane);
+        v[u][j] = two.x;
+        v[u][j + 1] = two.y;
+      }
     }
     float top = mx;
 #pragma unroll
@@ -922,10 +926,16 @@ __global__ void __launch_bounds__(32 * kMostJoin)
   }
   fwht_lanes<J>(a, lane);
   const float inv = 1.f / l;
+  char* out = static_cast<char*>(r.out) + (int64_t)row * D * (r.dtype == KH_F32 ? 4 : 2);
 #pragma unroll
-  for (int j = 0; j < J; ++j) {
-    const float v = l == 0.f ? 0.f : a[j] * inv;
-    st_any(r.out, r.dtype, (int64_t)row * D + 32 * j + lane, (r.dv_neg[j] >> lane) & 1 ? -v : v);
+  for (int j = 0; j < J; j += 2) {
+    const int e = 32 * j + 2 * lane;
+    const uint32_t neg = r.dv_neg[e >> 5] >> (e & 31);
+    float2 v = l == 0.f ? make_float2(0.f, 0.f) : make_float2(a[j] * inv, a[j + 1] * inv);
+    if (neg & 1) v.x = -v.x;
+    if (neg & 2) v.y = -v.y;
+    st_any(out, r.dtype, e, v.x);
+    st_any(out, r.dtype, e + 1, v.y);
   }
   if (r.lse && lane == 0) r.lse[row] = l == 0.f ? -INFINITY : (top + log2f(l)) * kLn2;
 }
