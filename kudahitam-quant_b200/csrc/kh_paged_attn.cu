@@ -46,7 +46,9 @@ namespace {
 //     largest element (2^-16 for bits that count once), weights to 2^-16 of
 //     the largest of their unit, whose roundings average out; together under
 //     a tenth of a bf16 step.
-//   PARTS = 4 (32-bit queries, 2 a block): q~ to 2^-28, weights to 2^-22.
+//   PARTS = 4 (32-bit queries, 2 a block): q~ to 2^-28, weights to 2^-31 (with
+//     three bytes, 2^-22, the result of 8 x 16 fp32 queries over rows up to
+//     40000 was off by 2.3e-6 of its norm, five times the plain form's error).
 // What bounds it is issue: a 32-row tile takes 128 logic operations at half
 // rate, 32 products of 7.5 cycles, and some 370 other instructions.  On a ragged
 // batch (32 sequences up to 8192 rows, 8 KV heads x 4, D 128, bf16) the kernel
@@ -90,9 +92,9 @@ template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
-  uint32_t y;
-  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(y) : "r"(a), "r"(b), "r"(sel));
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
   return y;
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
@@ -308,7 +310,7 @@ __global__ void __launch_bounds__(128) paged_prepare_kernel(const __grid_constan
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) {
-      out->sum[y] = sum;
+      out->sum[y] = mx < INFINITY ? sum : NAN;
       out->scale[y] = P.log_scale / up;  // sm_scale log2(e) / sqrt(D) and the scale above
     }
   }
@@ -501,8 +503,8 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
     }
   }
   // weight 1 as a whole number, and the most one may be
-  constexpr float kOne = PARTS == 2 ? 32768.f : 4194304.f;
-  constexpr float kMost = PARTS == 2 ? 65535.f : 8388607.f;
+  constexpr float kOne = PARTS == 2 ? 32768.f : 1073741824.f;
+  constexpr float kMost = PARTS == 2 ? 65535.f : 4294967040.f;
   const float va = ch * inv_sd * kOne;
   const float vb = 0.7978845608028654f * inv_sd * inv_sd * kOne;
   const float cap = r.softcap * kLog2e, inv_cap = r.softcap > 0.f ? 1.f / cap : 0.f;
@@ -608,6 +610,7 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
     }
   };
   // weights e = 2^(t2 - ref); true where they fit: a row's larger one decides
+  // (and a NaN among the attended, which whole numbers would lose)
   auto weigh = [&] {
     float top = 0.f;
 #pragma unroll
@@ -616,9 +619,9 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
       for (int nb = 0; nb < NB; ++nb) {
         const float e = ex2(tt[k >> 1][k & 1][nb] - ref[nb]);
         ee[k >> 1][k & 1][nb] = e;
-        const float most = fmaxf(fmaxf(ra[k >> 1][k & 1], rb[k >> 1][k & 1]), kOne * 0x1p-40f);
+        const float most = max_nan(max_nan(ra[k >> 1][k & 1], rb[k >> 1][k & 1]), kOne * 0x1p-40f);
         // nothing attended: 0 times whatever the row's norms hold
-        top = fmaxf(top, e == 0.f ? 0.f : e * most);
+        top = max_nan(top, e == 0.f ? 0.f : e * most);
       }
     return top <= kMost;
   };
@@ -629,13 +632,13 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
       float mx = kNoRef;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const float most = fmaxf(fmaxf(ra[k >> 1][k & 1], rb[k >> 1][k & 1]), kOne * 0x1p-40f);
+        const float most = max_nan(max_nan(ra[k >> 1][k & 1], rb[k >> 1][k & 1]), kOne * 0x1p-40f);
         const float x = tt[k >> 1][k & 1][nb];
-        if (x > -INFINITY) mx = fmaxf(mx, x + lg2(most * (1.f / kOne)));
+        if (x > -INFINITY) mx = max_nan(mx, x + lg2(most * (1.f / kOne)));
       }
 #pragma unroll
-      for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      if (mx == INFINITY) l[nb] = NAN;  // an infinite norm has no average
+      for (int o = 4; o < 32; o <<= 1) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      if (!(mx < INFINITY)) l[nb] = NAN;  // a norm that is not finite has no average
       const float to = fmaxf(ref[nb], ceilf(mx)), f = ex2(ref[nb] - to);
       int left = (int)fminf(to - ref[nb], 48.f);
       ref[nb] = to;
@@ -656,10 +659,15 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
             uint32_t h = acc[nb][i][k], o = acc[nb][i][k + 1];
             if constexpr (PARTS == 2) {
               o += ((h & lost) << 8) + half;
-            } else {  // the low lanes hold one column, in h
-              if (!low) o += (h & lost) << 8;
-              const uint32_t down = __shfl_xor_sync(0xffffffffu, o & lost, 1);
-              if (low) h += (down << 8) + half;
+            } else {
+              const uint32_t o2 = o + ((h & lost) << 8);
+              const uint32_t down = __shfl_xor_sync(0xffffffffu, o2 & lost, 1);
+              if (low) {
+                h += down << 8;
+                o += ((h & lost) << 8) + half;
+              } else {
+                o = o2;
+              }
             }
             acc[nb][i][k] = (int)(h >> sh);
             acc[nb][i][k + 1] = (int)(o >> sh);
@@ -678,22 +686,31 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
         for (int rr = 0; rr < 2; ++rr) {
           const float e = ee[hf][rr][nb];
           l[nb] += e;
-          // 2^23 + w: the low bits are w as a whole number
-          float x1 = fmaf(e, ra[hf][rr], 8388608.f), x2 = fmaf(e, rb[hf][rr], 8388608.f);
-          if (!full && tt[hf][rr][nb] == -INFINITY) x1 = x2 = 8388608.f;
-          u1[rr] = __float_as_uint(x1);
-          u2[rr] = __float_as_uint(x2);
+          const bool none = !full && tt[hf][rr][nb] == -INFINITY;
+          if constexpr (PARTS == 2) {
+            // 2^23 + w: the low bits are w as a whole number
+            const float x1 = fmaf(e, ra[hf][rr], 8388608.f), x2 = fmaf(e, rb[hf][rr], 8388608.f);
+            u1[rr] = none ? 0x4B000000u : __float_as_uint(x1);
+            u2[rr] = none ? 0x4B000000u : __float_as_uint(x2);
+          } else {
+            const float x1 = none ? 0.f : e * ra[hf][rr], x2 = none ? 0.f : e * rb[hf][rr];
+            w1s[nb] += x1;
+            w2s[nb] += x2;
+            u1[rr] = __float2uint_rn(x1);
+            u2[rr] = __float2uint_rn(x2);
+          }
         }
         i1 += u1[0] + u1[1];
         i2 += u2[0] + u2[1];
         // this lane's two columns, high byte first, of both rows
-        // (the low lanes' second is zero: the sign of byte 3, repeated)
-        const uint32_t sel = PARTS == 2 ? 0x4051u : low ? 0xfb40u : 0x5162u;
-        p1[hf][nb] = transpose8(prmt(u1[0], u1[1], sel));
-        p2[hf][nb] = transpose8(prmt(u2[0], u2[1], sel));
+        const uint32_t sel = PARTS == 2 || low ? 0x4051u : 0x6273u;
+        p1[hf][nb] = transpose8(__byte_perm(u1[0], u1[1], sel));
+        p2[hf][nb] = transpose8(__byte_perm(u2[0], u2[1], sel));
       }
-      w1s[nb] += (float)(i1 - 4u * 0x4B000000u);  // without the exponent fields
-      w2s[nb] += (float)(i2 - 4u * 0x4B000000u);
+      if constexpr (PARTS == 2) {
+        w1s[nb] += (float)(i1 - 4u * 0x4B000000u);  // without the exponent fields
+        w2s[nb] += (float)(i2 - 4u * 0x4B000000u);
+      }
     }
   };
   auto values = [&](const uint8_t* st, int p) {
@@ -789,7 +806,7 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
       if constexpr (PARTS == 2) {
         x = fmaf(h, 256.f, o);
       } else {
-        x = low ? h : fmaf(h, 65536.f, o * 256.f);
+        x = low ? fmaf(h, 256.f, o) : fmaf(h, 16777216.f, o * 65536.f);
         x += __shfl_xor_sync(0xffffffffu, x, 1);
       }
       return fmaf(x, 2.f / (float)(1 << (i & 7)), base) * is;

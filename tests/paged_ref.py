@@ -108,7 +108,7 @@ def check(got, lse, want, dtype):
       two operands rounded to fp16, 2^-11 |q| |K| sm_scale.
     p is off by twice that, relatively, as numerator and denominator move
     apart.  The weighted sum adds `dw` sum p |V_hat| (2^-20; 2^-11 for bf16, two
-    fp16 operands) and roundings of the weights to 2^-14 (2^-21 for fp32 queries)
+    fp16 operands) and roundings of the weights to 2^-14 (2^-24 for fp32 queries)
     of the largest weight of a unit: independent, so the root of their number
     counts, 1 / sqrt(12) of a step each; a whole 2^-14 is over 3 deviations.
     The output's own rounding is half a step."""
@@ -118,7 +118,7 @@ def check(got, lse, want, dtype):
         ds = ds + 2.0 ** -13.7 * peak
     if dtype == torch.bfloat16:
         ds, dw = torch.maximum(ds, 2.0 ** -11 * reach), 2.0 ** -11
-    extra = 2.0 ** (-21 if dtype == torch.float32 else -14) * largest
+    extra = 2.0 ** (-24 if dtype == torch.float32 else -14) * largest
     got = got.detach().cpu().double()
     # a value past the type's largest rounds to an infinity of its sign
     over = torch.isinf(got) & (out.abs() >= torch.finfo(dtype).max) & (got.sign() == out.sign())

@@ -337,6 +337,41 @@ def test_attention_with_uneven_levels(dtype, D, B, nq):
             want, dtype)
 
 
+@pytest.mark.parametrize("dtype,D,nq", [(BF, 128, 4), (FL, 128, 3), (HF, 256, 2), (FL, 256, 1)])
+def test_decode_with_values_that_are_not_finite(dtype, D, nq):
+    """A NaN or an infinity among a sequence's norms, or in one of its queries,
+    makes that result NaN and no other."""
+    lengths, page, H = [200, 150, 90], 16, 2
+    kc, vc, dk, dv, c = R.pools(32, H, page, D, 31)
+    table = R.tables(lengths, page, 32, 31)
+    g = torch.Generator().manual_seed(31)
+    q = torch.randn(3, H * nq, D, generator=g).to(dtype)
+    ln = torch.tensor(lengths, dtype=torch.int32).cuda()
+    run = lambda x: ops.paged_decode_attention(  # noqa: E731
+        x.cuda(), R.cuda(kc), R.cuda(vc), table.cuda(), ln, dk, dv, c).cpu().float()
+    R.check(run(q), None, R.attention(q, kc, vc, table, lengths, dk, dv, c), dtype)
+    for pool in (kc, vc):
+        for norms in (pool.norms, pool.rnorms):
+            for bad in (math.nan, math.inf):
+                for j in (0, 37, 149):
+                    row = (int(table[1, j // page]) * H + 1) * page + j % page
+                    old = norms[row].clone()
+                    norms[row] = bad
+                    out = run(q)
+                    norms[row] = old
+                    if not (pool is kc and bad == math.inf):  # may be a weight of zero
+                        assert torch.isnan(out[1, nq:]).all()
+                    assert torch.isfinite(out[[0, 2]]).all() and torch.isfinite(out[1, :nq]).all()
+    for bad in (math.nan, math.inf, -math.inf):
+        for e in (0, 5):
+            x = q.clone()
+            x[2, nq - 1, e] = bad
+            out = run(x)
+            assert torch.isnan(out[2, nq - 1]).all()
+            out[2, nq - 1] = 0
+            assert torch.isfinite(out).all()
+
+
 @pytest.mark.parametrize("dtype,D,H,nq,page,prefix,suffix", [
     (BF, 128, 2, 4, 64, 640, [3, 1, 100, 64]),
     (BF, 128, 1, 8, 48, 1001, [0, 7, 300]),
