@@ -62,9 +62,9 @@ struct PagedAttnRequest {
 // How a call's rows are cut, from what the host knows of it.
 struct PagedPlan {
   // the rows kernel: query rows of a group, groups of a KV head (the prefix's,
-  // and a sequence's own), their rows at most, units at most
+  // and a sequence's own), their rows, tiles of 32 and units at most
   int block = 1, pre_blocks = 0, own_blocks = 0;
-  int64_t pre_rows = 0, own_rows = 0, groups = 0, pairs = 0, max_units = 0;
+  int64_t pre_rows = 0, own_rows = 0, groups = 0, tiles = 0, max_units = 0;
   // the prefix on the tensor cores: chunks of chunk_rows rows
   int pre_chunks = 0;
   int64_t chunk_rows = 0;

@@ -66,7 +66,7 @@ namespace {
 // to 255 x 128 each), and what is summed as floats keeps its bits; the next
 // piece's record joins in.
 constexpr int kWarps = 4;
-constexpr int64_t kPieceRows = 16384;
+constexpr int64_t kPieceTiles = 512;
 
 template <int D>
 struct RowsCfg {
@@ -105,19 +105,21 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 
 // ---- how a call's rows are split
 //
-// All (group, row) pairs of the call lie one after another: first the prefix's
-// groups (KV head, block of NQ of every sequence's query rows), then for each
-// sequence its groups (KV head, block of NQ of its own).  They are cut into
-// units of equal length, one for every warp that the GPU holds (two to four a
-// warp made more records and measured the same, or 119 us instead of 110 on 8
-// sequences up to 40000 rows).  Lengths live on the device, so the cut is made
-// there: units from what max_len allows left a quarter of the SM time idle on
-// the ragged batch, CTAs with a chunk of a fixed length more.  A unit may hold
-// pieces of several groups; piece (unit u, group G) has record u + G, as a
-// unit's or a group's begin starts a new piece.
+// The tiles of 32 rows of all groups of the call lie one after another: first
+// those of the prefix's groups (KV head, block of NQ of every sequence's query
+// rows), then for each sequence those of its groups (KV head, block of NQ of
+// its own).  They are cut into units of equal length, one for every warp that
+// the GPU holds (two to four a warp made more records and measured the same, or
+// 119 us instead of 110 on 8 sequences up to 40000 rows).  Lengths live on the
+// device, so the cut is made there: units from what max_len allows left a
+// quarter of the SM time idle on the ragged batch, CTAs with a chunk of a fixed
+// length more.  Tiles and not rows are counted, as a group of one row costs its
+// tile: counted by rows, 17 x 4 x 5 queries with one own row each took 560 us.
+// A unit may hold pieces of several groups; piece (unit u, group G) has record
+// u + G, as a unit's or a group's begin starts a new piece.
 //
 // What the warps need is prepared by a launch before: where each sequence's
-// pairs start, its first row, the units, and each group's queries as operand
+// tiles start, its rows, the units, and each group's queries as operand
 // fragments.
 template <int D, int NB>
 struct Frags {  // of a group
@@ -224,7 +226,7 @@ __device__ __forceinline__ void write_query_tiles(const AttnParams& P, int64_t b
   }
 }
 
-// Block 0: starts, first rows, the units.  Then a group each; then, where the
+// Block 0: starts, own rows, the units.  Then a group each; then, where the
 // prefix goes to the tensor cores, sixteen rows of its operand each.
 template <int D, int PARTS, int NB>
 __global__ void __launch_bounds__(128) paged_prepare_kernel(const __grid_constant__ AttnParams P) {
@@ -243,8 +245,8 @@ __global__ void __launch_bounds__(128) paged_prepare_kernel(const __grid_constan
       int64_t n = 0;
       if (b < r.n_seqs) {
         const int64_t len = length_of(P, b), first = own_first(P, b, len);
-        n = max((int64_t)0, len - first);
-        P.first_row[b] = (int32_t)min(first, (int64_t)0x7fffffff);
+        n = (max((int64_t)0, len - first) + 31) / 32;
+        P.own[b] = make_int2((int)min(first, len), (int)len);
       }
       int64_t upto = n;
 #pragma unroll
@@ -265,9 +267,10 @@ __global__ void __launch_bounds__(128) paged_prepare_kernel(const __grid_constan
     if (threadIdx.x == 0) {
       P.starts[r.n_seqs] = base;
       const int64_t total =
-          r.n_kv_heads * (P.plan.pre_blocks * P.plan.pre_rows + base * P.plan.own_blocks);
+          r.n_kv_heads * (P.plan.pre_blocks * ((P.plan.pre_rows + 31) / 32) +
+                          base * P.plan.own_blocks);
       Units u;
-      u.size = max((int64_t)64, ((total + P.n_warps - 1) / P.n_warps + 31) / 32 * 32);
+      u.size = max((int64_t)2, (total + P.n_warps - 1) / P.n_warps);
       u.mul = ~uint64_t(0) / (uint64_t)u.size + 1;
       *P.units = u;
     }
@@ -386,7 +389,8 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
   // records.  The wait then comes at the end, so that this grid's completion
   // implies the prefix's.
   if (!P.pre_tensor) grid_dependency_wait();
-  const int64_t n_pre = r.n_kv_heads * P.plan.pre_blocks * P.plan.pre_rows;
+  const int64_t pre_tiles = (P.plan.pre_rows + 31) / 32;
+  const int64_t n_pre = r.n_kv_heads * P.plan.pre_blocks * pre_tiles;
   const int64_t per = (int64_t)r.n_kv_heads * P.plan.own_blocks, size = P.units->size;
   const int64_t total = n_pre + P.starts[r.n_seqs] * per;
   const int64_t unit = (int64_t)blockIdx.x * kWarps + warp;
@@ -399,13 +403,15 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
   const bool pre = at < n_pre;
   const int64_t b = pre ? 0 : find_sequence(P, at - n_pre, per, lane);
   const int64_t start = pre ? 0 : n_pre + P.starts[b] * per;
-  const int64_t rows = pre ? P.plan.pre_rows : P.starts[b + 1] - P.starts[b];
-  const int hz = (int)((at - start) / rows);
-  const int64_t begin = start + hz * rows;
-  const int lo = (pre ? 0 : P.first_row[b]) + (int)(at - begin);
-  const int hi = lo + (int)min(min(rows - (at - begin), end - at), kPieceRows);
+  const int64_t tiles = pre ? pre_tiles : P.starts[b + 1] - P.starts[b];
+  const int2 all = pre ? make_int2(0, (int)P.plan.pre_rows) : P.own[b];
+  const int hz = (int)((at - start) / tiles);
+  const int64_t begin = start + hz * tiles;
+  const int n_tiles = (int)min(min(tiles - (at - begin), end - at), kPieceTiles);
+  const int lo = all.x + 32 * (int)(at - begin);
+  const int hi = n_tiles < tiles - (at - begin) ? lo + 32 * n_tiles : all.y;
   const bool more = at > begin && at > unit * size;  // the record holds rows already
-  at += hi - lo;
+  at += n_tiles;
   const int blocks = pre ? P.plan.pre_blocks : P.plan.own_blocks;
   const int h = hz / blocks;
   const int64_t y0 = (int64_t)(hz - h * blocks) * NQ;
@@ -417,7 +423,6 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
 
   // ---- tiles of 32 rows: lane = row.  Its place in the table and in the page
   // moves on by 32 rows a tile; pages are read a tile before they are used.
-  const int n_tiles = (hi - lo + 31) >> 5;
   const int32_t* tab = r.table + b * r.table_stride;
   uint32_t block = P.page_div(lo + lane), off = lo + lane - block * r.page_size;
   int left = hi - lo - lane;
@@ -856,27 +861,28 @@ __global__ void __launch_bounds__(32 * kMostJoin, D == 128 ? 3 : 2)
     const float* at;
     int n;
   };
-  auto run = [&](int64_t begin, int64_t rows, int64_t group, int place) {
-    if (rows <= 0) return Run{P.records, 0};
+  auto run = [&](int64_t begin, int64_t tiles, int64_t group, int place) {
+    if (tiles <= 0) return Run{P.records, 0};
     const int64_t u = P.units->of(begin);
     return Run{P.records + (u + group) * stride + place * kRec,
-               (int)(P.units->of(begin + rows - 1) - u) + 1};
+               (int)(P.units->of(begin + tiles - 1) - u) + 1};
   };
   Run pre{P.records, 0}, own{P.records, 0};
   int64_t pre_stride = stride;
+  const int64_t pre_tiles = (P.plan.pre_rows + 31) / 32;
   if (P.plan.pre_chunks) {
     pre = Run{r.workspace + (int64_t)row * P.plan.pre_chunks * kRec, P.plan.pre_chunks};
     pre_stride = kRec;
   } else if (P.plan.pre_blocks) {
     const uint32_t i = b * r.n_q + y, z = i / P.plan.block;
     const int64_t group = (int64_t)h * P.plan.pre_blocks + z;
-    pre = run(group * P.plan.pre_rows, P.plan.pre_rows, group, i - z * P.plan.block);
+    pre = run(group * pre_tiles, pre_tiles, group, i - z * P.plan.block);
   }
   if (P.plan.own_blocks) {
-    const int64_t first = P.starts[b], rows = P.starts[b + 1] - first;
+    const int64_t first = P.starts[b], tiles = P.starts[b + 1] - first;
     const int z = y / P.plan.block, hz = h * P.plan.own_blocks + z;
     const int64_t per = (int64_t)r.n_kv_heads * P.plan.own_blocks;
-    own = run(r.n_kv_heads * P.plan.pre_blocks * P.plan.pre_rows + first * per + hz * rows, rows,
+    own = run(r.n_kv_heads * P.plan.pre_blocks * pre_tiles + first * per + hz * tiles, tiles,
               r.n_kv_heads * P.plan.pre_blocks + b * per + hz, y - z * P.plan.block);
   }
   const int n = pre.n + own.n;
@@ -973,26 +979,26 @@ kh_status launch_rows(AttnParams P, cudaStream_t stream) {
       ctas[dev & 63] = 0;
   });
   constexpr int kGroup = 128 * QueryTiles<D>::MT;
-  const int64_t tiles =
+  // the preparing launch's blocks, and the rows launch's
+  const int64_t operand =
       P.pre_tensor ? r.n_kv_heads * ((r.n_seqs * r.n_q + kGroup - 1) / kGroup) * (kGroup / 16) : 0;
-  const int64_t groups = P.plan.groups, pairs = P.plan.pairs;
-  if (P.plan.block != NQ || groups + tiles > 0x7ffffff0ll || pairs >= int64_t(1) << 36)
+  const int64_t groups = P.plan.groups;
+  if (P.plan.block != NQ || groups + operand > 0x7ffffff0ll || P.plan.tiles >= int64_t(1) << 36)
     return KH_EINVAL;
-  const int64_t grid =
-      std::min<int64_t>((int64_t)std::min(std::max(1, ctas[dev & 63]), kRowsCtas) *
-                            sm_count(),
-                        (pairs / 64 + kWarps) / kWarps);
+  const int64_t grid = std::min<int64_t>(
+      (int64_t)std::min(std::max(1, ctas[dev & 63]), kRowsCtas) * sm_count(),
+      (P.plan.tiles / 2 + kWarps) / kWarps);
   P.n_warps = grid * kWarps;
   static_assert(sizeof(Frags<D, NB>) <= kFragBytes, "workspace of the fragments");
-  if (groups + tiles > 0 &&
-      launch_programmatic(paged_prepare_kernel<D, PARTS, NB>, dim3((unsigned)(groups + tiles + 1)),
+  if (groups + operand > 0 &&
+      launch_programmatic(paged_prepare_kernel<D, PARTS, NB>, dim3((unsigned)(groups + operand + 1)),
                           dim3(128), 0, stream, P) != cudaSuccess)
     return KH_ELAUNCH;
   if (P.pre_tensor) {
     const kh_status st = launch_paged_prefix(P, stream);
     if (st != KH_OK) return st;
   }
-  if (pairs > 0) {
+  if (P.plan.tiles > 0) {
     if (launch_programmatic(kern, dim3((unsigned)grid), dim3(32 * kWarps), kSmem, stream, P) !=
         cudaSuccess)
       return KH_ELAUNCH;
@@ -1042,10 +1048,10 @@ kh_status launch_dim(const AttnParams& P, cudaStream_t stream) {
 int64_t prefix_tensor_rows(int D) { return D == 128 ? 32 : 16; }
 
 // The workspace, each part 16-byte aligned: a tensor-core prefix's records, by
-// query row and chunk; the other records; the sequences' starts and first rows;
+// query row and chunk; the other records; the sequences' starts and own rows;
 // the units; the groups' fragments; a tensor-core prefix's queries.
 struct Layout {
-  int64_t records, starts, first, units, frags, queries, bytes;
+  int64_t records, starts, own, units, frags, queries, bytes;
 };
 Layout layout_of(const PagedPlan& p, int64_t n_seqs, int n_q, int n_kv_heads, int D) {
   auto up = [](int64_t x) { return (x + 15) / 16 * 16; };
@@ -1053,8 +1059,8 @@ Layout layout_of(const PagedPlan& p, int64_t n_seqs, int n_q, int n_kv_heads, in
   Layout l;
   l.records = up(nq * n_kv_heads * p.pre_chunks * record);
   l.starts = l.records + up((p.max_units + p.groups) * p.block * record);
-  l.first = l.starts + up((n_seqs + 1) * 8);
-  l.units = l.first + up(n_seqs * 4);
+  l.own = l.starts + up((n_seqs + 1) * 8);
+  l.units = l.own + up(n_seqs * 8);
   l.frags = l.units + up(sizeof(Units));
   l.queries = l.frags + p.groups * kFragBytes;
   l.bytes = l.queries;
@@ -1089,8 +1095,9 @@ PagedPlan paged_plan(int64_t n_seqs, int n_q, int n_kv_heads, int D, int64_t max
   if (p.pre_rows > 0) p.pre_blocks = (int)((nq + p.block - 1) / p.block);
   if (p.own_rows > 0) p.own_blocks = (n_q + p.block - 1) / p.block;
   p.groups = n_kv_heads * (p.pre_blocks + n_seqs * p.own_blocks);
-  p.pairs = n_kv_heads * (p.pre_blocks * p.pre_rows + n_seqs * p.own_blocks * p.own_rows);
-  p.max_units = std::min<int64_t>((int64_t)kRowsCtas * kWarps * n_sms, p.pairs / 64 + 1);
+  p.tiles = n_kv_heads * (p.pre_blocks * ((p.pre_rows + 31) / 32) +
+                          n_seqs * p.own_blocks * ((p.own_rows + 31) / 32));
+  p.max_units = std::min<int64_t>((int64_t)kRowsCtas * kWarps * n_sms, p.tiles / 2 + 1);
   return p;
 }
 
@@ -1112,7 +1119,7 @@ kh_status launch_paged_attn(const PagedAttnRequest& r, cudaStream_t stream) {
   const Layout l = layout_of(P.plan, r.n_seqs, r.n_q, r.n_kv_heads, r.D);
   uint8_t* ws = reinterpret_cast<uint8_t*>(r.workspace);
   P.starts = reinterpret_cast<int64_t*>(ws + l.starts);
-  P.first_row = reinterpret_cast<int32_t*>(ws + l.first);
+  P.own = reinterpret_cast<int2*>(ws + l.own);
   P.units = reinterpret_cast<Units*>(ws + l.units);
   P.records = reinterpret_cast<float*>(ws + l.records);
   P.frags = ws + l.frags;

@@ -10,7 +10,7 @@ namespace kh {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// How the rows kernel's (group, row) pairs are cut (kh_paged_attn.cu).
+// How the rows kernel's tiles are cut (kh_paged_attn.cu).
 struct Units {
   int64_t size;
   uint64_t mul;  // floor(2^64 / size) + 1: x / size while x size < 2^64
@@ -32,7 +32,7 @@ struct AttnParams {
   int64_t n_warps;
   float* records;
   int64_t* starts;
-  int32_t* first_row;
+  int2* own;  // a sequence's own rows: first, end
   Units* units;
   void* frags;
   int pre_tensor;  // the prefix has its own launches (launch_paged_prefix)
