@@ -598,7 +598,8 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
         for (int nb = 0; nb < NB; ++nb) {
           float x = n.x * fmaf(a1[nb], joined(s1[hf][nb], rr), b1[nb]);
           x = fmaf(n.y, fmaf(a2[nb], joined(s2[hf][nb], rr), b2[nb]), x);
-          if (EXTRA && r.softcap > 0.f) x = soft_cap(x, cap, inv_cap);
+          if (EXTRA && r.softcap > 0.f)
+            x = PARTS == 2 ? soft_cap_16(x, cap, inv_cap) : soft_cap(x, cap, inv_cap);
           if (EXTRA && r.slopes) x = fmaf(slope[nb], (float)(j0 + row + 1 - q_hi[nb]), x);
           tt[hf][rr][nb] = x;
         }

@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
       // a score as an exponent of two, without the reference
       auto exponent = [&](int j, float x, float k) {
         x *= k;
-        if (EXTRA && r.softcap > 0.f) x = soft_cap(x, cap, inv_cap);
+        if (EXTRA && r.softcap > 0.f) x = soft_cap_16(x, cap, inv_cap);
         if (EXTRA && r.slopes) x = fmaf(slope, (float)(j0 + j + 1 - q_hi), x);
         return x;
       };
