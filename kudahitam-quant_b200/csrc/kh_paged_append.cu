@@ -226,11 +226,14 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const __grid_constant
 //
 // Many rows: a lane owns 64 elements of a row, so that six stages of the
 // transform stay in registers on packed adds and only the last one (two at
-// D = 256) crosses lanes, while 16 warps fit an SM (20, with 96 registers, spilled and measured 82 us where 16 measure 74).  A warp's tile is 2048
-// elements, 32 "slots" of 64: 16 or 8 rows in (token, head) order, so that a
-// token's angles serve its heads from L1.  Slots come by cp.async, 16 bytes
-// a lane, into a private double buffer; each is 16 bytes longer than it
-// needs to be, so that the lanes' 16-byte reads hit different banks.
+// D = 256) crosses lanes, while 16 warps fit an SM (20, with 96 registers,
+// spilled and measured 82 us where 16 measure 74: 32768 tokens of 8 heads, D 128,
+// bf16, all rotated).  A warp's tile is 2048 elements, 32 "slots" of 64: 16 or 8
+// rows in (token, head) order, so that a token's angles serve its heads from
+// L1.  Slots come by cp.async, 16 bytes a lane, into a private double buffer;
+// each is 16 bytes longer than it needs to be, so that the lanes' 16-byte reads
+// hit different banks.  What bounds it is issue: 82 instructions a row (the widest
+// parts: two shifts an element for its bits, a third of one for the borders).
 constexpr int kTileWarps = 4;
 constexpr int kTileCtas = 4;
 // From how many keys (tokens x heads) they come in tiles: fewer do not give the
