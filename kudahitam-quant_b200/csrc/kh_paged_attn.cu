@@ -41,14 +41,13 @@ namespace {
 //           layout into the operand's.
 // Queries and weights are fixed point, PARTS bytes of them a column each, and
 // sums are exact in 32 bits.  Bits count as 0 / 1: sum w sign = 2 sum w bit -
-// sum w, exactly too.
+// sum w, whose second sum is a product with ones, exact too (as a float sum of
+// 1800 weights it cost fp32 results 2.5e-6 of their norm, now 2.6e-7).
 //   PARTS = 2 (16-bit queries, 4 a block of 8 columns): q~ to 2^-13 of its
 //     largest element (2^-16 for bits that count once), weights to 2^-16 of
 //     the largest of their unit, whose roundings average out; together under
 //     a tenth of a bf16 step.
-//   PARTS = 4 (32-bit queries, 2 a block): q~ to 2^-28, weights to 2^-31 (with
-//     three bytes, 2^-22, the result of 8 x 16 fp32 queries over rows up to
-//     40000 was off by 2.3e-6 of its norm, five times the plain form's error).
+//   PARTS = 4 (32-bit queries, 2 a block): q~ to 2^-28, weights to 2^-31.
 // What bounds it is issue: a 32-row tile takes 128 logic operations at half
 // rate, 32 products of 7.5 cycles, and some 370 other instructions.  On a ragged
 // batch (32 sequences up to 8192 rows, 8 KV heads x 4, D 128, bf16) the kernel
@@ -514,14 +513,15 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
   const float vb = 0.7978845608028654f * inv_sd * inv_sd * kOne;
   const float cap = r.softcap * kLog2e, inv_cap = r.softcap > 0.f ? 1.f / cap : 0.f;
 
-  float ref[NB], l[NB], w1s[NB], w2s[NB];
-  int acc[NB][MT][4];
+  // the last tile's rows are all ones: sums of the weights themselves
+  float ref[NB], l[NB], w1s[NB];
+  int acc[NB][MT + 1][4];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     ref[nb] = kNoRef;
-    l[nb] = w1s[nb] = w2s[nb] = 0.f;
+    l[nb] = w1s[nb] = 0.f;
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int i = 0; i <= MT; ++i)
 #pragma unroll
       for (int k = 0; k < 4; ++k) acc[nb][i][k] = 0;
   }
@@ -651,7 +651,6 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
       if (first) continue;  // nothing summed yet
       l[nb] *= f;
       w1s[nb] *= f;
-      w2s[nb] *= f;
       // sums move right; what a column loses its next lower one takes up
 #pragma unroll 1
       while (__any_sync(0xffffffffu, left > 0)) {
@@ -659,7 +658,7 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
         const uint32_t lost = (1u << sh) - 1u, half = (1u << sh) >> 1;
         left -= sh;
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+        for (int i = 0; i <= MT; ++i)
 #pragma unroll
           for (int k = 0; k < 4; k += 2) {
             uint32_t h = acc[nb][i][k], o = acc[nb][i][k + 1];
@@ -684,7 +683,7 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
   auto pack = [&] {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      uint32_t i1 = 0u, i2 = 0u;
+      uint32_t i1 = 0u;
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
         uint32_t u1[2], u2[2];
@@ -701,25 +700,26 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
           } else {
             const float x1 = none ? 0.f : e * ra[hf][rr], x2 = none ? 0.f : e * rb[hf][rr];
             w1s[nb] += x1;
-            w2s[nb] += x2;
             u1[rr] = __float2uint_rn(x1);
             u2[rr] = __float2uint_rn(x2);
           }
         }
         i1 += u1[0] + u1[1];
-        i2 += u2[0] + u2[1];
         // this lane's two columns, high byte first, of both rows
         const uint32_t sel = PARTS == 2 || low ? 0x4051u : 0x6273u;
         p1[hf][nb] = transpose8(__byte_perm(u1[0], u1[1], sel));
         p2[hf][nb] = transpose8(__byte_perm(u2[0], u2[1], sel));
       }
-      if constexpr (PARTS == 2) {
+      if constexpr (PARTS == 2)
         w1s[nb] += (float)(i1 - 4u * 0x4B000000u);  // without the exponent fields
-        w2s[nb] += (float)(i2 - 4u * 0x4B000000u);
-      }
     }
   };
   auto values = [&](const uint8_t* st, int p) {
+    const auto& ones = p == 0 ? p1 : p2;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+      mma16832u(acc[nb][MT], 0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u, ones[0][nb],
+                ones[1][nb]);
     uint32_t x[2][W / 4], y[2][W / 4];  // even and odd bytes of four rows, by half
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
@@ -790,7 +790,6 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
     for (int o = 4; o < 32; o <<= 1) {
       l[nb] += __shfl_xor_sync(0xffffffffu, l[nb], o);
       w1s[nb] += __shfl_xor_sync(0xffffffffu, w1s[nb], o);
-      w2s[nb] += __shfl_xor_sync(0xffffffffu, w2s[nb], o);
     }
     const int y = nb * QB + mine;
     float* rec = P.records + ((unit + group) * NQ + y) * (int64_t)(D + 2);
@@ -805,9 +804,12 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
     }
     __syncwarp();
     if (y < nq && g == 0 && !low) *reinterpret_cast<float2*>(rec) = make_float2(ref[nb], l[nb]);
-    const float base = -w1s[nb] - w2s[nb] + (cm / ch) * w1s[nb];
-    auto element = [&](int i, int k) {  // 2 sum w bit, bit i counting 2^(i & 7) times
-      const float h = (float)acc[nb][i][2 * k], o = (float)acc[nb][i][2 * k + 1];
+    const float base = (cm / ch) * w1s[nb];
+    // 2 sum w bit - sum w, bit i counting 2^(i & 7) times: the difference is
+    // taken in whole numbers, it is small beside its parts
+    auto element = [&](int i, int k) {
+      const float h = (float)(2 * acc[nb][i][2 * k] - (acc[nb][MT][0] << (i & 7)));
+      const float o = (float)(2 * acc[nb][i][2 * k + 1] - (acc[nb][MT][1] << (i & 7)));
       float x;
       if constexpr (PARTS == 2) {
         x = fmaf(h, 256.f, o);
@@ -815,7 +817,7 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
         x = low ? fmaf(h, 256.f, o) : fmaf(h, 16777216.f, o * 65536.f);
         x += __shfl_xor_sync(0xffffffffu, x, 1);
       }
-      return fmaf(x, 2.f / (float)(1 << (i & 7)), base) * is;
+      return fmaf(x, 1.f / (float)(1 << (i & 7)), base) * is;
     };
     const int e0 = 2 + (D == 128 ? 16 : 32) * g;
 #pragma unroll
