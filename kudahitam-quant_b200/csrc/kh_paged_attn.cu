@@ -113,13 +113,19 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 // device, so the cut is made there: units from what max_len allows left a
 // quarter of the SM time idle on the ragged batch, CTAs with a chunk of a fixed
 // length more.  Tiles and not rows are counted, as a group of one row costs its
-// tile: counted by rows, 17 x 4 x 5 queries with one own row each took 560 us.
+// tile (counted by rows, 17 x 4 x 5 queries with one own row each took 560 us),
+// and kGap more places a group without anything in them, as starting a piece
+// takes a warp about as long as three tiles (without them a warp was left with
+// 37 short pieces: 64 x 32 fp16 queries over a prefix of 8192 rows and 32 own
+// rows each took 175 us, now 94).
 // A unit may hold pieces of several groups; piece (unit u, group G) has record
 // u + G, as a unit's or a group's begin starts a new piece.
 //
 // What the warps need is prepared by a launch before: where each sequence's
 // tiles start, its rows, the units, and each group's queries as operand
 // fragments.
+constexpr int64_t kGap = 3;
+
 template <int D, int NB>
 struct Frags {  // of a group
   static constexpr int kSteps = D / 32;
@@ -244,7 +250,7 @@ __global__ void __launch_bounds__(128) paged_prepare_kernel(const __grid_constan
       int64_t n = 0;
       if (b < r.n_seqs) {
         const int64_t len = length_of(P, b), first = own_first(P, b, len);
-        n = (max((int64_t)0, len - first) + 31) / 32;
+        n = first < len ? (len - first + 31) / 32 + kGap : 0;
         P.own[b] = make_int2((int)min(first, len), (int)len);
       }
       int64_t upto = n;
@@ -266,7 +272,7 @@ __global__ void __launch_bounds__(128) paged_prepare_kernel(const __grid_constan
     if (threadIdx.x == 0) {
       P.starts[r.n_seqs] = base;
       const int64_t total =
-          r.n_kv_heads * (P.plan.pre_blocks * ((P.plan.pre_rows + 31) / 32) +
+          r.n_kv_heads * (P.plan.pre_blocks * ((P.plan.pre_rows + 31) / 32 + kGap) +
                           base * P.plan.own_blocks);
       Units u;
       u.size = max((int64_t)2, (total + P.n_warps - 1) / P.n_warps);
@@ -389,7 +395,7 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
   // implies the prefix's.
   if (!P.pre_tensor) grid_dependency_wait();
   const int64_t pre_tiles = (P.plan.pre_rows + 31) / 32;
-  const int64_t n_pre = r.n_kv_heads * P.plan.pre_blocks * pre_tiles;
+  const int64_t n_pre = r.n_kv_heads * P.plan.pre_blocks * (pre_tiles + kGap);
   const int64_t per = (int64_t)r.n_kv_heads * P.plan.own_blocks, size = P.units->size;
   const int64_t total = n_pre + P.starts[r.n_seqs] * per;
   const int64_t unit = (int64_t)blockIdx.x * kWarps + warp;
@@ -402,10 +408,15 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
   const bool pre = at < n_pre;
   const int64_t b = pre ? 0 : find_sequence(P, at - n_pre, per, lane);
   const int64_t start = pre ? 0 : n_pre + P.starts[b] * per;
-  const int64_t tiles = pre ? pre_tiles : P.starts[b + 1] - P.starts[b];
+  const int64_t places = pre ? pre_tiles + kGap : P.starts[b + 1] - P.starts[b];
+  const int64_t tiles = places - kGap;
   const int2 all = pre ? make_int2(0, (int)P.plan.pre_rows) : P.own[b];
-  const int hz = (int)((at - start) / tiles);
-  const int64_t begin = start + hz * tiles;
+  const int hz = (int)((at - start) / places);
+  const int64_t begin = start + hz * places;
+  if (at - begin >= tiles) {  // the gap
+    at = begin + places;
+    continue;
+  }
   const int n_tiles = (int)min(min(tiles - (at - begin), end - at), kPieceTiles);
   const int lo = all.x + 32 * (int)(at - begin);
   const int hi = n_tiles < tiles - (at - begin) ? lo + 32 * n_tiles : all.y;
@@ -879,14 +890,14 @@ __global__ void __launch_bounds__(32 * kMostJoin, D == 128 ? 3 : 2)
   } else if (P.plan.pre_blocks) {
     const uint32_t i = b * r.n_q + y, z = i / P.plan.block;
     const int64_t group = (int64_t)h * P.plan.pre_blocks + z;
-    pre = run(group * pre_tiles, pre_tiles, group, i - z * P.plan.block);
+    pre = run(group * (pre_tiles + kGap), pre_tiles, group, i - z * P.plan.block);
   }
   if (P.plan.own_blocks) {
-    const int64_t first = P.starts[b], tiles = P.starts[b + 1] - first;
+    const int64_t first = P.starts[b], places = P.starts[b + 1] - first;
     const int z = y / P.plan.block, hz = h * P.plan.own_blocks + z;
     const int64_t per = (int64_t)r.n_kv_heads * P.plan.own_blocks;
-    own = run(r.n_kv_heads * P.plan.pre_blocks * pre_tiles + first * per + hz * tiles, tiles,
-              r.n_kv_heads * P.plan.pre_blocks + b * per + hz, y - z * P.plan.block);
+    own = run(r.n_kv_heads * P.plan.pre_blocks * (pre_tiles + kGap) + first * per + hz * places,
+              places - kGap, r.n_kv_heads * P.plan.pre_blocks + b * per + hz, y - z * P.plan.block);
   }
   const int n = pre.n + own.n;
   grid_dependency_wait();
@@ -1098,8 +1109,8 @@ PagedPlan paged_plan(int64_t n_seqs, int n_q, int n_kv_heads, int D, int64_t max
   if (p.pre_rows > 0) p.pre_blocks = (int)((nq + p.block - 1) / p.block);
   if (p.own_rows > 0) p.own_blocks = (n_q + p.block - 1) / p.block;
   p.groups = n_kv_heads * (p.pre_blocks + n_seqs * p.own_blocks);
-  p.tiles = n_kv_heads * (p.pre_blocks * ((p.pre_rows + 31) / 32) +
-                          n_seqs * p.own_blocks * ((p.own_rows + 31) / 32));
+  p.tiles = n_kv_heads * (p.pre_blocks * ((p.pre_rows + 31) / 32 + kGap) +
+                          n_seqs * p.own_blocks * ((p.own_rows + 31) / 32 + kGap));
   p.max_units = std::min<int64_t>((int64_t)kRowsCtas * kWarps * n_sms, p.tiles / 2 + 1);
   return p;
 }
