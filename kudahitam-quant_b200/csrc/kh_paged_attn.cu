@@ -44,10 +44,19 @@ namespace {
 // sum w, whose second sum is a product with ones, exact too (as a float sum of
 // 1800 weights it cost fp32 results 2.5e-6 of their norm, now 2.6e-7).
 //   PARTS = 2 (16-bit queries, 4 a block of 8 columns): q~ to 2^-13 of its
-//     largest element (2^-16 for bits that count once), weights to 2^-16 of
-//     the largest of their unit, whose roundings average out; together under
-//     a tenth of a bf16 step.
-//   PARTS = 4 (32-bit queries, 2 a block): q~ to 2^-28, weights to 2^-31.
+//     largest element (2^-16 for bits that count once), weights in steps of 2^-15
+//     to 2^-17 of the largest around them.
+//   PARTS = 4 (32-bit queries, 2 a block): q~ to 2^-28, weights in steps of 2^-30
+//     to 2^-32.
+// A long tail of rows far below a step would count in the softmax's
+// denominator and not in its values (a first row with 0.6 of the weight before
+// 32767 alike ones: 20% off), so
+//   - the step follows the weights: every kSpan tiles it comes down to them where
+//     they have become small, so that a heavy row costs the 256 rows around it
+//     their low bits and no more; and
+//   - a lane of 16-bit queries carries what each rounding left into its next
+//     row's weight, so that rounded weights sum to the true ones.
+// What remains is 0.41 of a step a row, of either sign: 2^-12 of one heavy row.
 // What bounds it is issue: a 32-row tile takes 128 logic operations at half
 // rate, 32 products of 7.5 cycles, and some 370 other instructions.  On a ragged
 // batch (32 sequences up to 8192 rows, 8 KV heads x 4, D 128, bf16) the kernel
@@ -59,13 +68,15 @@ namespace {
 //
 // A warp runs on its own: 32-row tiles in a ring of cp.async stages, one lane
 // fetching one row (so pages may end anywhere).  The reference exponent of a
-// column is a whole number and moves only when a weight would leave its range,
-// so that most tiles rescale nothing and sums move by shifts.
+// column moves up when a weight would leave its range, and down as above; the
+// sums so far are then folded into floats in shared memory, so that most tiles
+// rescale nothing.
 // A piece of a unit is at most 16384 rows: 32-bit sums hold those (weights up
 // to 255 x 128 each), and what is summed as floats keeps its bits; the next
 // piece's record joins in.
 constexpr int kWarps = 4;
 constexpr int64_t kPieceTiles = 512;
+constexpr int kSpan = 4;  // tiles (a power of two)
 
 template <int D>
 struct RowsCfg {
@@ -74,6 +85,10 @@ struct RowsCfg {
   static constexpr int kPlane = 32 * W * 4;             // one plane of a tile
   static constexpr int kStage = 4 * kPlane + 512 + 16;  // + norms by row + valid mask
   static constexpr int kRing = kWarps * kStages * kStage;
+  // a warp's folded sums: a lane's elements of each block of columns, and
+  // {reference, l, sum of the code plane's weights, -}, {that since the last fold, -}
+  template <int PARTS, int NB>
+  static constexpr int kFold = NB * (W * 4 / (PARTS / 2) + 8) * 32 * 4;
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
@@ -389,6 +404,11 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
   const int mine = PARTS == 2 ? t : t >> 1;   // this lane's query of a block
   const bool low = PARTS == 4 && (t & 1);     // it holds the query's low bytes
   uint8_t* ring = smem + warp * kStages * C::kStage;
+  // element x of block nb at [nb * kOwn / 4 + x / 4][lane], then the block's statistics
+  constexpr int kOwn = 2 * MT / (PARTS / 2);
+  float4* fold4 = reinterpret_cast<float4*>(smem + C::kRing +
+                                            warp * C::template kFold<PARTS, NB>) + lane;
+  float4* stat4 = fold4 + NB * (kOwn / 4) * 32;
   // After a prefix launch this grid may run beside it: that one signals its
   // dependents once all earlier work is done, and nothing here reads its
   // records.  The wait then comes at the end, so that this grid's completion
@@ -519,24 +539,37 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
   }
   // weight 1 as a whole number, and the most one may be
   constexpr float kOne = PARTS == 2 ? 32768.f : 1073741824.f;
-  constexpr float kMost = PARTS == 2 ? 65535.f : 4294967040.f;
+  constexpr float kMost = PARTS == 2 ? 65534.f : 4294967040.f;  // and a remainder
   const float va = ch * inv_sd * kOne;
   const float vb = 0.7978845608028654f * inv_sd * inv_sd * kOne;
   const float cap = r.softcap * kLog2e, inv_cap = r.softcap > 0.f ? 1.f / cap : 0.f;
 
   // the last tile's rows are all ones: sums of the weights themselves
-  float ref[NB], l[NB], w1s[NB];
+  float ref[NB];
+  float2 l[NB];     // and what its last addition lost
+  float top[NB];    // largest weight since the reference moved, or of the last kSpan tiles
+  float2 over[NB];  // what the last roundings left, of either plane
   int acc[NB][MT + 1][4];
+  // lanes start with remainders spread over a step: what they end with does too
+  const float2 over0 = make_float2((2 * g - 7) * 0.0625f, (7 - 2 * g) * 0.0625f);
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     ref[nb] = kNoRef;
-    l[nb] = w1s[nb] = 0.f;
+    l[nb] = make_float2(0.f, 0.f);
+    top[nb] = 0.f;
+    over[nb] = over0;
+    stat4[nb * 64] = make_float4(kNoRef, 0.f, 0.f, 0.f);
+    stat4[nb * 64 + 32] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int x = 0; x < kOwn / 4; ++x)
+      fold4[(nb * (kOwn / 4) + x) * 32] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int i = 0; i <= MT; ++i)
 #pragma unroll
       for (int k = 0; k < 4; ++k) acc[nb][i][k] = 0;
   }
   const int pg = (g >> 1) + 4 * (g & 1);  // pi(g)
+  const bool uneven = cm != 0.f;          // the levels' middle adds a part of the weights' sum
 
   // A tile's scores and a tile's values are independent: in the loop the next
   // tile's scores and exponents run between this tile's value products.
@@ -629,21 +662,67 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
   // weights e = 2^(t2 - ref); true where they fit: a row's larger one decides
   // (and a NaN among the attended, which whole numbers would lose)
   auto weigh = [&] {
-    float top = 0.f;
+    bool fit = true;
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
+    for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
+      for (int k = 0; k < 4; ++k) {
         const float e = ex2(tt[k >> 1][k & 1][nb] - ref[nb]);
         ee[k >> 1][k & 1][nb] = e;
         const float most = max_nan(max_nan(ra[k >> 1][k & 1], rb[k >> 1][k & 1]), kOne * 0x1p-40f);
         // nothing attended: 0 times whatever the row's norms hold
-        top = max_nan(top, e == 0.f ? 0.f : e * most);
+        top[nb] = max_nan(top[nb], e == 0.f ? 0.f : e * most);
       }
-    return top <= kMost;
+      fit = fit && top[nb] <= kMost;
+    }
+    return fit;
   };
-  // the reference moves up to the tile's largest, what has been summed follows
-  auto rescale = [&](bool first) {
+  // What has been summed joins the sums in shared memory.  2 sum w bit - sum w,
+  // bit i counting 2^(i & 7) times: the difference is taken in whole numbers, it
+  // is small beside its parts.
+  auto fold = [&] {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const float4 old = stat4[nb * 64];
+      const float to = fmaxf(old.x, ref[nb]), was = ex2(old.x - to), is = ex2(ref[nb] - to);
+      stat4[nb * 64] = make_float4(to, fmaf(old.y, was, (l[nb].x + l[nb].y) * is),
+                                   fmaf(old.z, was, stat4[nb * 64 + 32].x * is), 0.f);
+      stat4[nb * 64 + 32] = make_float4(0.f, 0.f, 0.f, 0.f);
+      l[nb] = make_float2(0.f, 0.f);
+      const int c0 = acc[nb][MT][0], c1 = acc[nb][MT][1];
+      auto element = [&](int i, int k) {
+        const int h = acc[nb][i][2 * k], o = acc[nb][i][2 * k + 1];
+        const float fh = (float)(2 * h - (c0 << (i & 7))), fo = (float)(2 * o - (c1 << (i & 7)));
+        float x = PARTS == 2 || low ? fmaf(fh, 256.f, fo) : fmaf(fh, 16777216.f, fo * 65536.f);
+        if (PARTS == 4) x += __shfl_xor_sync(0xffffffffu, x, 1);
+        return x * (is * (1.f / (float)(1 << (i & 7))));
+      };
+#pragma unroll
+      for (int x = 0; x < kOwn; x += 4) {
+        // elements of a lane in the order i, k; a lane of 32-bit queries has its k
+        float v[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          if constexpr (PARTS == 2) {
+            v[y] = element((x + y) >> 1, y & 1);
+          } else {
+            const float v0 = element(x + y, 0), v1 = element(x + y, 1);
+            v[y] = t & 1 ? v1 : v0;
+          }
+        }
+        float4* to = fold4 + (nb * (kOwn / 4) + x / 4) * 32;
+        const float4 sum = *to;
+        *to = make_float4(fmaf(sum.x, was, v[0]), fmaf(sum.y, was, v[1]), fmaf(sum.z, was, v[2]),
+                          fmaf(sum.w, was, v[3]));
+      }
+#pragma unroll
+      for (int i = 0; i <= MT; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[nb][i][k] = 0;
+    }
+  };
+  // the reference moves down by as much, or up to the tile's largest
+  auto refer = [&](const float(&down)[NB]) {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       float mx = kNoRef;
@@ -655,74 +734,59 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
       }
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      if (!(mx < INFINITY)) l[nb] = NAN;  // a norm that is not finite has no average
-      const float to = fmaxf(ref[nb], ceilf(mx)), f = ex2(ref[nb] - to);
-      int left = (int)fminf(to - ref[nb], 48.f);
-      ref[nb] = to;
-      if (first) continue;  // nothing summed yet
-      l[nb] *= f;
-      w1s[nb] *= f;
-      // sums move right; what a column loses its next lower one takes up
-#pragma unroll 1
-      while (__any_sync(0xffffffffu, left > 0)) {
-        const int sh = min(left, 16);
-        const uint32_t lost = (1u << sh) - 1u, half = (1u << sh) >> 1;
-        left -= sh;
-#pragma unroll
-        for (int i = 0; i <= MT; ++i)
-#pragma unroll
-          for (int k = 0; k < 4; k += 2) {
-            uint32_t h = acc[nb][i][k], o = acc[nb][i][k + 1];
-            if constexpr (PARTS == 2) {
-              o += ((h & lost) << 8) + half;
-            } else {
-              const uint32_t o2 = o + ((h & lost) << 8);
-              const uint32_t down = __shfl_xor_sync(0xffffffffu, o2 & lost, 1);
-              if (low) {
-                h += down << 8;
-                o += ((h & lost) << 8) + half;
-              } else {
-                o = o2;
-              }
-            }
-            acc[nb][i][k] = (int)(h >> sh);
-            acc[nb][i][k + 1] = (int)(o >> sh);
-          }
-      }
+      if (!(mx < INFINITY)) l[nb].x = NAN;  // a norm that is not finite has no average
+      ref[nb] = fmaxf(ref[nb] - down[nb], mx);
+      if (PARTS == 4) ref[nb] = ceilf(ref[nb]);  // then factors between references are exact
+      over[nb] = over0;
+      top[nb] = 0.f;
     }
+  };
+  // sum + x, its rounding in the next one: thousands of alike small weights
+  // behind a large one lose the same part of each, 1e-5 of fp32 results
+  auto add = [](float2& sum, float x) {
+    const float y = x + sum.y, to = sum.x + y;
+    sum = make_float2(to, y - (to - sum.x));
   };
   auto pack = [&] {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      uint32_t i1 = 0u;
+      add(l[nb], (ee[0][0][nb] + ee[0][1][nb]) + (ee[1][0][nb] + ee[1][1][nb]));
+      float w1s = 0.f;
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
         uint32_t u1[2], u2[2];
 #pragma unroll
         for (int rr = 0; rr < 2; ++rr) {
           const float e = ee[hf][rr][nb];
-          l[nb] += e;
           const bool none = !full && tt[hf][rr][nb] == -INFINITY;
           if constexpr (PARTS == 2) {
-            // 2^23 + w: the low bits are w as a whole number
-            const float x1 = fmaf(e, ra[hf][rr], 8388608.f), x2 = fmaf(e, rb[hf][rr], 8388608.f);
-            u1[rr] = none ? 0x4B000000u : __float_as_uint(x1);
-            u2[rr] = none ? 0x4B000000u : __float_as_uint(x2);
+            // 1.5 2^23 + w: the low bits are w as a whole number
+            const float2 big = make_float2(12582912.f, 12582912.f);
+            float2 x = __ffma2_rn(make_float2(e, e), make_float2(ra[hf][rr], rb[hf][rr]), over[nb]);
+            if (none) x = over[nb];  // rounds to 0, as it is half a step at most
+            const float2 w = __fadd2_rn(x, big);
+            over[nb] = __fadd2_rn(__fadd2_rn(big, make_float2(-w.x, -w.y)), x);
+            if (uneven) w1s += w.x - big.x;
+            u1[rr] = __float_as_uint(w.x);
+            u2[rr] = __float_as_uint(w.y);
           } else {
             const float x1 = none ? 0.f : e * ra[hf][rr], x2 = none ? 0.f : e * rb[hf][rr];
-            w1s[nb] += x1;
+            w1s += x1;
             u1[rr] = __float2uint_rn(x1);
             u2[rr] = __float2uint_rn(x2);
           }
         }
-        i1 += u1[0] + u1[1];
         // this lane's two columns, high byte first, of both rows
         const uint32_t sel = PARTS == 2 || low ? 0x4051u : 0x6273u;
         p1[hf][nb] = transpose8(__byte_perm(u1[0], u1[1], sel));
         p2[hf][nb] = transpose8(__byte_perm(u2[0], u2[1], sel));
       }
-      if constexpr (PARTS == 2)
-        w1s[nb] += (float)(i1 - 4u * 0x4B000000u);  // without the exponent fields
+      if (uneven) {
+        float4 sum = stat4[nb * 64 + 32];
+        float2 two = make_float2(sum.x, sum.y);
+        add(two, w1s);
+        stat4[nb * 64 + 32] = make_float4(two.x, two.y, 0.f, 0.f);
+      }
     }
   };
   auto values = [&](const uint8_t* st, int p) {
@@ -758,9 +822,27 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
         }
       }
   };
-  auto settle = [&](bool first) {
-    if (!__all_sync(0xffffffffu, weigh())) {
-      rescale(first);
+  // weights of tile i, with the reference where it should be
+  auto settle = [&](int i) {
+    float down[NB] = {};
+    bool falls = false;
+    if (i != 0 && (i & (kSpan - 1)) == 0) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1)
+          top[nb] = max_nan(top[nb], __shfl_xor_sync(0xffffffffu, top[nb], o));
+        // weights like the last ones leave a bit, and one more that kMost has
+        if (top[nb] <= 0.5f * kOne && top[nb] > 0.f) {
+          down[nb] = -1.f - lg2(top[nb] * (1.f / kOne));
+          falls = true;
+        }
+        top[nb] = 0.f;
+      }
+    }
+    if (!__all_sync(0xffffffffu, weigh() && !falls)) {
+      if (i != 0) fold();
+      refer(down);
       weigh();
     }
     pack();
@@ -770,7 +852,7 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
   __syncwarp();
   scores(ring);
   exponents(ring, lo);
-  settle(true);
+  settle(0);
   int stage = 0;
 #pragma unroll 1
   for (int tile = 0; tile + 1 < n_tiles; ++tile) {
@@ -785,7 +867,7 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
     values(st, 0);
     exponents(next, lo + (tile + 1) * 32);
     values(st, 1);
-    settle(false);
+    settle(tile + 1);
     __syncwarp();
   }
   values(ring + stage * C::kStage, 0);
@@ -795,53 +877,48 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
 
   // ---- the record: 16 consecutive elements a lane (32 at D = 256), tile i's
   // parts elements i and 8 + i of each 16
+  fold();
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
+    float4 now = stat4[nb * 64];
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) {
-      l[nb] += __shfl_xor_sync(0xffffffffu, l[nb], o);
-      w1s[nb] += __shfl_xor_sync(0xffffffffu, w1s[nb], o);
+      now.y += __shfl_xor_sync(0xffffffffu, now.y, o);
+      now.z += __shfl_xor_sync(0xffffffffu, now.z, o);
     }
     const int y = nb * QB + mine;
     float* rec = P.records + ((unit + group) * NQ + y) * (int64_t)(D + 2);
     float is = 1.f / kOne, was = 0.f;
     if (more && y < nq) {  // joins the record
       const float2 old = *reinterpret_cast<const float2*>(rec);
-      const float top = fmaxf(old.x, ref[nb]), f = ex2(ref[nb] - top);
-      ref[nb] = top;
+      const float to = fmaxf(old.x, now.x), f = ex2(now.x - to);
+      now.x = to;
       is *= f;
-      was = ex2(old.x - top);
-      l[nb] = fmaf(l[nb], f, old.y * was);
+      was = ex2(old.x - to);
+      now.y = fmaf(now.y, f, old.y * was);
     }
     __syncwarp();
-    if (y < nq && g == 0 && !low) *reinterpret_cast<float2*>(rec) = make_float2(ref[nb], l[nb]);
-    const float base = (cm / ch) * w1s[nb];
-    // 2 sum w bit - sum w, bit i counting 2^(i & 7) times: the difference is
-    // taken in whole numbers, it is small beside its parts
-    auto element = [&](int i, int k) {
-      const float h = (float)(2 * acc[nb][i][2 * k] - (acc[nb][MT][0] << (i & 7)));
-      const float o = (float)(2 * acc[nb][i][2 * k + 1] - (acc[nb][MT][1] << (i & 7)));
-      float x;
-      if constexpr (PARTS == 2) {
-        x = fmaf(h, 256.f, o);
-      } else {
-        x = low ? fmaf(h, 256.f, o) : fmaf(h, 16777216.f, o * 65536.f);
-        x += __shfl_xor_sync(0xffffffffu, x, 1);
-      }
-      return fmaf(x, 1.f / (float)(1 << (i & 7)), base) * is;
-    };
+    if (y < nq && g == 0 && !low) *reinterpret_cast<float2*>(rec) = make_float2(now.x, now.y);
+    const float base = (cm / ch) * now.z;
     const int e0 = 2 + (D == 128 ? 16 : 32) * g;
+    auto put = [&](int i, int k, float v0, float v1) {  // elements i and i + 1
+      float2 v = make_float2((v0 + base) * is, (v1 + base) * is);
+      float2* at2 = reinterpret_cast<float2*>(rec + e0 + 16 * (i >> 3) + 8 * k + (i & 7));
+      if (more) v = make_float2(fmaf(at2->x, was, v.x), fmaf(at2->y, was, v.y));
+      *at2 = v;
+    };
 #pragma unroll
-    for (int i = 0; i < MT; i += 2)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        float2 v = make_float2(element(i, k), element(i + 1, k));
-        if (y < nq && (PARTS == 2 || (t & 1) == k)) {
-          float2* at2 = reinterpret_cast<float2*>(rec + e0 + 16 * (i >> 3) + 8 * k + (i & 7));
-          if (more) v = make_float2(fmaf(at2->x, was, v.x), fmaf(at2->y, was, v.y));
-          *at2 = v;
-        }
+    for (int x = 0; x < kOwn; x += 4) {
+      const float4 v = fold4[(nb * (kOwn / 4) + x / 4) * 32];
+      if (y >= nq) continue;
+      if constexpr (PARTS == 2) {
+        put(x >> 1, 0, v.x, v.z);
+        put(x >> 1, 1, v.y, v.w);
+      } else {
+        put(x, t & 1, v.x, v.y);
+        put(x + 2, t & 1, v.z, v.w);
       }
+    }
   }
   __syncwarp();
   }
@@ -980,7 +1057,9 @@ __global__ void __launch_bounds__(32 * kMostJoin, D == 128 ? 3 : 2)
 template <int D, int PARTS, bool EXTRA, int NB>
 kh_status launch_rows(AttnParams P, cudaStream_t stream) {
   const PagedAttnRequest& r = P.r;
-  constexpr int NQ = NB * 8 / PARTS, kSmem = RowsCfg<D>::kRing;
+  constexpr int NQ = NB * 8 / PARTS;
+  constexpr int kSmem = RowsCfg<D>::kRing + kWarps * RowsCfg<D>::template kFold<PARTS, NB>;
+  static_assert(kRowsCtas * (kSmem + 1024) <= 233472, "shared memory of an SM");
   auto kern = paged_rows_kernel<D, PARTS, EXTRA, NB>;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return KH_ECUDA;

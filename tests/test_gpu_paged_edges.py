@@ -1,0 +1,139 @@
+"""The paged attention operators where their number formats end: one weight far
+above thousands of others, values and norms at the ends of their types, and
+batches whose places are not all in use."""
+import math
+
+import pytest
+import torch
+
+import paged_ref as R
+from kudahitam import _lib, lloyd_max, ops, rademacher
+
+pytestmark = pytest.mark.gpu
+
+BF, HF, FL = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.fixture(autouse=True)
+def _no_device_error():
+    _lib.call("kh_clear_device_error")
+    yield
+    assert _lib.device_error() == 0
+
+
+def _planted(D, page, targets, common, seed, sigma_v=1.0):
+    """One KV head whose row j has score targets[j] (natural units) for a query
+    `base`, and value rows that share `common` of their squared length.
+    (base, K pool, V pool, dk, dv, c)"""
+    n = len(targets)
+    pages = -(-n // page)
+    g = torch.Generator().manual_seed(seed)
+    dk, dv, c = rademacher(D, 2 * seed), rademacher(D, 2 * seed + 1), lloyd_max(1, D)
+    base = torch.randn(D, generator=g, dtype=torch.float64)
+    qt = (base * dk.double()) @ R.hadamard(D) / math.sqrt(D)
+    bits = (qt > 0).long()
+    # every key has the query's signs: s_j = norm_j sum |q~| (c1 + 0.5 / sqrt(D))
+    per = (qt.abs().sum() * (c[1].double() + 0.5 / math.sqrt(D))) / math.sqrt(D)
+    norm = torch.ones(pages * page, dtype=torch.float64)
+    norm[:n] = targets / per
+    k = ops.PackedKV((pages, 1, page, D), 1, R.words(bits.expand(pages * page, D)), norm.float(),
+                     R.words(bits.expand(pages * page, D)), (0.5 * norm).float())
+    x = math.sqrt(1 - common) * torch.randn(pages * page, D, generator=g, dtype=torch.float64)
+    x += math.sqrt(common) * torch.randn(D, generator=g, dtype=torch.float64)
+    code, res, vn, vr = R.compress(x * sigma_v, dv, c)
+    v = ops.PackedKV((pages, 1, page, D), 1, R.words(code), vn.float(), R.words(res), vr.float())
+    return base, k, v, dk, dv, c
+
+
+def _off(got, want):
+    return ((got.detach().cpu().double() - want).norm(dim=-1) / want.norm(dim=-1)).max().item()
+
+
+def _sink(n, share, sigma, D, common, seed, page=64):
+    """A first row of weight `share` beside n - 1 others of spread sigma."""
+    g = torch.Generator().manual_seed(seed + 1)
+    t = 2.0 + sigma * torch.randn(n, generator=g, dtype=torch.float64).clamp(-3, 3)
+    t[0] = torch.logsumexp(t[1:], 0) + math.log(share / (1 - share))
+    return _planted(D, page, t.clamp_min(1e-3), common, seed)
+
+
+def _queries(base, B, nq, dtype):
+    """Query rows along base, up to 2% longer or shorter."""
+    f = 1 + 0.02 * torch.linspace(-1, 1, B * nq, dtype=torch.float64)
+    return (f.view(B, nq, 1) * base).to(dtype)
+
+
+# Relative 2-norm of an output row's error.  The output's rounding: half a step
+# eps / 2 at most, 0.43 of that in the mean square over a binade, within 15% over
+# 128 elements: 1.9e-3 (bf16), 2.4e-4 (fp16).  The values' weights: 256 rows share the
+# step of the heaviest, 2^-15 of it, later ones have steps of a half, a quarter and
+# so on of that; 0.41 of a step a row (the difference of two remainders), at random:
+# sqrt(256 4/3) 0.41 2^-15 = 2.3e-4.  Scores of up to 20 (in log2), 16-bit queries' fixed
+# point 2^-13.7 sqrt(D) max |q~| / |q| of them at most, that over sqrt(D) in the mean
+# square (5e-5), times 2 share (1 - share) <= 1/2: under 1e-4.  Root sums 1.92e-3 and 3.5e-4.
+# fp32: exponents of 20 in three 32-bit roundings, 20 3 2^-24, a half of that as above:
+# 1.8e-6; weights of 2^-30 of the heaviest, all of one sign: 256 (1 + 1/2 + ...) 2^-31: 2.4e-7.
+WITHIN = {BF: 2e-3, HF: 4e-4, FL: 2.1e-6}
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FL])
+@pytest.mark.parametrize("D,B,nq,n,share,sigma,common", [
+    (128, 32, 4, 8192, 0.80, 0.0, 0.5), (128, 32, 4, 8192, 0.87, 0.5, 0.5),
+    (128, 512, 4, 32768, 0.50, 0.0, 0.5), (128, 512, 4, 32768, 0.62, 0.5, 0.5),
+    (128, 512, 4, 32768, 0.71, 1.0, 0.5), (128, 512, 4, 32768, 0.71, 1.0, 0.0),
+    (128, 256, 7, 32768, 0.66, 0.5, 0.5), (256, 256, 3, 16384, 0.67, 0.0, 0.5),
+    (256, 256, 8, 16384, 0.87, 1.0, 0.0), (128, 2, 2, 300, 0.90, 0.5, 0.5),
+])
+def test_small_weights_beside_a_large_one(dtype, D, B, nq, n, share, sigma, common):
+    """A first row that takes most of the weight, as contexts have it, and a
+    long tail whose rows each count little but together much."""
+    base, k, v, dk, dv, c = _sink(n, share, sigma, D, common, n + nq)
+    q = _queries(base, B, nq, dtype)
+    pages = k.shape[0]
+    table = torch.arange(pages, dtype=torch.int32).expand(B, -1).contiguous()
+    out = ops.paged_decode_attention(q.cuda(), R.cuda(k), R.cuda(v), table.cuda(),
+                                     torch.full((B,), n, dtype=torch.int32).cuda(), dk, dv, c)
+    few = [0, B // 2, B - 1]
+    want = R.attention(q[few], k, v, table[few], [n] * 3, dk, dv, c)[0]
+    assert _off(out[few], want) <= WITHIN[dtype]
+    # and the engine's attention over the same rows in one piece
+    one = ops.decode_attention(q[:1].float().cuda(), R.cuda(k), R.cuda(v), dk, dv, c, length=n)
+    assert _off(one, want[:1]) <= 1e-4
+    assert _off(out[:1], one.cpu().double()) <= WITHIN[dtype] + 1e-4
+
+
+@pytest.mark.parametrize("dtype,D,B,nq", [(BF, 128, 7, 4), (HF, 128, 16, 4), (HF, 256, 13, 7),
+                                          (FL, 128, 8, 4)])
+@pytest.mark.parametrize("n,share,sigma", [(8192, 0.8, 0.0), (32768, 0.62, 0.5)])
+def test_small_weights_beside_a_large_one_in_a_prefix(dtype, D, B, nq, n, share, sigma):
+    base, k, v, dk, dv, c = _sink(n, share, sigma, D, 0.5, n + B)
+    q = _queries(base, B, nq, dtype)
+    table = torch.arange(k.shape[0], dtype=torch.int32).expand(B, -1).contiguous()
+    out = ops.paged_prefix_attention(q.cuda(), R.cuda(k), R.cuda(v), table.cuda(),
+                                     torch.full((B,), n, dtype=torch.int32).cuda(), n, dk, dv, c)
+    few = [0, B - 1]
+    want = R.attention(q[few], k, v, table[few], [n] * 2, dk, dv, c)[0]
+    assert _off(out[few], want) <= WITHIN[dtype]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FL])
+@pytest.mark.parametrize("D,nq", [(128, 4), (128, 8), (256, 4)])
+def test_weights_that_rise_and_fall(dtype, D, nq):
+    """Heavy rows anywhere, each of another size, with every row in between far
+    below them and far above what came before."""
+    n, B = 16384, 256
+    g = torch.Generator().manual_seed(D + nq)
+    t = 4.0 + 0.5 * torch.randn(n, generator=g, dtype=torch.float64)
+    at = torch.tensor([0, 1, 31, 32, 255, 256, 257, 1000, 1031, 4000, 8191, 16383])
+    t[at] += torch.tensor([5.0, 1, 6, 2, 5, 7, 4, 3, 8, 1, 7, 8], dtype=torch.float64)
+    t[2000:3000] -= 3.0
+    base, k, v, dk, dv, c = _planted(D, 64, t, 0.5, n + nq)
+    q = _queries(base, B, nq, dtype)
+    table = torch.arange(k.shape[0], dtype=torch.int32).expand(B, -1).contiguous()
+    ln = torch.full((B,), n, dtype=torch.int32)
+    out, lse = ops.paged_decode_attention(q.cuda(), R.cuda(k), R.cuda(v), table.cuda(), ln.cuda(),
+                                          dk, dv, c, return_lse=True)
+    few = [0, B - 1]
+    want = R.attention(q[few], k, v, table[few], [n] * 2, dk, dv, c)
+    assert _off(out[few], want[0]) <= WITHIN[dtype]
+    assert (lse[few].cpu().double() - want[1]).abs().max() <= 2e-3
