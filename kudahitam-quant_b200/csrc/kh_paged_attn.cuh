@@ -88,10 +88,11 @@ __device__ __forceinline__ int64_t own_first(const AttnParams& P, int64_t b, int
   return max(first_of(P, b, len), P.r.prefix_len);
 }
 // cap tanh(t / cap): 1 - 2 / (e^2x + 1) loses what is left of small x, so
-// below 0.3 the odd series (its next term is under 2^-33 of x there).
+// below 0.3 the odd series (its next term is under 2^-33 of x there).  A NaN
+// stays one: it compares false twice.
 __device__ __forceinline__ float soft_cap(float t, float cap, float inv_cap) {
   const float x = t * inv_cap, a = fabsf(x);
-  const float big = copysignf(1.f - 2.f / (__expf(2.f * fminf(a, 20.f)) + 1.f), x);
+  const float big = copysignf(1.f - 2.f / (__expf(2.f * (a > 20.f ? 20.f : a)) + 1.f), x);
   const float z = x * x;
   float s = fmaf(z, 0.0035921280f, -0.0088632355f);
   s = fmaf(z, s, 0.021869488f);

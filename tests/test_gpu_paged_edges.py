@@ -137,3 +137,40 @@ def test_weights_that_rise_and_fall(dtype, D, nq):
     want = R.attention(q[few], k, v, table[few], [n] * 2, dk, dv, c)
     assert _off(out[few], want[0]) <= WITHIN[dtype]
     assert (lse[few].cpu().double() - want[1]).abs().max() <= 2e-3
+
+
+def _batch(lengths, page, H, D, nq, dtype, seed, pages=None):
+    need = pages or sum(-(-n // page) for n in lengths) + 1
+    kc, vc, dk, dv, c = R.pools(need, H, page, D, seed)
+    table = R.tables(lengths, page, need, seed)
+    g = torch.Generator().manual_seed(seed + 1)
+    q = torch.randn(len(lengths), H * nq, D, generator=g).to(dtype)
+    return q, kc, vc, table, torch.tensor(lengths, dtype=torch.int32).cuda(), dk, dv, c
+
+
+@pytest.mark.parametrize("dtype,D,nq", [(FL, 128, 2), (FL, 256, 1), (BF, 128, 4), (HF, 256, 5)])
+def test_capped_scores_keep_nan(dtype, D, nq):
+    """With a cap, too, a NaN in an attended row's norms or in a query (or an
+    infinity, whose products are NaN) makes that result NaN and no other."""
+    lengths, page, H = [200, 150, 90], 16, 2
+    q, kc, vc, table, ln, dk, dv, c = _batch(lengths, page, H, D, nq, dtype, 41)
+    run = lambda x: ops.paged_decode_attention(  # noqa: E731
+        x.cuda(), R.cuda(kc), R.cuda(vc), table.cuda(), ln, dk, dv, c, softcap=8.0).cpu().float()
+    R.check(run(q), None, R.attention(q, kc, vc, table, lengths, dk, dv, c, softcap=8.0), dtype)
+    for pool in (kc, vc):
+        for norms in (pool.norms, pool.rnorms):
+            for j in (0, 37, 149):
+                row = (int(table[1, j // page]) * H + 1) * page + j % page
+                old = norms[row].clone()
+                norms[row] = math.nan
+                out = run(q)
+                norms[row] = old
+                assert torch.isnan(out[1, nq:]).all()
+                assert torch.isfinite(out[[0, 2]]).all() and torch.isfinite(out[1, :nq]).all()
+    for bad in (math.nan, math.inf, -math.inf):
+        x = q.clone()
+        x[2, nq - 1, 5] = bad
+        out = run(x)
+        assert torch.isnan(out[2, nq - 1]).all()
+        out[2, nq - 1] = 0
+        assert torch.isfinite(out).all()
