@@ -636,11 +636,14 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
       for (int rr = 0; rr < 2; ++rr) {
         const int row = 16 * hf + pg + 8 * rr;
         const float4 n = nrm[row];
+        // NaN for an infinite norm too, whose products with bits of either sign have
+        // no sum: a score of minus infinity would count as not attended
+        const float nil = fmaf(n.y, 0.f, n.x * 0.f);
         ra[hf][rr] = n.z * va;
         rb[hf][rr] = n.w * vb;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-          float x = n.x * fmaf(a1[nb], joined(s1[hf][nb], rr), b1[nb]);
+          float x = fmaf(n.x, fmaf(a1[nb], joined(s1[hf][nb], rr), b1[nb]), nil);
           x = fmaf(n.y, fmaf(a2[nb], joined(s2[hf][nb], rr), b2[nb]), x);
           if (EXTRA && r.softcap > 0.f)
             x = PARTS == 2 ? soft_cap_16(x, cap, inv_cap) : soft_cap(x, cap, inv_cap);
@@ -667,11 +670,12 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
     for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const float e = ex2(tt[k >> 1][k & 1][nb] - ref[nb]);
+        const float x = tt[k >> 1][k & 1][nb], e = ex2(x - ref[nb]);
         ee[k >> 1][k & 1][nb] = e;
         const float most = max_nan(max_nan(ra[k >> 1][k & 1], rb[k >> 1][k & 1]), kOne * 0x1p-40f);
-        // nothing attended: 0 times whatever the row's norms hold
-        top[nb] = max_nan(top[nb], e == 0.f ? 0.f : e * most);
+        // nothing attended: 0 whatever the row's norms hold (but a weight that is
+        // only too small to tell from 0 makes NaN of an infinite one)
+        top[nb] = max_nan(top[nb], x == -INFINITY ? 0.f : e * most);
       }
       fit = fit && top[nb] <= kMost;
     }

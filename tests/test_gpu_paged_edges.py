@@ -174,3 +174,39 @@ def test_capped_scores_keep_nan(dtype, D, nq):
         assert torch.isnan(out[2, nq - 1]).all()
         out[2, nq - 1] = 0
         assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("dtype,D,nq,B,prefix", [
+    (FL, 128, 2, 3, 0), (BF, 128, 8, 3, 0), (HF, 256, 3, 3, 0), (BF, 128, 4, 3, 64), (BF, 128, 4, 12, 64),
+    (BF, 256, 4, 9, 64)])
+@pytest.mark.parametrize("softcap", [0.0, 10.0])
+def test_infinite_norms_of_attended_rows(dtype, D, nq, B, prefix, softcap):
+    """An infinity among the attended rows' norms has no average: NaN, whatever
+    the score's sign and however small the row's weight."""
+    page, H = 16, 1
+    lengths = [150 + b for b in range(B)]
+    q, kc, vc, table, ln, dk, dv, c = _batch(lengths, page, H, D, nq, dtype, 43)
+    table[:, :prefix // page] = table[0, :prefix // page]
+    # the row at 100 (or 7) counts nothing beside the last ones: 2^-500
+    slopes = torch.full((nq,), 10.0)
+
+    def run(sl):
+        a = (q.cuda(), R.cuda(kc), R.cuda(vc), table.cuda(), ln)
+        kw = dict(softcap=softcap, slopes=sl)
+        if prefix:
+            return ops.paged_prefix_attention(*a, prefix, dk, dv, c, **kw).cpu().float()
+        return ops.paged_decode_attention(*a, dk, dv, c, **kw).cpu().float()
+
+    assert torch.isfinite(run(None)).all() and torch.isfinite(run(slopes.cuda())).all()
+    for j in (7, 100):
+        hit = list(range(B)) if j < prefix else [1]
+        miss = [b for b in range(B) if b not in hit]
+        row = int(table[1, j // page]) * page + j % page
+        for norms in (kc.norms, kc.rnorms, vc.norms, vc.rnorms):
+            old = norms[row].clone()
+            norms[row] = math.inf
+            for sl in (None, slopes.cuda()):
+                out = run(sl)
+                assert torch.isnan(out[hit]).all(), (j, sl is None)
+                assert torch.isfinite(out[miss]).all()
+            norms[row] = old
