@@ -321,7 +321,8 @@ __global__ void __launch_bounds__(128) paged_prepare_kernel(const __grid_constan
     for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     // whole numbers that PARTS signed bytes hold: 127 x 256 + 127, or 127 x 2^24
     constexpr float kLargest = PARTS == 2 ? 32639.f : 2130706432.f;
-    const float up = mx > 0.f && mx < INFINITY ? kLargest / mx : 1.f;
+    // (at most 2^110, so that its inverse keeps its bits: smaller queries' scores are 0)
+    const float up = mx > 0.f && mx < INFINITY ? fminf(kLargest / mx, 0x1p110f) : 1.f;
 #pragma unroll
     for (int j = 0; j < W; ++j) {
       // element 32 j + lane: its bit's place in the masked byte counts 2^(bit & 3) times

@@ -210,3 +210,20 @@ def test_infinite_norms_of_attended_rows(dtype, D, nq, B, prefix, softcap):
                 assert torch.isnan(out[hit]).all(), (j, sl is None)
                 assert torch.isfinite(out[miss]).all()
             norms[row] = old
+
+
+@pytest.mark.parametrize("dtype,f", [(FL, 1e-32), (FL, 1e-38), (BF, 1e-36), (BF, 1e-38), (HF, 1e-7)])
+@pytest.mark.parametrize("D,B,nq", [(128, 3, 4), (256, 2, 3), (128, 10, 4)])
+def test_tiny_queries(dtype, f, D, B, nq):
+    """Queries so small that every score is 0 in 32 bits: the rows' average."""
+    lengths, page = [70 + 9 * b for b in range(B)], 16
+    q, kc, vc, table, ln, dk, dv, c = _batch(lengths, page, 1, D, nq, FL, 47)
+    q = (q * f).to(dtype)
+    want = R.attention(q, kc, vc, table, lengths, dk, dv, c)
+    a = (q.cuda(), R.cuda(kc), R.cuda(vc), table.cuda(), ln)
+    R.check(*ops.paged_decode_attention(*a, dk, dv, c, return_lse=True), want, dtype)
+    # one shared page, that of sequence 0
+    table[:, 0] = table[0, 0]
+    want = R.attention(q, kc, vc, table, lengths, dk, dv, c)
+    a = (q.cuda(), R.cuda(kc), R.cuda(vc), table.cuda(), ln)
+    R.check(*ops.paged_prefix_attention(*a, page, dk, dv, c, return_lse=True), want, dtype)
