@@ -172,9 +172,8 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
 
   if (warp >= C::kSoftWarps && warp < C::kSoftWarps + 4) {
     // ------------------------------------------------------------ decoding
-    // (no wait: what was before the queries' launch was done when this grid
-    // could start)
     if constexpr (D == 128) fewer_registers<kRegsDecode>();
+    grid_dependency_wait();
     const int i = threadIdx.x - 32 * C::kSoftWarps;  // row of the tile
     // at D = 256 a row is two threads', half its words each
     constexpr int kSplit = 128 / ROWS;
