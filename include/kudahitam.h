@@ -452,8 +452,10 @@ int kh_paged_append(const kh_paged_cache* cache, const void* k, const void* v, i
  *   lengths     device int32 [n_seqs], each at most max_len
  *   starts      device int32 [n_seqs] first attended row, or NULL (0)
  *   prefix_len  the first prefix_len rows are the same cached rows for every
- *               sequence: they are read through sequence 0's table row, once
- *               for all sequences.  0: nothing shared.
+ *               sequence, as far as it goes: they are read once for all, through
+ *               the table row of the first sequence that has all of them (else
+ *               of the longest), as far as that one goes; rows that none
+ *               attends too.  0: nothing shared.
  *   window      0, or how many of the last rows are attended
  *   softcap     0, or the cap; slopes: device float [n_kv_heads * n_q] or NULL
  *   workspace   kh_paged_workspace_bytes() bytes of device memory for the

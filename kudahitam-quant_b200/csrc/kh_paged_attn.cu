@@ -137,8 +137,8 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 // u + G, as a unit's or a group's begin starts a new piece.
 //
 // What the warps need is prepared by a launch before: where each sequence's
-// tiles start, its rows, the units, and each group's queries as operand
-// fragments.
+// tiles start, its rows, the units, through which sequence the prefix is read,
+// and each group's queries as operand fragments.
 constexpr int64_t kGap = 3;
 
 template <int D, int NB>
@@ -152,7 +152,7 @@ struct Frags {  // of a group
 struct Group {
   bool pre;
   int h, z;
-  int64_t b;  // sequence whose table is read
+  int64_t b;  // sequence (0 for the prefix)
 };
 __device__ __forceinline__ Group group_of(const AttnParams& P, int64_t i) {
   Group g;
@@ -260,11 +260,13 @@ __global__ void __launch_bounds__(128) paged_prepare_kernel(const __grid_constan
   grid_dependents_launch();
   if (blockIdx.x == 0) {
     int64_t base = 0;
+    uint64_t best = 0;  // (rows of the prefix, the lower of two sequences) as one number
     for (int64_t b0 = 0; b0 < r.n_seqs; b0 += 128) {
       const int64_t b = b0 + threadIdx.x;
       int64_t n = 0;
       if (b < r.n_seqs) {
         const int64_t len = length_of(P, b), first = own_first(P, b, len);
+        best = max(best, (uint64_t)min(len, r.prefix_len) << 32 | (uint64_t)(0xffffffffll - b));
         n = first < len ? (len - first + 31) / 32 + kGap : 0;
         P.own[b] = make_int2((int)min(first, len), (int)len);
       }
@@ -284,12 +286,21 @@ __global__ void __launch_bounds__(128) paged_prepare_kernel(const __grid_constan
       }
       if (b < r.n_seqs) P.starts[b] = before + upto - n;
     }
+#pragma unroll
+    for (int o = 16; o; o >>= 1)
+      best = max(best, (uint64_t)__shfl_xor_sync(0xffffffffu, best, o));
+    __syncthreads();
+    if (lane == 0) part[warp] = (int64_t)best;
+    __syncthreads();
     if (threadIdx.x == 0) {
+      for (int w = 1; w < 4; ++w) best = max(best, (uint64_t)part[w]);
+      Units u;
+      u.source = 0xffffffffll - (int64_t)(best & 0xffffffffu);
+      u.pre_end = (int64_t)(best >> 32);
       P.starts[r.n_seqs] = base;
       const int64_t total =
-          r.n_kv_heads * (P.plan.pre_blocks * ((P.plan.pre_rows + 31) / 32 + kGap) +
+          r.n_kv_heads * (P.plan.pre_blocks * ((u.pre_end + 31) / 32 + kGap) +
                           base * P.plan.own_blocks);
-      Units u;
       u.size = max((int64_t)2, (total + P.n_warps - 1) / P.n_warps);
       u.mul = ~uint64_t(0) / (uint64_t)u.size + 1;
       *P.units = u;
@@ -415,7 +426,7 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
   // before visible to it.  (Own rows beside the prefix's last CTAs without the wait: 64 x 32
   // queries behind a prompt of 8192 rows 42.8 us, with it 44.3.)
   grid_dependency_wait();
-  const int64_t pre_tiles = (P.plan.pre_rows + 31) / 32;
+  const int64_t pre_end = P.units->pre_end, pre_tiles = (pre_end + 31) / 32;
   const int64_t n_pre = r.n_kv_heads * P.plan.pre_blocks * (pre_tiles + kGap);
   const int64_t per = (int64_t)r.n_kv_heads * P.plan.own_blocks, size = P.units->size;
   const int64_t total = n_pre + P.starts[r.n_seqs] * per;
@@ -427,11 +438,11 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
   // ---- the piece: rows [lo, hi) of a sequence (or of the prefix, for every
   // sequence's queries) for query rows y0 .. y0 + nq of KV head h
   const bool pre = at < n_pre;
-  const int64_t b = pre ? 0 : find_sequence(P, at - n_pre, per, lane);
+  const int64_t b = pre ? P.units->source : find_sequence(P, at - n_pre, per, lane);
   const int64_t start = pre ? 0 : n_pre + P.starts[b] * per;
   const int64_t places = pre ? pre_tiles + kGap : P.starts[b + 1] - P.starts[b];
   const int64_t tiles = places - kGap;
-  const int2 all = pre ? make_int2(0, (int)P.plan.pre_rows) : P.own[b];
+  const int2 all = pre ? make_int2(0, (int)pre_end) : P.own[b];
   const int hz = (int)((at - start) / places);
   const int64_t begin = start + hz * places;
   if (at - begin >= tiles) {  // the gap
@@ -963,7 +974,7 @@ __global__ void __launch_bounds__(32 * kMostJoin, D == 128 ? 3 : 2)
   };
   Run pre{P.records, 0}, own{P.records, 0};
   int64_t pre_stride = stride;
-  const int64_t pre_tiles = (P.plan.pre_rows + 31) / 32;
+  const int64_t pre_tiles = P.plan.groups > 0 ? (P.units->pre_end + 31) / 32 : 0;
   if (P.plan.pre_chunks) {
     pre = Run{r.workspace + (int64_t)row * P.plan.pre_chunks * kRec, P.plan.pre_chunks};
     pre_stride = kRec;

@@ -10,10 +10,14 @@ namespace kh {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// How the rows kernel's tiles are cut (kh_paged_attn.cu).
+// How the rows kernel's tiles are cut (kh_paged_attn.cu), and whose prefix is read.
 struct Units {
   int64_t size;
   uint64_t mul;  // floor(2^64 / size) + 1: x / size while x size < 2^64
+  // The prefix is read through the table of the first sequence that has all of
+  // it, or else of the longest: places of a batch may be empty or short.
+  int64_t source;
+  int64_t pre_end;  // rows of it that `source` has
   __device__ __forceinline__ int64_t of(int64_t x) const {
     return (int64_t)__umul64hi((uint64_t)x, mul);
   }

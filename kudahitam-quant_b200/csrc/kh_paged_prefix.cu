@@ -184,14 +184,16 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
       float kn, krn, vn, vrn;
       bool on;
     };
+    const int32_t* table = r.table + P.units->source * r.table_stride;
+    const int end = (int)min((int64_t)hi, P.units->pre_end);
     auto page_of = [&](int t) {
       const uint32_t j = lo + t * ROWS + row;
-      return (t < n_tiles && (int)j < hi) ? r.table[P.page_div(j)] : -1;
+      return (t < n_tiles && (int)j < end) ? table[P.page_div(j)] : -1;
     };
     auto fetch = [&](int t, int page) {
       Row x;
       const uint32_t j = lo + t * ROWS + row;
-      const bool in = t < n_tiles && (int)j < hi;
+      const bool in = t < n_tiles && (int)j < end;
       x.on = in && (uint32_t)page < (uint32_t)r.n_pages;
       if (in && !x.on) flag_error(P.err, kErrBadIndex);
       x.kn = x.krn = x.vn = x.vrn = 0.f;

@@ -674,8 +674,10 @@ def paged_prefix_attention(q: torch.Tensor, k_cache: PackedKV, v_cache: PackedKV
                            slopes: Optional[torch.Tensor] = None, return_lse: bool = False):
     """``paged_decode_attention`` for a batch whose sequences begin with the
     same ``prefix_len`` cached rows: those are read once for all sequences,
-    through sequence 0's row of the block table; rows from prefix_len on are
-    each sequence's own.  ``lengths`` count the prefix."""
+    through the block table's row of the first sequence that has them all (or
+    else of the longest); rows from prefix_len on are each sequence's own.
+    ``lengths`` count the prefix; shorter sequences and empty places (length 0)
+    may stand anywhere in the batch."""
     return _paged_attention(q, k_cache, v_cache, block_table, lengths, int(prefix_len), dk, dv,
                             centroids, sm_scale, max_len, starts, window, softcap, slopes,
                             return_lse)

@@ -227,3 +227,47 @@ def test_tiny_queries(dtype, f, D, B, nq):
     want = R.attention(q, kc, vc, table, lengths, dk, dv, c)
     a = (q.cuda(), R.cuda(kc), R.cuda(vc), table.cuda(), ln)
     R.check(*ops.paged_prefix_attention(*a, page, dk, dv, c, return_lse=True), want, dtype)
+
+
+@pytest.mark.parametrize("dtype,D,nq", [(BF, 128, 4), (BF, 256, 4), (HF, 128, 2), (FL, 128, 3)])
+@pytest.mark.parametrize("lengths", [
+    [0] + [330 + 7 * b for b in range(11)],           # an unused place first
+    [100, 0, 300, 319, 330] + [340] * 7,              # short ones first
+    [0, 17, 160, 5, 200] + [130] * 7,                 # none reaches the prefix's end
+    [0] * 12,
+])
+def test_prefix_of_a_batch_whose_first_places_are_short(dtype, D, nq, lengths):
+    """The prefix is read through a sequence that has it: entries of the block
+    table behind a sequence's last page are out of range, for every sequence."""
+    prefix, page, H = 320, 32, 2
+    kc, vc, dk, dv, c = R.pools(prefix // page + 24, H, page, D, 53)
+    table = R.tables(lengths, page, kc.shape[0], 53, prefix)
+    R.poison(kc, vc, table, lengths)
+    q = torch.randn(len(lengths), H * nq, D, generator=torch.Generator().manual_seed(53)).to(dtype)
+    # a captured graph's max_len, not the lengths, fixes the launch
+    table = torch.cat([table, torch.full((len(lengths), 20 - table.shape[1]), 1 << 30,
+                                         dtype=torch.int32)], 1)
+    out, lse = ops.paged_prefix_attention(
+        q.cuda(), R.cuda(kc), R.cuda(vc), table.cuda(),
+        torch.tensor(lengths, dtype=torch.int32).cuda(), prefix, dk, dv, c, return_lse=True)
+    want = R.attention(q, kc, vc, table, lengths, dk, dv, c)
+    R.check(out, lse, want, dtype)
+    assert (out.cpu()[torch.isinf(want[1])] == 0).all()
+
+
+def test_prefix_source_far_behind_in_a_large_batch():
+    """Hundreds of unused places before the one that has the prefix."""
+    prefix, page, D, nq = 64, 16, 128, 2
+    for dtype in (BF, FL):
+        for at in (127, 128, 129, 700):
+            lengths = [3] * at + [70] + [0] * (705 - at - 1)
+            kc, vc, dk, dv, c = R.pools(3000, 1, page, D, 59)
+            table = R.tables(lengths, page, 3000, 59, prefix)
+            q = torch.randn(705, nq, D, generator=torch.Generator().manual_seed(59)).to(dtype)
+            out = ops.paged_prefix_attention(
+                q.cuda(), R.cuda(kc), R.cuda(vc), table.cuda(),
+                torch.tensor(lengths, dtype=torch.int32).cuda(), prefix, dk, dv, c).cpu()
+            few = [0, at]
+            want = R.attention(q[few], kc, vc, table[few], [3, 70], dk, dv, c)
+            R.check(out[few], None, want, dtype)
+            assert (out[at + 1:] == 0).all()
