@@ -538,7 +538,9 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
           const bool fits = all_whole ? weigh_even(c, x) : weigh_any(c, x, on);
           if (again || __all_sync(0xffffffffu, fits)) break;
           // a weight would leave fp16: the reference moves up to this chunk's
-          // largest, what has been summed and stored so far follows
+          // largest, what has been summed and stored so far follows.  It moves by
+          // whole numbers, and weights take their factor in two parts that fp16
+          // holds, so that the weights and l stay of one scale.
           float top = kNoRef;
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
@@ -546,10 +548,11 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
             const float y = exponent(j, x[i], kap[j] * down) + lg2(fmaxf(rv[j], 0x1p-40f));
             if (on >> i & 1) top = fmaxf(top, y);
           }
-          const float to = fmaxf(ref, top), f = ex2(ref - to);
+          const float to = fmaxf(ref, ceilf(top)), f = ex2(ref - to);
+          const float fa = ex2(fmaxf(ref - to, -14.f)), fb = ex2(fminf(ref - to + 14.f, 0.f));
           ref = to;
           l *= f;
-          const uint32_t f2 = pack_h2(f, f);
+          const uint32_t fa2 = pack_h2(fa, fa), fb2 = pack_h2(fb, fb);
 #pragma unroll 1
           for (int k = 0; k < c; ++k) {
             const uint32_t at = scores + 16 * k;
@@ -557,7 +560,8 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
             tmem_wait_ld();
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-              asm volatile("mul.rn.f16x2 %0, %0, %1;" : "+r"(p[i]) : "r"(f2));
+              asm volatile("mul.rn.f16x2 %0, %0, %1;\n\tmul.rn.f16x2 %0, %0, %2;"
+                           : "+r"(p[i]) : "r"(fa2), "r"(fb2));
             tmem_st16(at, p);
           }
           if (t > 0) {

@@ -271,3 +271,35 @@ def test_prefix_source_far_behind_in_a_large_batch():
             want = R.attention(q[few], kc, vc, table[few], [3, 70], dk, dv, c)
             R.check(out[few], None, want, dtype)
             assert (out[at + 1:] == 0).all()
+
+
+@pytest.mark.parametrize("D,page", [(128, 64), (256, 32)])
+@pytest.mark.parametrize("gap", [12.97, 13.48, 14.18, 14.72])
+def test_prefix_weights_of_a_tile_before_a_large_one(D, page, gap):
+    """Tensor-core prefix: a heavy row late in a tile that is already full of
+    weights far below it (2^-22.7 to 2^-25.2 times the first rows'); what those
+    add keeps its size."""
+    B, nq, n, last = 16, 4, 128, 127
+    t = torch.full((n,), 2.0, dtype=torch.float64)
+    mid = slice(32, 96) if D == 128 else slice(64, 96)  # a tile is 128 rows, or 64
+    t[mid] += math.log(1000.0)
+    t[last] += math.log(1000.0) + gap - math.log(64.0)
+    base, k, v, dk, dv, c = _planted(D, page, t, 0.0, 61)
+    # the rows before have one value, so that what they add shows along it
+    w = k.shape[0] * page
+    before = torch.arange(w) != last
+    for x in (v.code, v.res, v.norms, v.rnorms):
+        x[before] = x[0].clone()
+    q = base.expand(B, nq, D).to(BF)
+    table = torch.arange(k.shape[0], dtype=torch.int32).expand(B, -1).contiguous()
+    out = ops.paged_prefix_attention(q.cuda(), R.cuda(k), R.cuda(v), table.cuda(),
+                                     torch.full((B,), n, dtype=torch.int32).cuda(), n, dk, dv, c)
+    want = R.attention(q[:1], k, v, table[:1], [n], dk, dv, c)[0]
+    side = (R.rows(v, c, False)[0] @ R.hadamard(D)) * dv.double()
+    side = side / side.norm()
+    off = ((out[:1].cpu().double() - want) @ side).abs().max() / want.norm()
+    # Along one direction the output's roundings and the heavy row's (half steps, 2^-9 and
+    # 2^-12, of elements that have 1 / sqrt(D) of the norm each) are 2^-9 at most and
+    # 2^-9 0.43 / sqrt(D) in the mean square: 7.6e-5; four deviations are 3e-4.  The rest
+    # is the mass of the rows before, under 0.01 for these gaps, to 2^-8 of itself.
+    assert off <= 3e-4 + 0.01 * 2.0 ** -8
