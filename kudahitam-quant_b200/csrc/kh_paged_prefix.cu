@@ -101,6 +101,12 @@ constexpr float kTileScale = 0x1p-11f;
 // fp16 ends at 65504; 32 weights with this sum are all below it.
 constexpr float kMostSum = 32768.f;
 
+// A moved reference puts the largest weight just under 2^kLift: fp16's fixed steps
+// (2^-24, below 2^-14) are then 2^-32 of it, so that a long tail of small weights
+// is not rounded to one side by much of itself (from 2^0, 131072 alike rows with 0.13
+// of the weight were 2.5% off), and 32 as large ones still fit kMostSum four times.
+constexpr float kLift = 8.f;
+
 template <int N>
 __device__ __forceinline__ void more_registers() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -548,7 +554,7 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
             const float y = exponent(j, x[i], kap[j] * down) + lg2(fmaxf(rv[j], 0x1p-40f));
             if (on >> i & 1) top = fmaxf(top, y);
           }
-          const float to = fmaxf(ref, ceilf(top)), f = ex2(ref - to);
+          const float to = fmaxf(ref, ceilf(top) - kLift), f = ex2(ref - to);
           const float fa = ex2(fmaxf(ref - to, -14.f)), fb = ex2(fminf(ref - to + 14.f, 0.f));
           ref = to;
           l *= f;

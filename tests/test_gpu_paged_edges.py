@@ -303,3 +303,24 @@ def test_prefix_weights_of_a_tile_before_a_large_one(D, page, gap):
     # 2^-9 0.43 / sqrt(D) in the mean square: 7.6e-5; four deviations are 3e-4.  The rest
     # is the mass of the rows before, under 0.01 for these gaps, to 2^-8 of itself.
     assert off <= 3e-4 + 0.01 * 2.0 ** -8
+
+
+@pytest.mark.parametrize("n,share,sigma", [(131072, 0.87, 0.0), (131072, 0.62, 0.5), (32768, 0.71, 1.0)])
+@pytest.mark.parametrize("D", [128, 256])
+def test_prefix_in_one_chunk_with_a_heavy_row(n, share, sigma, D):
+    """Tensor-core prefix, so many query rows that a CTA has all of it: small
+    weights beside a large one.  WITHIN's bf16 output rounding 1.9e-3, and scores from two
+    fp16 operands that agree in sign everywhere, 2^-12 of 17 (in natural units)
+    times 2 share (1 - share) <= 1/2: 2.1e-3 at most, 0.43 of that in the mean
+    square.  Root sum 2.1e-3."""
+    per = 256 if D == 128 else 128
+    nq = 64
+    B = 148 * per // nq
+    base, k, v, dk, dv, c = _sink(n, share, sigma, D, 0.5, n + D, page=256)
+    q = _queries(base, B, nq, BF)
+    table = torch.arange(k.shape[0], dtype=torch.int32).expand(B, -1).contiguous()
+    out = ops.paged_prefix_attention(q.cuda(), R.cuda(k), R.cuda(v), table.cuda(),
+                                     torch.full((B,), n, dtype=torch.int32).cuda(), n, dk, dv, c)
+    few = [0, B - 1]
+    want = R.attention(q[few][:, :4], k, v, table[few], [n] * 2, dk, dv, c)[0]
+    assert _off(out[few][:, :4], want) <= 2.1e-3
