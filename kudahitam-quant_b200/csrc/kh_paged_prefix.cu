@@ -116,6 +116,18 @@ __device__ __forceinline__ void fewer_registers() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
+// Barrier of the four decoding warps, true where `in` is for all of them.
+__device__ __forceinline__ bool decoders_agree(bool in) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\t"
+      "barrier.cta.red.and.pred p, 1, 128, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(all)
+      : "r"((uint32_t)in)
+      : "memory");
+  return all != 0;
+}
+
 template <int D, bool EXTRA>
 __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
     paged_prefix_kernel(const __grid_constant__ AttnParams P) {
@@ -283,6 +295,7 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
     // two tiles' rows on their way while one is decoded, their pages one ahead
     Row now = fetch(0, page_of(0)), next = fetch(1, page_of(1));
     int page = page_of(2);
+    bool in = true;  // no wait has given up
 #pragma unroll 1
     for (int t = 0; t < n_tiles; ++t) {
       const int s = t % NS;
@@ -313,7 +326,8 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
           *reinterpret_cast<float4*>(range + 4 * (warp - C::kSoftWarps)) =
               make_float4(odd ? INFINITY : most[0], least[0], most[1], least[1]);
       }
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+      // a warp whose wait gave up comes here too, so that the four leave together
+      if (!decoders_agree(in)) break;
       float4 all = *reinterpret_cast<const float4*>(range);
 #pragma unroll
       for (int w = 1; w < 4; ++w) {
@@ -342,7 +356,6 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
       vb *= vi * kTileScale;
       // Keys, then values, through the same code: written out twice (and for
       // two tiles) it did not stay in the instruction cache beside the softmax.
-      bool in = true;
 #pragma unroll 1
       for (int kv = 0; kv < 2; ++kv) {
         in = __all_sync(0xffffffffu, mbar_wait(kv ? &vempty[s] : &kempty[s], ph ^ 1u, P.err));
@@ -371,7 +384,6 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
           x.kr[w] = x.vr[w];
         }
       }
-      if (!in) break;
     }
   } else if (warp >= C::kSoftWarps + 4) {
     // ------------------------------------------------------------ products
