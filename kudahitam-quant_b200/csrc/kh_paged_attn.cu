@@ -684,7 +684,7 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
       for (int k = 0; k < 4; ++k) {
         const float x = tt[k >> 1][k & 1][nb], e = ex2(x - ref[nb]);
         ee[k >> 1][k & 1][nb] = e;
-        const float most = max_nan(max_nan(ra[k >> 1][k & 1], rb[k >> 1][k & 1]), kOne * 0x1p-40f);
+        const float most = max_nan(max_nan(ra[k >> 1][k & 1], rb[k >> 1][k & 1]), kOne * kLeastNorm);
         // nothing attended: 0 whatever the row's norms hold (but a weight that is
         // only too small to tell from 0 makes NaN of an infinite one)
         top[nb] = max_nan(top[nb], x == -INFINITY ? 0.f : e * most);
@@ -744,7 +744,7 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
       float mx = kNoRef;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const float most = max_nan(max_nan(ra[k >> 1][k & 1], rb[k >> 1][k & 1]), kOne * 0x1p-40f);
+        const float most = max_nan(max_nan(ra[k >> 1][k & 1], rb[k >> 1][k & 1]), kOne * kLeastNorm);
         const float x = tt[k >> 1][k & 1][nb];
         if (x > -INFINITY) mx = max_nan(mx, x + lg2(most * (1.f / kOne)));
       }

@@ -161,5 +161,9 @@ __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
   return r;
 }
 constexpr float kNoRef = -1e30f;  // reference exponent before the first row
+// Values count in full down to this norm (weights times norms have the references;
+// at 2^-40 values of 1e-20 came out as noise); the weights alone then stay
+// under 2^100, and sums of them in range.
+constexpr float kLeastNorm = 0x1p-90f;
 
 }  // namespace kh

@@ -522,7 +522,7 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
         }
         const float s0 = sum.x + sum.y;
         lt = s0 * tile.y;
-        return s0 <= kMostSum && lt < 0x1p60f;
+        return s0 <= kMostSum && lt < 0x1p110f;
       };
       // Any tile: scales and places by column.
       auto weigh_any = [&](int c, const float (&x)[32], uint32_t on) {
@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
           p[i >> 1] = pack_h2(w[0], w[1]);
         }
         lt = sum;
-        return total <= kMostSum && sum < 0x1p60f;
+        return total <= kMostSum && sum < 0x1p110f;
       };
       const bool all_whole = __all_sync(0xffffffffu, whole);
 #pragma unroll 1
@@ -563,7 +563,7 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             const int j = 32 * c + i;
-            const float y = exponent(j, x[i], kap[j] * down) + lg2(fmaxf(rv[j], 0x1p-40f));
+            const float y = exponent(j, x[i], kap[j] * down) + lg2(fmaxf(rv[j], kLeastNorm));
             if (on >> i & 1) top = fmaxf(top, y);
           }
           const float to = fmaxf(ref, ceilf(top) - kLift), f = ex2(ref - to);

@@ -324,3 +324,24 @@ def test_prefix_in_one_chunk_with_a_heavy_row(n, share, sigma, D):
     few = [0, B - 1]
     want = R.attention(q[few][:, :4], k, v, table[few], [n] * 2, dk, dv, c)[0]
     assert _off(out[few][:, :4], want) <= 2.1e-3
+
+
+@pytest.mark.parametrize("dtype,D,B,nq", [(FL, 128, 3, 2), (FL, 256, 2, 1), (BF, 128, 3, 4),
+                                          (BF, 128, 10, 4), (BF, 256, 6, 4)])
+@pytest.mark.parametrize("scale", [1e-14, 1e-20, 1e-25, 1e25, 1e30])
+def test_values_of_any_size(dtype, D, B, nq, scale):
+    """All values scaled: the result is, too.  Some rows have none at all."""
+    lengths, page = [300 + 9 * b for b in range(B)], 16
+    q, kc, vc, table, ln, dk, dv, c = _batch(lengths, page, 1, D, nq, dtype, 67)
+    table[:, :16] = table[0, :16]
+    vc.norms *= scale
+    vc.rnorms *= scale
+    a = (q.cuda(), R.cuda(kc), R.cuda(vc), table.cuda(), ln)
+    for zeros in (False, True):
+        if zeros:
+            vc.norms[::3] = 0
+            vc.rnorms[::3] = 0
+            a = (q.cuda(), R.cuda(kc), R.cuda(vc), table.cuda(), ln)
+        want = R.attention(q, kc, vc, table, lengths, dk, dv, c)
+        R.check(*ops.paged_decode_attention(*a, dk, dv, c, return_lse=True), want, dtype)
+        R.check(*ops.paged_prefix_attention(*a, 256, dk, dv, c, return_lse=True), want, dtype)
