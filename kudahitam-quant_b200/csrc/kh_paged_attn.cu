@@ -43,11 +43,11 @@ namespace {
 // sums are exact in 32 bits.  Bits count as 0 / 1: sum w sign = 2 sum w bit -
 // sum w, whose second sum is a product with ones, exact too (as a float sum of
 // 1800 weights it cost fp32 results 2.5e-6 of their norm, now 2.6e-7).
-//   PARTS = 2 (16-bit queries, 4 a block of 8 columns): q~ to 2^-13 of its
-//     largest element (2^-16 for bits that count once), weights in steps of 2^-15
-//     to 2^-17 of the largest around them.
-//   PARTS = 4 (32-bit queries, 2 a block): q~ to 2^-28, weights in steps of 2^-30
-//     to 2^-32.
+//   PARTS = 2 (16-bit queries, 4 a block of 8 columns): q~ in steps of 2^-15 of
+//     its largest element (2^-14 for bits that count twice), weights of 2^-15 to 2^-17
+//     of the largest around them.
+//   PARTS = 4 (32-bit queries, 2 a block): q~ of 2^-31 to 2^-28, weights of 2^-30 to
+//     2^-32.
 // A long tail of rows far below a step would count in the softmax's
 // denominator and not in its values (a first row with 0.6 of the weight before
 // 32767 alike ones: 20% off), so
@@ -140,6 +140,13 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 // tiles start, its rows, the units, through which sequence the prefix is read,
 // and each group's queries as operand fragments.
 constexpr int64_t kGap = 3;
+
+// Keys' bits are masked in places 0 .. kPlaces - 1 of each byte, by moving the word
+// down: more places save moves and cost the queries bits.  Of 16-bit queries four
+// places left fp16 results 2.4e-4 to 2.7e-4 off (of which 2.1e-4 is their own
+// rounding), two leave 2.2e-4 to 2.4e-4 for 1 to 4% more time.
+template <int PARTS>
+constexpr int kPlaces = PARTS == 2 ? 2 : 4;
 
 template <int D, int NB>
 struct Frags {  // of a group
@@ -336,8 +343,8 @@ __global__ void __launch_bounds__(128) paged_prepare_kernel(const __grid_constan
     const float up = mx > 0.f && mx < INFINITY ? fminf(kLargest / mx, 0x1p110f) : 1.f;
 #pragma unroll
     for (int j = 0; j < W; ++j) {
-      // element 32 j + lane: its bit's place in the masked byte counts 2^(bit & 3) times
-      const float times = (float)(1 << (lane & 3));
+      // element 32 j + lane: its bit counts 2^place times
+      const float times = (float)(1 << (lane & (kPlaces<PARTS> - 1)));
       const float v = rintf(x[j] * up / times) * times;
       sum += v;
       qs[y][32 * j + lane] = v;
@@ -362,7 +369,7 @@ __global__ void __launch_bounds__(128) paged_prepare_kernel(const __grid_constan
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int bit = 2 * (i & 3) + o;
-        int v = (int)qs[y][32 * word + 8 * j + bit] >> (bit & 3);
+        int v = (int)qs[y][32 * word + 8 * j + bit] >> (bit & (kPlaces<PARTS> - 1));
         for (int d = PARTS - 1 - g % PARTS; d > 0; --d) v = (v - (((v + 128) & 255) - 128)) >> 8;
         f[o] |= (uint32_t)(v & 255) << (8 * j);
       }
@@ -604,10 +611,11 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
                 st + p * C::kPlane)[(16 * hf + pg + 8 * rr) * W + (D == 128 ? t : 2 * t + v)];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if (i == 2)
+        constexpr int kMove = kPlaces<PARTS>;
+        if (i && 2 * i % kMove == 0)
 #pragma unroll
-          for (int k = 0; k < 8; ++k) w[k >> 2][(k >> 1) & 1][k & 1] >>= 4;
-        const uint32_t m0 = 0x01010101u << ((2 * i) & 3), m1 = m0 << 1;
+          for (int k = 0; k < 8; ++k) w[k >> 2][(k >> 1) & 1][k & 1] >>= kMove;
+        const uint32_t m0 = 0x01010101u << (2 * i % kMove), m1 = m0 << 1;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
           const uint2 f = qf[nb * KS + v * 4 + i];
