@@ -1,5 +1,5 @@
 // kh_paged.h -- host-side requests of the paged cache operators, shared by the
-// C-ABI checks (kh_paged_api.cu) and the kernels.
+// C-ABI checks (kh_api.cu) and the kernels.
 #pragma once
 
 #include "kh_internal.h"

@@ -232,14 +232,16 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const __grid_constant
 // rows in (token, head) order, so that a token's angles serve its heads from
 // L1.  Slots come by cp.async, 16 bytes a lane, into a private double buffer;
 // each is 16 bytes longer than it needs to be, so that the lanes' 16-byte reads
-// hit different banks.  What bounds it is issue: 82 instructions a row (the widest
-// parts: two shifts an element for its bits, a third of one for the borders).
+// hit different banks.  What bounds it is latency: a warp's 64-element chain at 16
+// warps an SM uses 58% of the issue slots (82 instructions a row; the widest parts:
+// two shifts an element for its bits, a third of one for the borders).
 constexpr int kTileWarps = 4;
 constexpr int kTileCtas = 4;
-// From how many keys (tokens x heads) they come in tiles: fewer do not give the
-// 592 CTAs' warps a tile each.  Measured (us, a warp per row / tiles, bf16, whole
-// keys rotated), D 128: 4096 keys 6.9 / 10.1, 8192 11.2 / 9.4, 32768 36.1 / 14.0;
-// D 256: 4096 9.9 / 13.5, 8192 16.3 / 14.2, 32768 53.5 / 30.1.
+// From how many keys (tokens x heads) they come in tiles: of fewer, most warps
+// have no tile and the others' chain of 64 elements a lane is the time.  Measured (us,
+// a warp per row / tiles, bf16, whole keys rotated), D 128: 4096 keys 6.9 / 10.1,
+// 8192 11.2 / 9.4, 32768 36.1 / 14.0; D 256: 4096 9.9 / 13.5, 8192 16.3 / 14.2, 32768
+// 53.5 / 30.1.  Straight lines between the first two cross at 6700 keys.
 constexpr int64_t kTileRows = 6656;
 
 template <typename T>

@@ -8,11 +8,14 @@
 //   out = d_v . H (sum_j p_j (norm'_j / sqrt(D) c[code'_j] + g rnorm'_j / D sign'_j)),
 //   p = softmax(t); no row attended: zeros, lse = -inf.
 //
-// The rows of a call are cut into chunks of equal length: first those of the
-// shared prefix, which one CTA reads for every sequence, then each sequence's
-// own.  A chunk leaves a record (reference exponent m in log2 units,
-// l = sum 2^(t' - m), acc = sum 2^(t' - m) v~ with t' = t log2 e) per query
-// row; paged_combine_kernel merges them and leaves the transformed domain.
+// paged_prepare_kernel cuts a call's rows into units of equal length, those of
+// the shared prefix (read once for every sequence's queries) before each
+// sequence's own; a warp of paged_rows_kernel takes a unit, which may hold pieces
+// of several sequences or KV heads.  A piece leaves a record (reference exponent
+// m in log2 units, l = sum 2^(t' - m), acc = sum 2^(t' - m) v~ with
+// t' = t log2 e) per query row; paged_combine_kernel merges them and leaves the
+// transformed domain.  A prefix with many bf16 queries goes to kh_paged_prefix.cu
+// instead, a record per query row and chunk.
 #include <algorithm>
 #include <cfloat>
 #include <cmath>

@@ -28,9 +28,10 @@
 // for a second set of scores.  128 x 32 bf16 queries over 32768 rows of 8 KV heads
 // take 96 us, 715 TFLOP/s.
 //
-// Rounding to 16 bits: q~, K^, the weights and V^ to fp16 (half a step 2^-12
-// each); sums, exponents and l in 32 bits.  That is under a result of
-// bf16's own half step (2^-9), so only bf16 queries take this path.
+// Rounding to 16 bits: q~, K^, the weights and V^ to fp16 (half a step 2^-11
+// each); sums, exponents and l in 32 bits.  That is under a bf16 result's own
+// half step (2^-8), so only bf16 queries take this path: results are 1.86e-3 to
+// 1.89e-3 off, of which their own rounding is 1.66e-3.
 #include <algorithm>
 #include <cmath>
 #include <mutex>

@@ -298,10 +298,10 @@ def test_prefix_weights_of_a_tile_before_a_large_one(D, page, gap):
     side = (R.rows(v, c, False)[0] @ R.hadamard(D)) * dv.double()
     side = side / side.norm()
     off = ((out[:1].cpu().double() - want) @ side).abs().max() / want.norm()
-    # Along one direction the output's roundings and the heavy row's (half steps, 2^-9 and
-    # 2^-12, of elements that have 1 / sqrt(D) of the norm each) are 2^-9 at most and
-    # 2^-9 0.43 / sqrt(D) in the mean square: 7.6e-5; four deviations are 3e-4.  The rest
-    # is the mass of the rows before, under 0.01 for these gaps, to 2^-8 of itself.
+    # Along one direction the output's roundings (half steps, 2^-8 of elements that have
+    # 1 / sqrt(D) of the norm each) are 2^-8 0.43 / sqrt(D) in the mean square, the heavy
+    # row's (fp16) an eighth of that; two deviations are 3e-4 at D = 128.  The rest is the
+    # mass of the rows before, under 0.01 for these gaps, to 2^-8 of itself.
     assert off <= 3e-4 + 0.01 * 2.0 ** -8
 
 
@@ -309,10 +309,10 @@ def test_prefix_weights_of_a_tile_before_a_large_one(D, page, gap):
 @pytest.mark.parametrize("D", [128, 256])
 def test_prefix_in_one_chunk_with_a_heavy_row(n, share, sigma, D):
     """Tensor-core prefix, so many query rows that a CTA has all of it: small
-    weights beside a large one.  WITHIN's bf16 output rounding 1.9e-3, and scores from two
-    fp16 operands that agree in sign everywhere, 2^-12 of 17 (in natural units)
-    times 2 share (1 - share) <= 1/2: 2.1e-3 at most, 0.43 of that in the mean
-    square.  Root sum 2.1e-3."""
+    weights beside a large one.  WITHIN's bf16 output rounding 1.9e-3; a score of 17 (in
+    natural units) whose keys' elements are one number with one rounding to fp16,
+    2^-11 0.43 in the mean square, times share (1 - share) |V_0 - V| / |out| <= 0.19:
+    6.8e-4; values and weights in fp16, 2^-11 0.43 each.  Root sum 2.1e-3."""
     per = 256 if D == 128 else 128
     nq = 64
     B = 148 * per // nq
