@@ -47,27 +47,29 @@ namespace {
 // sum w, whose second sum is a product with ones, exact too (as a float sum of
 // 1800 weights it cost fp32 results 2.5e-6 of their norm, now 2.6e-7).
 //   PARTS = 2 (16-bit queries, 4 a block of 8 columns): q~ in steps of 2^-15 of
-//     its largest element (2^-14 for bits that count twice), weights of 2^-15 to 2^-17
-//     of the largest around them.
-//   PARTS = 4 (32-bit queries, 2 a block): q~ of 2^-31 to 2^-28, weights of 2^-30 to
-//     2^-32.
+//     its largest element (2^-14 for bits that count twice), weights in steps of
+//     2^-16 to 2^-14 (bf16: 2^-12) of the largest of the 128 rows around them.
+//   PARTS = 4 (32-bit queries, 2 a block): q~ of 2^-31 to 2^-28, weights of 2^-31 to
+//     2^-22.
 // A long tail of rows far below a step would count in the softmax's
-// denominator and not in its values (a first row with 0.6 of the weight before
-// 32767 alike ones: 20% off), so
+// denominator and not in its values (a first row with half of the weight before
+// 32767 alike ones: 2% off), so
 //   - the step follows the weights: every kSpan tiles it comes down to them where
 //     they have become small, so that a heavy row costs the 256 rows around it
 //     their low bits and no more; and
 //   - a lane of 16-bit queries carries what each rounding left into its next
 //     row's weight, so that rounded weights sum to the true ones.
 // What remains is 0.41 of a step a row, of either sign: 2^-12 of one heavy row.
-// What bounds it is issue: a 32-row tile takes 128 logic operations at half
-// rate, 32 products of 7.5 cycles, and some 370 other instructions.  On a ragged
+// Both cost the ragged batch below 4 us.
+// What bounds it is the latency of dependent instructions: a 32-row tile takes
+// some 730, 340 of them on the ALU at half rate, and 32 products of 7.5 cycles, and
+// three warps a scheduler issue on 55% of the cycles.  On a ragged
 // batch (32 sequences up to 8192 rows, 8 KV heads x 4, D 128, bf16) the kernel
-// takes 41 us (half of the cycles issue); as fp16 products, two elements a logic
-// operation, 63 us.  Two column blocks, where a KV head has queries for them,
+// takes 44.7 us; as fp16 products, two elements a logic operation, it took 63 us
+// when these took 41.  Two column blocks, where a KV head has queries for them,
 // take the same masked bits: 16 sequences of 4096 rows, 8 KV heads x 5 bf16
-// queries 33.9 us (one block at a time 37.6), x 16 54.9 (65.9), x 3 fp32 queries
-// 36.3 (39.8); at D 256 two blocks' sums do not fit the registers.
+// queries 36.4 us (one block at a time 40.4), x 16 61.9 (72.4), x 3 fp32 queries
+// 36.3 (40.2); at D 256 two blocks' sums do not fit the registers.
 //
 // A warp runs on its own: 32-row tiles in a ring of cp.async stages, one lane
 // fetching one row (so pages may end anywhere).  The reference exponent of a
@@ -90,8 +92,9 @@ struct RowsCfg {
   static constexpr int kRing = kWarps * kStages * kStage;
   // a warp's folded sums: a lane's elements of each block of columns, and
   // {reference, l, sum of the code plane's weights, -}, {that since the last fold, -}
+  // and, by column, constants that would take 7 registers a block
   template <int PARTS, int NB>
-  static constexpr int kFold = NB * (W * 4 / (PARTS / 2) + 8) * 32 * 4;
+  static constexpr int kFold = NB * ((W * 4 / (PARTS / 2) + 8) * 32 * 4 + 4 * 32);
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
@@ -135,7 +138,7 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 // and kGap more places a group without anything in them, as starting a piece
 // takes a warp about as long as three tiles (without them a warp was left with
 // 37 short pieces: 64 x 32 fp16 queries over a prefix of 8192 rows and 32 own
-// rows each took 175 us, now 94).
+// rows each took 175 us, and 94 with them).
 // A unit may hold pieces of several groups; piece (unit u, group G) has record
 // u + G, as a unit's or a group's begin starts a new piece.
 //
@@ -403,13 +406,16 @@ __device__ __forceinline__ int64_t find_sequence(const AttnParams& P, int64_t x,
   return lo;
 }
 
-// CTAs an SM that the registers are bounded for (168 of them).  Four or five at
-// D 128 measured 46 and 51 us on the ragged batch instead of 43.5, two at D 256
-// 54.6 instead of 49.2 for 13 x 28 fp16 queries over a prefix of 5001 rows.
-constexpr int kRowsCtas = 3;
+// CTAs an SM that the registers are bounded for: three (168 registers), or two where
+// a warp's sums would spill then: 16 sequences of 4096 rows, 8 KV heads x 16 bf16
+// queries 62.0 us (three: 63.3), 13 x 28 fp16 queries of D 256 over a prefix of 5001 rows
+// 44.8 (46.3).  Two elsewhere: ragged batch 48.9 (46.7), long fp32 contexts 131 (112).
+constexpr int kMostCtas = 3;
+template <int D, int NB>
+constexpr int kRowsCtas = D == 128 && NB == 1 ? kMostCtas : 2;
 
 template <int D, int PARTS, bool EXTRA, int NB>
-__global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
+__global__ void __launch_bounds__(32 * kWarps, kRowsCtas<D, NB>)
     paged_rows_kernel(const __grid_constant__ AttnParams P) {
   using C = RowsCfg<D>;
   using F = Frags<D, NB>;
@@ -431,6 +437,8 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
   float4* fold4 = reinterpret_cast<float4*>(smem + C::kRing +
                                             warp * C::template kFold<PARTS, NB>) + lane;
   float4* stat4 = fold4 + NB * (kOwn / 4) * 32;
+  // {a1, b1, a2, b2}, {slope, first and last row} of the query in block nb's column t
+  float4* col4 = stat4 - lane + NB * 64 + 2 * t;
   // Also behind a tensor-core prefix, which starts only when the preparing launch
   // is done: that orders the launches, but only a grid's own wait makes what came
   // before visible to it.  (Own rows beside the prefix's last CTAs without the wait: 64 x 32
@@ -537,41 +545,45 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
   //   t2 = norm (a1 M1 + b1) + rnorm (a2 M2 + b2), M the masked sums
   const float ch = 0.5f * (r.c1 - r.c0), cm = 0.5f * (r.c1 + r.c0);
   const float inv_sd = P.inv_sd;
-  float a1[NB], b1[NB], a2[NB], b2[NB], slope[NB];
-  int q_lo[NB], q_hi[NB];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     const int y = nb * QB + mine;
     const float k = frags->scale[y], sum = frags->sum[y] * k;
-    a1[nb] = 2.f * ch * k;
-    b1[nb] = (cm - ch) * sum;
-    a2[nb] = 2.f * inv_sd * k;
-    b2[nb] = -inv_sd * sum;
-    slope[nb] = 0.f;
-    q_lo[nb] = 0;
-    q_hi[nb] = 0x7fffffff;
+    float slope = 0.f;
+    int q_lo = 0, q_hi = 0x7fffffff;
     if (y < nq) {
       if (pre || (EXTRA && r.slopes)) {
         const int64_t len = length_of(P, seq_of(y));
-        q_hi[nb] = (int)len;
-        if (pre) q_lo[nb] = (int)min(first_of(P, seq_of(y), len), (int64_t)0x7fffffff);
+        q_hi = (int)len;
+        if (pre) q_lo = (int)min(first_of(P, seq_of(y), len), (int64_t)0x7fffffff);
       }
-      if (EXTRA && r.slopes) slope[nb] = r.slopes[head_of(y)] * kLog2e;
+      if (EXTRA && r.slopes) slope = r.slopes[head_of(y)] * kLog2e;
+    }
+    if (g == 0) {
+      col4[nb * 8] = make_float4(2.f * ch * k, (cm - ch) * sum, 2.f * inv_sd * k, -inv_sd * sum);
+      col4[nb * 8 + 1] = make_float4(slope, __int_as_float(q_lo), __int_as_float(q_hi), 0.f);
     }
   }
   // weight 1 as a whole number, and the most one may be
   constexpr float kOne = PARTS == 2 ? 32768.f : 1073741824.f;
   constexpr float kMost = PARTS == 2 ? 65534.f : 4294967040.f;  // and a remainder
+  // A span's largest weight that lets the step come down: what that costs is sums
+  // being folded, what it saves is noise of 0.41 of a step a row.  fp16 results have
+  // no room for it, bf16's own rounding is eight times as large; 32-bit queries'
+  // weights are that far from their steps.
+  const float fall = kOne * (PARTS == 4 ? 0x1p-8f : r.dtype == KH_BF16 ? 0.125f : 0.5f);
   const float va = ch * inv_sd * kOne;
   const float vb = 0.7978845608028654f * inv_sd * inv_sd * kOne;
   const float cap = r.softcap * kLog2e, inv_cap = r.softcap > 0.f ? 1.f / cap : 0.f;
 
   // the last tile's rows are all ones: sums of the weights themselves
   float ref[NB];
-  float2 l[NB];     // and what its last addition lost
+  float2 l[NB];     // and what its last addition lost (of 32-bit queries)
   float top[NB];    // largest weight since the reference moved, or of the last kSpan tiles
   float2 over[NB];  // what the last roundings left, of either plane
   int acc[NB][MT + 1][4];
+  uint32_t folded = 0;  // blocks with sums in shared memory
+  const bool uneven = cm != 0.f;  // the levels' middle adds a part of the weights' sum
   // lanes start with remainders spread over a step: what they end with does too
   const float2 over0 = make_float2((2 * g - 7) * 0.0625f, (7 - 2 * g) * 0.0625f);
 #pragma unroll
@@ -580,18 +592,13 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
     l[nb] = make_float2(0.f, 0.f);
     top[nb] = 0.f;
     over[nb] = over0;
-    stat4[nb * 64] = make_float4(kNoRef, 0.f, 0.f, 0.f);
-    stat4[nb * 64 + 32] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int x = 0; x < kOwn / 4; ++x)
-      fold4[(nb * (kOwn / 4) + x) * 32] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (uneven) stat4[nb * 64 + 32] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int i = 0; i <= MT; ++i)
 #pragma unroll
       for (int k = 0; k < 4; ++k) acc[nb][i][k] = 0;
   }
   const int pg = (g >> 1) + 4 * (g & 1);  // pi(g)
-  const bool uneven = cm != 0.f;          // the levels' middle adds a part of the weights' sum
 
   // A tile's scores and a tile's values are independent: in the loop the next
   // tile's scores and exponents run between this tile's value products.
@@ -643,7 +650,10 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
     full = valid == 0xffffffffu;
     if (pre) {
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) full = full && j0 >= q_lo[nb] && j0 + 32 <= q_hi[nb];
+      for (int nb = 0; nb < NB; ++nb) {
+        const float4 col = col4[nb * 8 + 1];
+        full = full && j0 >= __float_as_int(col.y) && j0 + 32 <= __float_as_int(col.z);
+      }
       full = __all_sync(0xffffffffu, full);
     }
     // a query's masked sum from its columns' (2 PARTS bytes of them)
@@ -653,6 +663,9 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
       const float y = __shfl_xor_sync(0xffffffffu, x, 1);
       return low ? fmaf(y, 65536.f, x) : fmaf(x, 65536.f, y);
     };
+    float4 ab[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) ab[nb] = col4[nb * 8];
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
@@ -666,11 +679,14 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
         rb[hf][rr] = n.w * vb;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-          float x = fmaf(n.x, fmaf(a1[nb], joined(s1[hf][nb], rr), b1[nb]), nil);
-          x = fmaf(n.y, fmaf(a2[nb], joined(s2[hf][nb], rr), b2[nb]), x);
+          float x = fmaf(n.x, fmaf(ab[nb].x, joined(s1[hf][nb], rr), ab[nb].y), nil);
+          x = fmaf(n.y, fmaf(ab[nb].z, joined(s2[hf][nb], rr), ab[nb].w), x);
           if (EXTRA && r.softcap > 0.f)
             x = PARTS == 2 ? soft_cap_16(x, cap, inv_cap) : soft_cap(x, cap, inv_cap);
-          if (EXTRA && r.slopes) x = fmaf(slope[nb], (float)(j0 + row + 1 - q_hi[nb]), x);
+          if (EXTRA && r.slopes) {
+            const float4 col = col4[nb * 8 + 1];
+            x = fmaf(col.x, (float)(j0 + row + 1 - __float_as_int(col.z)), x);
+          }
           tt[hf][rr][nb] = x;
         }
       }
@@ -680,96 +696,111 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
           const int row = 16 * (k >> 1) + pg + 8 * (k & 1), j = j0 + row;
-          const bool on = ((valid >> row) & 1) && j >= q_lo[nb] && j < q_hi[nb];
+          const float4 col = col4[nb * 8 + 1];
+          const bool on = ((valid >> row) & 1) && j >= __float_as_int(col.y) &&
+                          j < __float_as_int(col.z);
           if (!on) tt[k >> 1][k & 1][nb] = -INFINITY;
         }
     }
   };
   // weights e = 2^(t2 - ref); true where they fit: a row's larger one decides
   // (and a NaN among the attended, which whole numbers would lose)
-  auto weigh = [&] {
-    bool fit = true;
+  auto weigh = [&](int nb) {
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float x = tt[k >> 1][k & 1][nb], e = ex2(x - ref[nb]);
-        ee[k >> 1][k & 1][nb] = e;
-        const float most = max_nan(max_nan(ra[k >> 1][k & 1], rb[k >> 1][k & 1]), kOne * kLeastNorm);
-        // nothing attended: 0 whatever the row's norms hold (but a weight that is
-        // only too small to tell from 0 makes NaN of an infinite one)
-        top[nb] = max_nan(top[nb], x == -INFINITY ? 0.f : e * most);
-      }
-      fit = fit && top[nb] <= kMost;
+    for (int k = 0; k < 4; ++k) {
+      const float x = tt[k >> 1][k & 1][nb], e = ex2(x - ref[nb]);
+      ee[k >> 1][k & 1][nb] = e;
+      const float most = max_nan(max_nan(ra[k >> 1][k & 1], rb[k >> 1][k & 1]), kOne * kLeastNorm);
+      // nothing attended: 0 whatever the row's norms hold (but a weight that is
+      // only too small to tell from 0 makes NaN of an infinite one)
+      top[nb] = max_nan(top[nb], x == -INFINITY ? 0.f : e * most);
     }
-    return fit;
+    return top[nb] <= kMost;
   };
-  // What has been summed joins the sums in shared memory.  2 sum w bit - sum w,
-  // bit i counting 2^(i & 7) times: the difference is taken in whole numbers, it
-  // is small beside its parts.
-  auto fold = [&] {
+  // Four elements of a lane's sums, in the order i, k (a lane of 32-bit queries has
+  // its k), times `is`.  2 sum w bit - sum w, bit i counting 2^(i & 7) times: the
+  // difference is taken in whole numbers, it is small beside its parts.
+  auto sums = [&](int nb, int x, float is, float (&v)[4]) {
+    const int c0 = acc[nb][MT][0], c1 = acc[nb][MT][1];
+    auto element = [&](int i, int k) {
+      const int h = acc[nb][i][2 * k], o = acc[nb][i][2 * k + 1];
+      const float fh = (float)(2 * h - (c0 << (i & 7))), fo = (float)(2 * o - (c1 << (i & 7)));
+      float x = PARTS == 2 || low ? fmaf(fh, 256.f, fo) : fmaf(fh, 16777216.f, fo * 65536.f);
+      if (PARTS == 4) x += __shfl_xor_sync(0xffffffffu, x, 1);
+      return x * (is * (1.f / (float)(1 << (i & 7))));
+    };
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      const float4 old = stat4[nb * 64];
-      const float to = fmaxf(old.x, ref[nb]), was = ex2(old.x - to), is = ex2(ref[nb] - to);
-      stat4[nb * 64] = make_float4(to, fmaf(old.y, was, (l[nb].x + l[nb].y) * is),
-                                   fmaf(old.z, was, stat4[nb * 64 + 32].x * is), 0.f);
-      stat4[nb * 64 + 32] = make_float4(0.f, 0.f, 0.f, 0.f);
-      l[nb] = make_float2(0.f, 0.f);
-      const int c0 = acc[nb][MT][0], c1 = acc[nb][MT][1];
-      auto element = [&](int i, int k) {
-        const int h = acc[nb][i][2 * k], o = acc[nb][i][2 * k + 1];
-        const float fh = (float)(2 * h - (c0 << (i & 7))), fo = (float)(2 * o - (c1 << (i & 7)));
-        float x = PARTS == 2 || low ? fmaf(fh, 256.f, fo) : fmaf(fh, 16777216.f, fo * 65536.f);
-        if (PARTS == 4) x += __shfl_xor_sync(0xffffffffu, x, 1);
-        return x * (is * (1.f / (float)(1 << (i & 7))));
-      };
-#pragma unroll
-      for (int x = 0; x < kOwn; x += 4) {
-        // elements of a lane in the order i, k; a lane of 32-bit queries has its k
-        float v[4];
-#pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          if constexpr (PARTS == 2) {
-            v[y] = element((x + y) >> 1, y & 1);
-          } else {
-            const float v0 = element(x + y, 0), v1 = element(x + y, 1);
-            v[y] = t & 1 ? v1 : v0;
-          }
-        }
-        float4* to = fold4 + (nb * (kOwn / 4) + x / 4) * 32;
-        const float4 sum = *to;
-        *to = make_float4(fmaf(sum.x, was, v[0]), fmaf(sum.y, was, v[1]), fmaf(sum.z, was, v[2]),
-                          fmaf(sum.w, was, v[3]));
+    for (int y = 0; y < 4; ++y) {
+      if constexpr (PARTS == 2) {
+        v[y] = element((x + y) >> 1, y & 1);
+      } else {
+        const float v0 = element(x + y, 0), v1 = element(x + y, 1);
+        v[y] = t & 1 ? v1 : v0;
       }
-#pragma unroll
-      for (int i = 0; i <= MT; ++i)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) acc[nb][i][k] = 0;
     }
+  };
+  // A block's reference, l and sum of the code plane's weights, with what is in
+  // shared memory; `was` and `is` scale that and the sums in registers.
+  auto totals = [&](int nb, float& was, float& is) {
+    float4 now = make_float4(ref[nb], l[nb].x + l[nb].y, uneven ? stat4[nb * 64 + 32].x : 0.f, 0.f);
+    was = 0.f;
+    is = 1.f;
+    if ((folded >> nb) & 1) {
+      const float4 old = stat4[nb * 64];
+      now.x = fmaxf(old.x, ref[nb]);
+      was = ex2(old.x - now.x);
+      is = ex2(ref[nb] - now.x);
+      now.y = fmaf(old.y, was, now.y * is);
+      now.z = fmaf(old.z, was, now.z * is);
+    }
+    return now;
+  };
+  // What has been summed joins the sums in shared memory.
+  auto fold = [&](int nb) {
+    float was, is;
+    stat4[nb * 64] = totals(nb, was, is);
+    if (uneven) stat4[nb * 64 + 32] = make_float4(0.f, 0.f, 0.f, 0.f);
+    l[nb] = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int x = 0; x < kOwn; x += 4) {
+      float v[4];
+      sums(nb, x, is, v);
+      float4* to = fold4 + (nb * (kOwn / 4) + x / 4) * 32;
+      if ((folded >> nb) & 1) {
+        const float4 sum = *to;
+        v[0] = fmaf(sum.x, was, v[0]);
+        v[1] = fmaf(sum.y, was, v[1]);
+        v[2] = fmaf(sum.z, was, v[2]);
+        v[3] = fmaf(sum.w, was, v[3]);
+      }
+      *to = make_float4(v[0], v[1], v[2], v[3]);
+    }
+    folded |= 1u << nb;
+#pragma unroll
+    for (int i = 0; i <= MT; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[nb][i][k] = 0;
   };
   // the reference moves down by as much, or up to the tile's largest
-  auto refer = [&](const float(&down)[NB]) {
+  auto refer = [&](int nb, float down) {
+    float mx = kNoRef;
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      float mx = kNoRef;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float most = max_nan(max_nan(ra[k >> 1][k & 1], rb[k >> 1][k & 1]), kOne * kLeastNorm);
-        const float x = tt[k >> 1][k & 1][nb];
-        if (x > -INFINITY) mx = max_nan(mx, x + lg2(most * (1.f / kOne)));
-      }
-#pragma unroll
-      for (int o = 4; o < 32; o <<= 1) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      if (!(mx < INFINITY)) l[nb].x = NAN;  // a norm that is not finite has no average
-      ref[nb] = fmaxf(ref[nb] - down[nb], mx);
-      if (PARTS == 4) ref[nb] = ceilf(ref[nb]);  // then factors between references are exact
-      over[nb] = over0;
-      top[nb] = 0.f;
+    for (int k = 0; k < 4; ++k) {
+      const float most = max_nan(max_nan(ra[k >> 1][k & 1], rb[k >> 1][k & 1]), kOne * kLeastNorm);
+      const float x = tt[k >> 1][k & 1][nb];
+      if (x > -INFINITY) mx = max_nan(mx, x + lg2(most * (1.f / kOne)));
     }
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    if (!(mx < INFINITY)) l[nb].x = NAN;  // a norm that is not finite has no average
+    ref[nb] = fmaxf(ref[nb] - down, mx);
+    if (PARTS == 4) ref[nb] = ceilf(ref[nb]);  // then factors between references are exact
+    over[nb] = over0;
+    top[nb] = 0.f;
   };
   // sum + x, its rounding in the next one: thousands of alike small weights
-  // behind a large one lose the same part of each, 1e-5 of fp32 results
+  // behind a large one lose the same part of each, 1e-5 of fp32 results (of a piece
+  // of 16384 rows 2^-15 at most, which 16-bit results are left with)
   auto add = [](float2& sum, float x) {
     const float y = x + sum.y, to = sum.x + y;
     sum = make_float2(to, y - (to - sum.x));
@@ -777,7 +808,9 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
   auto pack = [&] {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      add(l[nb], (ee[0][0][nb] + ee[0][1][nb]) + (ee[1][0][nb] + ee[1][1][nb]));
+      const float sum = (ee[0][0][nb] + ee[0][1][nb]) + (ee[1][0][nb] + ee[1][1][nb]);
+      if (PARTS == 4) add(l[nb], sum);
+      else l[nb].x += sum;
       float w1s = 0.f;
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
@@ -852,7 +885,7 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
   // weights of tile i, with the reference where it should be
   auto settle = [&](int i) {
     float down[NB] = {};
-    bool falls = false;
+    uint32_t move = 0;  // blocks of which one does
     if (i != 0 && (i & (kSpan - 1)) == 0) {
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
@@ -860,17 +893,25 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
         for (int o = 4; o < 32; o <<= 1)
           top[nb] = max_nan(top[nb], __shfl_xor_sync(0xffffffffu, top[nb], o));
         // weights like the last ones leave a bit, and one more that kMost has
-        if (top[nb] <= 0.5f * kOne && top[nb] > 0.f) {
+        if (top[nb] <= fall && top[nb] > 0.f) {
           down[nb] = -1.f - lg2(top[nb] * (1.f / kOne));
-          falls = true;
+          move |= 1u << nb;
         }
         top[nb] = 0.f;
       }
     }
-    if (!__all_sync(0xffffffffu, weigh() && !falls)) {
-      if (i != 0) fold();
-      refer(down);
-      weigh();
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+      if (!weigh(nb)) move |= 1u << nb;
+    move = __reduce_or_sync(0xffffffffu, move);
+    if (move) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+        if ((move >> nb) & 1) {
+          if (i != 0) fold(nb);
+          refer(nb, down[nb]);
+          weigh(nb);
+        }
     }
     pack();
   };
@@ -904,10 +945,10 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
 
   // ---- the record: 16 consecutive elements a lane (32 at D = 256), tile i's
   // parts elements i and 8 + i of each 16
-  fold();
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    float4 now = stat4[nb * 64];
+    float fold_was, fold_is;
+    float4 now = totals(nb, fold_was, fold_is);
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) {
       now.y += __shfl_xor_sync(0xffffffffu, now.y, o);
@@ -936,14 +977,22 @@ __global__ void __launch_bounds__(32 * kWarps, kRowsCtas)
     };
 #pragma unroll
     for (int x = 0; x < kOwn; x += 4) {
-      const float4 v = fold4[(nb * (kOwn / 4) + x / 4) * 32];
+      float v[4];
+      sums(nb, x, fold_is, v);
+      if ((folded >> nb) & 1) {
+        const float4 sum = fold4[(nb * (kOwn / 4) + x / 4) * 32];
+        v[0] = fmaf(sum.x, fold_was, v[0]);
+        v[1] = fmaf(sum.y, fold_was, v[1]);
+        v[2] = fmaf(sum.z, fold_was, v[2]);
+        v[3] = fmaf(sum.w, fold_was, v[3]);
+      }
       if (y >= nq) continue;
       if constexpr (PARTS == 2) {
-        put(x >> 1, 0, v.x, v.z);
-        put(x >> 1, 1, v.y, v.w);
+        put(x >> 1, 0, v[0], v[2]);
+        put(x >> 1, 1, v[1], v[3]);
       } else {
-        put(x, t & 1, v.x, v.y);
-        put(x + 2, t & 1, v.z, v.w);
+        put(x, t & 1, v[0], v[1]);
+        put(x + 2, t & 1, v[2], v[3]);
       }
     }
   }
@@ -1083,7 +1132,7 @@ kh_status launch_rows(AttnParams P, cudaStream_t stream) {
   const PagedAttnRequest& r = P.r;
   constexpr int NQ = NB * 8 / PARTS;
   constexpr int kSmem = RowsCfg<D>::kRing + kWarps * RowsCfg<D>::template kFold<PARTS, NB>;
-  static_assert(kRowsCtas * (kSmem + 1024) <= 233472, "shared memory of an SM");
+  static_assert(kRowsCtas<D, NB> * (kSmem + 1024) <= 233472, "shared memory of an SM");
   auto kern = paged_rows_kernel<D, PARTS, EXTRA, NB>;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return KH_ECUDA;
@@ -1103,7 +1152,7 @@ kh_status launch_rows(AttnParams P, cudaStream_t stream) {
   if (P.plan.block != NQ || groups + operand > 0x7ffffff0ll || P.plan.tiles >= int64_t(1) << 36)
     return KH_EINVAL;
   const int64_t grid = std::min<int64_t>(
-      (int64_t)std::min(std::max(1, ctas[dev & 63]), kRowsCtas) * sm_count(),
+      (int64_t)std::min(std::max(1, ctas[dev & 63]), kRowsCtas<D, NB>) * sm_count(),
       (P.plan.tiles / 2 + kWarps) / kWarps);
   P.n_warps = grid * kWarps;
   static_assert(sizeof(Frags<D, NB>) <= kFragBytes, "workspace of the fragments");
@@ -1156,12 +1205,12 @@ kh_status launch_dim(const AttnParams& P, cudaStream_t stream) {
 // products have 128 query rows whatever there are, the rows kernel's time grows
 // with them.  Measured (us, rows kernel / tensor cores, 8 KV heads, bf16):
 //                 16 rows      32           48           64           128
-//   D 128, 1024   15.5 / 18.3  16.8 / 18.4  18.6 / 18.6  19.6 / 18.6  24.8 / 19.0
-//   D 128, 8192   24.3 / 30.9  33.0 / 30.2  40.7 / 31.1  51.6 / 30.7  88.0 / 31.8
-//   D 256, 1024   18.3 / 20.5  21.7 / 20.5  23.4 / 22.3  26.2 / 24.7  34.5 / 29.3
-//   D 256, 8192   33.1 / 33.9  51.0 / 32.7  66.9 / 34.8  87.6 / 34.0   132 / 35.1
-// (Of one KV head and 1024 rows the rows kernel stays ahead up to 64 query
-// rows, by 1 us at D 128 and 4 us at D 256.)
+//   D 128, 1024   14.7 / 17.4  15.8 / 17.6  16.8 / 18.7  17.8 / 18.6  20.9 / 18.4
+//   D 128, 8192   21.8 / 31.8  26.7 / 30.7  32.4 / 31.7  37.7 / 30.8  59.4 / 30.5
+//   D 256, 1024   16.5 / 19.9  17.3 / 20.0  19.1 / 20.7  21.3 / 20.5  28.1 / 20.5
+//   D 256, 8192   26.3 / 34.4  37.5 / 33.7  49.6 / 33.7  61.8 / 33.8   109 / 33.0
+// (Of one KV head and 1024 rows the rows kernel stays ahead up to 128 query
+// rows, by 2 us at D 128 and 2 to 5 us at D 256.)
 int64_t prefix_tensor_rows(int D) { return D == 128 ? 32 : 16; }
 
 // The workspace, each part 16-byte aligned: a tensor-core prefix's records, by
@@ -1218,7 +1267,7 @@ PagedPlan paged_plan(int64_t n_seqs, int n_q, int n_kv_heads, int D, int64_t max
   p.groups = n_kv_heads * (p.pre_blocks + n_seqs * p.own_blocks);
   p.tiles = n_kv_heads * (p.pre_blocks * ((p.pre_rows + 31) / 32 + kGap) +
                           n_seqs * p.own_blocks * ((p.own_rows + 31) / 32 + kGap));
-  p.max_units = std::min<int64_t>((int64_t)kRowsCtas * kWarps * n_sms, p.tiles / 2 + 1);
+  p.max_units = std::min<int64_t>((int64_t)kMostCtas * kWarps * n_sms, p.tiles / 2 + 1);
   return p;
 }
 
