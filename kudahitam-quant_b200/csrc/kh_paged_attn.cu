@@ -60,7 +60,7 @@ namespace {
 //   - a lane of 16-bit queries carries what each rounding left into its next
 //     row's weight, so that rounded weights sum to the true ones.
 // What remains is 0.41 of a step a row, of either sign: 2^-12 of one heavy row.
-// Both cost the ragged batch below 4 us.
+// Both cost the ragged batch below 3 us.
 // What bounds it is the latency of dependent instructions: a 32-row tile takes
 // some 730, 340 of them on the ALU at half rate, and 32 products of 7.5 cycles, and
 // three warps a scheduler issue on 55% of the cycles.  On a ragged
@@ -1207,8 +1207,8 @@ kh_status launch_dim(const AttnParams& P, cudaStream_t stream) {
 //                 16 rows      32           48           64           128
 //   D 128, 1024   14.7 / 17.4  15.8 / 17.6  16.8 / 18.7  17.8 / 18.6  20.9 / 18.4
 //   D 128, 8192   21.8 / 31.8  26.7 / 30.7  32.4 / 31.7  37.7 / 30.8  59.4 / 30.5
-//   D 256, 1024   16.5 / 19.9  17.3 / 20.0  19.1 / 20.7  21.3 / 20.5  28.1 / 20.5
-//   D 256, 8192   26.3 / 34.4  37.5 / 33.7  49.6 / 33.7  61.8 / 33.8   109 / 33.0
+//   D 256, 1024   16.5 / 19.9  17.3 / 20.1  19.1 / 21.0  21.3 / 20.5  28.1 / 20.6
+//   D 256, 8192   26.3 / 34.4  37.5 / 34.2  49.6 / 35.5  61.8 / 34.5   109 / 33.1
 // (Of one KV head and 1024 rows the rows kernel stays ahead up to 128 query
 // rows, by 2 us at D 128 and 2 to 5 us at D 256.)
 int64_t prefix_tensor_rows(int D) { return D == 128 ? 32 : 16; }

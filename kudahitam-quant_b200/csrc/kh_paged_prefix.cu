@@ -604,6 +604,13 @@ __global__ void __launch_bounds__(PreCfg<D>::kThreads, 1)
       }
       if (!ok) break;
       tmem_wait_st();
+      // With two score buffers the softmax may be a tile ahead of the products,
+      // and the wait for the last of them below would return at once while the
+      // one before it runs: that one is waited for here, while it can only be the
+      // latest or the one before.
+      if (C::SB == 2 && t > 0 && t == n_tiles - 1)
+        ok = __all_sync(0xffffffffu, mbar_wait(&odone[m], (uint32_t)((t - 1) & 1), P.err));
+      if (!ok) break;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&pfull[i]);

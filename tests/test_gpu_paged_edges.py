@@ -362,3 +362,24 @@ def test_scores_of_16_bit_queries(dtype, D, nq):
     _, want, _, _, peak, _ = R.attention(q, kc, vc, table, [1] * B, dk, dv, c)
     off = ((lse.cpu().double() - want) / peak).square().mean().sqrt()
     assert off <= 1.15 * 0.456 * 2.0 ** -15 / math.sqrt(D)
+
+
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("B,nq,n", [(7, 8, 13017), (64, 9, 2472), (64, 9, 11945), (64, 9, 2652),
+                                    (16, 3, 300), (40, 4, 64)])
+def test_prefix_chunks_of_a_few_tiles(D, B, nq, n):
+    """Tensor-core prefix that is all there is: its sums leave after the last
+    product, in every run."""
+    page = 64
+    kc, vc, dk, dv, c = R.pools(-(-n // page), 1, page, D, 73)
+    q = torch.randn(B, nq, D, generator=torch.Generator().manual_seed(73)).to(BF)
+    table = torch.randperm(kc.shape[0], generator=torch.Generator().manual_seed(n)).int()
+    table = table.expand(B, -1).contiguous()
+    a = (q.cuda(), R.cuda(kc), R.cuda(vc), table.cuda(),
+         torch.full((B,), n, dtype=torch.int32).cuda(), n, dk, dv, c)
+    out, lse = ops.paged_prefix_attention(*a, return_lse=True)
+    few = [0, B - 1]
+    want = R.attention(q[few], kc, vc, table[few], [n] * 2, dk, dv, c)
+    R.check(out[few], lse[few], want, BF)
+    for _ in range(20):
+        assert torch.equal(ops.paged_prefix_attention(*a), out)
