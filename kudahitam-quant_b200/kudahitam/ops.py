@@ -677,7 +677,9 @@ def paged_prefix_attention(q: torch.Tensor, k_cache: PackedKV, v_cache: PackedKV
     through the block table's row of the first sequence that has them all (or
     else of the longest); rows from prefix_len on are each sequence's own.
     ``lengths`` count the prefix; shorter sequences and empty places (length 0)
-    may stand anywhere in the batch."""
+    may stand anywhere in the batch.  With many bf16 query rows a KV head the
+    prefix's scores come from fp16 operands (off by up to 2^-11 |q| |K|
+    sm_scale); ``paged_decode_attention`` keeps them finer."""
     return _paged_attention(q, k_cache, v_cache, block_table, lengths, int(prefix_len), dk, dv,
                             centroids, sm_scale, max_len, starts, window, softcap, slopes,
                             return_lse)
