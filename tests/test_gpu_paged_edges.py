@@ -383,3 +383,34 @@ def test_prefix_chunks_of_a_few_tiles(D, B, nq, n):
     R.check(out[few], lse[few], want, BF)
     for _ in range(20):
         assert torch.equal(ops.paged_prefix_attention(*a), out)
+
+
+@pytest.mark.parametrize("dtype,D,B,nq", [(BF, 128, 12, 4), (BF, 256, 9, 4), (FL, 128, 3, 2)])
+def test_prefix_in_a_graph_while_places_come_and_go(dtype, D, B, nq):
+    """A captured call replayed with other lengths, the first place empty in
+    some, beside eager calls on another stream."""
+    prefix, page = 320, 32
+    full = [prefix + 40 + b for b in range(B)]
+    kc, vc, dk, dv, c = R.pools(prefix // page + 3 * B, 1, page, D, 79)
+    table = R.tables(full, page, kc.shape[0], 79, prefix)
+    q = torch.randn(B, nq, D, generator=torch.Generator().manual_seed(79)).to(dtype)
+    kg, vg, tg, qg = R.cuda(kc), R.cuda(vc), table.cuda(), q.cuda()
+    ln = torch.tensor(full, dtype=torch.int32).cuda()
+    run = lambda n: ops.paged_prefix_attention(qg, kg, vg, tg, n, prefix, dk, dv, c)  # noqa: E731
+    run(ln)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(ln)
+    side = torch.cuda.Stream()
+    other = torch.tensor([0] + [n - 7 for n in full[1:]], dtype=torch.int32).cuda()
+    alone = run(other)
+    for lengths in (full, [0] + full[1:], [5, 0] + [n - 30 for n in full[2:]], [0] * B, full):
+        ln.copy_(torch.tensor(lengths, dtype=torch.int32))
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            beside = [run(other) for _ in range(4)]
+        for _ in range(4):
+            graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, alone) for x in beside)
+        R.check(out, None, R.attention(q, kc, vc, table, lengths, dk, dv, c), dtype)
